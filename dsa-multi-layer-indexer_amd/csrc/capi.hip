@@ -380,7 +380,7 @@ extern "C" {
 
 const char* dsa_last_error(void) { return g_err; }
 
-const char* dsa_version(void) { return "dsa_mli 0.4.0 gfx950"; }
+const char* dsa_version(void) { return "dsa_mli 0.5.0 gfx950"; }
 
 size_t dsa_layer_args_bytes(void) { return sizeof(dsa_layer_args); }
 
@@ -726,6 +726,136 @@ int dsa_append_latent_rows(const void* latent_bf16, const int32_t* slots, int n,
   DSA_REQUIRE(kv_rows >= 1, DSA_ERR_INVALID_ARG, "dsa_append_latent_rows: kv_rows must be >= 1");
   return hip_status(dsa::launch_append_latent(latent_bf16, slots, n, kv_pool, (long)kv_rows, (hipStream_t)stream),
                     "append latent rows");
+}
+
+
+int dsa_rms_norm(const void* x, int dtype, int64_t x_stride, const void* residual, int64_t residual_stride,
+                 const void* weight, int weight_dtype, double eps, void* y, void* codes, float* scales, int group,
+                 void* residual_out, int64_t residual_out_stride, int n, int D, void* stream) {
+  DSA_REQUIRE(n >= 0, DSA_ERR_INVALID_ARG, "dsa_rms_norm: n must be >= 0 (got %d)", n);
+  if (n == 0) return DSA_OK;
+  DSA_REQUIRE(x && weight && ((y != nullptr) != (codes != nullptr)) && (!codes || scales), DSA_ERR_INVALID_ARG,
+              "dsa_rms_norm: x, weight and one of y and codes with scales are required");
+  DSA_REQUIRE(!residual_out || residual, DSA_ERR_INVALID_ARG, "dsa_rms_norm: residual_out without a residual");
+  DSA_REQUIRE(dtype >= 0 && dtype <= 2, DSA_ERR_INVALID_ARG, "dsa_rms_norm: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+  DSA_REQUIRE(weight_dtype == dtype || weight_dtype == 0, DSA_ERR_INVALID_ARG,
+              "dsa_rms_norm: the weight must be fp32 or of x's type");
+  DSA_REQUIRE(D >= 1 && D <= DSA_NORM_MAX_DIM, DSA_ERR_UNSUPPORTED, "dsa_rms_norm: D must be in [1, %d] (got %d)",
+              DSA_NORM_MAX_DIM, D);
+  DSA_REQUIRE(group == 0 || group == 128, DSA_ERR_UNSUPPORTED, "dsa_rms_norm: group must be 128 or 0 (got %d)", group);
+  DSA_REQUIRE(x_stride >= 0 && residual_stride >= 0 && (!residual_out || n == 1 || residual_out_stride >= D),
+              DSA_ERR_INVALID_ARG, "dsa_rms_norm: bad row stride");
+  dsa::NormArgs A{};
+  A.x = x, A.r = residual, A.w = weight, A.y = y, A.codes = static_cast<uint8_t*>(codes), A.scales = scales;
+  A.h = residual_out, A.xs = (long)x_stride, A.rs = (long)residual_stride, A.hs = (long)residual_out_stride;
+  A.n = n, A.D = D, A.group = group, A.w_f32 = weight_dtype == 0, A.eps = (float)eps;
+  return hip_status(dsa::launch_rms_norm(A, dtype, (hipStream_t)stream), "rms norm");
+}
+
+int dsa_rotary(const void* x, int dtype, int64_t x_token_stride, int64_t x_head_stride, const void* pos, int pos_bytes,
+               const float* cos_sin, int64_t max_pos, void* out, int64_t out_token_stride, int64_t out_head_stride,
+               int n, int H, int D, int R, int start, int interleaved, int inverse, void* stream) {
+  DSA_REQUIRE(n >= 0 && H >= 0, DSA_ERR_INVALID_ARG, "dsa_rotary: n and H must be >= 0 (got %d, %d)", n, H);
+  if (n == 0 || H == 0) return DSA_OK;
+  DSA_REQUIRE(x && pos && cos_sin && out, DSA_ERR_INVALID_ARG, "dsa_rotary: null pointer");
+  DSA_REQUIRE(dtype >= 0 && dtype <= 2, DSA_ERR_INVALID_ARG, "dsa_rotary: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+  DSA_REQUIRE(pos_bytes == 4 || pos_bytes == 8, DSA_ERR_INVALID_ARG, "dsa_rotary: pos_bytes must be 4 or 8");
+  DSA_REQUIRE(R >= 2 && R % 2 == 0 && start >= 0 && D <= 65536 && start + R <= D, DSA_ERR_INVALID_ARG,
+              "dsa_rotary: %d values from %d on of a head of %d", R, start, D);
+  DSA_REQUIRE((int64_t)H * D < ((int64_t)1 << 31), DSA_ERR_UNSUPPORTED, "dsa_rotary: H * D must be < 2^31");
+  DSA_REQUIRE(max_pos >= 1, DSA_ERR_INVALID_ARG, "dsa_rotary: max_pos must be >= 1");
+  dsa::RopeArgs A{};
+  A.x = x, A.out = out, A.pos = pos, A.table = cos_sin, A.max_pos = (long)max_pos;
+  A.xn = (long)x_token_stride, A.xh = (long)x_head_stride, A.on = (long)out_token_stride, A.oh = (long)out_head_stride;
+  A.n = n, A.H = H, A.D = D, A.R = R, A.start = start, A.pos64 = pos_bytes == 8;
+  A.interleaved = interleaved != 0, A.inverse = inverse != 0, A.copy = out != x;
+  return hip_status(dsa::launch_rotary(A, dtype, (hipStream_t)stream), "rotary");
+}
+
+int dsa_append_tokens(const int32_t* rows, const int32_t* pos, int n, const int32_t* page_table, int B, int pt_stride,
+                      const float* cos_sin, int64_t table_rows, int dtype, const void* latent, int64_t latent_stride,
+                      const void* norm_weight, int norm_weight_dtype, double eps, int interleaved, void* kv_pool,
+                      int64_t kv_rows, int row_bytes, const void* keys, int64_t keys_stride, int index_interleaved,
+                      void* index_k, int64_t num_pages, void* stream) {
+  DSA_REQUIRE(n >= 0, DSA_ERR_INVALID_ARG, "dsa_append_tokens: n must be >= 0 (got %d)", n);
+  if (n == 0) return DSA_OK;
+  DSA_REQUIRE(rows && pos && page_table && (latent || keys), DSA_ERR_INVALID_ARG,
+              "dsa_append_tokens: rows, pos, page_table and a latent or keys are required");
+  DSA_REQUIRE(B >= 1 && pt_stride >= 1, DSA_ERR_INVALID_ARG, "dsa_append_tokens: B and pt_stride must be >= 1");
+  DSA_REQUIRE(!cos_sin || table_rows >= 1, DSA_ERR_INVALID_ARG, "dsa_append_tokens: table_rows must be >= 1");
+  DSA_REQUIRE(dtype >= 0 && dtype <= 2, DSA_ERR_INVALID_ARG,
+              "dsa_append_tokens: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+  DSA_REQUIRE(!norm_weight || norm_weight_dtype == dtype || norm_weight_dtype == 0, DSA_ERR_INVALID_ARG,
+              "dsa_append_tokens: the norm weight must be fp32 or of the latent's type");
+  DSA_REQUIRE(!latent || (kv_pool && kv_rows >= 1 && aligned16(kv_pool)), DSA_ERR_INVALID_ARG,
+              "dsa_append_tokens: a latent needs a 16-byte aligned kv_pool of kv_rows >= 1 rows");
+  DSA_REQUIRE(!latent || row_bytes == DSA_LATENT_ROW_BYTES || row_bytes == DSA_FP4_ROW_BYTES, DSA_ERR_UNSUPPORTED,
+              "dsa_append_tokens: row_bytes must be %d or %d (got %d)", DSA_LATENT_ROW_BYTES, DSA_FP4_ROW_BYTES,
+              row_bytes);
+  DSA_REQUIRE(!keys || (index_k && num_pages >= 1 && aligned16(index_k)), DSA_ERR_INVALID_ARG,
+              "dsa_append_tokens: keys need a 16-byte aligned index_k of num_pages >= 1 pages");
+  DSA_REQUIRE(latent_stride >= 0 && keys_stride >= 0, DSA_ERR_INVALID_ARG, "dsa_append_tokens: bad row stride");
+  dsa::AppendArgs A{};
+  A.rows = rows, A.pos = pos, A.page_table = page_table, A.table = cos_sin, A.table_rows = (long)table_rows;
+  A.latent = latent, A.latent_stride = (long)latent_stride, A.norm_w = norm_weight, A.norm_w_f32 = norm_weight_dtype == 0;
+  A.eps = eps, A.interleaved = interleaved != 0, A.pool = static_cast<uint8_t*>(kv_pool), A.kv_rows = (long)kv_rows;
+  A.keys = keys, A.keys_stride = (long)keys_stride, A.index_interleaved = index_interleaved != 0;
+  A.index_k = static_cast<uint8_t*>(index_k), A.num_pages = (long)num_pages;
+  A.n = n, A.B = B, A.pt_stride = pt_stride;
+  return hip_status(dsa::launch_append_tokens(A, dtype, latent ? row_bytes : DSA_LATENT_ROW_BYTES, (hipStream_t)stream),
+                    "append tokens");
+}
+
+int dsa_read_latent_rows(const void* kv_pool, int64_t kv_rows, int row_bytes, const int32_t* slots, int n,
+                         void* out_bf16, void* stream) {
+  DSA_REQUIRE(n >= 0, DSA_ERR_INVALID_ARG, "dsa_read_latent_rows: n must be >= 0 (got %d)", n);
+  if (n == 0) return DSA_OK;
+  DSA_REQUIRE(kv_pool && slots && out_bf16, DSA_ERR_INVALID_ARG, "dsa_read_latent_rows: null pointer");
+  DSA_REQUIRE(kv_rows >= 1, DSA_ERR_INVALID_ARG, "dsa_read_latent_rows: kv_rows must be >= 1");
+  DSA_REQUIRE(row_bytes == DSA_LATENT_ROW_BYTES || row_bytes == DSA_FP4_ROW_BYTES, DSA_ERR_UNSUPPORTED,
+              "dsa_read_latent_rows: row_bytes must be %d or %d (got %d)", DSA_LATENT_ROW_BYTES, DSA_FP4_ROW_BYTES,
+              row_bytes);
+  DSA_REQUIRE(aligned16(kv_pool) && aligned16(out_bf16), DSA_ERR_INVALID_ARG,
+              "dsa_read_latent_rows: kv_pool and out must be 16-byte aligned");
+  return hip_status(dsa::launch_read_latent(kv_pool, (long)kv_rows, row_bytes, slots, n, out_bf16, (hipStream_t)stream),
+                    "read latent rows");
+}
+
+size_t dsa_mla_fp4_workspace_bytes(int B, int H, int nsplit) {
+  if (B < 1 || B > 65535 || H < 16 || H % 16 || H > 16 * 64 || nsplit < 0 || nsplit > 128) return 0;
+  return dsa::mla_fp4_workspace_bytes(B, H, nsplit);
+}
+
+static int mla_fp4(const void* q_bf16, const void* kv_pool, int64_t kv_rows, const int32_t* idx,
+                   const int32_t* page_table, int pt_stride, const int32_t* seq_lens, void* workspace, void* out_bf16,
+                   int B, int H, int keys, int nsplit, float sm_scale, void* stream) {
+  int rc = check_mla(q_bf16, kv_pool, kv_rows, idx, workspace, out_bf16, B, H, keys, nsplit,
+                     /*idx_required=*/page_table == nullptr);
+  if (rc) return rc;
+  dsa::Mla4Args A{};
+  A.q = static_cast<const uint16_t*>(q_bf16), A.pool = static_cast<const uint8_t*>(kv_pool), A.kv_rows = (long)kv_rows;
+  A.idx = idx, A.dense_pt = page_table, A.dense_pt_stride = pt_stride, A.dense_lens = seq_lens;
+  A.out = static_cast<uint16_t*>(out_bf16), A.sm_log2 = sm_scale * 1.4426950408889634f;
+  A.B = B, A.H = H, A.keys = keys;
+  return hip_status(dsa::launch_mla_fp4(A, nsplit, workspace, (hipStream_t)stream), "4-bit MLA launch");
+}
+
+int dsa_sparse_mla_decode_fp4(const void* q_bf16, const void* kv_pool, int64_t kv_rows, const int32_t* idx,
+                              void* workspace, void* out_bf16, int B, int H, int topk, int nsplit, float sm_scale,
+                              void* stream) {
+  return mla_fp4(q_bf16, kv_pool, kv_rows, idx, nullptr, 0, nullptr, workspace, out_bf16, B, H, topk, nsplit, sm_scale,
+                 stream);
+}
+
+int dsa_dense_mla_decode_fp4(const void* q_bf16, const void* kv_pool, int64_t kv_rows, const int32_t* page_table,
+                             int pt_stride, const int32_t* seq_lens, void* workspace, void* out_bf16, int B, int H,
+                             int nsplit, float sm_scale, void* stream) {
+  DSA_REQUIRE(page_table && seq_lens && pt_stride >= 1, DSA_ERR_INVALID_ARG,
+              "dsa_dense_mla_decode_fp4: page_table, seq_lens and pt_stride >= 1 are required");
+  DSA_REQUIRE((int64_t)pt_stride * DSA_PAGE_TOKENS <= (int64_t)1 << 30, DSA_ERR_UNSUPPORTED,
+              "dsa_dense_mla_decode_fp4: pt_stride too large");
+  return mla_fp4(q_bf16, kv_pool, kv_rows, nullptr, page_table, pt_stride, seq_lens, workspace, out_bf16, B, H,
+                 pt_stride * DSA_PAGE_TOKENS, nsplit, sm_scale, stream);
 }
 
 }  // extern "C"

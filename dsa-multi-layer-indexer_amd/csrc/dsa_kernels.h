@@ -134,4 +134,70 @@ hipError_t launch_append_keys(const void* k_bf16, const int* rows, const int* po
 hipError_t launch_append_latent(const void* lat_bf16, const int* slots, int n, void* pool, long kv_rows,
                                 hipStream_t s);
 
+// RMS norm with the residual's addition, and rotary positions (norm_rope.hip).
+// Strides in elements; element types as above.
+struct NormArgs {
+  const void* x;      // [n, D], row stride xs
+  const void* r;      // residual, row stride rs, or nullptr
+  const void* w;      // [D]
+  void* y;            // [n, D] contiguous, or nullptr: codes and scales
+  uint8_t* codes;     // [n, D] contiguous
+  float* scales;      // [n, groups]
+  void* h;            // x + r, row stride hs, or nullptr
+  long xs, rs, hs;
+  int n, D, group;    // group 128, or 0: one scale a row
+  int w_f32;          // the weight is fp32 (else of x's type)
+  float eps;
+};
+struct RopeArgs {
+  const void* x;
+  void* out;          // [n, H, D]; x itself, or disjoint from it
+  const void* pos;    // [n] int32 or int64
+  const float* table; // [max_pos, R]: cos of the R/2 pairs, then sin
+  long xn, xh, on, oh;
+  int n, H, D, R, start, pos64, inverse, interleaved;
+  int copy;           // out is not x: the other elements too
+  long max_pos;
+};
+hipError_t launch_rms_norm(const NormArgs& A, int dtype, hipStream_t s);
+hipError_t launch_rotary(const RopeArgs& A, int dtype, hipStream_t s);
+
+// Appends to the paged caches and reads of latent rows (latent_cache.hip).
+struct AppendArgs {
+  const int* rows;    // [n]
+  const int* pos;     // [n]
+  const int* page_table;
+  const float* table; // [table_rows, 64], or nullptr: no rotation
+  const void* latent; // [n, 576], row stride latent_stride, or nullptr
+  const void* norm_w; // [512] or nullptr
+  const void* keys;   // [n, 128], row stride keys_stride, or nullptr
+  uint8_t* pool;
+  uint8_t* index_k;
+  long latent_stride, keys_stride, table_rows, kv_rows, num_pages;
+  double eps;
+  int n, B, pt_stride, norm_w_f32, interleaved, index_interleaved;
+};
+hipError_t launch_append_tokens(const AppendArgs& A, int dtype, int row_bytes, hipStream_t s);
+hipError_t launch_read_latent(const void* pool, long kv_rows, int row_bytes, const int* slots, int n, void* out,
+                              hipStream_t s);
+
+// Sparse / dense MLA decode over 400-byte latent rows (mla_fp4.hip).
+struct Mla4Args {
+  const uint16_t* q;     // [B, H, 576] bf16
+  const uint8_t* pool;   // [kv_rows, 400]
+  long kv_rows;
+  const int* idx;        // [B, keys] KV slots (dense: unused)
+  const int* dense_pt;   // [B, dense_pt_stride] or nullptr
+  const int* dense_lens; // [B]
+  uint16_t* out;         // [B, H, 512] bf16
+  float sm_log2;         // sm_scale * log2(e)
+  int B, H, keys, dense_pt_stride;  // keys: of a selection, or those a dense row may hold
+  // filled by the launcher
+  float* part_o;         // [chunks, H, 512]
+  float* part_ml;        // [chunks, H, 2]
+  int chunks, units, per_row;
+};
+size_t mla_fp4_workspace_bytes(int B, int H, int nsplit);
+hipError_t launch_mla_fp4(Mla4Args A, int nsplit, void* workspace, hipStream_t s);
+
 }  // namespace dsa

@@ -22,7 +22,7 @@ INCLUDE = REPO_DIR / "include"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libdsa_mli.so"
 SOURCES = ["libdsa_mli.hip", "capi.hip", "mla_rows.hip", "prefill.hip", "prefill_logits.hip", "select_rows.hip",
-           "quant.hip", "sol.hip"]
+           "quant.hip", "norm_rope.hip", "latent_cache.hip", "mla_fp4.hip", "sol.hip"]
 ARCH = "gfx950"
 
 

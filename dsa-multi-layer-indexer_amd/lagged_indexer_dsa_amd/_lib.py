@@ -30,6 +30,8 @@ LATENT_DIM = 512
 ROPE_DIM = 64
 QK_DIM = 576
 LATENT_ROW_BYTES = 656
+FP4_ROW_BYTES = 400
+NORM_MAX_DIM = 32768
 TOPK_MAX_CTX = 262144
 SELECTION_MAX_CTX = 524288
 
@@ -37,6 +39,7 @@ _vp = ctypes.c_void_p
 _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 
 class DsaError(RuntimeError):
@@ -102,6 +105,16 @@ SIGNATURES = {
     "dsa_pack_latent_rows": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp]),
     "dsa_selection_set": (_i32, [_vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
     "dsa_prefill_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp]),
+    "dsa_rms_norm": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i32, _f64, _vp, _vp, _vp, _i32, _vp, _i64, _i32, _i32,
+                            _vp]),
+    "dsa_rotary": (_i32, [_vp, _i32, _i64, _i64, _vp, _i32, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32,
+                          _i32, _i32, _vp]),
+    "dsa_append_tokens": (_i32, [_vp, _vp, _i32, _vp, _i32, _i32, _vp, _i64, _i32, _vp, _i64, _vp, _i32, _f64, _i32,
+                                 _vp, _i64, _i32, _vp, _i64, _i32, _vp, _i64, _vp]),
+    "dsa_read_latent_rows": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _vp]),
+    "dsa_mla_fp4_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i32]),
+    "dsa_sparse_mla_decode_fp4": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp]),
+    "dsa_dense_mla_decode_fp4": (_i32, [_vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _f32, _vp]),
 }
 
 

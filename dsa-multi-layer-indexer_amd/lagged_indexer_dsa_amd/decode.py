@@ -46,6 +46,9 @@ class DecodeLayer:
     dense: bool = False               # attention over the whole prefix (full layer / DENSE cold start)
 
     def __post_init__(self) -> None:
+        if self.kv_pool.dim() != 2 or self.kv_pool.shape[1] != _lib.LATENT_ROW_BYTES:
+            raise RuntimeError("a decode layer's kv_pool must be [rows, 656] uint8 (4-bit rows are attended by "
+                               "ops.sparse_mla_decode and ops.dense_mla_decode)")
         B = self.q_bf16.shape[0]
         dev = self.q_bf16.device
         self.scores = torch.empty(B, self.slab_stride, dtype=torch.float32, device=dev)

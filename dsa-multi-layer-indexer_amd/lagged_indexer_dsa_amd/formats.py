@@ -4,6 +4,8 @@
   (reference K:540-546, K:630, K:2428; serving index-K buffer P:339-342).
 * latent KV row (656 B): [512 e4m3][4 x f32 scale, one per 128 dims]
   [64 x bf16 rope] (K:1114, K:1355-1395; SGLang fp8 KV layout P:800-803).
+* 4-bit latent row (400 B): [256 B: 512 e2m1, value 2i in the low half of byte
+  i][16 x e8m0 scale, one per 32 dims][64 x bf16 rope].
 * page table: int32 [B, pt_stride]; token g of row b is in physical page
   page_table[b, g // 64], slot g % 64; its latent row is KV slot
   page_table[b, g // 64] * 64 + g % 64 (hp_page_to_slot, K:1142-1144).
@@ -18,7 +20,7 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import INDEX_DIM, INDEX_PAGE_BYTES, LATENT_DIM, LATENT_ROW_BYTES, PAGE_TOKENS, ROPE_DIM
+from ._lib import FP4_ROW_BYTES, INDEX_DIM, INDEX_PAGE_BYTES, LATENT_DIM, LATENT_ROW_BYTES, PAGE_TOKENS, ROPE_DIM
 
 E4M3_MAX = 448.0
 
@@ -88,6 +90,33 @@ def pack_latent_rows(latent: torch.Tensor, rope: torch.Tensor) -> torch.Tensor:
     return rows
 
 
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+
+
+def pack_latent_rows_fp4(latent: torch.Tensor, rope: torch.Tensor) -> torch.Tensor:
+    """[n,512] latent + [n,64] rope -> [n,400] uint8 rows: per 32 values the
+    smallest power of two s with max(amax, 1e-6) <= 6 s, codes the nearest
+    e2m1 of x / s (ties to the even code); a group with a NaN or an infinity
+    gets the scale byte 255."""
+    n = latent.shape[0]
+    x = latent.float().reshape(n, 16, 32)
+    ok = x.isfinite().all(-1, keepdim=True)
+    x = torch.where(ok, x, 0.0)
+    m, e = torch.frexp(x.abs().amax(-1, keepdim=True).clamp_min(1e-6))
+    e = e - 3 + (m > 0.75).to(e.dtype)
+    a = torch.ldexp(x.abs().double(), -e)
+    step = torch.where(a < 2, 0.5, torch.where(a < 4, 1.0, 2.0))
+    a = (a / step).round() * step
+    levels = torch.tensor(_E2M1, dtype=torch.float64, device=x.device)
+    codes = torch.bucketize(a, levels).to(torch.uint8) | (x.signbit().to(torch.uint8) << 3)
+    rows = torch.empty(n, FP4_ROW_BYTES, dtype=torch.uint8, device=latent.device)
+    codes = codes.reshape(n, LATENT_DIM // 2, 2)
+    rows[:, :LATENT_DIM // 2] = codes[..., 0] | (codes[..., 1] << 4)
+    rows[:, LATENT_DIM // 2:LATENT_DIM // 2 + 16] = torch.where(ok, e + 127, 255).to(torch.uint8).reshape(n, 16)
+    rows[:, LATENT_DIM // 2 + 16:] = rope.to(torch.bfloat16).contiguous().view(torch.uint8).reshape(n, 2 * ROPE_DIM)
+    return rows
+
+
 def write_latent_rows(pool: torch.Tensor, page_table_row: torch.Tensor, rows: torch.Tensor,
                       start: int = 0) -> None:
     """Store packed latent rows of tokens start..start+n at their KV slots."""
@@ -110,5 +139,9 @@ def new_index_pool(num_pages: int, device) -> torch.Tensor:
     return torch.zeros(num_pages, INDEX_PAGE_BYTES, dtype=torch.uint8, device=device)
 
 
-def new_latent_pool(num_pages: int, device) -> torch.Tensor:
-    return torch.zeros(num_pages * PAGE_TOKENS, LATENT_ROW_BYTES, dtype=torch.uint8, device=device)
+def new_latent_pool(num_pages: int, device, bits: int = 8) -> torch.Tensor:
+    """An empty pool of 656-byte (bits 8) or 400-byte (bits 4) latent rows."""
+    if bits not in (4, 8):
+        raise ValueError(f"latent rows are kept in 8 or 4 bits, got {bits}")
+    row = LATENT_ROW_BYTES if bits == 8 else FP4_ROW_BYTES
+    return torch.zeros(num_pages * PAGE_TOKENS, row, dtype=torch.uint8, device=device)

@@ -13,12 +13,15 @@ from . import _lib
 from ._lib import (
     DSA_TOPK_POSITION_ORDER,
     DSA_TOPK_SORTED,
+    FP4_ROW_BYTES,
     INDEX_DIM,
     INDEX_PAGE_BYTES,
     LATENT_DIM,
     LATENT_ROW_BYTES,
+    NORM_MAX_DIM,
     PAGE_TOKENS,
     QK_DIM,
+    ROPE_DIM,
 )
 
 
@@ -145,10 +148,13 @@ def select_rows(scores: torch.Tensor, k: int, pad_value: int) -> torch.Tensor | 
 
 def sparse_mla_workspace(B: int, H: int, nsplit: int, device) -> torch.Tensor:
     """Zero-filled workspace (split partials + the splits' barriers; every
-    call leaves the barriers ready).  nsplit=0 sizes it for any split count."""
-    nbytes = _lib.load().dsa_sparse_mla_workspace_bytes(B, H, nsplit)
+    call leaves the barriers ready), for pools of either row format.  nsplit=0
+    sizes it for any split count."""
+    lib = _lib.load()
+    nbytes = lib.dsa_sparse_mla_workspace_bytes(B, H, nsplit)
     if nbytes == 0:
         raise RuntimeError(f"bad sparse MLA workspace shape B={B} H={H} nsplit={nsplit}")
+    nbytes = max(nbytes, lib.dsa_mla_fp4_workspace_bytes(B, H, nsplit))
     return torch.zeros(nbytes // 4, dtype=torch.float32, device=device)
 
 
@@ -171,17 +177,58 @@ def _resolve_nsplit(nsplit: int, B: int, H: int, keys: int) -> int:
     return nsplit or max(1, _lib.load().dsa_sparse_mla_auto_nsplit(B, H, keys))
 
 
+def _here(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    """All on one device, the one the call's kernels go to."""
+    dev = first.device
+    if dev.index != torch.cuda.current_device():
+        raise RuntimeError(f"tensors are on {dev}, the current device is cuda:{torch.cuda.current_device()}")
+    for t in others:
+        if t is not None and t.device != dev:
+            raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
+
+
+def _fp4_call(q, kv_pool, sm_scale, nsplit: int, workspace, out, *others):
+    """What a decode call over 400-byte rows checks besides its keys."""
+    qs = q.shape
+    if len(qs) != 3 or qs[2] != QK_DIM or q.dtype != torch.bfloat16:
+        raise RuntimeError("q must be [B, H, 576] bfloat16")
+    if kv_pool.dtype != torch.uint8:
+        raise RuntimeError("kv_pool must be [rows, 400] uint8")
+    B, H, _ = qs
+    nbytes = _lib.load().dsa_mla_fp4_workspace_bytes(B, H, nsplit)
+    if workspace is None:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    else:
+        _dev(workspace)
+        _need_bytes("4-bit MLA workspace", workspace, nbytes)
+    if out is None:
+        out = torch.empty(B, H, LATENT_DIM, dtype=torch.bfloat16, device=q.device)
+    else:
+        _dev(out)
+        _need_shape("out", out, (B, H, LATENT_DIM), torch.bfloat16)
+    _here(q, kv_pool, workspace, out, *others)
+    return B, H, QK_DIM ** -0.5 if sm_scale is None else float(sm_scale), workspace, out
+
+
 def sparse_mla_decode(q: torch.Tensor, kv_pool: torch.Tensor, idx: torch.Tensor,
                       sm_scale: float | None = None, nsplit: int = 0,
                       workspace: torch.Tensor | None = None,
                       out: torch.Tensor | None = None) -> torch.Tensor:
-    """Split-K sparse MLA over the fp8 656-byte latent pool.
+    """Split-K sparse MLA over the latent pool, in 656-byte fp8 rows or in
+    400-byte 4-bit ones.
 
-    q [B,H,576] bf16; kv_pool [rows,656] uint8; idx [B,topk] int32 KV slots
-    (out-of-range = masked)  ->  out [B,H,512] bf16.
+    q [B,H,576] bf16; kv_pool [rows,656] or [rows,400] uint8; idx [B,topk]
+    int32 KV slots (out-of-range = masked)  ->  out [B,H,512] bf16.
     Reference: attention_core.py:121-146 sparse_mla_core; K:2950-2966.
     """
     _dev(q, kv_pool, idx)
+    if kv_pool.dim() == 2 and kv_pool.shape[1] == FP4_ROW_BYTES:
+        B, H, sm_scale, workspace, out = _fp4_call(q, kv_pool, sm_scale, nsplit, workspace, out, idx)
+        if idx.dim() != 2 or idx.shape[0] != B or idx.dtype != torch.int32:
+            raise RuntimeError("idx must be [B, topk] int32")
+        _lib.call("dsa_sparse_mla_decode_fp4", q.data_ptr(), kv_pool.data_ptr(), kv_pool.shape[0], idx.data_ptr(),
+                  workspace.data_ptr(), out.data_ptr(), B, H, idx.shape[1], nsplit, sm_scale, _stream())
+        return out
     if q.dim() != 3 or q.shape[2] != QK_DIM or q.dtype != torch.bfloat16:
         raise RuntimeError("q must be [B, H, 576] bfloat16")
     B, H, _ = q.shape
@@ -214,11 +261,20 @@ def dense_mla_decode(q: torch.Tensor, kv_pool: torch.Tensor, page_table: torch.T
     """Dense MLA of each decode row over its first seq_lens[b] tokens, their
     latent rows found through the page table (64-token pages).
 
-    q [B,H,576] bf16; kv_pool [rows,656] uint8; page_table [B,pt] int32;
-    seq_lens [B] int32  ->  out [B,H,512] bf16.
+    q [B,H,576] bf16; kv_pool [rows,656] or [rows,400] uint8; page_table
+    [B,pt] int32; seq_lens [B] int32  ->  out [B,H,512] bf16.
     Reference: attention_core.py:142-160 dense_mla_core; model.py:104-114.
     """
     _dev(q, kv_pool, page_table, seq_lens)
+    if kv_pool.dim() == 2 and kv_pool.shape[1] == FP4_ROW_BYTES:
+        B, H, sm_scale, workspace, out = _fp4_call(q, kv_pool, sm_scale, nsplit, workspace, out, page_table, seq_lens)
+        if page_table.dim() != 2 or page_table.shape[0] != B or page_table.dtype != torch.int32:
+            raise RuntimeError("page_table must be [B, pt_stride] int32")
+        _need_shape("seq_lens", seq_lens, (B,), torch.int32)
+        _lib.call("dsa_dense_mla_decode_fp4", q.data_ptr(), kv_pool.data_ptr(), kv_pool.shape[0],
+                  page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(), workspace.data_ptr(),
+                  out.data_ptr(), B, H, nsplit, sm_scale, _stream())
+        return out
     if q.dim() != 3 or q.shape[2] != QK_DIM or q.dtype != torch.bfloat16:
         raise RuntimeError("q must be [B, H, 576] bfloat16")
     B, H, _ = q.shape
@@ -413,3 +469,297 @@ def append_latent_rows(kv_pool: torch.Tensor, slots: torch.Tensor, latent: torch
     _need_shape("slots", slots, (n,), torch.int32)
     _lib.call("dsa_append_latent_rows", latent.data_ptr(), slots.data_ptr(), n, kv_pool.data_ptr(),
               kv_pool.shape[0], _stream())
+
+
+# ---- around the cached attention: norm, rotation, cache appends and reads ----
+
+def _rows_of(name: str, x: torch.Tensor, D: int | None = None) -> torch.Tensor:
+    """x [..., D] as rows [n, D] without a copy; the last dim contiguous."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise RuntimeError("lagged_indexer_dsa_amd ops need GPU (HIP) tensors; there is no CPU path")
+    shape = x.shape
+    if not shape or (D is not None and shape[-1] != D):
+        raise RuntimeError(f"{name} must be [..., {'D' if D is None else D}], got {tuple(shape)}")
+    if shape[-1] > 1 and x.stride(-1) != 1:
+        raise RuntimeError(f"{name}'s last dimension must be contiguous")
+    if len(shape) != 2:
+        try:
+            x = x.view(-1, shape[-1]) if x.numel() else x.reshape(0, shape[-1])
+        except RuntimeError:
+            raise RuntimeError(f"{name}'s leading dimensions must be one stride apart, got strides {x.stride()}") from None
+    return x
+
+
+def _span(t: torch.Tensor) -> tuple[int, int]:
+    """The bytes a non-empty tensor lies in."""
+    end = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1
+    at = t.data_ptr()
+    return at, at + end * t.element_size()
+
+
+def _need_apart(name: str, out: torch.Tensor, *inputs: torch.Tensor | None) -> None:
+    """An output's bytes hold none of the inputs'."""
+    lo, hi = _span(out)
+    for t in inputs:
+        if t is not None:
+            a, b = _span(t)
+            if a < hi and lo < b:
+                raise RuntimeError(f"{name} overlaps an input")
+
+
+def _norm(x, weight, eps, residual, out, out_q, out_scale, group, out_residual):
+    xr = _rows_of("x", x)
+    n, D = xr.shape
+    dtype = x.dtype
+    if dtype not in _PACK_DTYPES:
+        raise RuntimeError(f"x must be float32, bfloat16 or float16, got {dtype}")
+    if not 1 <= D <= NORM_MAX_DIM:
+        raise RuntimeError(f"x's rows must hold 1 to {NORM_MAX_DIM} values, got {D}")
+    _dev(weight)
+    if weight.shape != (D,) or (weight.dtype != dtype and weight.dtype != torch.float32):
+        raise RuntimeError(f"weight must be [{D}] of x's type or float32, got {weight.dtype} {tuple(weight.shape)}")
+    rr = hr = None
+    h = None
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != dtype:
+            raise RuntimeError(f"residual must be {dtype} {tuple(x.shape)}, got {residual.dtype} {tuple(residual.shape)}")
+        rr = _rows_of("residual", residual)
+        if out_residual is None:
+            h = hr = torch.empty(x.shape, dtype=dtype, device=x.device)
+            hr = _rows_of("out_residual", hr)
+        else:
+            h = out_residual
+            if h.shape != x.shape or h.dtype != dtype:
+                raise RuntimeError(f"out_residual must be {dtype} {tuple(x.shape)}, got {h.dtype} {tuple(h.shape)}")
+            hr = _rows_of("out_residual", h)
+            if n > 1 and hr.stride(0) < D:
+                raise RuntimeError("out_residual's rows overlap")
+            if n and (hr.data_ptr() != rr.data_ptr() or hr.stride(0) != rr.stride(0)):
+                _need_apart("out_residual", hr, xr, rr, weight)
+            elif n:
+                _need_apart("out_residual", hr, xr, weight)
+    elif out_residual is not None:
+        raise RuntimeError("out_residual without a residual")
+    _here(x, weight, residual, h, out, out_q, out_scale)
+    if n and (out is not None or out_q is not None or out_scale is not None):
+        for name, t in (("out", out), ("out_q", out_q), ("out_scale", out_scale)):
+            if t is not None and t.numel():
+                _need_apart(name, t, xr, rr, hr, weight)
+        if out_q is not None and out_scale is not None:
+            _need_apart("out_scale", out_scale, out_q)
+    if n:
+        _lib.call("dsa_rms_norm", xr.data_ptr(), _PACK_DTYPES[dtype], xr.stride(0), _ptr(rr),
+                  0 if rr is None else rr.stride(0), weight.data_ptr(), _PACK_DTYPES[weight.dtype], eps, _ptr(out),
+                  _ptr(out_q), _ptr(out_scale), group, _ptr(hr), 0 if hr is None else hr.stride(0), n, D, _stream())
+    return h
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
+             out: torch.Tensor | None = None, out_residual: torch.Tensor | None = None):
+    """h = x + residual (or x); h / sqrt(mean(h^2) + eps) * weight over the last
+    dim, in fp32 -> out, of x's type; with a residual (out, h).
+
+    x [..., D] fp32, bf16 or fp16 (rows any one stride apart, D up to 32768),
+    residual of the same shape and type, weight [D] of x's type or fp32.
+    out_residual may be residual itself.  h is rounded to x's type only as it is
+    stored.  Reference: dsa_layer.py:32-52 RMSNorm.
+    """
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    else:
+        _dev(out)
+        _need_shape("out", out, x.shape, x.dtype)
+    h = _norm(x, weight, eps, residual, out, None, None, 0, out_residual)
+    return out if residual is None else (out, h)
+
+
+def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
+                   group: int = 128, out_q: torch.Tensor | None = None, out_scale: torch.Tensor | None = None,
+                   out_residual: torch.Tensor | None = None):
+    """:func:`rms_norm` with its output in e4m3: (codes uint8 [..., D], scales
+    fp32 [..., groups]) and, with a residual, h.
+
+    group 128: a scale per 128 values (the last group may be short); group 0:
+    one per row.  scale = max(amax, 1e-6) / 448; a NaN makes its group's scale
+    and codes NaN.  Reference: dsa_layer.py:32-52 and the act_quant before an
+    fp8 product (inference/modeling/kernels.py:35-117).
+    """
+    if group not in (0, 128):
+        raise RuntimeError(f"group must be 128 or 0, got {group}")
+    shape = x.shape
+    if not shape:
+        raise RuntimeError("x must be [..., D]")
+    sshape = (*shape[:-1], -(-shape[-1] // 128) if group else 1)
+    if out_q is None:
+        out_q = torch.empty(shape, dtype=torch.uint8, device=x.device)
+    else:
+        _dev(out_q)
+        _need_shape("out_q", out_q, shape, torch.uint8)
+    if out_scale is None:
+        out_scale = torch.empty(sshape, dtype=torch.float32, device=x.device)
+    else:
+        _dev(out_scale)
+        _need_shape("out_scale", out_scale, sshape, torch.float32)
+    h = _norm(x, weight, eps, residual, None, out_q, out_scale, group, out_residual)
+    return (out_q, out_scale) if residual is None else (out_q, out_scale, h)
+
+
+def rotary(x: torch.Tensor, pos: torch.Tensor, cos_sin: torch.Tensor, interleaved: bool = False, start: int = 0,
+           inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Values start .. start + R - 1 of every head turned by its token's
+    position: (a, b) -> (a cos - b sin, b cos + a sin), in fp32.
+
+    x [n, H, D] or [n, D] fp32, bf16 or fp16, any strides but a contiguous last
+    dim (a slice of wider heads); pos [n] int32 or int64; cos_sin [positions, R]
+    fp32 (``rope.build_rope_table``).  Pairs are i and i + R/2 or, interleaved,
+    2i and 2i + 1; inverse turns back (and is the gradient's direction).  out:
+    x itself (only the turned values are touched), a tensor that does not
+    overlap it, or None for a new one; the other values are copied then.  A
+    token whose position is not in the table (padding, say -1) is not turned.
+    Reference: rope.py:25-84 apply_rotary.
+    """
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise RuntimeError("lagged_indexer_dsa_amd ops need GPU (HIP) tensors; there is no CPU path")
+    _dev(pos, cos_sin)
+    shape = x.shape
+    if len(shape) == 3:
+        n, H, D = shape
+        xn, xh, xd = x.stride()
+    elif len(shape) == 2:
+        (n, D), H = shape, 1
+        xn, xd = x.stride()
+        xh = 0
+    else:
+        raise RuntimeError(f"x must be [n, H, D] or [n, D], got {tuple(shape)}")
+    if x.dtype not in _PACK_DTYPES:
+        raise RuntimeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
+    if pos.shape != (n,) or pos.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError(f"pos must be [{n}] int32 or int64, got {pos.dtype} {tuple(pos.shape)}")
+    if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32:
+        raise RuntimeError("cos_sin must be [positions, R] float32")
+    P, R = cos_sin.shape
+    if R < 2 or R % 2 or start < 0 or start + R > D or P < 1:
+        raise RuntimeError(f"a table of {P} positions and {R} values does not fit values {start} on of {D}")
+    if D > 1 and xd != 1:
+        raise RuntimeError("x's last dimension must be contiguous")
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    elif out.shape != shape or out.dtype != x.dtype:
+        raise RuntimeError(f"out must be {x.dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
+    _here(x, pos, cos_sin, out)
+    on, oh = (out.stride(0), out.stride(1)) if len(shape) == 3 else (out.stride(0), 0)
+    if D > 1 and out.stride(-1) != 1:
+        raise RuntimeError("out's last dimension must be contiguous")
+    if n == 0 or H == 0:
+        return out
+    # no two heads of out at one place: the larger stride steps over the others
+    (small, ns), (large, nl) = sorted(((on, n), (oh, H)))
+    if (ns > 1 and small < D) or (nl > 1 and large < (ns - 1) * small + D):
+        raise RuntimeError(f"out's heads overlap (strides {out.stride()})")
+    same = out.data_ptr() == x.data_ptr()
+    if same and (on, oh) != (xn, xh):
+        raise RuntimeError("out is x with other strides")
+    _need_apart("out", out, pos, cos_sin, *(() if same else (x,)))
+    _lib.call("dsa_rotary", x.data_ptr(), _PACK_DTYPES[x.dtype], xn, xh, pos.data_ptr(), pos.element_size(),
+              cos_sin.data_ptr(), P, out.data_ptr(), on, oh, n, H, D, R, start, interleaved, inverse, _stream())
+    return out
+
+
+def append_tokens(page_table: torch.Tensor, rows: torch.Tensor, pos: torch.Tensor,
+                  kv_pool: torch.Tensor | None = None, latent: torch.Tensor | None = None,
+                  index_k: torch.Tensor | None = None, keys: torch.Tensor | None = None,
+                  cos_sin: torch.Tensor | None = None, norm_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                  interleaved: bool = False, index_interleaved: bool = False) -> None:
+    """New tokens into the paged caches, in one launch: token i belongs to
+    request rows[i] at position pos[i], its page in page_table [B, pt_stride]
+    int32.
+
+    latent [n, 576] (512 latent | 64 rope): the latent part normed when
+    norm_weight [512] is given, the rope part turned when cos_sin [positions, 64]
+    is given (:func:`rotary`'s pairs and table), into kv_pool: [rows, 656]
+    uint8 (e4m3, a scale per 128) or [rows, 400] (4-bit e2m1, a power-of-two
+    scale per 32).  keys [n, 128]: the first 64 turned, into index_k [pages,
+    8448].  Either pair may be left out.  latent and keys are fp32, bf16 or
+    fp16, rows any one stride apart; norm_weight of the same type or fp32.  A
+    token without a request, page, slot or table row is skipped; two tokens of
+    one slot must hold the same values.
+    Reference: sglang overlay P:252-363, P:789; dsa_layer.py:92-143.
+    """
+    _dev(page_table, rows, pos)
+    n = rows.shape[0] if rows.dim() == 1 else -1
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or not page_table.numel():
+        raise RuntimeError("page_table must be [B, pt_stride] int32")
+    if n < 0 or rows.dtype != torch.int32:
+        raise RuntimeError("rows must be [n] int32")
+    _need_shape("pos", pos, (n,), torch.int32)
+    if latent is None and keys is None:
+        raise RuntimeError("append_tokens needs a latent, keys or both")
+    if (latent is None) != (kv_pool is None) or (keys is None) != (index_k is None):
+        raise RuntimeError("latent goes with kv_pool, keys with index_k")
+    ls = ks = row_bytes = kv_rows = pages = table_rows = w_dtype = 0
+    dtype = (keys if latent is None else latent).dtype
+    if dtype not in _PACK_DTYPES:
+        raise RuntimeError(f"latent and keys must be float32, bfloat16 or float16, got {dtype}")
+    if latent is not None:
+        ls = _append_rows("latent", latent, n, QK_DIM, dtype)
+        _dev(kv_pool)
+        kv_rows, row_bytes = kv_pool.shape if kv_pool.dim() == 2 else (0, 0)
+        if row_bytes not in (LATENT_ROW_BYTES, FP4_ROW_BYTES) or kv_pool.dtype != torch.uint8 or not kv_rows:
+            raise RuntimeError("kv_pool must be [rows, 656] or [rows, 400] uint8")
+        if norm_weight is not None:
+            _dev(norm_weight)
+            if norm_weight.shape != (LATENT_DIM,) or norm_weight.dtype not in (dtype, torch.float32):
+                raise RuntimeError("norm_weight must be [512] of the latent's type or float32")
+            w_dtype = _PACK_DTYPES[norm_weight.dtype]
+    elif norm_weight is not None:
+        raise RuntimeError("norm_weight without a latent")
+    if keys is not None:
+        ks = _append_rows("keys", keys, n, INDEX_DIM, dtype)
+        _dev(index_k)
+        if index_k.dim() != 2 or index_k.shape[1] != INDEX_PAGE_BYTES or index_k.dtype != torch.uint8 or not len(index_k):
+            raise RuntimeError("index_k must be [pages, 8448] uint8")
+        pages = index_k.shape[0]
+    if cos_sin is not None:
+        _dev(cos_sin)
+        if cos_sin.dim() != 2 or cos_sin.shape[1] != ROPE_DIM or cos_sin.dtype != torch.float32 or not len(cos_sin):
+            raise RuntimeError("cos_sin must be [positions, 64] float32")
+        table_rows = cos_sin.shape[0]
+    _here(page_table, rows, pos, kv_pool, latent, index_k, keys, cos_sin, norm_weight)
+    _lib.call("dsa_append_tokens", rows.data_ptr(), pos.data_ptr(), n, page_table.data_ptr(), page_table.shape[0],
+              page_table.shape[1], _ptr(cos_sin), table_rows, _PACK_DTYPES[dtype], _ptr(latent), ls,
+              _ptr(norm_weight), w_dtype, eps, interleaved, _ptr(kv_pool), kv_rows, row_bytes, _ptr(keys), ks,
+              index_interleaved, _ptr(index_k), pages, _stream())
+
+
+def _append_rows(name: str, x: torch.Tensor, n: int, width: int, dtype) -> int:
+    """The row stride of an append's input."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise RuntimeError("lagged_indexer_dsa_amd ops need GPU (HIP) tensors; there is no CPU path")
+    if x.shape != (n, width) or x.dtype != dtype or x.stride(1) != 1:
+        raise RuntimeError(f"{name} must be {dtype} [{n}, {width}] with a contiguous last dimension, got {x.dtype} "
+                           f"{tuple(x.shape)}")
+    return x.stride(0)
+
+
+def read_latent_rows(kv_pool: torch.Tensor, slots: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values of cached latent rows, bf16 [n, 576] (512 latent | 64 rope):
+    what the attention reads of KV slots slots [n] int32 of a pool of 656- or
+    400-byte rows.  With them the prefill ops attend a cached prefix.  A slot
+    outside the pool gives zeros.  Reference: P:789 dequantize_k_cache.
+    """
+    _dev(kv_pool, slots)
+    kv_rows, row_bytes = kv_pool.shape if kv_pool.dim() == 2 else (0, 0)
+    if row_bytes not in (LATENT_ROW_BYTES, FP4_ROW_BYTES) or kv_pool.dtype != torch.uint8 or not kv_rows:
+        raise RuntimeError("kv_pool must be [rows, 656] or [rows, 400] uint8")
+    if slots.dim() != 1 or slots.dtype != torch.int32:
+        raise RuntimeError("slots must be [n] int32")
+    n = slots.shape[0]
+    if out is None:
+        out = torch.empty(n, QK_DIM, dtype=torch.bfloat16, device=kv_pool.device)
+    else:
+        _dev(out)
+        _need_shape("out", out, (n, QK_DIM), torch.bfloat16)
+    _here(kv_pool, slots, out)
+    _lib.call("dsa_read_latent_rows", kv_pool.data_ptr(), kv_rows, row_bytes, slots.data_ptr(), n, out.data_ptr(),
+              _stream())
+    return out

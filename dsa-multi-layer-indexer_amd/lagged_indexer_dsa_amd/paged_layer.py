@@ -17,6 +17,10 @@ timed hot path.  Shapes the kernels accept: kv_lora_rank 512, rope 64
 (576-wide absorbed queries), index_head_dim 128, index_n_heads 16/32/48/64,
 attention heads a multiple of 16.
 
+With ``kv_bits=4`` the latent pool holds 400-byte rows (39 % less cache); the
+keys and rows of new tokens are then stored by ``ops.append_tokens`` and the
+attention is a launch of its own beside the layer's scan and top-k.
+
 Index convention: selections cross this API as token positions, int64
 ``[B, 1, topk]`` like ``select_topk`` returns them, with the sentinel
 ``S_kv`` (the row length) for unused entries.  They come back in ascending
@@ -32,13 +36,15 @@ import torch
 
 from . import _lib, ops
 from ._lib import INDEX_DIM, LATENT_DIM, PAGE_TOKENS, QK_DIM, LayerArgs
+from .formats import new_latent_pool
 
 
 class PagedDSALayer:
     """Paged caches of one layer for ``batch`` rows of up to ``max_ctx``
     tokens each (identity paging: row b owns pages [b*npg, (b+1)*npg))."""
 
-    def __init__(self, layer, batch: int, max_ctx: int, device=None, nsplit: int = 0) -> None:
+    def __init__(self, layer, batch: int, max_ctx: int, device=None, nsplit: int = 0,
+                 kv_bits: int = 8) -> None:
         cfg = layer.config
         if cfg.kv_lora_rank + cfg.qk_rope_head_dim != QK_DIM or cfg.kv_lora_rank != LATENT_DIM:
             raise ValueError("the fp8 latent format needs kv_lora_rank 512 and qk_rope_head_dim 64")
@@ -55,7 +61,8 @@ class PagedDSALayer:
         self.page_table = (torch.arange(B, dtype=torch.int32, device=dev)[:, None] * self.npg
                            + torch.arange(self.npg, dtype=torch.int32, device=dev)[None, :]).contiguous()
         self.index_k = torch.zeros(B * self.npg, _lib.INDEX_PAGE_BYTES, dtype=torch.uint8, device=dev)
-        self.kv_pool = torch.zeros(B * self.cap, _lib.LATENT_ROW_BYTES, dtype=torch.uint8, device=dev)
+        self.kv_bits = int(kv_bits)
+        self.kv_pool = new_latent_pool(B * self.npg, dev, self.kv_bits)
         self.seq_lens = torch.zeros(B, dtype=torch.int32, device=dev)
         self.length = 0
         self.scores = torch.empty(B, self.cap, dtype=torch.float32, device=dev)
@@ -79,10 +86,15 @@ class PagedDSALayer:
         pos = torch.arange(self.length, self.length + S, dtype=torch.int32, device=kv.device)
         rows = self._rows.repeat_interleave(S)
         posb = pos.repeat(B)
-        ops.append_index_keys(self.index_k, self.page_table, rows, posb,
-                              index_k.reshape(B * S, INDEX_DIM).to(torch.bfloat16).contiguous())
-        slots = (rows.long() * self.cap + posb.long()).to(torch.int32)
-        ops.append_latent_rows(self.kv_pool, slots, kv.reshape(B * S, QK_DIM).to(torch.bfloat16).contiguous())
+        keys = index_k.reshape(B * S, INDEX_DIM).to(torch.bfloat16).contiguous()
+        latent = kv.reshape(B * S, QK_DIM).to(torch.bfloat16).contiguous()
+        if self.kv_bits == 4:
+            ops.append_tokens(self.page_table, rows, posb, kv_pool=self.kv_pool, latent=latent, index_k=self.index_k,
+                              keys=keys)
+        else:
+            ops.append_index_keys(self.index_k, self.page_table, rows, posb, keys)
+            slots = (rows.long() * self.cap + posb.long()).to(torch.int32)
+            ops.append_latent_rows(self.kv_pool, slots, latent)
         self.length += S
         self.seq_lens.fill_(self.length)
 
@@ -139,18 +151,28 @@ class PagedDSALayer:
             a.Hidx = self.Hidx
         a.scores, a.topk_scratch, a.next_idx = (self.scores.data_ptr(), self.topk_scratch.data_ptr(),
                                                 self.next_idx.data_ptr())
-        a.q_bf16, a.kv_pool, a.kv_rows = q_bf16.data_ptr(), self.kv_pool.data_ptr(), self.kv_pool.shape[0]
-        a.workspace, a.out_bf16 = self.workspace.data_ptr(), self.out.data_ptr()
-        if attn_indices is None:
-            a.dense = 1
-        else:
+        if attn_indices is not None:
             self.attend.copy_(self._to_slots(attn_indices))
-            a.attend_idx = self.attend.data_ptr()
+        if self.kv_bits == 4:
+            if attn_indices is None:
+                ops.dense_mla_decode(q_bf16, self.kv_pool, self.page_table, self.seq_lens, nsplit=self.nsplit,
+                                     workspace=self.workspace, out=self.out)
+            else:
+                ops.sparse_mla_decode(q_bf16, self.kv_pool, self.attend, nsplit=self.nsplit, workspace=self.workspace,
+                                      out=self.out)
+        else:
+            a.q_bf16, a.kv_pool, a.kv_rows = q_bf16.data_ptr(), self.kv_pool.data_ptr(), self.kv_pool.shape[0]
+            a.workspace, a.out_bf16 = self.workspace.data_ptr(), self.out.data_ptr()
+            if attn_indices is None:
+                a.dense = 1
+            else:
+                a.attend_idx = self.attend.data_ptr()
         a.page_table, a.seq_lens = self.page_table.data_ptr(), self.seq_lens.data_ptr()
         a.B, a.H, a.topk, a.nsplit = self.B, self.H, self.topk, self.nsplit
         a.pt_stride, a.slab_stride = self.npg, self.cap
         a.sm_scale = QK_DIM ** -0.5
-        _lib.call("dsa_decode_layer", ctypes.byref(a), torch.cuda.current_stream().cuda_stream)
+        if produce_indexer or self.kv_bits == 8:
+            _lib.call("dsa_decode_layer", ctypes.byref(a), torch.cuda.current_stream().cuda_stream)
         o_latent = self.out.float().reshape(self.B, 1, self.H, LATENT_DIM).to(x_norm.dtype)
         hidden = lay._project_output(o_latent)
         nxt = self._to_positions(self.next_idx) if produce_indexer else None

@@ -28,6 +28,10 @@
  *   latent KV row : 656 bytes = [512 e4m3][4 fp32 scales, one per 128 dims]
  *                   [64 bf16 rope]; the row of token g of row b is KV slot
  *                   page_table[b*pt_stride + g/64]*64 + g%64.
+ *   4-bit latent row : 400 bytes = [256 B: 512 e2m1, value 2i in the low half
+ *                   of byte i][16 e8m0 scales, one per 32 values][64 bf16 rope],
+ *                   at the same KV slots; value = e2m1 * 2^(byte - 127), a
+ *                   scale byte of 255 makes its 32 values NaN.
  *   e4m3          : OCP float8 e4m3fn (bias 7, max 448, 0x7f/0xff = NaN).
  */
 #ifndef DSA_MLI_H
@@ -52,6 +56,8 @@ extern "C" {
 #define DSA_ROPE_DIM 64
 #define DSA_QK_DIM 576
 #define DSA_LATENT_ROW_BYTES 656  /* 512 + 4*4 + 64*2 */
+#define DSA_FP4_ROW_BYTES 400     /* 512/2 + 16 + 64*2 */
+#define DSA_NORM_MAX_DIM 32768    /* longest row of dsa_rms_norm */
 #define DSA_TOPK_MAX_CTX 262144   /* longest row the top-k select accepts */
 #define DSA_SELECTION_MAX_CTX 524288 /* longest context of dsa_selection_set */
 
@@ -421,6 +427,96 @@ int dsa_selection_set(const void* idx, int idx_bytes, int B, int S, int n, int T
                       void* stream);
 int dsa_prefill_attention(const void* q_bf16, const void* keys, const uint32_t* bits, void* workspace, void* out_bf16,
                           int B, int S, int H, int T, float sm_scale, void* stream);
+
+/*
+ * (8) RMS norm with the residual's addition.  dtype codes as in (6a).
+ *   h = x + residual (or x),  y = h / sqrt(mean(h^2) + eps) * weight, in fp32;
+ *   x, residual [n, D] with row strides in elements (the last dim contiguous;
+ *   a stride of 0 repeats one row), weight [D] of x's type or fp32.
+ *   Either y [n, D] of x's type, or codes [n, D] e4m3 with scales:
+ *   max(amax |y|, 1e-6) / 448 per 128 values (group 128: [n, ceil(D/128)], the
+ *   last group may be short) or per row (group 0: [n, 1]); a NaN makes its
+ *   group's scale and codes NaN.  y and codes contiguous.
+ *   residual_out (may be NULL; may be residual itself, with its stride): h
+ *   rounded to x's type.  Outputs must not overlap inputs otherwise.
+ *   1 <= D <= DSA_NORM_MAX_DIM.
+ * Replaces: RMSNorm (dsa_layer.py:32-52) and the act_quant before an fp8
+ * product (inference/modeling/kernels.py:35-117; this library's scale rule).
+ */
+int dsa_rms_norm(const void* x, int dtype, int64_t x_stride, const void* residual, int64_t residual_stride,
+                 const void* weight, int weight_dtype, double eps, void* y, void* codes, float* scales, int group,
+                 void* residual_out, int64_t residual_out_stride, int n, int D, void* stream);
+
+/*
+ * (9) Rotary positions: values start .. start + R - 1 of every head of x
+ * [n, H, D] turned by its token's position, pair (a, b) -> (a c - b s,
+ * b c + a s) in fp32, rounded once; pairs are i and i + R/2, or (interleaved)
+ * 2i and 2i + 1; inverse: by -s (the operation's adjoint).
+ *   cos_sin [max_pos, R] fp32: R/2 cosines, then R/2 sines; pos [n] int32 or
+ *   int64 (pos_bytes).  Strides in elements, the last dim contiguous.
+ *   out may be x itself (same strides; the other values are not touched) or a
+ *   tensor that does not overlap it (the other values are copied).  A token
+ *   whose position is outside the table is padding: not turned.
+ * Replaces: apply_rotary (rope.py:25-84).
+ */
+int dsa_rotary(const void* x, int dtype, int64_t x_token_stride, int64_t x_head_stride, const void* pos, int pos_bytes,
+               const float* cos_sin, int64_t max_pos, void* out, int64_t out_token_stride, int64_t out_head_stride,
+               int n, int H, int D, int R, int start, int interleaved, int inverse, void* stream);
+
+/*
+ * (10) Append new tokens to the paged caches in one launch.  Token i belongs
+ * to request rows[i] at position pos[i]; its page is
+ * page_table[rows[i]*pt_stride + pos[i]/64].
+ *   latent [n, 576] (NULL: none): the first 512 values normed by (8)'s rule,
+ *     in fp64, when norm_weight [512] is given; stored at the token's KV slot
+ *     of kv_pool as 656-byte rows ((6)'s rule, but a NaN makes its group's
+ *     scale and codes NaN) or 400-byte ones (row_bytes): per 32 values, e the
+ *     smallest integer with max(amax, 1e-6) <= 6 * 2^e, scale byte e + 127,
+ *     codes e2m1_rne(x * 2^-e); a group with a NaN or an infinity gets the
+ *     byte 255.  The last 64 turned by (9)'s rule when cos_sin [table_rows, 64]
+ *     is given, rounded to bf16.
+ *   keys [n, 128] (NULL: none): the first 64 values turned, quantised into
+ *     index_k as in (6).
+ *   latent, keys and a norm_weight that is not fp32 are of one type; row
+ *   strides in elements.  A token whose request, position, page, slot or table
+ *   row is out of range is skipped.  Two tokens of a call with one slot must
+ *   hold the same values.
+ * Replaces: forward_hide_operands' key side (P:252-363, P:789) with the norm
+ * and rope before it (DL:92-143).
+ */
+int dsa_append_tokens(const int32_t* rows, const int32_t* pos, int n, const int32_t* page_table, int B, int pt_stride,
+                      const float* cos_sin, int64_t table_rows, int dtype, const void* latent, int64_t latent_stride,
+                      const void* norm_weight, int norm_weight_dtype, double eps, int interleaved, void* kv_pool,
+                      int64_t kv_rows, int row_bytes, const void* keys, int64_t keys_stride, int index_interleaved,
+                      void* index_k, int64_t num_pages, void* stream);
+
+/*
+ * (11) Latent rows as values: out [n, 576] bf16 = the 512 dequantised values
+ * and 64 rope values of KV slots slots[i], of 656- or 400-byte rows; a slot
+ * outside [0, kv_rows) gives zeros.
+ * Replaces: dequantize_k_cache (P:789).
+ */
+int dsa_read_latent_rows(const void* kv_pool, int64_t kv_rows, int row_bytes, const int32_t* slots, int n,
+                         void* out_bf16, void* stream);
+
+/*
+ * (12) (3) and (3a) over a pool of 400-byte rows.  workspace:
+ * dsa_mla_fp4_workspace_bytes(B, H, nsplit) bytes, no initialisation; calls
+ * that overlap in time must not share it.  A workspace large enough for both
+ * may serve (3), (3a) and these in turn: the barriers at its start are left as
+ * they are.  nsplit: the chunks of keys a row is
+ * cut into, 1 to 128 (0: what fills the device once); dense rows (up to 256)
+ * share B * nsplit chunks by their lengths, so where a row is cut, and the
+ * last bits of its output, depend on the other rows' lengths (the same call
+ * always gives the same).  No workgroup waits for another.
+ */
+size_t dsa_mla_fp4_workspace_bytes(int B, int H, int nsplit);
+int dsa_sparse_mla_decode_fp4(const void* q_bf16, const void* kv_pool, int64_t kv_rows, const int32_t* idx,
+                              void* workspace, void* out_bf16, int B, int H, int topk, int nsplit, float sm_scale,
+                              void* stream);
+int dsa_dense_mla_decode_fp4(const void* q_bf16, const void* kv_pool, int64_t kv_rows, const int32_t* page_table,
+                             int pt_stride, const int32_t* seq_lens, void* workspace, void* out_bf16, int B, int H,
+                             int nsplit, float sm_scale, void* stream);
 
 #ifdef __cplusplus
 }

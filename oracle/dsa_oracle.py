@@ -189,6 +189,85 @@ def dequant_latent_rows(rows: np.ndarray) -> np.ndarray:
     return np.concatenate([nope, rope], axis=1).astype(np.float32)
 
 
+# 4-bit latent row: 256 B of e2m1 pairs | 16 e8m0 scales | 64 bf16 rope.
+FP4_ROW_BYTES = 400
+E2M1_VALUES = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def pack_latent_rows_fp4(latent: np.ndarray, rope: np.ndarray) -> np.ndarray:
+    """[n,512] f32 latent + [n,64] rope -> [n,400] bytes.  Per 32 values: the
+    smallest power of two s with max(amax, 1e-6) <= 6 s, codes by exhaustive
+    comparison with the eight magnitudes (a tie goes to the even code); a group
+    with a NaN or an infinity has the scale byte 255."""
+    n = latent.shape[0]
+    x = np.asarray(latent, np.float32).reshape(n, 16, 32).astype(np.float64)
+    ok = np.isfinite(x).all(-1)
+    x = np.where(ok[..., None], x, 0.0)
+    top = np.maximum(np.abs(x).max(-1), np.float64(np.float32(1e-6)))
+    e = np.full(top.shape, -40)
+    while np.any(top > 6 * 2.0 ** e):
+        e = e + (top > 6 * 2.0 ** e)
+    a = np.abs(x) / 2.0 ** e[..., None]
+    d = np.abs(a[..., None] - E2M1_VALUES)
+    # ties: prefer the even code by listing even codes first
+    order = np.array([0, 2, 4, 6, 1, 3, 5, 7])
+    codes = order[np.argmin(d[..., order], axis=-1)] + 8 * np.signbit(x)
+    sign = np.signbit(np.asarray(latent, np.float32).reshape(n, 16, 32)) & ok[..., None]
+    codes = ((codes & 7) | (8 * sign)).reshape(n, 256, 2).astype(np.uint8)
+    rows = np.zeros((n, FP4_ROW_BYTES), dtype=np.uint8)
+    rows[:, :256] = codes[..., 0] | (codes[..., 1] << 4)
+    rows[:, 256:272] = np.where(ok, e + 127, 255).astype(np.uint8)
+    rows[:, 272:] = bf16_bits(bf16_rn(rope)).view(np.uint8).reshape(n, 128)
+    return rows
+
+
+def dequant_latent_rows_fp4(rows: np.ndarray) -> np.ndarray:
+    """[n,400] bytes -> [n,576] float32 (every value is a bf16; 2^128 and above
+    are infinite)."""
+    rows = np.asarray(rows, dtype=np.uint8)
+    n = rows.shape[0]
+    codes = np.stack([rows[:, :256] & 15, rows[:, :256] >> 4], axis=-1).reshape(n, 16, 32)
+    v = E2M1_VALUES[codes & 7] * np.where(codes & 8, -1.0, 1.0)
+    s = rows[:, 256:272].astype(np.int64)
+    v = np.where((s == 255)[..., None], np.nan, v * 2.0 ** (s - 127)[..., None])
+    v = np.where(np.abs(v) >= 2.0 ** 128, np.copysign(np.inf, v), v)
+    rope = bf16_from_bits(rows[:, 272:].copy().view(np.uint16))
+    return np.concatenate([v.reshape(n, LATENT_DIM), rope], axis=1).astype(np.float32)
+
+
+def rms_norm(x: np.ndarray, w: np.ndarray, eps: float, residual: np.ndarray | None = None):
+    """(y, h) in float64: h = x (+ residual), y = h / sqrt(mean(h^2) + eps) * w."""
+    h = np.asarray(x, np.float64) + (0.0 if residual is None else np.asarray(residual, np.float64))
+    return h / np.sqrt((h * h).mean(-1, keepdims=True) + eps) * np.asarray(w, np.float64), h
+
+
+def rotate(x: np.ndarray, cos: np.ndarray, sin: np.ndarray, interleaved: bool, inverse: bool = False) -> np.ndarray:
+    """Pairs of x [..., R] turned by cos, sin [..., R/2], in float64."""
+    x, cos, sin = (np.asarray(a, np.float64) for a in (x, cos, sin))
+    R = x.shape[-1]
+    ia, ib = (np.arange(0, R, 2), np.arange(1, R, 2)) if interleaved else (np.arange(R // 2), np.arange(R // 2, R))
+    s = -sin if inverse else sin
+    out = np.empty_like(x)
+    out[..., ia] = x[..., ia] * cos - x[..., ib] * s
+    out[..., ib] = x[..., ib] * cos + x[..., ia] * s
+    return out
+
+
+def mla_decode_values(q: np.ndarray, kv: np.ndarray, idx: np.ndarray, sm_scale: float) -> np.ndarray:
+    """out[b] = softmax(sm q[b] . kv[idx]) kv[idx, :512] over the idx[b] inside
+    kv [rows, 576], in float64; no valid index: 0."""
+    B, H, _ = q.shape
+    out = np.zeros((B, H, LATENT_DIM))
+    for b in range(B):
+        sel = idx[b][(idx[b] >= 0) & (idx[b] < kv.shape[0])]
+        if sel.size:
+            k = kv[sel].astype(np.float64)
+            s = q[b].astype(np.float64) @ k.T * sm_scale
+            p = np.exp(s - s.max(-1, keepdims=True))
+            out[b] = p @ k[:, :LATENT_DIM] / p.sum(-1, keepdims=True)
+    return out
+
+
 def slot_of(page_table_row: np.ndarray, g: np.ndarray) -> np.ndarray:
     """Token position -> KV slot through the page table (hp_page_to_slot, K:1142-1144)."""
     g = np.asarray(g, dtype=np.int64)

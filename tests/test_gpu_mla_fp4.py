@@ -1,0 +1,236 @@
+"""GPU: decode attention over 400-byte latent rows against float64.
+
+Bound.  The keys' values are exact.  A score is off by fp32's sums of 576
+products: under 2^-14 for these inputs (36 chained sums a lane at 2^-24 of at
+most 60); each probability then by 2^-14, by 2^-16 in its two bf16 terms and
+some fp32 roundings: 2^-12 of sum p |v| in all.  The output is rounded to bf16
+once (2^-8 of it).
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import dsa_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+SM = 576 ** -0.5
+
+
+def _pool(seed, n):
+    rng = np.random.default_rng(seed)
+    lat = rng.standard_normal((n, 512)).astype(np.float32) * np.exp(0.5 * rng.standard_normal((n, 1))).astype(np.float32)
+    return O.pack_latent_rows_fp4(lat, rng.standard_normal((n, 64)).astype(np.float32))
+
+
+def _q(seed, B, H, scale=1.0):
+    rng = np.random.default_rng(seed + 77)
+    return O.bf16_rn((rng.standard_normal((B, H, 576)) * scale).astype(np.float32))
+
+
+def _dev(a, dev, bf16=False):
+    if bf16:
+        return torch.from_numpy(O.bf16_bits(a).view(np.int16)).view(torch.bfloat16).to(dev)
+    return torch.from_numpy(np.ascontiguousarray(a)).to(dev)
+
+
+def _check(out, q, kv, idx, sm=SM):
+    ref = O.mla_decode_values(q, kv, idx, sm)
+    got = out.double().cpu().numpy()
+    for b in range(len(q)):
+        sel = idx[b][(idx[b] >= 0) & (idx[b] < len(kv))]
+        if not sel.size:
+            assert not got[b].any(), f"row {b} has no key"
+            continue
+        k = kv[sel].astype(np.float64)
+        s = q[b].astype(np.float64) @ k.T * sm
+        p = np.exp(s - s.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        bound = 2.0 ** -8 * np.abs(ref[b]) + 2.0 ** -12 * (p @ np.abs(k[:, :512]))
+        err = np.abs(got[b] - ref[b])
+        assert np.all(err <= bound), f"row {b}: {float((err / bound).max())} of the bound"
+
+
+SPARSE = [(1, 16, 1, 64, 0), (1, 16, 2048, 5000, 0), (3, 32, 777, 3000, 0), (2, 128, 130, 400, 0), (1, 16, 2048, 5000, 1),
+          (2, 48, 300, 1000, 5), (300, 16, 65, 500, 0), (1, 1024, 40, 64, 0), (5, 16, 1000, 1200, 128), (260, 16, 200, 512, 3)]
+
+
+@pytest.mark.parametrize("B,H,topk,n,nsplit", SPARSE)
+def test_sparse(dev, B, H, topk, n, nsplit):
+    from lagged_indexer_dsa_amd import ops
+
+    print(f"[fp4 sparse] {(B, H, topk, n, nsplit)}", flush=True)
+    rng = np.random.default_rng(B + topk)
+    rows = _pool(n, n)
+    q = _q(n, B, H)
+    idx = np.stack([rng.permutation(n)[:topk] if topk <= n else np.r_[rng.permutation(n), np.full(topk - n, -1)]
+                    for _ in range(B)]).astype(np.int32)
+    drop = rng.random(idx.shape)
+    idx[drop < 0.02] = -1
+    idx[(drop > 0.98)] = n + 5
+    if B > 2:
+        idx[1] = -1                                       # a row that attends nothing
+        idx[2, 1:] = -1                                   # a row of one key, first place
+        idx[2, 0] = n - 1
+    qd, pool, id_ = _dev(q, dev, True), _dev(rows, dev), _dev(idx, dev)
+    out = ops.sparse_mla_decode(qd, pool, id_, nsplit=nsplit)
+    _check(out, q, O.dequant_latent_rows_fp4(rows), idx)
+    # the same call, the same bits; with a workspace full of anything, too
+    ws = ops.sparse_mla_workspace(B, H, nsplit, dev)
+    ws.view(torch.uint8)[ops._lib.load().dsa_sparse_mla_barrier_bytes(B, H, 0):].fill_(0xFF)
+    again = ops.sparse_mla_decode(qd, pool, id_, nsplit=nsplit, workspace=ws, out=torch.full_like(out, 3.0))
+    assert torch.equal(again, out)
+
+
+DENSE = [(1, 16, [1], 0), (1, 16, [4097], 0), (3, 64, [777, 0, 5000], 0), (2, 128, [130, 2000], 0), (8, 32, [64] * 8, 0),
+         (4, 16, [0, 0, 0, 0], 0), (5, 16, [1, 63, 64, 65, 9000], 7), (1, 16, [20000], 128), (70, 16, None, 0),
+         (300, 16, None, 0), (2, 1024, [100, 257], 0), (257, 16, None, 2), (130, 32, None, 4)]
+
+
+@pytest.mark.parametrize("B,H,lens,nsplit", DENSE)
+def test_dense(dev, B, H, lens, nsplit):
+    from lagged_indexer_dsa_amd import ops
+
+    print(f"[fp4 dense] {(B, H, lens, nsplit)}", flush=True)
+    rng = np.random.default_rng(B * H)
+    lens = np.array(lens if lens is not None else rng.integers(0, 400, B), dtype=np.int32)
+    pts = max(1, int(lens.max()) // 64 + 2)
+    need = -(-lens // 64)
+    pages = int(need.sum()) + 1
+    perm = rng.permutation(pages)
+    pt = np.full((B, pts), -1, dtype=np.int32)
+    at = 0
+    for b in range(B):
+        pt[b, :need[b]] = perm[at:at + need[b]]
+        at += need[b]
+    rows = _pool(B, pages * 64)
+    q = _q(B, B, H)
+    idx = np.full((B, max(1, int(lens.max()))), -1, dtype=np.int64)
+    for b in range(B):
+        j = np.arange(lens[b])
+        idx[b, :lens[b]] = pt[b, j // 64] * 64 + j % 64
+    args = [_dev(q, dev, True), _dev(rows, dev), _dev(pt, dev), _dev(lens, dev)]
+    out = ops.dense_mla_decode(*args, nsplit=nsplit)
+    _check(out, q, O.dequant_latent_rows_fp4(rows), idx)
+    again = ops.dense_mla_decode(*args, nsplit=nsplit, workspace=ops.sparse_mla_workspace(B, H, nsplit, dev),
+                                 out=torch.full_like(out, 3.0))
+    assert torch.equal(again, out)
+    if B == 3:  # lengths past the table are cut to it; pages that are not there are not attended
+        over = _dev(np.array([pts * 64 + 999, -4, 5000], dtype=np.int32), dev)
+        cut = np.full((3, pts * 64), -1, dtype=np.int64)
+        for b, n in ((0, pts * 64), (2, 5000)):
+            j = np.arange(n)
+            cut[b, :n] = np.where(pt[b, j // 64] >= 0, pt[b, j // 64] * 64 + j % 64, -1)
+        _check(ops.dense_mla_decode(*args[:3], over), q, O.dequant_latent_rows_fp4(rows), cut)
+
+
+def test_sharp_and_growing_scores(dev):
+    """Scores whose maximum rises along the row by far more than the sums'
+    slack, and rows where one key outweighs the others."""
+    from lagged_indexer_dsa_amd import ops
+
+    print("[fp4] growing scores", flush=True)
+    n = 3000
+    rng = np.random.default_rng(4)
+    lat = rng.standard_normal((n, 512)).astype(np.float32)
+    lat *= np.linspace(0.05, 40, n, dtype=np.float32)[:, None]
+    rows = O.pack_latent_rows_fp4(lat, np.zeros((n, 64), np.float32))
+    kv = O.dequant_latent_rows_fp4(rows)
+    idx = np.stack([np.arange(n), np.arange(n)[::-1], rng.permutation(n)]).astype(np.int32)
+    q = _q(9, 3, 16, 0.3)
+    for nsplit in (1, 4, 0):
+        out = ops.sparse_mla_decode(_dev(q, dev, True), _dev(rows, dev), _dev(idx, dev), nsplit=nsplit)
+        ref = O.mla_decode_values(q, kv, idx, SM)
+        # scores to about 300: an fp32 sum's error there (2^-24 * 36 * 5000)
+        # moves a probability by 2^-6 of itself at most
+        for b in range(3):
+            s = q[b].astype(np.float64) @ kv[idx[b]].T.astype(np.float64) * SM
+            p = np.exp(s - s.max(-1, keepdims=True))
+            p /= p.sum(-1, keepdims=True)
+            bound = 2.0 ** -8 * np.abs(ref[b]) + 2.0 ** -6 * (p @ np.abs(kv[idx[b], :512].astype(np.float64)))
+            assert np.all(np.abs(out[b].double().cpu().numpy() - ref[b]) <= bound)
+
+
+def test_nan_stays_where_it_is(dev):
+    """A NaN group in a row that is not attended reaches nothing; attended, it
+    makes its dims (through the score, all of them) NaN for that request only."""
+    from lagged_indexer_dsa_amd import ops
+
+    print("[fp4] NaN", flush=True)
+    rows = _pool(1, 640)
+    rows[100, 256 + 3] = 255
+    rows[101, 272:274] = np.array([0x7f80], np.uint16).view(np.uint8)     # rope infinity
+    q = _q(1, 3, 16)
+    idx = np.stack([np.r_[np.arange(100), np.arange(102, 302)], np.r_[np.arange(200, 499), 100], np.arange(300, 600)])
+    out = ops.sparse_mla_decode(_dev(q, dev, True), _dev(rows, dev), _dev(idx.astype(np.int32), dev)).cpu()
+    kv = O.dequant_latent_rows_fp4(rows)
+    assert out[1].isnan().all() and not out[[0, 2]].isnan().any()
+    clean = kv.copy()
+    clean[100:102] = 0
+    _check(out[[0, 2]], q[[0, 2]], clean, idx[[0, 2]])
+    lens = torch.tensor([100, 0], dtype=torch.int32, device=dev)
+    pt = torch.arange(10, dtype=torch.int32, device=dev).repeat(2, 1)
+    d = ops.dense_mla_decode(_dev(q[:2], dev, True), _dev(rows, dev), pt, lens).cpu()
+    assert d.isfinite().all() and not d[1].any()
+
+
+def test_far_slots(dev):
+    from lagged_indexer_dsa_amd import ops
+
+    print("[fp4] far slots", flush=True)
+    n = ((1 << 32) // 400 + 4096) // 64 * 64
+    pool = torch.zeros(n, 400, dtype=torch.uint8, device=dev)
+    rows = _pool(6, 256)
+    pool[n - 256:] = _dev(rows, dev)
+    q = _q(6, 1, 16)
+    idx = (n - 256 + np.arange(256)).astype(np.int32)[None]
+    out = ops.sparse_mla_decode(_dev(q, dev, True), pool, _dev(idx, dev))
+    _check(out, q, O.dequant_latent_rows_fp4(rows), np.arange(256)[None])
+    pt = _dev((n // 64 - 4 + np.arange(4)).astype(np.int32)[None], dev)
+    out = ops.dense_mla_decode(_dev(q, dev, True), pool, pt, torch.tensor([256], dtype=torch.int32, device=dev))
+    _check(out, q, O.dequant_latent_rows_fp4(rows), np.arange(256)[None])
+
+
+def test_one_workspace_for_both_formats(dev):
+    """Calls over 8- and 4-bit rows take turns with a workspace."""
+    from lagged_indexer_dsa_amd import _lib, formats as F, ops
+
+    print("[fp4] shared workspace", flush=True)
+    g = torch.Generator(device=dev).manual_seed(2)
+    lat, rope = torch.randn(4096, 512, device=dev, generator=g), torch.randn(4096, 64, device=dev, generator=g)
+    p8, p4 = F.pack_latent_rows(lat, rope), F.pack_latent_rows_fp4(lat, rope)
+    q = torch.randn(2, 16, 576, device=dev, generator=g).to(torch.bfloat16)
+    idx = torch.stack([torch.randperm(4096, generator=g, device=dev)[:2048] for _ in range(2)]).int()
+    ref8, ref4 = ops.sparse_mla_decode(q, p8, idx), ops.sparse_mla_decode(q, p4, idx)
+    assert float((ref8.float() - ref4.float()).norm() / ref8.float().norm()) < 0.5   # the same rows, coarser
+    ws = ops.sparse_mla_workspace(2, 16, 0, dev)
+    _lib.sync_timeouts(reset=True)
+    for _ in range(3):
+        assert torch.equal(ops.sparse_mla_decode(q, p4, idx, workspace=ws), ref4)
+        got8 = ops.sparse_mla_decode(q, p8, idx, workspace=ws)
+        assert float((got8.float() - ref8.float()).abs().max()) <= 2.0 ** -6 * float(ref8.float().abs().max())
+    assert _lib.sync_timeouts() == 0
+
+
+def test_refusals(dev):
+    from lagged_indexer_dsa_amd import ops
+
+    print("[fp4] refusals", flush=True)
+    q = torch.zeros(2, 16, 576, dtype=torch.bfloat16, device=dev)
+    pool = torch.zeros(128, 400, dtype=torch.uint8, device=dev)
+    idx = torch.zeros(2, 64, dtype=torch.int32, device=dev)
+    pt, lens = idx[:, :2].contiguous(), idx[:, 0].contiguous()
+    s, d = ops.sparse_mla_decode, ops.dense_mla_decode
+    for f in (lambda: s(q.float(), pool, idx), lambda: s(q[..., :512].contiguous(), pool, idx),
+              lambda: s(q, pool.view(torch.int8), idx), lambda: s(q, pool, idx.long()), lambda: s(q, pool, idx[:1]),
+              lambda: s(q[:, :8].contiguous(), pool, idx), lambda: s(q, pool, idx, nsplit=129),
+              lambda: s(q, pool, idx, nsplit=16, workspace=torch.zeros(64, device=dev)),
+              lambda: s(q, pool, idx, out=torch.zeros(2, 16, 512, device=dev)), lambda: s(q, pool[:0], idx),
+              lambda: s(q, pool, idx[:, :0].contiguous()), lambda: s(q, pool, idx[:, ::2]),
+              lambda: d(q, pool, pt.long(), lens), lambda: d(q, pool, pt, lens[:1]), lambda: d(q, pool, pt[:1], lens),
+              lambda: d(q, pool, pt, lens.long()), lambda: d(q, pool, pt[:, :0].contiguous(), lens)):
+        with pytest.raises(RuntimeError):
+            f()

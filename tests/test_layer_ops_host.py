@@ -1,0 +1,231 @@
+"""CPU: contracts of the operators around the cached attention (no launch):
+rope tables against their formulas, the 4-bit row format's builder against the
+oracle's exhaustive one, refusals of CPU tensors, and the C ABI's argument
+checks, which answer before anything is launched."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import dsa_oracle as O
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from lagged_indexer_dsa_amd import _lib
+
+    if not _lib.LIB_PATH.exists():
+        pytest.skip("library not built (run __graft_entry__.build())")
+    return _lib.load()
+
+
+# ---- rope tables ----
+
+def test_plain_table_is_the_formula():
+    from lagged_indexer_dsa_amd.rope import build_rope_table
+
+    t = build_rope_table(70001, 64).double().numpy()
+    p, i = np.arange(70001)[:, None], np.arange(32)[None, :]
+    a = p * 10000.0 ** (-2 * i / 64)
+    # one rounding to fp32 of values at most 1; the angle's float64 error is
+    # under 70000 * 2^-52, below a tenth of an fp32 half step
+    assert np.abs(t[:, :32] - np.cos(a)).max() <= 2.0 ** -24
+    assert np.abs(t[:, 32:] - np.sin(a)).max() <= 2.0 ** -24
+
+
+def test_scaled_frequencies():
+    from lagged_indexer_dsa_amd.rope import RopeScaling, build_rope_table, rope_frequencies
+
+    f = rope_frequencies(64, 10000.0)
+    lin = rope_frequencies(64, 10000.0, RopeScaling("linear", 8.0))
+    assert torch.allclose(lin * 8, f, rtol=1e-15)
+    ntk = rope_frequencies(64, 10000.0, RopeScaling("ntk", 8.0))
+    assert ntk[0] == f[0] and math.isclose(float(ntk[-1]), float(f[-1]) / 8, rel_tol=1e-12)
+    yarn = rope_frequencies(64, 10000.0, RopeScaling("yarn", 40.0))
+    turns = 4096 * f / (2 * math.pi)
+    assert torch.equal(yarn[turns > 40], f[turns > 40])                # fast pairs stay
+    slow = turns < 0.7
+    assert torch.allclose(yarn[slow], f[slow] / 40, rtol=1e-15)        # slow ones are stretched
+    assert bool(((yarn <= f) & (yarn >= f / 40 * (1 - 1e-12))).all()) and bool((yarn[:-1] > yarn[1:]).all())
+    t = build_rope_table(4, 64, scaling=RopeScaling("yarn", 40.0))
+    assert math.isclose(float(t[0, 0]), 0.1 * math.log(40.0) + 1, rel_tol=1e-7)
+    t = build_rope_table(4, 64, scaling=RopeScaling("yarn", 40.0, mscale_all_dim=1.0))
+    assert float(t[0, 0]) == 1.0
+
+
+def test_rope_refusals():
+    from lagged_indexer_dsa_amd.rope import RopeScaling, build_rope_table
+
+    for kw in (dict(max_pos=0), dict(max_pos=4, dim=63), dict(max_pos=4, dim=0), dict(max_pos=4, theta=1.0),
+               dict(max_pos=4, dim=2, scaling=RopeScaling("ntk", 2.0))):
+        with pytest.raises(ValueError):
+            build_rope_table(**kw)
+    for a in (("cubic", 2.0), ("linear", 0.5), ("linear", float("nan")), ("yarn", float("inf"))):
+        with pytest.raises(ValueError):
+            RopeScaling(*a)
+    with pytest.raises(ValueError):
+        RopeScaling("yarn", 2.0, beta_fast=1.0, beta_slow=2.0)
+
+
+# ---- the 4-bit row ----
+
+def fp4_edge_rows() -> np.ndarray:
+    """Rows of 512 whose groups hold every code, every midpoint and its
+    neighbours, at several scales; zero, tiny, huge and non-finite groups."""
+    mags = np.array([0, .25, .5, .75, 1, 1.25, 1.5, 1.75, 2, 2.5, 3, 3.5, 4, 5, 6], np.float32)
+    near = np.concatenate([mags, np.nextafter(mags, np.float32(9)), np.nextafter(mags, np.float32(-9))])
+    vals = np.concatenate([near, -near]).astype(np.float32)
+    groups = []
+    for k in (-20, -3, 0, 1, 90, 120):
+        for i in range(0, len(vals), 31):
+            part = vals[i:i + 31]
+            part = part[np.abs(part) <= 6]
+            g = np.zeros(32, np.float32)
+            g[:len(part)], g[31] = part, 6.0
+            groups.append(g * np.float32(2.0 ** k))
+    groups.append(np.zeros(32, np.float32))
+    groups.append(np.full(32, 1e-9, np.float32))
+    groups.append(np.full(32, -1e-40, np.float32))
+    groups.append(np.linspace(-3e38, 3.4e38, 32, dtype=np.float32))
+    for bad in (np.nan, np.inf, -np.inf):
+        g = np.linspace(-2, 2, 32, dtype=np.float32)
+        g[7] = bad
+        groups.append(g)
+    for top in (6.0, np.nextafter(np.float32(6), np.float32(7)), 3.0, 7.9, 8.0, 1e-6, 1.2e-6):
+        g = np.linspace(-1, 1, 32, dtype=np.float32) * np.float32(top)
+        groups.append(g)
+    while len(groups) % 16:
+        groups.append(np.zeros(32, np.float32))
+    return np.stack(groups).reshape(-1, 512)
+
+
+def test_fp4_builder_equals_oracle():
+    from lagged_indexer_dsa_amd import formats as F
+
+    rng = np.random.default_rng(3)
+    lat = np.concatenate([fp4_edge_rows(), rng.standard_normal((40, 512)).astype(np.float32) * 7])
+    rope = rng.standard_normal((len(lat), 64)).astype(np.float32)
+    ref = O.pack_latent_rows_fp4(lat, rope)
+    got = F.pack_latent_rows_fp4(torch.from_numpy(lat), torch.from_numpy(rope)).numpy()
+    finite = np.isfinite(lat).reshape(len(lat), 16, 32).all(-1)
+    assert np.array_equal(got[:, 256:], ref[:, 256:])
+    codes = np.repeat(finite, 16, axis=1)                      # the codes of a NaN group mean nothing
+    assert np.array_equal(got[:, :256][codes], ref[:, :256][codes])
+    # what they read back as: within half a code step of the value, none saturated
+    # (3.4e38 lies nearest to 4 * 2^126 = 2^128, which bf16 holds as infinity)
+    back = O.dequant_latent_rows_fp4(ref)[:, :512].reshape(-1, 32)
+    x, ok = lat.reshape(-1, 32).astype(np.float64), finite.reshape(-1)
+    s = 2.0 ** (ref[:, 256:272].reshape(-1).astype(np.float64) - 127)[:, None]
+    half = np.where(np.abs(x) < 2 * s, 0.25, np.where(np.abs(x) < 4 * s, 0.5, 1.0)) * s
+    over = np.abs(x) >= 3.5 * 2.0 ** 126
+    assert (over & ok[:, None]).any() and np.isinf(back[over & ok[:, None]]).all()
+    assert np.all((np.abs(back - x) <= half)[ok & ~over.any(1)]) and np.all((np.abs(back - x) <= half)[~over & ok[:, None]])
+    assert np.isnan(back[~ok]).all() and (~ok).sum() == 3
+
+
+def test_new_latent_pool_formats():
+    from lagged_indexer_dsa_amd import formats as F
+
+    assert F.new_latent_pool(2, "cpu").shape == (128, 656)
+    assert F.new_latent_pool(2, "cpu", bits=4).shape == (128, 400)
+    with pytest.raises(ValueError):
+        F.new_latent_pool(2, "cpu", bits=6)
+
+
+# ---- refusals ----
+
+def test_ops_refuse_cpu_tensors():
+    from lagged_indexer_dsa_amd import ops
+
+    x, w = torch.zeros(2, 64), torch.ones(64)
+    i = torch.zeros(2, dtype=torch.int32)
+    for call in (lambda: ops.rms_norm(x, w), lambda: ops.rms_norm_quant(x, w), lambda: ops.rotary(x, i, torch.zeros(4, 64)),
+                 lambda: ops.append_tokens(i[None], i, i, index_k=torch.zeros(1, 8448, dtype=torch.uint8),
+                                           keys=torch.zeros(2, 128)),
+                 lambda: ops.read_latent_rows(torch.zeros(4, 400, dtype=torch.uint8), i),
+                 lambda: ops.sparse_mla_decode(torch.zeros(1, 16, 576, dtype=torch.bfloat16),
+                                               torch.zeros(4, 400, dtype=torch.uint8), i[None])):
+        with pytest.raises(RuntimeError, match="no CPU path"):
+            call()
+
+
+def test_decode_layer_refuses_4bit_pool():
+    from lagged_indexer_dsa_amd.decode import DecodeLayer
+
+    with pytest.raises(RuntimeError, match="656"):
+        DecodeLayer(q_fp8=None, w=None, index_k=None, q_bf16=torch.zeros(1, 16, 576, dtype=torch.bfloat16),
+                    kv_pool=torch.zeros(64, 400, dtype=torch.uint8), page_table=torch.zeros(1, 1, dtype=torch.int32),
+                    seq_lens=torch.zeros(1, dtype=torch.int32), slab_stride=64)
+
+
+def test_norm_contract(lib):
+    from lagged_indexer_dsa_amd._lib import DSA_ERR_INVALID_ARG, DSA_ERR_UNSUPPORTED, DSA_OK
+
+    def call(x=16, dt=1, xs=64, r=None, rs=0, w=16, wd=1, y=16, c=None, s=None, g=0, h=None, hs=0, n=2, D=64):
+        return lib.dsa_rms_norm(x, dt, xs, r, rs, w, wd, 1e-6, y, c, s, g, h, hs, n, D, None)
+    assert call(n=0, x=None) == DSA_OK
+    for kw in (dict(n=-1), dict(x=None), dict(w=None), dict(y=None), dict(c=16), dict(y=None, c=16), dict(dt=3),
+               dict(wd=2), dict(h=16), dict(r=16, rs=64, h=16, hs=63), dict(xs=-64)):
+        assert call(**kw) == DSA_ERR_INVALID_ARG, kw
+    for kw in (dict(D=0), dict(D=32769), dict(y=None, c=16, s=16, g=64)):
+        assert call(**kw) == DSA_ERR_UNSUPPORTED, kw
+    assert b"dsa_rms_norm" in lib.dsa_last_error()
+
+
+def test_rotary_contract(lib):
+    from lagged_indexer_dsa_amd._lib import DSA_ERR_INVALID_ARG, DSA_ERR_UNSUPPORTED, DSA_OK
+
+    def call(x=16, dt=1, pos=16, pb=4, t=16, P=8, o=16, n=2, H=2, D=64, R=64, start=0):
+        return lib.dsa_rotary(x, dt, H * D, D, pos, pb, t, P, o, H * D, D, n, H, D, R, start, 0, 0, None)
+    assert call(n=0, x=None) == DSA_OK
+    for kw in (dict(n=-1), dict(x=None), dict(pos=None), dict(t=None), dict(o=None), dict(dt=5), dict(pb=2), dict(P=0),
+               dict(R=0), dict(R=63), dict(R=66), dict(start=2), dict(start=-2, R=32), dict(D=65538)):
+        assert call(**kw) == DSA_ERR_INVALID_ARG, kw
+    assert call(H=1 << 26) == DSA_ERR_UNSUPPORTED
+    assert b"dsa_rotary" in lib.dsa_last_error()
+
+
+def test_append_and_read_contract(lib):
+    from lagged_indexer_dsa_amd._lib import DSA_ERR_INVALID_ARG, DSA_ERR_UNSUPPORTED, DSA_OK
+
+    def call(rows=16, pos=16, n=2, pt=16, B=1, pts=4, cs=16, cr=8, dt=1, lat=16, ls=576, w=None, wd=0, pool=16, kv=64,
+             rb=656, k=16, ks=128, idx=16, pages=1):
+        return lib.dsa_append_tokens(rows, pos, n, pt, B, pts, cs, cr, dt, lat, ls, w, wd, 1e-6, 0, pool, kv, rb, k, ks, 0,
+                                     idx, pages, None)
+    assert call(n=0, rows=None) == DSA_OK
+    for kw in (dict(n=-1), dict(rows=None), dict(pos=None), dict(pt=None), dict(lat=None, k=None), dict(B=0), dict(pts=0),
+               dict(cr=0), dict(dt=3), dict(w=16, wd=2), dict(pool=None), dict(kv=0), dict(pool=24), dict(idx=None),
+               dict(pages=0), dict(idx=24), dict(ls=-1)):
+        assert call(**kw) == DSA_ERR_INVALID_ARG, kw
+    assert call(rb=512) == DSA_ERR_UNSUPPORTED
+    r = lib.dsa_read_latent_rows
+    assert r(None, 4, 656, None, 0, None, None) == DSA_OK
+    assert r(16, 4, 656, 16, -1, 16, None) == DSA_ERR_INVALID_ARG
+    assert r(16, 0, 656, 16, 2, 16, None) == DSA_ERR_INVALID_ARG
+    assert r(16, 4, 656, None, 2, 16, None) == DSA_ERR_INVALID_ARG
+    assert r(24, 4, 656, 16, 2, 16, None) == DSA_ERR_INVALID_ARG
+    assert r(16, 4, 600, 16, 2, 16, None) == DSA_ERR_UNSUPPORTED
+
+
+def test_fp4_mla_contract(lib):
+    from lagged_indexer_dsa_amd._lib import DSA_ERR_INVALID_ARG, DSA_ERR_UNSUPPORTED
+
+    f, d, ws = lib.dsa_sparse_mla_decode_fp4, lib.dsa_dense_mla_decode_fp4, lib.dsa_mla_fp4_workspace_bytes
+    assert f(16, 16, 10, 16, 16, 16, 1, 24, 2048, 0, 0.04, None) == DSA_ERR_UNSUPPORTED
+    assert f(16, 16, 10, 16, 16, 16, 1, 16, 2048, 129, 0.04, None) == DSA_ERR_UNSUPPORTED
+    assert f(16, 16, 10, None, 16, 16, 1, 16, 2048, 0, 0.04, None) == DSA_ERR_INVALID_ARG
+    assert f(16, 16, 0, 16, 16, 16, 1, 16, 2048, 0, 0.04, None) == DSA_ERR_INVALID_ARG
+    assert f(16, 24, 10, 16, 16, 16, 1, 16, 2048, 0, 0.04, None) == DSA_ERR_INVALID_ARG
+    assert d(16, 16, 10, None, 4, 16, 16, 16, 1, 16, 0, 0.04, None) == DSA_ERR_INVALID_ARG
+    assert d(16, 16, 10, 16, 0, 16, 16, 16, 1, 16, 0, 0.04, None) == DSA_ERR_INVALID_ARG
+    assert d(16, 16, 10, 16, (1 << 24) + 1, 16, 16, 16, 1, 16, 0, 0.04, None) == DSA_ERR_UNSUPPORTED
+    assert d(16, 16, 10, 16, 4, 16, None, 16, 1, 16, 0, 0.04, None) == DSA_ERR_INVALID_ARG
+    assert ws(1, 15, 8) == 0 and ws(0, 16, 8) == 0 and ws(1, 16, 129) == 0
+    barriers = 25 * 64 * 4
+    assert ws(1, 16, 8) == barriers + 8 * 16 * 514 * 4
+    assert ws(3, 32, 8) == 3 * 2 * barriers + 24 * 32 * 514 * 4
+    assert ws(2, 16, 128) >= ws(2, 16, 64) and ws(7, 16, 1) == 16
