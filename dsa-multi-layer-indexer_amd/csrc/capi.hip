@@ -729,80 +729,80 @@ int dsa_append_latent_rows(const void* latent_bf16, const int32_t* slots, int n,
 }
 
 
-int dsa_rms_norm(const void* x, int dtype, int64_t x_stride, const void* residual, int64_t residual_stride,
-                 const void* weight, int weight_dtype, double eps, void* y, void* codes, float* scales, int group,
-                 void* residual_out, int64_t residual_out_stride, int n, int D, void* stream) {
-  DSA_REQUIRE(n >= 0, DSA_ERR_INVALID_ARG, "dsa_rms_norm: n must be >= 0 (got %d)", n);
-  if (n == 0) return DSA_OK;
-  DSA_REQUIRE(x && weight && ((y != nullptr) != (codes != nullptr)) && (!codes || scales), DSA_ERR_INVALID_ARG,
-              "dsa_rms_norm: x, weight and one of y and codes with scales are required");
-  DSA_REQUIRE(!residual_out || residual, DSA_ERR_INVALID_ARG, "dsa_rms_norm: residual_out without a residual");
-  DSA_REQUIRE(dtype >= 0 && dtype <= 2, DSA_ERR_INVALID_ARG, "dsa_rms_norm: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
-  DSA_REQUIRE(weight_dtype == dtype || weight_dtype == 0, DSA_ERR_INVALID_ARG,
+int dsa_rms_norm(const dsa_norm_args* a, void* stream) {
+  DSA_REQUIRE(a && a->n >= 0, DSA_ERR_INVALID_ARG, "dsa_rms_norm: args with n >= 0 are required");
+  if (a->n == 0) return DSA_OK;
+  DSA_REQUIRE(a->x && a->weight && ((a->y != nullptr) != (a->codes != nullptr)) && (!a->codes || a->scales),
+              DSA_ERR_INVALID_ARG, "dsa_rms_norm: x, weight and one of y and codes with scales are required");
+  DSA_REQUIRE(!a->residual_out || a->residual, DSA_ERR_INVALID_ARG, "dsa_rms_norm: residual_out without a residual");
+  DSA_REQUIRE(a->dtype >= 0 && a->dtype <= 2, DSA_ERR_INVALID_ARG,
+              "dsa_rms_norm: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+  DSA_REQUIRE(a->weight_dtype == a->dtype || a->weight_dtype == 0, DSA_ERR_INVALID_ARG,
               "dsa_rms_norm: the weight must be fp32 or of x's type");
-  DSA_REQUIRE(D >= 1 && D <= DSA_NORM_MAX_DIM, DSA_ERR_UNSUPPORTED, "dsa_rms_norm: D must be in [1, %d] (got %d)",
-              DSA_NORM_MAX_DIM, D);
-  DSA_REQUIRE(group == 0 || group == 128, DSA_ERR_UNSUPPORTED, "dsa_rms_norm: group must be 128 or 0 (got %d)", group);
-  DSA_REQUIRE(x_stride >= 0 && residual_stride >= 0 && (!residual_out || n == 1 || residual_out_stride >= D),
+  DSA_REQUIRE(a->D >= 1 && a->D <= DSA_NORM_MAX_DIM, DSA_ERR_UNSUPPORTED, "dsa_rms_norm: D must be in [1, %d] (got %d)",
+              DSA_NORM_MAX_DIM, a->D);
+  DSA_REQUIRE(a->group == 0 || a->group == 128, DSA_ERR_UNSUPPORTED, "dsa_rms_norm: group must be 128 or 0 (got %d)",
+              a->group);
+  DSA_REQUIRE(a->x_stride >= 0 && a->residual_stride >= 0 &&
+                  (!a->residual_out || a->n == 1 || a->residual_out_stride >= a->D),
               DSA_ERR_INVALID_ARG, "dsa_rms_norm: bad row stride");
   dsa::NormArgs A{};
-  A.x = x, A.r = residual, A.w = weight, A.y = y, A.codes = static_cast<uint8_t*>(codes), A.scales = scales;
-  A.h = residual_out, A.xs = (long)x_stride, A.rs = (long)residual_stride, A.hs = (long)residual_out_stride;
-  A.n = n, A.D = D, A.group = group, A.w_f32 = weight_dtype == 0, A.eps = (float)eps;
-  return hip_status(dsa::launch_rms_norm(A, dtype, (hipStream_t)stream), "rms norm");
+  A.x = a->x, A.r = a->residual, A.w = a->weight, A.y = a->y, A.codes = static_cast<uint8_t*>(a->codes);
+  A.scales = a->scales, A.h = a->residual_out;
+  A.xs = (long)a->x_stride, A.rs = (long)a->residual_stride, A.hs = (long)a->residual_out_stride;
+  A.n = a->n, A.D = a->D, A.group = a->group, A.w_f32 = a->weight_dtype == 0, A.eps = (float)a->eps;
+  return hip_status(dsa::launch_rms_norm(A, a->dtype, (hipStream_t)stream), "rms norm");
 }
 
-int dsa_rotary(const void* x, int dtype, int64_t x_token_stride, int64_t x_head_stride, const void* pos, int pos_bytes,
-               const float* cos_sin, int64_t max_pos, void* out, int64_t out_token_stride, int64_t out_head_stride,
-               int n, int H, int D, int R, int start, int interleaved, int inverse, void* stream) {
-  DSA_REQUIRE(n >= 0 && H >= 0, DSA_ERR_INVALID_ARG, "dsa_rotary: n and H must be >= 0 (got %d, %d)", n, H);
-  if (n == 0 || H == 0) return DSA_OK;
-  DSA_REQUIRE(x && pos && cos_sin && out, DSA_ERR_INVALID_ARG, "dsa_rotary: null pointer");
-  DSA_REQUIRE(dtype >= 0 && dtype <= 2, DSA_ERR_INVALID_ARG, "dsa_rotary: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
-  DSA_REQUIRE(pos_bytes == 4 || pos_bytes == 8, DSA_ERR_INVALID_ARG, "dsa_rotary: pos_bytes must be 4 or 8");
-  DSA_REQUIRE(R >= 2 && R % 2 == 0 && start >= 0 && D <= 65536 && start + R <= D, DSA_ERR_INVALID_ARG,
-              "dsa_rotary: %d values from %d on of a head of %d", R, start, D);
-  DSA_REQUIRE((int64_t)H * D < ((int64_t)1 << 31), DSA_ERR_UNSUPPORTED, "dsa_rotary: H * D must be < 2^31");
-  DSA_REQUIRE(max_pos >= 1, DSA_ERR_INVALID_ARG, "dsa_rotary: max_pos must be >= 1");
+int dsa_rotary(const dsa_rotary_args* a, void* stream) {
+  DSA_REQUIRE(a && a->n >= 0 && a->H >= 0, DSA_ERR_INVALID_ARG, "dsa_rotary: args with n and H >= 0 are required");
+  if (a->n == 0 || a->H == 0) return DSA_OK;
+  DSA_REQUIRE(a->x && a->pos && a->cos_sin && a->out, DSA_ERR_INVALID_ARG, "dsa_rotary: null pointer");
+  DSA_REQUIRE(a->dtype >= 0 && a->dtype <= 2, DSA_ERR_INVALID_ARG,
+              "dsa_rotary: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+  DSA_REQUIRE(a->pos_bytes == 4 || a->pos_bytes == 8, DSA_ERR_INVALID_ARG, "dsa_rotary: pos_bytes must be 4 or 8");
+  DSA_REQUIRE(a->R >= 2 && a->R % 2 == 0 && a->start >= 0 && a->D <= 65536 && a->start + a->R <= a->D,
+              DSA_ERR_INVALID_ARG, "dsa_rotary: %d values from %d on of a head of %d", a->R, a->start, a->D);
+  DSA_REQUIRE((int64_t)a->H * a->D < ((int64_t)1 << 31), DSA_ERR_UNSUPPORTED, "dsa_rotary: H * D must be < 2^31");
+  DSA_REQUIRE(a->max_pos >= 1, DSA_ERR_INVALID_ARG, "dsa_rotary: max_pos must be >= 1");
   dsa::RopeArgs A{};
-  A.x = x, A.out = out, A.pos = pos, A.table = cos_sin, A.max_pos = (long)max_pos;
-  A.xn = (long)x_token_stride, A.xh = (long)x_head_stride, A.on = (long)out_token_stride, A.oh = (long)out_head_stride;
-  A.n = n, A.H = H, A.D = D, A.R = R, A.start = start, A.pos64 = pos_bytes == 8;
-  A.interleaved = interleaved != 0, A.inverse = inverse != 0, A.copy = out != x;
-  return hip_status(dsa::launch_rotary(A, dtype, (hipStream_t)stream), "rotary");
+  A.x = a->x, A.out = a->out, A.pos = a->pos, A.table = a->cos_sin, A.max_pos = (long)a->max_pos;
+  A.xn = (long)a->x_token_stride, A.xh = (long)a->x_head_stride;
+  A.on = (long)a->out_token_stride, A.oh = (long)a->out_head_stride;
+  A.n = a->n, A.H = a->H, A.D = a->D, A.R = a->R, A.start = a->start, A.pos64 = a->pos_bytes == 8;
+  A.interleaved = a->interleaved != 0, A.inverse = a->inverse != 0, A.copy = a->out != a->x;
+  return hip_status(dsa::launch_rotary(A, a->dtype, (hipStream_t)stream), "rotary");
 }
 
-int dsa_append_tokens(const int32_t* rows, const int32_t* pos, int n, const int32_t* page_table, int B, int pt_stride,
-                      const float* cos_sin, int64_t table_rows, int dtype, const void* latent, int64_t latent_stride,
-                      const void* norm_weight, int norm_weight_dtype, double eps, int interleaved, void* kv_pool,
-                      int64_t kv_rows, int row_bytes, const void* keys, int64_t keys_stride, int index_interleaved,
-                      void* index_k, int64_t num_pages, void* stream) {
-  DSA_REQUIRE(n >= 0, DSA_ERR_INVALID_ARG, "dsa_append_tokens: n must be >= 0 (got %d)", n);
-  if (n == 0) return DSA_OK;
-  DSA_REQUIRE(rows && pos && page_table && (latent || keys), DSA_ERR_INVALID_ARG,
+int dsa_append_tokens(const dsa_append_args* a, void* stream) {
+  DSA_REQUIRE(a && a->n >= 0, DSA_ERR_INVALID_ARG, "dsa_append_tokens: args with n >= 0 are required");
+  if (a->n == 0) return DSA_OK;
+  DSA_REQUIRE(a->rows && a->pos && a->page_table && (a->latent || a->keys), DSA_ERR_INVALID_ARG,
               "dsa_append_tokens: rows, pos, page_table and a latent or keys are required");
-  DSA_REQUIRE(B >= 1 && pt_stride >= 1, DSA_ERR_INVALID_ARG, "dsa_append_tokens: B and pt_stride must be >= 1");
-  DSA_REQUIRE(!cos_sin || table_rows >= 1, DSA_ERR_INVALID_ARG, "dsa_append_tokens: table_rows must be >= 1");
-  DSA_REQUIRE(dtype >= 0 && dtype <= 2, DSA_ERR_INVALID_ARG,
+  DSA_REQUIRE(a->B >= 1 && a->pt_stride >= 1, DSA_ERR_INVALID_ARG, "dsa_append_tokens: B and pt_stride must be >= 1");
+  DSA_REQUIRE(!a->cos_sin || a->table_rows >= 1, DSA_ERR_INVALID_ARG, "dsa_append_tokens: table_rows must be >= 1");
+  DSA_REQUIRE(a->dtype >= 0 && a->dtype <= 2, DSA_ERR_INVALID_ARG,
               "dsa_append_tokens: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
-  DSA_REQUIRE(!norm_weight || norm_weight_dtype == dtype || norm_weight_dtype == 0, DSA_ERR_INVALID_ARG,
+  DSA_REQUIRE(!a->norm_weight || a->norm_weight_dtype == a->dtype || a->norm_weight_dtype == 0, DSA_ERR_INVALID_ARG,
               "dsa_append_tokens: the norm weight must be fp32 or of the latent's type");
-  DSA_REQUIRE(!latent || (kv_pool && kv_rows >= 1 && aligned16(kv_pool)), DSA_ERR_INVALID_ARG,
+  DSA_REQUIRE(!a->latent || (a->kv_pool && a->kv_rows >= 1 && aligned16(a->kv_pool)), DSA_ERR_INVALID_ARG,
               "dsa_append_tokens: a latent needs a 16-byte aligned kv_pool of kv_rows >= 1 rows");
-  DSA_REQUIRE(!latent || row_bytes == DSA_LATENT_ROW_BYTES || row_bytes == DSA_FP4_ROW_BYTES, DSA_ERR_UNSUPPORTED,
-              "dsa_append_tokens: row_bytes must be %d or %d (got %d)", DSA_LATENT_ROW_BYTES, DSA_FP4_ROW_BYTES,
-              row_bytes);
-  DSA_REQUIRE(!keys || (index_k && num_pages >= 1 && aligned16(index_k)), DSA_ERR_INVALID_ARG,
+  DSA_REQUIRE(!a->latent || a->row_bytes == DSA_LATENT_ROW_BYTES || a->row_bytes == DSA_FP4_ROW_BYTES,
+              DSA_ERR_UNSUPPORTED, "dsa_append_tokens: row_bytes must be %d or %d (got %d)", DSA_LATENT_ROW_BYTES,
+              DSA_FP4_ROW_BYTES, a->row_bytes);
+  DSA_REQUIRE(!a->keys || (a->index_k && a->num_pages >= 1 && aligned16(a->index_k)), DSA_ERR_INVALID_ARG,
               "dsa_append_tokens: keys need a 16-byte aligned index_k of num_pages >= 1 pages");
-  DSA_REQUIRE(latent_stride >= 0 && keys_stride >= 0, DSA_ERR_INVALID_ARG, "dsa_append_tokens: bad row stride");
+  DSA_REQUIRE(a->latent_stride >= 0 && a->keys_stride >= 0, DSA_ERR_INVALID_ARG, "dsa_append_tokens: bad row stride");
   dsa::AppendArgs A{};
-  A.rows = rows, A.pos = pos, A.page_table = page_table, A.table = cos_sin, A.table_rows = (long)table_rows;
-  A.latent = latent, A.latent_stride = (long)latent_stride, A.norm_w = norm_weight, A.norm_w_f32 = norm_weight_dtype == 0;
-  A.eps = eps, A.interleaved = interleaved != 0, A.pool = static_cast<uint8_t*>(kv_pool), A.kv_rows = (long)kv_rows;
-  A.keys = keys, A.keys_stride = (long)keys_stride, A.index_interleaved = index_interleaved != 0;
-  A.index_k = static_cast<uint8_t*>(index_k), A.num_pages = (long)num_pages;
-  A.n = n, A.B = B, A.pt_stride = pt_stride;
-  return hip_status(dsa::launch_append_tokens(A, dtype, latent ? row_bytes : DSA_LATENT_ROW_BYTES, (hipStream_t)stream),
+  A.rows = a->rows, A.pos = a->pos, A.page_table = a->page_table, A.table = a->cos_sin, A.table_rows = (long)a->table_rows;
+  A.latent = a->latent, A.latent_stride = (long)a->latent_stride;
+  A.norm_w = a->norm_weight, A.norm_w_f32 = a->norm_weight_dtype == 0, A.eps = a->eps;
+  A.interleaved = a->interleaved != 0, A.pool = static_cast<uint8_t*>(a->kv_pool), A.kv_rows = (long)a->kv_rows;
+  A.keys = a->keys, A.keys_stride = (long)a->keys_stride, A.index_interleaved = a->index_interleaved != 0;
+  A.index_k = static_cast<uint8_t*>(a->index_k), A.num_pages = (long)a->num_pages;
+  A.n = a->n, A.B = a->B, A.pt_stride = a->pt_stride;
+  return hip_status(dsa::launch_append_tokens(A, a->dtype, a->latent ? a->row_bytes : DSA_LATENT_ROW_BYTES,
+                                              (hipStream_t)stream),
                     "append tokens");
 }
 

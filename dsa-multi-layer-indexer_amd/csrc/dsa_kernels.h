@@ -158,6 +158,7 @@ struct RopeArgs {
   int n, H, D, R, start, pos64, inverse, interleaved;
   int copy;           // out is not x: the other elements too
   long max_pos;
+  int heads, tokens;  // filled by the launcher: of each, those of a workgroup
 };
 hipError_t launch_rms_norm(const NormArgs& A, int dtype, hipStream_t s);
 hipError_t launch_rotary(const RopeArgs& A, int dtype, hipStream_t s);

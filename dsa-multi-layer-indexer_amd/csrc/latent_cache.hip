@@ -42,24 +42,54 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
+// Where a token goes.  slot < 0: nowhere (no request, page, row or table row).
+struct Place {
+  int pos;
+  long page, slot;
+};
+__device__ __forceinline__ Place place_of(const AppendArgs& A, int t) {
+  Place p{A.pos[t], -1, -1};
+  const int r = A.rows[t];
+  if (r < 0 || r >= A.B || p.pos < 0 || p.pos / DSA_PAGE_TOKENS >= A.pt_stride || (A.table && p.pos >= A.table_rows))
+    return p;
+  p.page = A.page_table[(long)r * A.pt_stride + p.pos / DSA_PAGE_TOKENS];
+  p.slot = p.page < 0 ? -1 : p.page * DSA_PAGE_TOKENS + p.pos % DSA_PAGE_TOKENS;
+  return p;
+}
+
+// A wave's latent row: 8 values of the latent part a lane, a pair of the
+// rope part for lanes 0-31.  All inputs are on their way before the place is
+// known.
 template <int DT, bool WIDE, int BYTES>
-__device__ __forceinline__ void append_latent_row(const AppendArgs& A, int t, int pos, long slot) {
-  const int lane = threadIdx.x & (kWave - 1);
+__device__ __forceinline__ void append_latent_row(const AppendArgs& A, int t) {
+  constexpr int kHalf = DSA_ROPE_DIM / 2;
+  const int lane = threadIdx.x & (kWave - 1), pair = lane & (kHalf - 1);
   const long src = (long)t * A.latent_stride;
-  float x[8];
+  float x[8], w[8];
   load8<DT, WIDE>(A.latent, src + 8 * lane, x);
+  const int ia = A.interleaved ? 2 * pair : pair, ib = A.interleaved ? 2 * pair + 1 : pair + kHalf;
+  const float a = load_elem<DT>(A.latent, src + DSA_LATENT_DIM + ia);
+  const float b = load_elem<DT>(A.latent, src + DSA_LATENT_DIM + ib);
+  if (A.norm_w) {
+    if (A.norm_w_f32) load8<kF32, WIDE>(A.norm_w, 8 * lane, w);
+    else load8<DT, WIDE>(A.norm_w, 8 * lane, w);
+  }
+  const Place p = place_of(A, t);
+  if (p.slot < 0 || p.slot >= A.kv_rows) return;
+  float c = 1.f, s = 0.f;
+  if (A.table) {
+    c = A.table[(long)p.pos * DSA_ROPE_DIM + pair];
+    s = A.table[(long)p.pos * DSA_ROPE_DIM + kHalf + pair];
+  }
   if (A.norm_w) {
     double ss = 0.0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) ss = __builtin_fma((double)x[e], (double)x[e], ss);
-    const double rs = 1.0 / sqrt(wave_sum64(ss) / DSA_LATENT_DIM + A.eps);
+    const double rs = rsqrt(wave_sum64(ss) * (1.0 / DSA_LATENT_DIM) + A.eps);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float w = A.norm_w_f32 ? load_elem<kF32>(A.norm_w, 8 * lane + e) : load_elem<DT>(A.norm_w, 8 * lane + e);
-      x[e] = (float)((double)x[e] * rs * (double)w);
-    }
+    for (int e = 0; e < 8; ++e) x[e] = (float)((double)x[e] * rs * (double)w[e]);
   }
-  uint8_t* dst = A.pool + slot * BYTES;
+  uint8_t* dst = A.pool + p.slot * BYTES;
   if constexpr (BYTES == DSA_LATENT_ROW_BYTES) {
     const float scale = row_scale<true>(x);
     *reinterpret_cast<v2u_t*>(dst + 8 * lane) = quant8<true>(x, scale);
@@ -69,45 +99,39 @@ __device__ __forceinline__ void append_latent_row(const AppendArgs& A, int t, in
     reinterpret_cast<uint32_t*>(dst)[lane] = quant8_fp4(x, sb);
     if ((lane & 3) == 0) dst[DSA_LATENT_DIM / 2 + (lane >> 2)] = (uint8_t)sb;
   }
-  if (lane < DSA_ROPE_DIM / 2) {
-    constexpr int kHalf = DSA_ROPE_DIM / 2;
+  if (lane < kHalf) {
     uint16_t* rope = reinterpret_cast<uint16_t*>(dst + BYTES - 2 * DSA_ROPE_DIM);
-    const int ia = A.interleaved ? 2 * lane : lane, ib = A.interleaved ? 2 * lane + 1 : lane + kHalf;
-    const float a = load_elem<DT>(A.latent, src + DSA_LATENT_DIM + ia);
-    const float b = load_elem<DT>(A.latent, src + DSA_LATENT_DIM + ib);
     float ya = a, yb = b;
-    if (A.table) {
-      const float c = A.table[(long)pos * DSA_ROPE_DIM + lane], s = A.table[(long)pos * DSA_ROPE_DIM + kHalf + lane];
-      turn(a, b, c, s, ya, yb);
-    }
-    const uint32_t w = pack_bf16x2(ya, yb);
+    if (A.table) turn(a, b, c, s, ya, yb);
+    const uint32_t v = pack_bf16x2(ya, yb);
     if (A.interleaved) {
-      reinterpret_cast<uint32_t*>(rope)[lane] = w;
+      reinterpret_cast<uint32_t*>(rope)[lane] = v;
     } else {
-      rope[lane] = (uint16_t)w;
-      rope[lane + kHalf] = (uint16_t)(w >> 16);
+      rope[lane] = (uint16_t)v;
+      rope[lane + kHalf] = (uint16_t)(v >> 16);
     }
   }
 }
 
+// 16 lanes' index key, 8 values each; lanes 0-7 hold the turned half.
 template <int DT, bool WIDE>
-__device__ __forceinline__ void append_key(const AppendArgs& A, int t, int pos, long page) {
+__device__ __forceinline__ void append_key(const AppendArgs& A, int t) {
   const int i = threadIdx.x & 15;
   const long src = (long)t * A.keys_stride;
-  float x[8];
+  float x[8], o[8];  // o: lane i ^ 4's, the partners of the half layout
   load8<DT, WIDE>(A.keys, src + 8 * i, x);
-  if (A.table && i < DSA_ROPE_DIM / 8) {  // lanes 0-7 hold the rotated half
+  const bool turned = A.table && i < DSA_ROPE_DIM / 8;
+  if (turned && !A.index_interleaved) load8<DT, WIDE>(A.keys, src + 8 * (i ^ 4), o);
+  const Place p = place_of(A, t);
+  if (p.page < 0 || p.page >= A.num_pages) return;
+  if (turned) {
     constexpr int kHalf = DSA_ROPE_DIM / 2;
-    const float* cs = A.table + (long)pos * DSA_ROPE_DIM;
+    const float* cs = A.table + (long)p.pos * DSA_ROPE_DIM;
     if (A.index_interleaved) {
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const float c = cs[4 * i + p], s = cs[kHalf + 4 * i + p], a = x[2 * p], b = x[2 * p + 1];
-        turn(a, b, c, s, x[2 * p], x[2 * p + 1]);
-      }
-    } else {  // the partner's 8 are lane i ^ 4's
-      float o[8];
-      load8<DT, WIDE>(A.keys, src + 8 * (i ^ 4), o);
+      for (int k = 0; k < 4; ++k)
+        turn(x[2 * k], x[2 * k + 1], cs[4 * i + k], cs[kHalf + 4 * i + k], x[2 * k], x[2 * k + 1]);
+    } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float c = cs[8 * (i & 3) + e], s = cs[kHalf + 8 * (i & 3) + e];
@@ -116,8 +140,8 @@ __device__ __forceinline__ void append_key(const AppendArgs& A, int t, int pos, 
     }
   }
   const float scale = row_scale<true>(x);
-  uint8_t* base = A.index_k + page * DSA_INDEX_PAGE_BYTES;
-  const int slot = pos % DSA_PAGE_TOKENS;
+  uint8_t* base = A.index_k + p.page * DSA_INDEX_PAGE_BYTES;
+  const int slot = p.pos % DSA_PAGE_TOKENS;
   *reinterpret_cast<v2u_t*>(base + slot * DSA_INDEX_DIM + 8 * i) = quant8<true>(x, scale);
   if (i == 0) reinterpret_cast<float*>(base + DSA_PAGE_TOKENS * DSA_INDEX_DIM)[slot] = scale;
 }
@@ -128,27 +152,20 @@ template <int DT, bool WIDE, int BYTES>
 __global__ __launch_bounds__(kAppendThreads) void append_tokens_kernel(const AppendArgs A) {
   const long unit = (long)blockIdx.x * kAppendUnits + wave_id();
   const long n_lat = A.latent ? A.n : 0;
-  const int lane = threadIdx.x & (kWave - 1);
-  const long at = unit < n_lat ? unit : 4 * (unit - n_lat) + (lane >> 4);
-  if (at >= A.n) return;
-  const int t = (int)at, r = A.rows[t], pos = A.pos[t];
-  // a token without a request, a page or a table row is skipped
-  if (r < 0 || r >= A.B || pos < 0 || pos / DSA_PAGE_TOKENS >= A.pt_stride || (A.table && pos >= A.table_rows)) return;
-  const long page = A.page_table[(long)r * A.pt_stride + pos / DSA_PAGE_TOKENS];
-  if (page < 0) return;
   if (unit < n_lat) {
-    const long slot = page * DSA_PAGE_TOKENS + pos % DSA_PAGE_TOKENS;
-    if (slot < A.kv_rows) append_latent_row<DT, WIDE, BYTES>(A, t, pos, slot);
-  } else if (page < A.num_pages) {
-    append_key<DT, WIDE>(A, t, pos, page);
+    append_latent_row<DT, WIDE, BYTES>(A, (int)unit);
+    return;
   }
+  const long t = 4 * (unit - n_lat) + ((threadIdx.x & (kWave - 1)) >> 4);
+  if (A.keys && t < A.n) append_key<DT, WIDE>(A, (int)t);
 }
 
 template <int DT>
 static hipError_t launch_append_dt(const AppendArgs& A, int row_bytes, hipStream_t s) {
   constexpr int es = DT == kF32 ? 4 : 2;
   const auto on16 = [](const void* p, long stride) { return (((uintptr_t)p | (uintptr_t)(stride * es)) & 15) == 0; };
-  const bool wide = (!A.latent || on16(A.latent, A.latent_stride)) && (!A.keys || on16(A.keys, A.keys_stride));
+  const bool wide = (!A.latent || on16(A.latent, A.latent_stride)) && (!A.keys || on16(A.keys, A.keys_stride)) &&
+                    on16(A.norm_w, 0);
   const long units = (A.latent ? A.n : 0) + (A.keys ? (A.n + 3L) / 4 : 0);
   const dim3 grid((unsigned)((units + kAppendUnits - 1) / kAppendUnits));
   const auto go = [&](auto kernel) {
@@ -168,41 +185,60 @@ hipError_t launch_append_tokens(const AppendArgs& A, int dtype, int row_bytes, h
   return launch_append_dt<kF16>(A, row_bytes, s);
 }
 
-// ---- reading rows back: one wave a row ----
+// ---- reading rows back: a wave takes kReadRows rows, all in flight ----
+
+constexpr int kReadRows = 4;
 
 template <int BYTES>
 __global__ __launch_bounds__(kAppendThreads) void read_latent_kernel(const uint8_t* pool, long kv_rows, const int* slots,
                                                                       int n, uint16_t* out) {
-  const int t = blockIdx.x * kAppendUnits + wave_id(), lane = threadIdx.x & (kWave - 1);
-  if (t >= n) return;
-  const long slot = slots[t];
-  uint4* dst = reinterpret_cast<uint4*>(out + (long)t * DSA_QK_DIM);
-  const bool ok = slot >= 0 && slot < kv_rows;
-  const uint8_t* src = pool + (ok ? slot : 0) * BYTES;
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (ok) {
-    if constexpr (BYTES == DSA_LATENT_ROW_BYTES) {
-      const v2u_t c = *reinterpret_cast<const v2u_t*>(src + 8 * lane);
-      const float sc = reinterpret_cast<const float*>(src + DSA_LATENT_DIM)[lane >> 4];
-      float f[8];
-      e4m3x4_to_f32(c[0], f);
-      e4m3x4_to_f32(c[1], f + 4);
-      v = make_uint4(pack_bf16x2(f[0] * sc, f[1] * sc), pack_bf16x2(f[2] * sc, f[3] * sc),
-                     pack_bf16x2(f[4] * sc, f[5] * sc), pack_bf16x2(f[6] * sc, f[7] * sc));
+  constexpr bool kFp8 = BYTES == DSA_LATENT_ROW_BYTES;
+  const int lane = threadIdx.x & (kWave - 1);
+  const long t0 = ((long)blockIdx.x * kAppendUnits + wave_id()) * kReadRows;
+  uint2 code[kReadRows];
+  float sc[kReadRows];
+  uint4 rope[kReadRows];
+#pragma unroll
+  for (int k = 0; k < kReadRows; ++k) {
+    code[k] = make_uint2(0, 0);
+    sc[k] = 0.f;
+    rope[k] = make_uint4(0, 0, 0, 0);
+    const long slot = t0 + k < n ? slots[t0 + k] : -1;
+    if (slot < 0 || slot >= kv_rows) continue;
+    const uint8_t* src = pool + slot * BYTES;
+    if constexpr (kFp8) {
+      code[k] = *reinterpret_cast<const uint2*>(src + 8 * lane);
+      sc[k] = reinterpret_cast<const float*>(src + DSA_LATENT_DIM)[lane >> 4];
     } else {
-      v = dequant8_fp4(reinterpret_cast<const uint32_t*>(src)[lane],
-                       __uint_as_float((uint32_t)src[DSA_LATENT_DIM / 2 + (lane >> 2)] << 23));
+      code[k].x = reinterpret_cast<const uint32_t*>(src)[lane];
+      sc[k] = __uint_as_float((uint32_t)src[DSA_LATENT_DIM / 2 + (lane >> 2)] << 23);
     }
+    if (lane < DSA_ROPE_DIM / 8) rope[k] = *reinterpret_cast<const uint4*>(src + BYTES - 2 * DSA_ROPE_DIM + 16 * lane);
   }
-  dst[lane] = v;
-  if (lane < DSA_ROPE_DIM / 8)
-    dst[kWave + lane] = ok ? *reinterpret_cast<const uint4*>(src + BYTES - 2 * DSA_ROPE_DIM + 16 * lane) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int k = 0; k < kReadRows; ++k) {
+    if (t0 + k >= n) return;
+    uint4 v;
+    if constexpr (kFp8) {
+      float f[8];
+      e4m3x4_to_f32(code[k].x, f);
+      e4m3x4_to_f32(code[k].y, f + 4);
+      v = make_uint4(pack_bf16x2(f[0] * sc[k], f[1] * sc[k]), pack_bf16x2(f[2] * sc[k], f[3] * sc[k]),
+                     pack_bf16x2(f[4] * sc[k], f[5] * sc[k]), pack_bf16x2(f[6] * sc[k], f[7] * sc[k]));
+    } else {
+      v = dequant8_fp4(code[k].x, sc[k]);
+    }
+    uint4* dst = reinterpret_cast<uint4*>(out + (t0 + k) * DSA_QK_DIM);
+    dst[lane] = v;
+    if (lane < DSA_ROPE_DIM / 8) dst[kWave + lane] = rope[k];
+  }
 }
 
 hipError_t launch_read_latent(const void* pool, long kv_rows, int row_bytes, const int* slots, int n, void* out,
                               hipStream_t s) {
   if (n <= 0) return hipSuccess;
-  const dim3 grid((unsigned)((n + kAppendUnits - 1) / kAppendUnits));
+  constexpr int per = kAppendUnits * kReadRows;
+  const dim3 grid((unsigned)(((long)n + per - 1) / per));
   const uint8_t* p = static_cast<const uint8_t*>(pool);
   uint16_t* o = static_cast<uint16_t*>(out);
   if (row_bytes == DSA_LATENT_ROW_BYTES)

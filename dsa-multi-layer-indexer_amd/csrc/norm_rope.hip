@@ -10,6 +10,8 @@
 //   rotary: (a, b) -> (a c - b s, b c + a s) with c, s of the token's position;
 //   a, b = elements i, i + R/2 (half) or 2i, 2i + 1 (interleaved); the
 //   inverse turns by -s, which is also the operation's adjoint.
+#include <algorithm>
+
 #include "dsa_kernels.h"
 #include "quant_core.h"
 
@@ -31,62 +33,128 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+// V vectors of 8 elements a lane, as they come from memory.
+template <int DT, int V>
+struct RawRow {
+  uint4 v[V][DT == kF32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ void unpack8(const uint4* v, float* x) {
+  if constexpr (DT == kF32) {
+    const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e]);
+  } else {
+    const uint32_t w[4] = {v[0].x, v[0].y, v[0].z, v[0].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (DT == kBF16) {
+        x[2 * e] = bf16_lo(w[e]);
+        x[2 * e + 1] = bf16_hi(w[e]);
+      } else {
+        x[2 * e] = (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
+        x[2 * e + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
+      }
+    }
+  }
+}
+// Row `p`'s vectors of thread t of T (zeros past D).
+template <int DT, int V>
+__device__ __forceinline__ void load_raw(const void* p, int t, int T, int D, RawRow<DT, V>& r) {
+  constexpr int es = DT == kF32 ? 4 : 2, k = DT == kF32 ? 2 : 1;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int i = 8 * (v * T + t);
+#pragma unroll
+    for (int c = 0; c < k; ++c)
+      r.v[v][c] = i < D ? reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + (long)i * es)[c]
+                        : make_uint4(0, 0, 0, 0);
+  }
+}
+
 // A row is held by T threads, V vectors of 8 elements each (vector v of
 // thread t: elements 8 (v T + t) ..); the 16 lanes of a DPP row hold 128
 // consecutive elements, one quantisation group.  WIDE: D a multiple of 8 and
-// every row on 16-byte boundaries.
-template <int DT, int T, int V, bool WIDE>
-__global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(const NormArgs A) {
-  constexpr int kBlock = T < 256 ? 256 : T, kRows = kBlock / T, kWaves = T / kWave;
-  __shared__ float red[2][kWaves];
-  __shared__ uint32_t redm[2][kWaves];
-  const int t = threadIdx.x % T, D = A.D, wv = t / kWave;
+// every row on 16-byte boundaries.  ONE_WAVE: T is a wave, kNormRows rows a
+// workgroup; otherwise the workgroup is the row's T threads.  Workgroups go
+// on to further rows, with the weight in registers and the next row in
+// flight from before the reduction on.
+constexpr int kNormRows = 4;
+constexpr int kNormWaves = 16;  // most waves a row
+
+template <int DT, int V, bool WIDE, bool ONE_WAVE>
+__global__ __launch_bounds__(ONE_WAVE ? kNormRows* kWave : kNormWaves* kWave) void rms_norm_kernel(const NormArgs A) {
+  constexpr int es = DT == kF32 ? 4 : 2;
+  __shared__ float red[2][kNormWaves];
+  __shared__ uint32_t redm[2][kNormWaves];
+  const int T = ONE_WAVE ? kWave : (int)blockDim.x, waves = T / kWave;
+  const int t = ONE_WAVE ? (int)threadIdx.x & (kWave - 1) : (int)threadIdx.x, D = A.D, wv = wave_id();
+  const long stride = (long)gridDim.x * (ONE_WAVE ? kNormRows : 1);
+  long row = (long)blockIdx.x * (ONE_WAVE ? kNormRows : 1) + (ONE_WAVE ? wv : 0);
+  if (row >= A.n) return;  // (whole rows' threads)
+  const auto at = [&](const void* p, long r, long rs) { return static_cast<const uint8_t*>(p) + r * rs * es; };
+  RawRow<DT, V> x, r;
+  if constexpr (WIDE) {
+    load_raw<DT, V>(at(A.x, row, A.xs), t, T, D, x);
+    if (A.r) load_raw<DT, V>(at(A.r, row, A.rs), t, T, D, r);
+  }
   float w[V][8];
 #pragma unroll
-  for (int v = 0; v < V; ++v)
+  for (int v = 0; v < V; ++v) {
+    const int i = 8 * (v * T + t);
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int i = 8 * (v * T + t) + e;
-      w[v][e] = i >= D ? 0.f : A.w_f32 ? load_elem<kF32>(A.w, i) : load_elem<DT>(A.w, i);
+      for (int e = 0; e < 8; ++e) w[v][e] = 0.f;
+      if (i < D) {
+        if (A.w_f32) load8<kF32>(A.w, i, w[v]);
+        else load8<DT>(A.w, i, w[v]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        w[v][e] = i + e >= D ? 0.f : A.w_f32 ? load_elem<kF32>(A.w, i + e) : load_elem<DT>(A.w, i + e);
     }
-  int par = 0;
-  for (long row = (long)blockIdx.x * kRows + threadIdx.x / T; row < A.n; row += (long)gridDim.x * kRows, par ^= 1) {
+  }
+  for (int par = 0; row < A.n; row += stride, par ^= 1) {
     float h[V][8];
     float ss = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int i = 8 * (v * T + t);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h[v][e] = 0.f;
       if constexpr (WIDE) {
-        if (i < D) {
-          load8<DT>(A.x, row * A.xs + i, h[v]);
-          if (A.r) {
-            float r[8];
-            load8<DT>(A.r, row * A.rs + i, r);
+        unpack8<DT>(x.v[v], h[v]);
+        if (A.r) {
+          float f[8];
+          unpack8<DT>(r.v[v], f);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) h[v][e] += r[e];
-          }
+          for (int e = 0; e < 8; ++e) h[v][e] += f[e];
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < 8; ++e) {
+          h[v][e] = 0.f;
           if (i + e < D) {
             h[v][e] = load_elem<DT>(A.x, row * A.xs + i + e);
             if (A.r) h[v][e] += load_elem<DT>(A.r, row * A.rs + i + e);
           }
+        }
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(h[v][e], h[v][e], ss);
       if (A.h && (!WIDE || i < D)) store8<DT, WIDE>(A.h, row * A.hs + i, h[v], row * A.hs + D);
     }
+    if constexpr (WIDE) {
+      if (const long next = row + stride; next < A.n) {
+        load_raw<DT, V>(at(A.x, next, A.xs), t, T, D, x);
+        if (A.r) load_raw<DT, V>(at(A.r, next, A.rs), t, T, D, r);
+      }
+    }
     ss = wave_sum(ss);
-    if constexpr (kWaves > 1) {
+    if (!ONE_WAVE && waves > 1) {
       if ((t & (kWave - 1)) == 0) red[par][wv] = ss;
       __syncthreads();
       ss = 0.f;
-#pragma unroll
-      for (int k = 0; k < kWaves; ++k) ss += red[par][k];
+      for (int k = 0; k < waves; ++k) ss += red[par][k];
     }
     const float rs = 1.f / sqrtf(ss / (float)D + A.eps);
 #pragma unroll
@@ -106,11 +174,10 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(const NormA
 #pragma unroll
       for (int v = 0; v < V; ++v) am = max(am, amax_bits<true>(h[v]));
       am = wave_reduce<2>(am);
-      if constexpr (kWaves > 1) {
+      if (!ONE_WAVE && waves > 1) {
         if ((t & (kWave - 1)) == 0) redm[par][wv] = am;
         __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kWaves; ++k) am = max(am, redm[par][k]);
+        for (int k = 0; k < waves; ++k) am = max(am, redm[par][k]);
       }
     }
     const int groups = A.group ? (D + 127) / 128 : 1;
@@ -133,13 +200,14 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rms_norm_kernel(const NormA
   }
 }
 
-template <int DT, int T, int V>
+template <int DT, int V, bool ONE_WAVE>
 static hipError_t launch_norm(const NormArgs& A, bool wide, hipStream_t s) {
-  constexpr int kBlock = T < 256 ? 256 : T, kRows = kBlock / T;
-  const long blocks = ((long)A.n + kRows - 1) / kRows;
-  const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : (1 << 20)));
-  const auto kernel = wide ? rms_norm_kernel<DT, T, V, true> : rms_norm_kernel<DT, T, V, false>;
-  hipLaunchKernelGGL(kernel, grid, dim3(kBlock), 0, s, A);
+  const int vecs = (A.D + 7) / 8;
+  const int threads = ONE_WAVE ? kNormRows * kWave : ((vecs + V - 1) / V + kWave - 1) / kWave * kWave;
+  const long blocks = ONE_WAVE ? ((long)A.n + kNormRows - 1) / kNormRows : A.n;
+  const long most = (long)device_cu_count() * (2048 / threads);  // what is resident at once
+  const auto kernel = wide ? rms_norm_kernel<DT, V, true, ONE_WAVE> : rms_norm_kernel<DT, V, false, ONE_WAVE>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(threads), 0, s, A);
   return hipGetLastError();
 }
 
@@ -148,14 +216,11 @@ static hipError_t launch_norm_dim(const NormArgs& A, hipStream_t s) {
   constexpr int es = DT == kF32 ? 4 : 2;
   const auto on16 = [](const void* p, long stride) { return (((uintptr_t)p | (uintptr_t)(stride * es)) & 15) == 0; };
   const bool wide = A.D % 8 == 0 && on16(A.x, A.xs) && (!A.r || on16(A.r, A.rs)) && (!A.h || on16(A.h, A.hs)) &&
-                    (!A.y || on16(A.y, 0)) && ((uintptr_t)A.codes & 7) == 0;
-  if (A.D <= 512) return launch_norm<DT, 64, 1>(A, wide, s);
-  if (A.D <= 1024) return launch_norm<DT, 64, 2>(A, wide, s);
-  if (A.D <= 2048) return launch_norm<DT, 256, 1>(A, wide, s);
-  if (A.D <= 4096) return launch_norm<DT, 256, 2>(A, wide, s);
-  if (A.D <= 8192) return launch_norm<DT, 256, 4>(A, wide, s);
-  if (A.D <= 16384) return launch_norm<DT, 1024, 2>(A, wide, s);
-  return launch_norm<DT, 1024, 4>(A, wide, s);
+                    (!A.y || on16(A.y, 0)) && ((uintptr_t)A.codes & 7) == 0 && on16(A.w, 0);
+  if (A.D <= 512) return launch_norm<DT, 1, true>(A, wide, s);
+  if (A.D <= 8192) return launch_norm<DT, 1, false>(A, wide, s);
+  if (A.D <= 16384) return launch_norm<DT, 2, false>(A, wide, s);
+  return launch_norm<DT, 4, false>(A, wide, s);
 }
 
 hipError_t launch_rms_norm(const NormArgs& A, int dtype, hipStream_t s) {
@@ -167,90 +232,114 @@ hipError_t launch_rms_norm(const NormArgs& A, int dtype, hipStream_t s) {
 
 // ---- rotary positions ----
 
-// One item: WIDE a vector of 8 elements (of a half: and its partners R/2
-// on), otherwise a pair; behind them, where the output is another tensor,
-// the elements outside the rotated part (vectors of 8, or one by one).
-// A workgroup takes whole tokens, so that a thread's table entries serve all
-// its heads (kRopeThreads is a multiple of the items of every width that is
-// a power of two).
-constexpr int kRopeThreads = 256;
+// One item of a head: WIDE a vector of 8 elements of the rotated part (half:
+// and its partners R/2 on), otherwise a pair; behind them, where the output
+// is another tensor, the elements outside the rotated part (vectors of 8, or
+// one by one).  A thread keeps its item and goes through heads, kRopeBatch at
+// a time, so that the table is read once for all of them and several loads
+// are in flight.
+constexpr int kRopeThreads = 256, kRopeBatch = 4;
 
 template <int DT, bool WIDE, bool INTER>
 __global__ __launch_bounds__(kRopeThreads) void rotary_kernel(const RopeArgs A) {
   const int rot_items = WIDE ? A.R / (INTER ? 8 : 16) : A.R / 2;
   const int items = rot_items + (A.copy ? (A.D - A.R) / (WIDE ? 8 : 1) : 0);
-  const int per = A.H * items;                                  // items a token
-  const int tok = per < kRopeThreads ? kRopeThreads / per : 1;  // tokens a workgroup
+  const int per = items * A.heads;  // threads a token (items of as many heads)
   const int lt = per < kRopeThreads ? (int)threadIdx.x / per : 0;
-  const long token = (long)blockIdx.x * tok + lt;
-  if (lt >= tok || token >= A.n) return;
+  const int tid = (int)threadIdx.x - lt * per;
+  const long token = (long)blockIdx.x * A.tokens + lt;
+  if (lt >= A.tokens || token >= A.n) return;
   const long pos = A.pos64 ? static_cast<const int64_t*>(A.pos)[token] : (long)static_cast<const int32_t*>(A.pos)[token];
   const bool in = pos >= 0 && pos < A.max_pos;
+  if (!in && !A.copy) return;
   const float* cs = A.table + (in ? pos : 0) * A.R;
   const float sign = A.inverse ? -1.f : 1.f;
-  const int hr = A.R / 2;
-  for (int j = (int)threadIdx.x - lt * per; j < per; j += kRopeThreads) {
-    const int head = j / items, it = j - head * items;
-    const long xi = token * A.xn + head * A.xh, oi = token * A.on + head * A.oh;
-    if (it >= rot_items) {  // outside the rotated part
-      int d = (it - rot_items) * (WIDE ? 8 : 1);
-      d += d >= A.start ? A.R : 0;
-      if constexpr (WIDE) {
-        float x[8];
-        load8<DT>(A.x, xi + d, x);
-        store8<DT, true>(A.out, oi + d, x, 0);
-      } else {
-        if constexpr (DT == kF32) static_cast<float*>(A.out)[oi + d] = static_cast<const float*>(A.x)[xi + d];
-        else static_cast<uint16_t*>(A.out)[oi + d] = static_cast<const uint16_t*>(A.x)[xi + d];
-      }
-      continue;
-    }
-    if (!in && !A.copy) return;
-    if constexpr (WIDE && INTER) {
-      const int d = A.start + 8 * it;
-      float x[8], y[8];
-      load8<DT>(A.x, xi + d, x);
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const float c = in ? cs[4 * it + p] : 1.f, sn = in ? sign * cs[hr + 4 * it + p] : 0.f;
-        turn(x[2 * p], x[2 * p + 1], c, sn, y[2 * p], y[2 * p + 1]);
-      }
-      store8<DT, true>(A.out, oi + d, in ? y : x, 0);
-    } else if constexpr (WIDE) {
-      const int d = A.start + 8 * it;
-      float a[8], b[8], ya[8], yb[8];
-      load8<DT>(A.x, xi + d, a);
-      load8<DT>(A.x, xi + d + hr, b);
-#pragma unroll
-      for (int p = 0; p < 8; ++p) {
-        const float c = in ? cs[8 * it + p] : 1.f, sn = in ? sign * cs[hr + 8 * it + p] : 0.f;
-        turn(a[p], b[p], c, sn, ya[p], yb[p]);
-      }
-      store8<DT, true>(A.out, oi + d, in ? ya : a, 0);
-      store8<DT, true>(A.out, oi + d + hr, in ? yb : b, 0);
+  const int hr = A.R / 2, h0 = tid / items + (int)blockIdx.y * A.heads, hstep = (int)gridDim.y * A.heads;
+  for (int it = tid % items; it < items; it += kRopeThreads) {  // (one pass unless a head has more items)
+    const bool turned = it < rot_items;
+    constexpr int kC = WIDE ? (INTER ? 4 : 8) : 1, kE = WIDE ? 8 : 1, kPart = (INTER && WIDE) ? 1 : 2;
+    int d = WIDE ? 8 * it : INTER ? 2 * it : it;
+    if (turned) {
+      d += A.start;
     } else {
-      const int da = A.start + (INTER ? 2 * it : it), db = INTER ? da + 1 : da + hr;
-      const float a = load_elem<DT>(A.x, xi + da), b = load_elem<DT>(A.x, xi + db);
-      const float c = in ? cs[it] : 1.f, sn = in ? sign * cs[hr + it] : 0.f;
-      float ya[8], yb[8];
-      turn(a, b, c, sn, ya[0], yb[0]);
-      if (!in) ya[0] = a, yb[0] = b;
-      store8<DT, false>(A.out, oi + da, ya, oi + da + 1);
-      store8<DT, false>(A.out, oi + db, yb, oi + db + 1);
+      d = (it - rot_items) * kE;
+      d += d >= A.start ? A.R : 0;
+    }
+    const int d2 = d + (WIDE || !INTER ? hr : 1);  // the partners (kPart == 2)
+    float c[kC], sn[kC];
+#pragma unroll
+    for (int k = 0; k < kC; ++k) c[k] = 1.f, sn[k] = 0.f;
+    if (turned && in) {
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int k = 0; k < kC; k += 4) {
+          const v4f a = *reinterpret_cast<const v4f*>(cs + kC * it + k);
+          const v4f b = *reinterpret_cast<const v4f*>(cs + hr + kC * it + k);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[k + e] = a[e], sn[k + e] = sign * b[e];
+        }
+      } else {
+        c[0] = cs[it], sn[0] = sign * cs[hr + it];
+      }
+    }
+    for (int hb = h0; hb < A.H; hb += hstep * kRopeBatch) {
+      float x[kRopeBatch][kPart][kE];
+#pragma unroll
+      for (int k = 0; k < kRopeBatch; ++k) {
+        const int h = hb + k * hstep;
+        if (h >= A.H) break;
+        const long xi = token * A.xn + h * A.xh;
+        if constexpr (WIDE) {
+          load8<DT>(A.x, xi + d, x[k][0]);
+          if constexpr (kPart == 2)
+            if (turned) load8<DT>(A.x, xi + d2, x[k][1]);
+        } else {
+          x[k][0][0] = load_elem<DT>(A.x, xi + d);
+          if (turned) x[k][1][0] = load_elem<DT>(A.x, xi + d2);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kRopeBatch; ++k) {
+        const int h = hb + k * hstep;
+        if (h >= A.H) break;
+        const long oi = token * A.on + h * A.oh;
+        if (turned && in) {
+          if constexpr (kPart == 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) turn(x[k][0][2 * e], x[k][0][2 * e + 1], c[e], sn[e], x[k][0][2 * e], x[k][0][2 * e + 1]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < kE; ++e) turn(x[k][0][e], x[k][1][e], c[e], sn[e], x[k][0][e], x[k][1][e]);
+          }
+        }
+        if constexpr (WIDE) {
+          store8<DT, true>(A.out, oi + d, x[k][0], 0);
+          if constexpr (kPart == 2)
+            if (turned) store8<DT, true>(A.out, oi + d2, x[k][1], 0);
+        } else {
+          store8<DT, false>(A.out, oi + d, x[k][0], oi + d + 1);
+          if (turned) store8<DT, false>(A.out, oi + d2, x[k][1], oi + d2 + 1);
+        }
+      }
     }
   }
 }
 
 template <int DT>
-static hipError_t launch_rotary_dt(const RopeArgs& A, hipStream_t s) {
+static hipError_t launch_rotary_dt(RopeArgs A, hipStream_t s) {
   constexpr int es = DT == kF32 ? 4 : 2;
   const uintptr_t strides = (uintptr_t)((A.xn | A.xh | A.on | A.oh) * es);
   const bool wide = A.R % (A.interleaved ? 8 : 16) == 0 && A.start % 8 == 0 && (!A.copy || A.D % 8 == 0) &&
-                    (((uintptr_t)A.x | (uintptr_t)A.out | strides) & 15) == 0;
+                    (((uintptr_t)A.x | (uintptr_t)A.out | (uintptr_t)A.table | strides) & 15) == 0;
   const int items = (wide ? A.R / (A.interleaved ? 8 : 16) : A.R / 2) + (A.copy ? (A.D - A.R) / (wide ? 8 : 1) : 0);
-  const long per = (long)A.H * items;
-  const int tok = per < kRopeThreads ? (int)(kRopeThreads / per) : 1;
-  const dim3 grid((unsigned)(((long)A.n + tok - 1) / tok));
+  // a workgroup: as many heads of a token as fit, then as many tokens
+  A.heads = items >= kRopeThreads ? 1 : std::min(A.H, kRopeThreads / items);
+  A.tokens = std::max(1, kRopeThreads / (A.heads * items));
+  const long x = ((long)A.n + A.tokens - 1) / A.tokens;
+  // few tokens: their heads over several workgroups
+  const int turns = (A.H + A.heads - 1) / A.heads;
+  const int y = (int)std::max(1L, std::min({(long)turns, 65535L, 2L * device_cu_count() / x}));
+  const dim3 grid((unsigned)x, (unsigned)y);
   const auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, dim3(kRopeThreads), 0, s, A);
     return hipGetLastError();

@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 import torch  # noqa: F401  (loads torch's HIP runtime before ours)
@@ -66,6 +67,12 @@ class LayerArgs(ctypes.Structure):
     ]
 
 
+# dsa_norm_args, dsa_rotary_args, dsa_append_args, packed in one go (a field of
+# a ctypes structure costs about as much as the whole packing)
+NORM_ARGS = struct.Struct("@7P3qd5i0q")
+ROTARY_ARGS = struct.Struct("@4P5q9i0q")
+APPEND_ARGS = struct.Struct("@9P5qd8i0q")
+
 _LIB: ctypes.CDLL | None = None
 
 # (name, restype, argtypes) for every symbol of include/dsa_mli.h
@@ -105,12 +112,9 @@ SIGNATURES = {
     "dsa_pack_latent_rows": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp]),
     "dsa_selection_set": (_i32, [_vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp]),
     "dsa_prefill_attention": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp]),
-    "dsa_rms_norm": (_i32, [_vp, _i32, _i64, _vp, _i64, _vp, _i32, _f64, _vp, _vp, _vp, _i32, _vp, _i64, _i32, _i32,
-                            _vp]),
-    "dsa_rotary": (_i32, [_vp, _i32, _i64, _i64, _vp, _i32, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _i32, _i32,
-                          _i32, _i32, _vp]),
-    "dsa_append_tokens": (_i32, [_vp, _vp, _i32, _vp, _i32, _i32, _vp, _i64, _i32, _vp, _i64, _vp, _i32, _f64, _i32,
-                                 _vp, _i64, _i32, _vp, _i64, _i32, _vp, _i64, _vp]),
+    "dsa_rms_norm": (_i32, [ctypes.c_char_p, _vp]),
+    "dsa_rotary": (_i32, [ctypes.c_char_p, _vp]),
+    "dsa_append_tokens": (_i32, [ctypes.c_char_p, _vp]),
     "dsa_read_latent_rows": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _vp]),
     "dsa_mla_fp4_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i32]),
     "dsa_sparse_mla_decode_fp4": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp]),

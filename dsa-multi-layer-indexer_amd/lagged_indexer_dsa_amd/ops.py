@@ -33,8 +33,13 @@ def _dev(*tensors: torch.Tensor) -> None:
             raise RuntimeError("lagged_indexer_dsa_amd ops need contiguous tensors")
 
 
+_current_device = torch._C._cuda_getDevice
+
+
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # torch.cuda.current_stream().cuda_stream without building the two objects
+    # around it (0.2 us against 2.7, a fifth of a small call)
+    return torch._C._cuda_getCurrentRawStream(_current_device())
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -177,14 +182,17 @@ def _resolve_nsplit(nsplit: int, B: int, H: int, keys: int) -> int:
     return nsplit or max(1, _lib.load().dsa_sparse_mla_auto_nsplit(B, H, keys))
 
 
-def _here(first: torch.Tensor, *others: torch.Tensor | None) -> None:
-    """All on one device, the one the call's kernels go to."""
-    dev = first.device
-    if dev.index != torch.cuda.current_device():
-        raise RuntimeError(f"tensors are on {dev}, the current device is cuda:{torch.cuda.current_device()}")
-    for t in others:
-        if t is not None and t.device != dev:
-            raise RuntimeError(f"tensors on different devices: {dev} and {t.device}")
+def _here(dev: int, *tensors: torch.Tensor | None) -> None:
+    """All on device `dev`, the one the call's kernels go to."""
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            if dev < 0 or t.get_device() < 0:
+                raise RuntimeError("lagged_indexer_dsa_amd ops need GPU (HIP) tensors; there is no CPU path")
+            raise RuntimeError(f"tensors on different devices: cuda:{dev} and {t.device}")
+    if dev < 0:
+        raise RuntimeError("lagged_indexer_dsa_amd ops need GPU (HIP) tensors; there is no CPU path")
+    if dev != _current_device():
+        raise RuntimeError(f"tensors are on cuda:{dev}, the current device is cuda:{_current_device()}")
 
 
 def _fp4_call(q, kv_pool, sm_scale, nsplit: int, workspace, out, *others):
@@ -195,18 +203,18 @@ def _fp4_call(q, kv_pool, sm_scale, nsplit: int, workspace, out, *others):
     if kv_pool.dtype != torch.uint8:
         raise RuntimeError("kv_pool must be [rows, 400] uint8")
     B, H, _ = qs
+    _here(q.get_device(), kv_pool, workspace, out, *others)
     nbytes = _lib.load().dsa_mla_fp4_workspace_bytes(B, H, nsplit)
     if workspace is None:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     else:
-        _dev(workspace)
         _need_bytes("4-bit MLA workspace", workspace, nbytes)
+        if not workspace.is_contiguous():
+            raise RuntimeError("the 4-bit MLA workspace must be contiguous")
     if out is None:
         out = torch.empty(B, H, LATENT_DIM, dtype=torch.bfloat16, device=q.device)
     else:
-        _dev(out)
         _need_shape("out", out, (B, H, LATENT_DIM), torch.bfloat16)
-    _here(q, kv_pool, workspace, out, *others)
     return B, H, QK_DIM ** -0.5 if sm_scale is None else float(sm_scale), workspace, out
 
 
@@ -473,21 +481,20 @@ def append_latent_rows(kv_pool: torch.Tensor, slots: torch.Tensor, latent: torch
 
 # ---- around the cached attention: norm, rotation, cache appends and reads ----
 
-def _rows_of(name: str, x: torch.Tensor, D: int | None = None) -> torch.Tensor:
-    """x [..., D] as rows [n, D] without a copy; the last dim contiguous."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise RuntimeError("lagged_indexer_dsa_amd ops need GPU (HIP) tensors; there is no CPU path")
-    shape = x.shape
-    if not shape or (D is not None and shape[-1] != D):
-        raise RuntimeError(f"{name} must be [..., {'D' if D is None else D}], got {tuple(shape)}")
-    if shape[-1] > 1 and x.stride(-1) != 1:
+def _row_stride(name: str, x: torch.Tensor, n: int, D: int) -> int:
+    """The stride between the n rows of x [..., D]; refuses what has none."""
+    if x.is_contiguous():
+        return D
+    st = x.stride()
+    if D > 1 and st[-1] != 1:
         raise RuntimeError(f"{name}'s last dimension must be contiguous")
-    if len(shape) != 2:
-        try:
-            x = x.view(-1, shape[-1]) if x.numel() else x.reshape(0, shape[-1])
-        except RuntimeError:
-            raise RuntimeError(f"{name}'s leading dimensions must be one stride apart, got strides {x.stride()}") from None
-    return x
+    if n <= 1:
+        return D
+    dims = [(k, t) for k, t in zip(x.shape[:-1], st[:-1]) if k > 1]
+    for (k, t), (_, outer) in zip(dims[1:], dims[:-1]):
+        if outer != k * t:
+            raise RuntimeError(f"{name}'s leading dimensions must be one stride apart, got strides {st}")
+    return dims[-1][1]
 
 
 def _span(t: torch.Tensor) -> tuple[int, int]:
@@ -507,51 +514,66 @@ def _need_apart(name: str, out: torch.Tensor, *inputs: torch.Tensor | None) -> N
                 raise RuntimeError(f"{name} overlaps an input")
 
 
-def _norm(x, weight, eps, residual, out, out_q, out_scale, group, out_residual):
-    xr = _rows_of("x", x)
-    n, D = xr.shape
-    dtype = x.dtype
-    if dtype not in _PACK_DTYPES:
-        raise RuntimeError(f"x must be float32, bfloat16 or float16, got {dtype}")
+def _norm(x, weight, eps, residual, outs, group, out_residual):
+    """Checks and launch of a norm; outs: its output and, quantised, the
+    scales, as the caller gave them (None: new ones).  Returns all outputs."""
+    shape, dt = x.shape, x.dtype
+    dtype = _PACK_DTYPES.get(dt)
+    if dtype is None:
+        raise RuntimeError(f"x must be float32, bfloat16 or float16, got {dt}")
+    dev = x.get_device()
+    D = shape[-1] if shape else 0
     if not 1 <= D <= NORM_MAX_DIM:
-        raise RuntimeError(f"x's rows must hold 1 to {NORM_MAX_DIM} values, got {D}")
-    _dev(weight)
-    if weight.shape != (D,) or (weight.dtype != dtype and weight.dtype != torch.float32):
-        raise RuntimeError(f"weight must be [{D}] of x's type or float32, got {weight.dtype} {tuple(weight.shape)}")
-    rr = hr = None
-    h = None
+        raise RuntimeError(f"x must be [..., D] with D from 1 to {NORM_MAX_DIM}, got {tuple(shape)}")
+    _here(dev, weight, residual, out_residual, *outs)
+    n = x.numel() // D
+    wt = weight.dtype
+    if weight.shape != (D,) or (wt != dt and wt != torch.float32) or not weight.is_contiguous():
+        raise RuntimeError(f"weight must be [{D}] of x's type or float32, got {wt} {tuple(weight.shape)}")
+    quant = len(outs) == 2
+    if quant:
+        sshape = (*shape[:-1], -(-D // 128) if group else 1)
+        kinds = (("out_q", shape, torch.uint8), ("out_scale", sshape, torch.float32))
+    else:
+        kinds = (("out", shape, dt),)
+    res = []
+    for t, (name, want, kind) in zip(outs, kinds):
+        if t is None:
+            t = torch.empty(want, dtype=kind, device=x.device)
+        else:
+            _need_shape(name, t, want, kind)
+            if n:
+                _need_apart(name, t, x, residual, weight, out_residual, *res)
+        res.append(t)
+    xs, rs, hs, rp, hp = _row_stride("x", x, n, D), 0, 0, 0, 0
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != dtype:
-            raise RuntimeError(f"residual must be {dtype} {tuple(x.shape)}, got {residual.dtype} {tuple(residual.shape)}")
-        rr = _rows_of("residual", residual)
+        if residual.dtype != dt or residual.shape != shape:
+            raise RuntimeError(f"residual must be {dt} {tuple(shape)}, got {residual.dtype} {tuple(residual.shape)}")
+        rs, rp = _row_stride("residual", residual, n, D), residual.data_ptr()
         if out_residual is None:
-            h = hr = torch.empty(x.shape, dtype=dtype, device=x.device)
-            hr = _rows_of("out_residual", hr)
+            h = torch.empty(shape, dtype=dt, device=x.device)
+            hs = D
         else:
             h = out_residual
-            if h.shape != x.shape or h.dtype != dtype:
-                raise RuntimeError(f"out_residual must be {dtype} {tuple(x.shape)}, got {h.dtype} {tuple(h.shape)}")
-            hr = _rows_of("out_residual", h)
-            if n > 1 and hr.stride(0) < D:
+            if h.dtype != dt or h.shape != shape:
+                raise RuntimeError(f"out_residual must be {dt} {tuple(shape)}, got {h.dtype} {tuple(h.shape)}")
+            hs = _row_stride("out_residual", h, n, D)
+            if n > 1 and hs < D:
                 raise RuntimeError("out_residual's rows overlap")
-            if n and (hr.data_ptr() != rr.data_ptr() or hr.stride(0) != rr.stride(0)):
-                _need_apart("out_residual", hr, xr, rr, weight)
-            elif n:
-                _need_apart("out_residual", hr, xr, weight)
+            if n:
+                same = h is residual or (h.data_ptr() == rp and hs == rs)
+                _need_apart("out_residual", h, x, weight, None if same else residual)
+        hp = h.data_ptr()
+        res.append(h)
     elif out_residual is not None:
         raise RuntimeError("out_residual without a residual")
-    _here(x, weight, residual, h, out, out_q, out_scale)
-    if n and (out is not None or out_q is not None or out_scale is not None):
-        for name, t in (("out", out), ("out_q", out_q), ("out_scale", out_scale)):
-            if t is not None and t.numel():
-                _need_apart(name, t, xr, rr, hr, weight)
-        if out_q is not None and out_scale is not None:
-            _need_apart("out_scale", out_scale, out_q)
     if n:
-        _lib.call("dsa_rms_norm", xr.data_ptr(), _PACK_DTYPES[dtype], xr.stride(0), _ptr(rr),
-                  0 if rr is None else rr.stride(0), weight.data_ptr(), _PACK_DTYPES[weight.dtype], eps, _ptr(out),
-                  _ptr(out_q), _ptr(out_scale), group, _ptr(hr), 0 if hr is None else hr.stride(0), n, D, _stream())
-    return h
+        y = res[0].data_ptr()
+        a = _lib.NORM_ARGS.pack(x.data_ptr(), rp, weight.data_ptr(), 0 if quant else y, y if quant else 0,
+                                res[1].data_ptr() if quant else 0, hp, xs, rs, hs, eps, n, D, dtype, _PACK_DTYPES[wt],
+                                group)
+        _lib.call("dsa_rms_norm", a, torch._C._cuda_getCurrentRawStream(dev))
+    return res
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
@@ -561,16 +583,12 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
 
     x [..., D] fp32, bf16 or fp16 (rows any one stride apart, D up to 32768),
     residual of the same shape and type, weight [D] of x's type or fp32.
-    out_residual may be residual itself.  h is rounded to x's type only as it is
-    stored.  Reference: dsa_layer.py:32-52 RMSNorm.
+    out_residual may be residual itself; otherwise outputs must not overlap
+    inputs.  h is rounded to x's type only as it is stored.
+    Reference: dsa_layer.py:32-52 RMSNorm.
     """
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    else:
-        _dev(out)
-        _need_shape("out", out, x.shape, x.dtype)
-    h = _norm(x, weight, eps, residual, out, None, None, 0, out_residual)
-    return out if residual is None else (out, h)
+    res = _norm(x, weight, eps, residual, (out,), 0, out_residual)
+    return res[0] if residual is None else tuple(res)
 
 
 def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
@@ -586,22 +604,7 @@ def rms_norm_quant(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, res
     """
     if group not in (0, 128):
         raise RuntimeError(f"group must be 128 or 0, got {group}")
-    shape = x.shape
-    if not shape:
-        raise RuntimeError("x must be [..., D]")
-    sshape = (*shape[:-1], -(-shape[-1] // 128) if group else 1)
-    if out_q is None:
-        out_q = torch.empty(shape, dtype=torch.uint8, device=x.device)
-    else:
-        _dev(out_q)
-        _need_shape("out_q", out_q, shape, torch.uint8)
-    if out_scale is None:
-        out_scale = torch.empty(sshape, dtype=torch.float32, device=x.device)
-    else:
-        _dev(out_scale)
-        _need_shape("out_scale", out_scale, sshape, torch.float32)
-    h = _norm(x, weight, eps, residual, None, out_q, out_scale, group, out_residual)
-    return (out_q, out_scale) if residual is None else (out_q, out_scale, h)
+    return tuple(_norm(x, weight, eps, residual, (out_q, out_scale), group, out_residual))
 
 
 def rotary(x: torch.Tensor, pos: torch.Tensor, cos_sin: torch.Tensor, interleaved: bool = False, start: int = 0,
@@ -618,50 +621,54 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, cos_sin: torch.Tensor, interleave
     token whose position is not in the table (padding, say -1) is not turned.
     Reference: rope.py:25-84 apply_rotary.
     """
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise RuntimeError("lagged_indexer_dsa_amd ops need GPU (HIP) tensors; there is no CPU path")
-    _dev(pos, cos_sin)
-    shape = x.shape
+    shape, dt, st, pt = x.shape, x.dtype, x.stride(), pos.dtype
+    dev = x.get_device()
+    _here(dev, pos, cos_sin, out)
     if len(shape) == 3:
         n, H, D = shape
-        xn, xh, xd = x.stride()
+        xn, xh, xd = st
     elif len(shape) == 2:
         (n, D), H = shape, 1
-        xn, xd = x.stride()
-        xh = 0
+        (xn, xd), xh = st, 0
     else:
         raise RuntimeError(f"x must be [n, H, D] or [n, D], got {tuple(shape)}")
-    if x.dtype not in _PACK_DTYPES:
-        raise RuntimeError(f"x must be float32, bfloat16 or float16, got {x.dtype}")
-    if pos.shape != (n,) or pos.dtype not in (torch.int32, torch.int64):
-        raise RuntimeError(f"pos must be [{n}] int32 or int64, got {pos.dtype} {tuple(pos.shape)}")
-    if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32:
-        raise RuntimeError("cos_sin must be [positions, R] float32")
-    P, R = cos_sin.shape
+    dtype = _PACK_DTYPES.get(dt)
+    if dtype is None:
+        raise RuntimeError(f"x must be float32, bfloat16 or float16, got {dt}")
+    if pos.shape != (n,) or (pt != torch.int32 and pt != torch.int64) or not pos.is_contiguous():
+        raise RuntimeError(f"pos must be contiguous [{n}] int32 or int64, got {pt} {tuple(pos.shape)}")
+    table = cos_sin.shape
+    if len(table) != 2 or cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous():
+        raise RuntimeError("cos_sin must be contiguous [positions, R] float32")
+    P, R = table
     if R < 2 or R % 2 or start < 0 or start + R > D or P < 1:
         raise RuntimeError(f"a table of {P} positions and {R} values does not fit values {start} on of {D}")
-    if D > 1 and xd != 1:
+    if xd != 1 and D > 1:
         raise RuntimeError("x's last dimension must be contiguous")
+    xp = x.data_ptr()
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
-    elif out.shape != shape or out.dtype != x.dtype:
-        raise RuntimeError(f"out must be {x.dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
-    _here(x, pos, cos_sin, out)
-    on, oh = (out.stride(0), out.stride(1)) if len(shape) == 3 else (out.stride(0), 0)
-    if D > 1 and out.stride(-1) != 1:
-        raise RuntimeError("out's last dimension must be contiguous")
-    if n == 0 or H == 0:
-        return out
-    # no two heads of out at one place: the larger stride steps over the others
-    (small, ns), (large, nl) = sorted(((on, n), (oh, H)))
-    if (ns > 1 and small < D) or (nl > 1 and large < (ns - 1) * small + D):
-        raise RuntimeError(f"out's heads overlap (strides {out.stride()})")
-    same = out.data_ptr() == x.data_ptr()
-    if same and (on, oh) != (xn, xh):
-        raise RuntimeError("out is x with other strides")
-    _need_apart("out", out, pos, cos_sin, *(() if same else (x,)))
-    _lib.call("dsa_rotary", x.data_ptr(), _PACK_DTYPES[x.dtype], xn, xh, pos.data_ptr(), pos.element_size(),
-              cos_sin.data_ptr(), P, out.data_ptr(), on, oh, n, H, D, R, start, interleaved, inverse, _stream())
+        out = torch.empty(shape, dtype=dt, device=x.device)
+        on, oh = H * D, D
+    else:
+        if out.shape != shape or out.dtype != dt:
+            raise RuntimeError(f"out must be {dt} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
+        ot = out.stride()
+        if ot[-1] != 1 and D > 1:
+            raise RuntimeError("out's last dimension must be contiguous")
+        on, oh = (ot[0], ot[1]) if len(shape) == 3 else (ot[0], 0)
+        # no two heads of out at one place: the larger stride steps over the others
+        (small, ns), (large, nl) = ((on, n), (oh, H)) if on < oh else ((oh, H), (on, n))
+        if (ns > 1 and small < D) or (nl > 1 and large < (ns - 1) * small + D):
+            raise RuntimeError(f"out's heads overlap (strides {ot})")
+        if n and H:
+            same = out.data_ptr() == xp
+            if same and (on, oh) != (xn, xh):
+                raise RuntimeError("out is x with other strides")
+            _need_apart("out", out, pos, cos_sin, None if same else x)
+    if n and H:
+        a = _lib.ROTARY_ARGS.pack(xp, pos.data_ptr(), cos_sin.data_ptr(), out.data_ptr(), xn, xh, on, oh, P, n, H, D, R,
+                                  start, dtype, 4 if pt == torch.int32 else 8, interleaved, inverse)
+        _lib.call("dsa_rotary", a, torch._C._cuda_getCurrentRawStream(dev))
     return out
 
 
@@ -685,60 +692,64 @@ def append_tokens(page_table: torch.Tensor, rows: torch.Tensor, pos: torch.Tenso
     one slot must hold the same values.
     Reference: sglang overlay P:252-363, P:789; dsa_layer.py:92-143.
     """
-    _dev(page_table, rows, pos)
-    n = rows.shape[0] if rows.dim() == 1 else -1
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or not page_table.numel():
-        raise RuntimeError("page_table must be [B, pt_stride] int32")
-    if n < 0 or rows.dtype != torch.int32:
-        raise RuntimeError("rows must be [n] int32")
-    _need_shape("pos", pos, (n,), torch.int32)
-    if latent is None and keys is None:
-        raise RuntimeError("append_tokens needs a latent, keys or both")
-    if (latent is None) != (kv_pool is None) or (keys is None) != (index_k is None):
-        raise RuntimeError("latent goes with kv_pool, keys with index_k")
-    ls = ks = row_bytes = kv_rows = pages = table_rows = w_dtype = 0
-    dtype = (keys if latent is None else latent).dtype
-    if dtype not in _PACK_DTYPES:
-        raise RuntimeError(f"latent and keys must be float32, bfloat16 or float16, got {dtype}")
+    dev = rows.get_device()
+    _here(dev, page_table, pos, kv_pool, latent, index_k, keys, cos_sin, norm_weight)
+    pts = page_table.shape
+    if len(pts) != 2 or 0 in pts or page_table.dtype != torch.int32 or not page_table.is_contiguous():
+        raise RuntimeError("page_table must be contiguous [B, pt_stride] int32")
+    n = rows.numel()
+    if rows.shape != (n,) or rows.dtype != torch.int32 or not rows.is_contiguous():
+        raise RuntimeError("rows must be contiguous [n] int32")
+    if pos.shape != (n,) or pos.dtype != torch.int32 or not pos.is_contiguous():
+        raise RuntimeError(f"pos must be contiguous [{n}] int32")
+    if (latent is None) != (kv_pool is None) or (keys is None) != (index_k is None) or (latent is None and keys is None):
+        raise RuntimeError("latent goes with kv_pool, keys with index_k, and one of them is needed")
+    dt = (keys if latent is None else latent).dtype
+    dtype = _PACK_DTYPES.get(dt)
+    if dtype is None:
+        raise RuntimeError(f"latent and keys must be float32, bfloat16 or float16, got {dt}")
+    lp = ls = wp = wt = pp = kv_rows = row_bytes = kp = ks = ip = pages = tp = table_rows = 0
     if latent is not None:
-        ls = _append_rows("latent", latent, n, QK_DIM, dtype)
-        _dev(kv_pool)
-        kv_rows, row_bytes = kv_pool.shape if kv_pool.dim() == 2 else (0, 0)
-        if row_bytes not in (LATENT_ROW_BYTES, FP4_ROW_BYTES) or kv_pool.dtype != torch.uint8 or not kv_rows:
-            raise RuntimeError("kv_pool must be [rows, 656] or [rows, 400] uint8")
+        ls, lp = _append_rows("latent", latent, n, QK_DIM, dt), latent.data_ptr()
+        pool = kv_pool.shape
+        kv_rows, row_bytes = pool if len(pool) == 2 else (0, 0)
+        if (row_bytes != LATENT_ROW_BYTES and row_bytes != FP4_ROW_BYTES) or not kv_rows or kv_pool.dtype != torch.uint8 \
+                or not kv_pool.is_contiguous():
+            raise RuntimeError("kv_pool must be contiguous [rows, 656] or [rows, 400] uint8")
+        pp = kv_pool.data_ptr()
         if norm_weight is not None:
-            _dev(norm_weight)
-            if norm_weight.shape != (LATENT_DIM,) or norm_weight.dtype not in (dtype, torch.float32):
+            nt = norm_weight.dtype
+            if norm_weight.shape != (LATENT_DIM,) or (nt != dt and nt != torch.float32) or not norm_weight.is_contiguous():
                 raise RuntimeError("norm_weight must be [512] of the latent's type or float32")
-            w_dtype = _PACK_DTYPES[norm_weight.dtype]
+            wp, wt = norm_weight.data_ptr(), _PACK_DTYPES[nt]
     elif norm_weight is not None:
         raise RuntimeError("norm_weight without a latent")
     if keys is not None:
-        ks = _append_rows("keys", keys, n, INDEX_DIM, dtype)
-        _dev(index_k)
-        if index_k.dim() != 2 or index_k.shape[1] != INDEX_PAGE_BYTES or index_k.dtype != torch.uint8 or not len(index_k):
-            raise RuntimeError("index_k must be [pages, 8448] uint8")
-        pages = index_k.shape[0]
+        ks, kp = _append_rows("keys", keys, n, INDEX_DIM, dt), keys.data_ptr()
+        idx = index_k.shape
+        if len(idx) != 2 or idx[1] != INDEX_PAGE_BYTES or not idx[0] or index_k.dtype != torch.uint8 \
+                or not index_k.is_contiguous():
+            raise RuntimeError("index_k must be contiguous [pages, 8448] uint8")
+        ip, pages = index_k.data_ptr(), idx[0]
     if cos_sin is not None:
-        _dev(cos_sin)
-        if cos_sin.dim() != 2 or cos_sin.shape[1] != ROPE_DIM or cos_sin.dtype != torch.float32 or not len(cos_sin):
-            raise RuntimeError("cos_sin must be [positions, 64] float32")
-        table_rows = cos_sin.shape[0]
-    _here(page_table, rows, pos, kv_pool, latent, index_k, keys, cos_sin, norm_weight)
-    _lib.call("dsa_append_tokens", rows.data_ptr(), pos.data_ptr(), n, page_table.data_ptr(), page_table.shape[0],
-              page_table.shape[1], _ptr(cos_sin), table_rows, _PACK_DTYPES[dtype], _ptr(latent), ls,
-              _ptr(norm_weight), w_dtype, eps, interleaved, _ptr(kv_pool), kv_rows, row_bytes, _ptr(keys), ks,
-              index_interleaved, _ptr(index_k), pages, _stream())
+        table = cos_sin.shape
+        if len(table) != 2 or table[1] != ROPE_DIM or not table[0] or cos_sin.dtype != torch.float32 \
+                or not cos_sin.is_contiguous():
+            raise RuntimeError("cos_sin must be contiguous [positions, 64] float32")
+        tp, table_rows = cos_sin.data_ptr(), table[0]
+    a = _lib.APPEND_ARGS.pack(rows.data_ptr(), pos.data_ptr(), page_table.data_ptr(), tp, lp, wp, pp, kp, ip, table_rows,
+                              ls, kv_rows, ks, pages, eps, n, pts[0], pts[1], dtype, wt, row_bytes, interleaved,
+                              index_interleaved)
+    _lib.call("dsa_append_tokens", a, torch._C._cuda_getCurrentRawStream(dev))
 
 
 def _append_rows(name: str, x: torch.Tensor, n: int, width: int, dtype) -> int:
     """The row stride of an append's input."""
-    if not isinstance(x, torch.Tensor) or not x.is_cuda:
-        raise RuntimeError("lagged_indexer_dsa_amd ops need GPU (HIP) tensors; there is no CPU path")
-    if x.shape != (n, width) or x.dtype != dtype or x.stride(1) != 1:
+    st = x.stride()
+    if x.shape != (n, width) or x.dtype != dtype or st[1] != 1:
         raise RuntimeError(f"{name} must be {dtype} [{n}, {width}] with a contiguous last dimension, got {x.dtype} "
                            f"{tuple(x.shape)}")
-    return x.stride(0)
+    return st[0]
 
 
 def read_latent_rows(kv_pool: torch.Tensor, slots: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -747,19 +758,20 @@ def read_latent_rows(kv_pool: torch.Tensor, slots: torch.Tensor, out: torch.Tens
     400-byte rows.  With them the prefill ops attend a cached prefix.  A slot
     outside the pool gives zeros.  Reference: P:789 dequantize_k_cache.
     """
-    _dev(kv_pool, slots)
-    kv_rows, row_bytes = kv_pool.shape if kv_pool.dim() == 2 else (0, 0)
-    if row_bytes not in (LATENT_ROW_BYTES, FP4_ROW_BYTES) or kv_pool.dtype != torch.uint8 or not kv_rows:
-        raise RuntimeError("kv_pool must be [rows, 656] or [rows, 400] uint8")
-    if slots.dim() != 1 or slots.dtype != torch.int32:
-        raise RuntimeError("slots must be [n] int32")
-    n = slots.shape[0]
+    dev = kv_pool.get_device()
+    _here(dev, slots, out)
+    pool = kv_pool.shape
+    kv_rows, row_bytes = pool if len(pool) == 2 else (0, 0)
+    if (row_bytes != LATENT_ROW_BYTES and row_bytes != FP4_ROW_BYTES) or not kv_rows or kv_pool.dtype != torch.uint8 \
+            or not kv_pool.is_contiguous():
+        raise RuntimeError("kv_pool must be contiguous [rows, 656] or [rows, 400] uint8")
+    n = slots.numel()
+    if slots.shape != (n,) or slots.dtype != torch.int32 or not slots.is_contiguous():
+        raise RuntimeError("slots must be contiguous [n] int32")
     if out is None:
         out = torch.empty(n, QK_DIM, dtype=torch.bfloat16, device=kv_pool.device)
     else:
-        _dev(out)
         _need_shape("out", out, (n, QK_DIM), torch.bfloat16)
-    _here(kv_pool, slots, out)
     _lib.call("dsa_read_latent_rows", kv_pool.data_ptr(), kv_rows, row_bytes, slots.data_ptr(), n, out.data_ptr(),
-              _stream())
+              torch._C._cuda_getCurrentRawStream(dev))
     return out

@@ -443,9 +443,16 @@ int dsa_prefill_attention(const void* q_bf16, const void* keys, const uint32_t* 
  * Replaces: RMSNorm (dsa_layer.py:32-52) and the act_quant before an fp8
  * product (inference/modeling/kernels.py:35-117; this library's scale rule).
  */
-int dsa_rms_norm(const void* x, int dtype, int64_t x_stride, const void* residual, int64_t residual_stride,
-                 const void* weight, int weight_dtype, double eps, void* y, void* codes, float* scales, int group,
-                 void* residual_out, int64_t residual_out_stride, int n, int D, void* stream);
+typedef struct dsa_norm_args {
+  const void *x, *residual, *weight; /* residual may be NULL */
+  void *y, *codes;                   /* one of them */
+  float* scales;                     /* with codes */
+  void* residual_out;                /* may be NULL */
+  int64_t x_stride, residual_stride, residual_out_stride;
+  double eps;
+  int n, D, dtype, weight_dtype, group;
+} dsa_norm_args;
+int dsa_rms_norm(const dsa_norm_args* args, void* stream);
 
 /*
  * (9) Rotary positions: values start .. start + R - 1 of every head of x
@@ -459,9 +466,14 @@ int dsa_rms_norm(const void* x, int dtype, int64_t x_stride, const void* residua
  *   whose position is outside the table is padding: not turned.
  * Replaces: apply_rotary (rope.py:25-84).
  */
-int dsa_rotary(const void* x, int dtype, int64_t x_token_stride, int64_t x_head_stride, const void* pos, int pos_bytes,
-               const float* cos_sin, int64_t max_pos, void* out, int64_t out_token_stride, int64_t out_head_stride,
-               int n, int H, int D, int R, int start, int interleaved, int inverse, void* stream);
+typedef struct dsa_rotary_args {
+  const void *x, *pos;
+  const float* cos_sin;
+  void* out;
+  int64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride, max_pos;
+  int n, H, D, R, start, dtype, pos_bytes, interleaved, inverse;
+} dsa_rotary_args;
+int dsa_rotary(const dsa_rotary_args* args, void* stream);
 
 /*
  * (10) Append new tokens to the paged caches in one launch.  Token i belongs
@@ -484,11 +496,18 @@ int dsa_rotary(const void* x, int dtype, int64_t x_token_stride, int64_t x_head_
  * Replaces: forward_hide_operands' key side (P:252-363, P:789) with the norm
  * and rope before it (DL:92-143).
  */
-int dsa_append_tokens(const int32_t* rows, const int32_t* pos, int n, const int32_t* page_table, int B, int pt_stride,
-                      const float* cos_sin, int64_t table_rows, int dtype, const void* latent, int64_t latent_stride,
-                      const void* norm_weight, int norm_weight_dtype, double eps, int interleaved, void* kv_pool,
-                      int64_t kv_rows, int row_bytes, const void* keys, int64_t keys_stride, int index_interleaved,
-                      void* index_k, int64_t num_pages, void* stream);
+typedef struct dsa_append_args {
+  const int32_t *rows, *pos, *page_table; /* [n], [n], [B, pt_stride] */
+  const float* cos_sin;
+  const void *latent, *norm_weight;
+  void* kv_pool;
+  const void* keys;
+  void* index_k;
+  int64_t table_rows, latent_stride, kv_rows, keys_stride, num_pages;
+  double eps;
+  int n, B, pt_stride, dtype, norm_weight_dtype, row_bytes, interleaved, index_interleaved;
+} dsa_append_args;
+int dsa_append_tokens(const dsa_append_args* args, void* stream);
 
 /*
  * (11) Latent rows as values: out [n, 576] bf16 = the 512 dequantised values

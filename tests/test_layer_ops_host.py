@@ -6,6 +6,8 @@ checks, which answer before anything is launched."""
 from __future__ import annotations
 
 import math
+import shutil
+import subprocess
 
 import numpy as np
 import pytest
@@ -162,11 +164,30 @@ def test_decode_layer_refuses_4bit_pool():
                     seq_lens=torch.zeros(1, dtype=torch.int32), slab_stride=64)
 
 
+def test_packed_arguments_are_the_headers_structures(tmp_path):
+    """The Python side packs the argument structures field by field: their
+    sizes and last fields' places as a C compiler lays out the header."""
+    from conftest import REPO
+    from lagged_indexer_dsa_amd._lib import APPEND_ARGS, NORM_ARGS, ROTARY_ARGS
+
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if not cc:
+        pytest.skip("no C compiler")
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stddef.h>\n#include "dsa_mli.h"\n' + "".join(
+        f'_Static_assert(sizeof({t}) == {p.size} && offsetof({t}, {f}) == {at}, "{t}");\n'
+        for t, p, f, at in (("dsa_norm_args", NORM_ARGS, "group", 104), ("dsa_rotary_args", ROTARY_ARGS, "inverse", 104),
+                            ("dsa_append_args", APPEND_ARGS, "index_interleaved", 148))))
+    subprocess.run([cc, "-std=c11", "-fsyntax-only", f"-I{REPO / 'include'}", str(src)], check=True)
+
+
 def test_norm_contract(lib):
-    from lagged_indexer_dsa_amd._lib import DSA_ERR_INVALID_ARG, DSA_ERR_UNSUPPORTED, DSA_OK
+    from lagged_indexer_dsa_amd._lib import NORM_ARGS, DSA_ERR_INVALID_ARG, DSA_ERR_UNSUPPORTED, DSA_OK
 
     def call(x=16, dt=1, xs=64, r=None, rs=0, w=16, wd=1, y=16, c=None, s=None, g=0, h=None, hs=0, n=2, D=64):
-        return lib.dsa_rms_norm(x, dt, xs, r, rs, w, wd, 1e-6, y, c, s, g, h, hs, n, D, None)
+        p = [v or 0 for v in (x, r, w, y, c, s, h)]
+        return lib.dsa_rms_norm(NORM_ARGS.pack(*p, xs, rs, hs, 1e-6, n, D, dt, wd, g), None)
+    assert lib.dsa_rms_norm(None, None) == DSA_ERR_INVALID_ARG
     assert call(n=0, x=None) == DSA_OK
     for kw in (dict(n=-1), dict(x=None), dict(w=None), dict(y=None), dict(c=16), dict(y=None, c=16), dict(dt=3),
                dict(wd=2), dict(h=16), dict(r=16, rs=64, h=16, hs=63), dict(xs=-64)):
@@ -177,10 +198,12 @@ def test_norm_contract(lib):
 
 
 def test_rotary_contract(lib):
-    from lagged_indexer_dsa_amd._lib import DSA_ERR_INVALID_ARG, DSA_ERR_UNSUPPORTED, DSA_OK
+    from lagged_indexer_dsa_amd._lib import ROTARY_ARGS, DSA_ERR_INVALID_ARG, DSA_ERR_UNSUPPORTED, DSA_OK
 
     def call(x=16, dt=1, pos=16, pb=4, t=16, P=8, o=16, n=2, H=2, D=64, R=64, start=0):
-        return lib.dsa_rotary(x, dt, H * D, D, pos, pb, t, P, o, H * D, D, n, H, D, R, start, 0, 0, None)
+        p = [v or 0 for v in (x, pos, t, o)]
+        return lib.dsa_rotary(ROTARY_ARGS.pack(*p, H * D, D, H * D, D, P, n, H, D, R, start, dt, pb, 0, 0), None)
+    assert lib.dsa_rotary(None, None) == DSA_ERR_INVALID_ARG
     assert call(n=0, x=None) == DSA_OK
     for kw in (dict(n=-1), dict(x=None), dict(pos=None), dict(t=None), dict(o=None), dict(dt=5), dict(pb=2), dict(P=0),
                dict(R=0), dict(R=63), dict(R=66), dict(start=2), dict(start=-2, R=32), dict(D=65538)):
@@ -190,12 +213,13 @@ def test_rotary_contract(lib):
 
 
 def test_append_and_read_contract(lib):
-    from lagged_indexer_dsa_amd._lib import DSA_ERR_INVALID_ARG, DSA_ERR_UNSUPPORTED, DSA_OK
+    from lagged_indexer_dsa_amd._lib import APPEND_ARGS, DSA_ERR_INVALID_ARG, DSA_ERR_UNSUPPORTED, DSA_OK
 
     def call(rows=16, pos=16, n=2, pt=16, B=1, pts=4, cs=16, cr=8, dt=1, lat=16, ls=576, w=None, wd=0, pool=16, kv=64,
              rb=656, k=16, ks=128, idx=16, pages=1):
-        return lib.dsa_append_tokens(rows, pos, n, pt, B, pts, cs, cr, dt, lat, ls, w, wd, 1e-6, 0, pool, kv, rb, k, ks, 0,
-                                     idx, pages, None)
+        p = [v or 0 for v in (rows, pos, pt, cs, lat, w, pool, k, idx)]
+        return lib.dsa_append_tokens(APPEND_ARGS.pack(*p, cr, ls, kv, ks, pages, 1e-6, n, B, pts, dt, wd, rb, 0, 0), None)
+    assert lib.dsa_append_tokens(None, None) == DSA_ERR_INVALID_ARG
     assert call(n=0, rows=None) == DSA_OK
     for kw in (dict(n=-1), dict(rows=None), dict(pos=None), dict(pt=None), dict(lat=None, k=None), dict(B=0), dict(pts=0),
                dict(cr=0), dict(dt=3), dict(w=16, wd=2), dict(pool=None), dict(kv=0), dict(pool=24), dict(idx=None),
