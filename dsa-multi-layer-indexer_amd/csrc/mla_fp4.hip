@@ -218,7 +218,7 @@ __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A
   if (wave >= 4 && tiles) e0 = entry(0), e1 = entry(1), e2 = entry(2), e3 = entry(3);
   // the queries' way in: lines of 64 bytes of 16 heads
   const uint8_t* qsrc = reinterpret_cast<const uint8_t*>(A.q) + (long)b * A.H * (DSA_QK_DIM * 2) + p16;
-  #pragma unroll
+#pragma unroll
   for (int k = 0; k < (2 * kM4QLines + 7) / 8; ++k) {
     const int x = wave + 8 * k;
     if (x >= 2 * kM4QLines) break;
@@ -540,12 +540,17 @@ __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A
   }
 }
 
-// The chunks of a row meet: a workgroup takes 64 of the items (quad, half,
-// head) of a (row, head block), a lane each; its waves take the chunks in turn,
-// and their sums meet in LDS.  Always in the same order.
-constexpr int kM4Quads = DSA_LATENT_DIM / 8;
+// The chunks of a row meet: a workgroup takes 8 heads x 8 of the 128 pieces of
+// four dims (64 bytes of each head's output), a lane each; its waves take the
+// chunks in turn, and their sums meet in LDS.  Always in the same order.
+//
+// Bound by the partial sums it reads, 64 KB a chunk and 32 heads: 16.8 MB and
+// 8.4 us after 64 chunks of 128 heads (a fifth of that is the ragged rows'
+// plan), 2.8 us for 16 chunks of 16 heads.  16 waves a workgroup where a row has
+// many chunks (42 each: 7.1 us), else 4 (16 waves took 4.2 us for 16 chunks).
+constexpr int kM4Quads = DSA_LATENT_DIM / 8;  // of eight dims, two pieces each
 constexpr int kM4MergeAhead = 4;
-constexpr int kM4MergeFew = 16;  // chunks of a row (on average) that 4 waves take
+constexpr int kM4MergeFew = 16;  // chunks of a row, on average, that 4 waves take
 
 template <int W>
 __global__ __launch_bounds__(W* kWave) void mla_fp4_merge_kernel(const Mla4Args A) {
@@ -553,7 +558,7 @@ __global__ __launch_bounds__(W* kWave) void mla_fp4_merge_kernel(const Mla4Args 
   __shared__ v4f so[W][kWave];
   const int lane = threadIdx.x & (kWave - 1), wv = wave_id();
   const int nhb = m4_blocks(A.H), heads = m4_heads(A.H), per = kM4Quads * 2 * heads / kWave;
-  const int hb = (int)(blockIdx.x / per % nhb), b = (int)(blockIdx.x / per / nhb);
+  const int hb = (int)(blockIdx.x / per), b = (int)blockIdx.y;
   const M4Plan p = m4_plan_row(A, b, lane);
   if (p.count == 1) return;  // (the same in the whole workgroup)
   const int eights = heads / 8, at8 = (int)(blockIdx.x % per);
@@ -610,8 +615,10 @@ __global__ __launch_bounds__(W* kWave) void mla_fp4_merge_kernel(const Mla4Args 
 }
 
 // Chunks the rows share: nsplit a row, or (0) what fills the chip once, one
-// workgroup a CU; at most kM4MergeMax where one row may take them all (kM4Ragged rows and
-// fewer).
+// workgroup a CU; at most kM4MergeMax where one row may take them all
+// (kM4Ragged rows and fewer).  Measured around 0's choice: 32 rows of 2048
+// selected keys, 16 heads: 26.0 us at 2 a row, 19.4 at 4, 18.5 at 8 (0's), 23.5
+// at 16; 8 rows of 16K keys, 128 heads: 76.8 at 4, 52.0 at 8 (0's), 55.8 at 16.
 static int m4_chunks(int B, int H, int nsplit) {
   const long want = nsplit > 0 ? (long)B * nsplit : (long)(device_cu_count() / m4_blocks(H));
   return (int)std::max((long)B, B <= kM4Ragged ? std::min(want, (long)kM4MergeMax) : want);
@@ -634,7 +641,7 @@ hipError_t launch_mla_fp4(Mla4Args A, int nsplit, void* workspace, hipStream_t s
   });
   if (e != hipSuccess) return e;
   const int blocks = m4_blocks(A.H);
-  const int row_units = (A.keys + kM4Unit - 1) / kM4Unit;
+  const int row_units = (A.keys - 1) / kM4Unit + 1;
   A.chunks = m4_chunks(A.B, A.H, nsplit);
   A.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + attn_workspace_bytes(A.B, A.H, 0));
   A.part_ml = A.part_o + (size_t)A.chunks * blocks * m4_heads(A.H) * DSA_LATENT_DIM;
@@ -650,10 +657,9 @@ hipError_t launch_mla_fp4(Mla4Args A, int nsplit, void* workspace, hipStream_t s
   hipLaunchKernelGGL(kernel, grid, dim3(kM4Threads), kM4Lds, s, A);
   if (hipError_t r = hipGetLastError()) return r;
   if (A.units && A.per_row == 1) return hipSuccess;
-  const int items = blocks * kM4Quads * 2 * m4_heads(A.H);  // of a row
+  const dim3 merge_grid((unsigned)(blocks * kM4Quads * 2 * m4_heads(A.H) / kWave), (unsigned)A.B);
   const bool many = (A.units ? A.per_row : A.chunks / A.B) > kM4MergeFew;
-  hipLaunchKernelGGL(many ? mla_fp4_merge_kernel<16> : mla_fp4_merge_kernel<4>, dim3((unsigned)((long)A.B * items / kWave)),
-                     dim3(kWave * (many ? 16 : 4)), 0, s, A);
+  hipLaunchKernelGGL(many ? mla_fp4_merge_kernel<16> : mla_fp4_merge_kernel<4>, merge_grid, dim3(kWave * (many ? 16 : 4)), 0, s, A);
   return hipGetLastError();
 }
 

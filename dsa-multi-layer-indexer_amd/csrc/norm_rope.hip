@@ -72,26 +72,25 @@ __device__ __forceinline__ void load_raw(const void* p, int t, int T, int D, Raw
   }
 }
 
-// A row is held by T threads, V vectors of 8 elements each (vector v of
-// thread t: elements 8 (v T + t) ..); the 16 lanes of a DPP row hold 128
+// A workgroup of T threads holds a row, V vectors of 8 elements each (vector v
+// of thread t: elements 8 (v T + t) ..); the 16 lanes of a DPP row hold 128
 // consecutive elements, one quantisation group.  WIDE: D a multiple of 8 and
-// every row on 16-byte boundaries.  ONE_WAVE: T is a wave, kNormRows rows a
-// workgroup; otherwise the workgroup is the row's T threads.  Workgroups go
-// on to further rows, with the weight in registers and the next row in
-// flight from before the reduction on.
-constexpr int kNormRows = 4;
+// every row on 16-byte boundaries.  Workgroups go on to further rows, with the
+// weight in registers and the next row in flight from before the reduction on.
+//
+// Bound by its bytes: 8191 rows of 7168 bf16 with a residual, to e4m3 with a
+// scale per 128 values, move 412 MB in 82 us, 5.0 TB/s (a large copy: 5.2).  A
+// row a workgroup, the weight read again for each: 195 us.  One token: 2.9 us,
+// a launch and two trips to memory.
 constexpr int kNormWaves = 16;  // most waves a row
 
-template <int DT, int V, bool WIDE, bool ONE_WAVE>
-__global__ __launch_bounds__(ONE_WAVE ? kNormRows* kWave : kNormWaves* kWave) void rms_norm_kernel(const NormArgs A) {
+template <int DT, int V, bool WIDE>
+__global__ __launch_bounds__(kNormWaves* kWave) void rms_norm_kernel(const NormArgs A) {
   constexpr int es = DT == kF32 ? 4 : 2;
   __shared__ float red[2][kNormWaves];
   __shared__ uint32_t redm[2][kNormWaves];
-  const int T = ONE_WAVE ? kWave : (int)blockDim.x, waves = T / kWave;
-  const int t = ONE_WAVE ? (int)threadIdx.x & (kWave - 1) : (int)threadIdx.x, D = A.D, wv = wave_id();
-  const long stride = (long)gridDim.x * (ONE_WAVE ? kNormRows : 1);
-  long row = (long)blockIdx.x * (ONE_WAVE ? kNormRows : 1) + (ONE_WAVE ? wv : 0);
-  if (row >= A.n) return;  // (whole rows' threads)
+  const int T = (int)blockDim.x, waves = T / kWave, t = (int)threadIdx.x, D = A.D, wv = wave_id();
+  long row = blockIdx.x;
   const auto at = [&](const void* p, long r, long rs) { return static_cast<const uint8_t*>(p) + r * rs * es; };
   RawRow<DT, V> x, r;
   if constexpr (WIDE) {
@@ -115,7 +114,7 @@ __global__ __launch_bounds__(ONE_WAVE ? kNormRows* kWave : kNormWaves* kWave) vo
         w[v][e] = i + e >= D ? 0.f : A.w_f32 ? load_elem<kF32>(A.w, i + e) : load_elem<DT>(A.w, i + e);
     }
   }
-  for (int par = 0; row < A.n; row += stride, par ^= 1) {
+  for (int par = 0; row < A.n; row += gridDim.x, par ^= 1) {
     float h[V][8];
     float ss = 0.f;
 #pragma unroll
@@ -144,13 +143,13 @@ __global__ __launch_bounds__(ONE_WAVE ? kNormRows* kWave : kNormWaves* kWave) vo
       if (A.h && (!WIDE || i < D)) store8<DT, WIDE>(A.h, row * A.hs + i, h[v], row * A.hs + D);
     }
     if constexpr (WIDE) {
-      if (const long next = row + stride; next < A.n) {
+      if (const long next = row + gridDim.x; next < A.n) {
         load_raw<DT, V>(at(A.x, next, A.xs), t, T, D, x);
         if (A.r) load_raw<DT, V>(at(A.r, next, A.rs), t, T, D, r);
       }
     }
     ss = wave_sum(ss);
-    if (!ONE_WAVE && waves > 1) {
+    if (waves > 1) {
       if ((t & (kWave - 1)) == 0) red[par][wv] = ss;
       __syncthreads();
       ss = 0.f;
@@ -174,7 +173,7 @@ __global__ __launch_bounds__(ONE_WAVE ? kNormRows* kWave : kNormWaves* kWave) vo
 #pragma unroll
       for (int v = 0; v < V; ++v) am = max(am, amax_bits<true>(h[v]));
       am = wave_reduce<2>(am);
-      if (!ONE_WAVE && waves > 1) {
+      if (waves > 1) {
         if ((t & (kWave - 1)) == 0) redm[par][wv] = am;
         __syncthreads();
         for (int k = 0; k < waves; ++k) am = max(am, redm[par][k]);
@@ -200,14 +199,13 @@ __global__ __launch_bounds__(ONE_WAVE ? kNormRows* kWave : kNormWaves* kWave) vo
   }
 }
 
-template <int DT, int V, bool ONE_WAVE>
+template <int DT, int V>
 static hipError_t launch_norm(const NormArgs& A, bool wide, hipStream_t s) {
   const int vecs = (A.D + 7) / 8;
-  const int threads = ONE_WAVE ? kNormRows * kWave : ((vecs + V - 1) / V + kWave - 1) / kWave * kWave;
-  const long blocks = ONE_WAVE ? ((long)A.n + kNormRows - 1) / kNormRows : A.n;
+  const int threads = ((vecs + V - 1) / V + kWave - 1) / kWave * kWave;
   const long most = (long)device_cu_count() * (2048 / threads);  // what is resident at once
-  const auto kernel = wide ? rms_norm_kernel<DT, V, true, ONE_WAVE> : rms_norm_kernel<DT, V, false, ONE_WAVE>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(threads), 0, s, A);
+  const auto kernel = wide ? rms_norm_kernel<DT, V, true> : rms_norm_kernel<DT, V, false>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)std::min((long)A.n, most)), dim3(threads), 0, s, A);
   return hipGetLastError();
 }
 
@@ -217,10 +215,11 @@ static hipError_t launch_norm_dim(const NormArgs& A, hipStream_t s) {
   const auto on16 = [](const void* p, long stride) { return (((uintptr_t)p | (uintptr_t)(stride * es)) & 15) == 0; };
   const bool wide = A.D % 8 == 0 && on16(A.x, A.xs) && (!A.r || on16(A.r, A.rs)) && (!A.h || on16(A.h, A.hs)) &&
                     (!A.y || on16(A.y, 0)) && ((uintptr_t)A.codes & 7) == 0 && on16(A.w, 0);
-  if (A.D <= 512) return launch_norm<DT, 1, true>(A, wide, s);
-  if (A.D <= 8192) return launch_norm<DT, 1, false>(A, wide, s);
-  if (A.D <= 16384) return launch_norm<DT, 2, false>(A, wide, s);
-  return launch_norm<DT, 4, false>(A, wide, s);
+  // the fewest vectors a thread that 1024 threads allow: 7168 values in one
+  // (896 threads) 82.8 us, in two 84.8, in four 108.7 (8191 rows, as above)
+  if (A.D <= 8192) return launch_norm<DT, 1>(A, wide, s);
+  if (A.D <= 16384) return launch_norm<DT, 2>(A, wide, s);
+  return launch_norm<DT, 4>(A, wide, s);
 }
 
 hipError_t launch_rms_norm(const NormArgs& A, int dtype, hipStream_t s) {
@@ -238,6 +237,11 @@ hipError_t launch_rms_norm(const NormArgs& A, int dtype, hipStream_t s) {
 // one by one).  A thread keeps its item and goes through heads, kRopeBatch at
 // a time, so that the table is read once for all of them and several loads
 // are in flight.
+//
+// Bound by its bytes: 64 values of each of 128 heads of 4097 tokens, 384 bytes
+// apart on the way in, take 32 us for 134 MB (4.2 TB/s).  One item a thread,
+// the table read again for every head: 44 us; batches of 1, 2 and 8 heads:
+// 33.0, 32.4 and 32.6.  32 tokens of 16 heads: 3.1 us, a launch and its latency.
 constexpr int kRopeThreads = 256, kRopeBatch = 4;
 
 template <int DT, bool WIDE, bool INTER>
@@ -336,7 +340,8 @@ static hipError_t launch_rotary_dt(RopeArgs A, hipStream_t s) {
   A.heads = items >= kRopeThreads ? 1 : std::min(A.H, kRopeThreads / items);
   A.tokens = std::max(1, kRopeThreads / (A.heads * items));
   const long x = ((long)A.n + A.tokens - 1) / A.tokens;
-  // few tokens: their heads over several workgroups
+  // few tokens: their heads over several workgroups (a token of 128 heads of
+  // 192 values: 3.4 us; in one workgroup 6.3)
   const int turns = (A.H + A.heads - 1) / A.heads;
   const int y = (int)std::max(1L, std::min({(long)turns, 65535L, 2L * device_cu_count() / x}));
   const dim3 grid((unsigned)x, (unsigned)y);

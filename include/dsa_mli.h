@@ -524,8 +524,8 @@ int dsa_read_latent_rows(const void* kv_pool, int64_t kv_rows, int row_bytes, co
  * that overlap in time must not share it.  A workspace large enough for both
  * may serve (3), (3a) and these in turn: the barriers at its start are left as
  * they are.  nsplit: the chunks of keys a row is
- * cut into, 1 to 128 (0: what fills the device once); dense rows (up to 256)
- * share B * nsplit chunks by their lengths, so where a row is cut, and the
+ * cut into, 1 to 128 (0: what fills the device once); dense rows (256 or fewer)
+ * share B * nsplit chunks (512 at most) by their lengths, so where a row is cut, and the
  * last bits of its output, depend on the other rows' lengths (the same call
  * always gives the same).  No workgroup waits for another.
  */
