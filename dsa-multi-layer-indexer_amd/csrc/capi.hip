@@ -761,7 +761,8 @@ int dsa_rotary(const dsa_rotary_args* a, void* stream) {
   DSA_REQUIRE(a->dtype >= 0 && a->dtype <= 2, DSA_ERR_INVALID_ARG,
               "dsa_rotary: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
   DSA_REQUIRE(a->pos_bytes == 4 || a->pos_bytes == 8, DSA_ERR_INVALID_ARG, "dsa_rotary: pos_bytes must be 4 or 8");
-  DSA_REQUIRE(a->R >= 2 && a->R % 2 == 0 && a->start >= 0 && a->D <= 65536 && a->start + a->R <= a->D,
+  DSA_REQUIRE(a->R >= 2 && a->R % 2 == 0 && a->start >= 0 && a->D <= 65536 &&
+                  (int64_t)a->start + a->R <= a->D,
               DSA_ERR_INVALID_ARG, "dsa_rotary: %d values from %d on of a head of %d", a->R, a->start, a->D);
   DSA_REQUIRE((int64_t)a->H * a->D < ((int64_t)1 << 31), DSA_ERR_UNSUPPORTED, "dsa_rotary: H * D must be < 2^31");
   DSA_REQUIRE(a->max_pos >= 1, DSA_ERR_INVALID_ARG, "dsa_rotary: max_pos must be >= 1");

@@ -159,7 +159,7 @@ def sparse_mla_workspace(B: int, H: int, nsplit: int, device) -> torch.Tensor:
     nbytes = lib.dsa_sparse_mla_workspace_bytes(B, H, nsplit)
     if nbytes == 0:
         raise RuntimeError(f"bad sparse MLA workspace shape B={B} H={H} nsplit={nsplit}")
-    nbytes = max(nbytes, lib.dsa_mla_fp4_workspace_bytes(B, H, nsplit))
+    nbytes = max(nbytes, *(lib.dsa_mla_fp4_workspace_bytes(B, H, n) for n in (nsplit, nsplit or 128)))
     return torch.zeros(nbytes // 4, dtype=torch.float32, device=device)
 
 

@@ -128,6 +128,29 @@ def test_dense(dev, B, H, lens, nsplit):
         _check(ops.dense_mla_decode(*args[:3], over), q, O.dequant_latent_rows_fp4(rows), cut)
 
 
+@pytest.mark.parametrize("H,nsplit", [(16, 1), (48, 1), (32, 2)])
+def test_every_count_of_tiles(dev, H, nsplit):
+    """Chunks of one to nine tiles (128 keys) and their borders: the first three
+    tiles are on their way from the start, later ones follow a tile behind."""
+    from lagged_indexer_dsa_amd import ops
+
+    print(f"[fp4 tiles] {(H, nsplit)}", flush=True)
+    lens = np.array([n * 128 + d for n in range(1, 9) for d in (-1, 0, 1)], dtype=np.int32)
+    B, pts = len(lens), 17
+    rng = np.random.default_rng(H)
+    pt = rng.permutation(B * pts).reshape(B, pts).astype(np.int32)
+    rows, q = _pool(H, B * pts * 64), _q(3, B, H)
+    idx = np.full((B, int(lens.max())), -1, dtype=np.int64)
+    for b in range(B):
+        j = np.arange(lens[b])
+        idx[b, :lens[b]] = pt[b, j // 64] * 64 + j % 64
+    out = ops.dense_mla_decode(_dev(q, dev, True), _dev(rows, dev), _dev(pt, dev), _dev(lens, dev), nsplit=nsplit)
+    _check(out, q, O.dequant_latent_rows_fp4(rows), idx)
+    # the same keys as selections
+    out = ops.sparse_mla_decode(_dev(q, dev, True), _dev(rows, dev), _dev(idx.astype(np.int32), dev), nsplit=nsplit)
+    _check(out, q, O.dequant_latent_rows_fp4(rows), idx)
+
+
 def test_sharp_and_growing_scores(dev):
     """Scores whose maximum rises along the row by far more than the sums'
     slack, and rows where one key outweighs the others."""
@@ -214,6 +237,54 @@ def test_one_workspace_for_both_formats(dev):
         got8 = ops.sparse_mla_decode(q, p8, idx, workspace=ws)
         assert float((got8.float() - ref8.float()).abs().max()) <= 2.0 ** -6 * float(ref8.float().abs().max())
     assert _lib.sync_timeouts() == 0
+
+
+def test_graphs_on_one_workspace_and_calls_at_once(dev):
+    """Two captured calls of other sizes and formats share a workspace and are
+    replayed in turn; calls on two streams with a workspace each run together."""
+    from lagged_indexer_dsa_amd import formats as F, ops
+
+    print("[fp4] graphs", flush=True)
+    g = torch.Generator(device=dev).manual_seed(5)
+    lat, rope = torch.randn(4096, 512, device=dev, generator=g), torch.randn(4096, 64, device=dev, generator=g)
+    p4, p8 = F.pack_latent_rows_fp4(lat, rope), F.pack_latent_rows(lat, rope)
+    q = torch.randn(2, 32, 576, device=dev, generator=g).to(torch.bfloat16)
+    idx = torch.stack([torch.randperm(4096, generator=g, device=dev)[:2048] for _ in range(2)]).int()
+    pt = torch.arange(64, device=dev, dtype=torch.int32).reshape(2, 32)
+    lens = torch.tensor([2048, 700], dtype=torch.int32, device=dev)
+    ws = ops.sparse_mla_workspace(2, 32, 0, dev)
+    outs = [torch.zeros(2, 32, 512, dtype=torch.bfloat16, device=dev) for _ in range(3)]
+    calls = [lambda: ops.sparse_mla_decode(q, p4, idx, workspace=ws, out=outs[0]),
+             lambda: ops.dense_mla_decode(q, p4, pt, lens, nsplit=5, workspace=ws, out=outs[1]),
+             lambda: ops.sparse_mla_decode(q, p8, idx, nsplit=8, workspace=ws, out=outs[2])]
+    want = [f().clone() for f in calls]
+    graphs = []
+    for f in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            f()
+    for turn in range(4):
+        for o in outs:
+            o.zero_()
+        for k in (turn % 3, (turn + 1) % 3, (turn + 2) % 3):
+            graphs[k].replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w), f"turn {turn}"
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    spaces = [ops.sparse_mla_workspace(2, 32, 0, dev) for _ in streams]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k].append(ops.sparse_mla_decode(q, p4, idx, workspace=spaces[k]) if k else
+                              ops.dense_mla_decode(q, p4, pt, lens, nsplit=5, workspace=spaces[k]))
+    torch.cuda.synchronize()
+    for o in got[0]:
+        assert torch.equal(o, want[1])
+    for o in got[1]:
+        assert torch.equal(o, want[0])
 
 
 def test_refusals(dev):

@@ -206,7 +206,8 @@ def test_rotary_contract(lib):
     assert lib.dsa_rotary(None, None) == DSA_ERR_INVALID_ARG
     assert call(n=0, x=None) == DSA_OK
     for kw in (dict(n=-1), dict(x=None), dict(pos=None), dict(t=None), dict(o=None), dict(dt=5), dict(pb=2), dict(P=0),
-               dict(R=0), dict(R=63), dict(R=66), dict(start=2), dict(start=-2, R=32), dict(D=65538)):
+               dict(R=0), dict(R=63), dict(R=66), dict(start=2), dict(start=-2, R=32), dict(D=65538),
+               dict(start=2 ** 31 - 2, R=4), dict(start=4, R=2 ** 31 - 2)):
         assert call(**kw) == DSA_ERR_INVALID_ARG, kw
     assert call(H=1 << 26) == DSA_ERR_UNSUPPORTED
     assert b"dsa_rotary" in lib.dsa_last_error()
@@ -253,3 +254,14 @@ def test_fp4_mla_contract(lib):
     assert ws(1, 16, 8) == barriers + 8 * 16 * 514 * 4
     assert ws(3, 32, 8) == 3 * 2 * barriers + 24 * 32 * 514 * 4
     assert ws(2, 16, 128) >= ws(2, 16, 64) and ws(7, 16, 1) == 16
+
+
+def test_workspace_for_any_split_count(lib):
+    """The workspace of nsplit 0 holds every split count, of either format."""
+    from lagged_indexer_dsa_amd import ops
+
+    for B, H in ((1, 16), (4, 48), (5, 16), (3, 128), (6, 80)):
+        nbytes = ops.sparse_mla_workspace(B, H, 0, "cpu").numel() * 4
+        for n in range(0, 129):
+            assert nbytes >= lib.dsa_mla_fp4_workspace_bytes(B, H, n), (B, H, n)
+            assert nbytes >= lib.dsa_sparse_mla_workspace_bytes(B, H, n), (B, H, n)
