@@ -196,6 +196,7 @@ struct Mla4Args {
   // filled by the launcher
   float* part_o;         // [chunks, H, 512]
   float* part_ml;        // [chunks, H, 2]
+  int2* plan;            // [B] rows that share chunks: first chunk and their count
   int chunks, units, per_row;
 };
 size_t mla_fp4_workspace_bytes(int B, int H, int nsplit);

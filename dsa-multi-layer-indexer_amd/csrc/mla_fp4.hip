@@ -21,7 +21,7 @@
 // moving.  So a tile passes through LDS once in 4 bits: a transpose of the bf16
 // values there cost 16 clocks a KB written.
 //
-// Measured: 8 rows of 16K keys, 128 heads: 52 us in a graph, merge included.  A
+// Measured: 8 rows of 16K keys, 128 heads: 51 us in a graph, merge included.  A
 // tile takes 4.5K clocks, 2.7K of them the matrix unit's (1.9 GHz with all CUs
 // at it); the start of a chunk 4 us (entries, then rows and queries), its end
 // and the launch 4.  The same work in workgroups of 4 waves that each score and
@@ -91,91 +91,69 @@ __device__ __forceinline__ float m4_halves(float v, F op) {
   return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// The chunks of the rows, the same in every wave that asks.  Row b's keys are
-// cut into chunks of `units` * kM4Unit; their partials lie behind those of
-// the rows before it.
+// Row b's keys are cut into chunks of `units` * kM4Unit; their partials lie
+// behind those of the rows before it.
 struct M4Plan {
   int units;  // of kM4Unit keys, a chunk
   int first;  // chunk number of the row's first
-  int count;  // chunks of the row
+  int count;  // chunks of the row, at least one
 };
 
 __device__ __forceinline__ int m4_row_keys(const Mla4Args& A, int b) {
   return A.dense_pt ? max(0, min(A.dense_lens[b], A.keys)) : A.keys;
 }
 
-// Ragged rows (at most kM4Ragged) share A.chunks chunks: the smallest chunk with
-// which all rows' chunks fit, or one chunk a row.  Lane l holds rows 64k + l.
-struct M4Shares {
-  int units;                  // of kM4Unit keys, a chunk
-  uint32_t c[kM4Ragged / 64];  // chunks of the row
-};
-__device__ __forceinline__ M4Shares m4_shares(const Mla4Args& A, int lane) {
-  constexpr int kPer = kM4Ragged / 64;
-  M4Shares p;
-  uint32_t u[kPer], total = 0, longest = 0;
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    const int b = 64 * k + lane;
-    u[k] = b < A.B ? (uint32_t)(m4_row_keys(A, b) + kM4Unit - 1) / kM4Unit : 0u;
-  }
-#pragma unroll
-  for (int k = 0; k < kPer; ++k) {
-    if (64 * k >= A.B) break;
-    total += wave_reduce<0>(u[k]);
-    longest = max(longest, wave_reduce<2>(u[k]));
-  }
-  uint32_t cu = max(1u, (total + A.chunks - 1) / A.chunks);
-  // (rows' last chunks may be short, so this many fit in any case)
-  const uint32_t enough = A.chunks > A.B ? (total + A.chunks - A.B - 1) / (uint32_t)(A.chunks - A.B) : longest;
-  for (;;) {
-    uint32_t n = 0;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-      p.c[k] = 0;
-      if (64 * k >= A.B) continue;
-      p.c[k] = (u[k] + cu - 1) / cu;
-      if (cu < enough) n += wave_reduce<0>(p.c[k]);
-    }
-    if (cu >= enough || n <= (uint32_t)A.chunks) break;
-    cu = min(cu + max(1u, cu / 16), enough);
-  }
-  p.units = (int)cu;
-  return p;
-}
-
-// Row b's chunks.
-__device__ __forceinline__ M4Plan m4_plan_row(const Mla4Args& A, int b, int lane) {
-  if (A.units) return {A.units, b * A.per_row, A.per_row};  // rows of one length (selections), or a chunk a row
-  const M4Shares s = m4_shares(A, lane);
-  M4Plan p = {s.units, 0, 0};
-#pragma unroll
-  for (int k = 0; k < kM4Ragged / 64; ++k) {
-    if (64 * k > b) break;
-    p.first += (int)wave_reduce<0>(64 * k + lane < b ? s.c[k] : 0u);
-    if (b < 64 * k + 64) p.count = __builtin_amdgcn_readlane((int)s.c[k], b & 63);
-  }
-  return p;
-}
-
-// The row of chunk `id` (-1: none) and its plan.
+// The row of chunk `id` (-1: none) and its plan, the same in every wave.
+// Selections, and dense rows where there is no chunk to spare, are cut alike.
+// Other dense rows (at most kM4Ragged) share A.chunks chunks: the smallest chunk
+// with which all rows' fit.  Lane l holds rows 64k + l.
 __device__ __forceinline__ int m4_plan_chunk(const Mla4Args& A, int id, int lane, M4Plan& p) {
   if (A.units) {
     const int b = id / A.per_row;
     p = {A.units, b * A.per_row, A.per_row};
     return b < A.B ? b : -1;
   }
-  const M4Shares s = m4_shares(A, lane);
-  p.units = s.units;
+  constexpr int kPer = kM4Ragged / 64;
+  uint32_t u[kPer], c[kPer], total = 0;
+#pragma unroll
+  for (int k = 0; k < kPer; ++k) {
+    const int b = 64 * k + lane;
+    u[k] = b < A.B ? (uint32_t)(m4_row_keys(A, b) + kM4Unit - 1) / kM4Unit : 0u;
+  }
+#pragma unroll
+  for (int k = 0; k < kPer; ++k)
+    if (64 * k < A.B) total += wave_reduce<0>(u[k]);
+  const auto chunks = [&](uint32_t cu) {  // of all rows (an empty one has one too)
+    uint32_t n = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      c[k] = 64 * k + lane < A.B ? max(1u, (u[k] + cu - 1) / cu) : 0u;
+      if (64 * k < A.B) n += wave_reduce<0>(c[k]);
+    }
+    return n;
+  };
+  // the search ends at a size that fits in any case: a row's last chunk may be short
+  uint32_t lo = max(1u, (total + A.chunks - 1) / A.chunks);
+  uint32_t hi = max(lo, (total + (uint32_t)(A.chunks - A.B) - 1) / (uint32_t)(A.chunks - A.B));
+  uint32_t n = chunks(lo);
+  if (n > (uint32_t)A.chunks) {
+    while (hi - lo > 1) {  // lo does not fit, hi does
+      const uint32_t mid = (lo + hi) / 2;
+      (chunks(mid) > (uint32_t)A.chunks ? lo : hi) = mid;
+    }
+    lo = hi;
+    n = chunks(lo);
+  }
+  p.units = (int)lo;
   int before = 0;
 #pragma unroll
-  for (int k = 0; k < kM4Ragged / 64; ++k) {
+  for (int k = 0; k < kPer; ++k) {
     if (64 * k >= A.B) break;
-    const int end = before + (int)wave_scan_incl<0>(s.c[k]);
-    const uint64_t hit = __ballot(id < end && id >= end - (int)s.c[k]);
+    const int end = before + (int)wave_scan_incl<0>(c[k]);
+    const uint64_t hit = __ballot(id < end && id >= end - (int)c[k]);
     if (hit) {
       const int src = __builtin_ctzll(hit);
-      p.count = __builtin_amdgcn_readlane((int)s.c[k], src);
+      p.count = __builtin_amdgcn_readlane((int)c[k], src);
       p.first = __builtin_amdgcn_readlane(end, src) - p.count;
       return 64 * k + src;
     }
@@ -198,6 +176,7 @@ __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A
   M4Plan plan;
   const int b = m4_plan_chunk(A, id, lane, plan);
   if (b < 0) return;  // (the same in the whole workgroup)
+  if (!A.units && id == plan.first && hb == 0 && t == 0) A.plan[b] = make_int2(plan.first, plan.count);  // for the merge
   const int total = m4_row_keys(A, b);
   const long j0 = (long)(id - plan.first) * plan.units * kM4Unit;
   const uint32_t keys = (uint32_t)max(min((long)total - j0, (long)plan.units * kM4Unit), 0L);
@@ -544,10 +523,11 @@ __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A
 // four dims (64 bytes of each head's output), a lane each; its waves take the
 // chunks in turn, and their sums meet in LDS.  Always in the same order.
 //
-// Bound by the partial sums it reads, 64 KB a chunk and 32 heads: 16.8 MB and
-// 8.4 us after 64 chunks of 128 heads (a fifth of that is the ragged rows'
-// plan), 2.8 us for 16 chunks of 16 heads.  16 waves a workgroup where a row has
-// many chunks (42 each: 7.1 us), else 4 (16 waves took 4.2 us for 16 chunks).
+// Bound by the partial sums it reads, 64 KB a chunk and 32 heads: 16.8 MB in
+// 5.2 us after 64 chunks of 128 heads, 2.5 us for 16 chunks of 16 heads.  16
+// waves a workgroup where a row has many chunks (42 each: 6.3 us), else 4 (16
+// waves took 4.2 us for 16 chunks).  Workgroups that go on to further pieces:
+// 1-2 us more for split rows, 2 less for 100 rows that are not.
 constexpr int kM4Quads = DSA_LATENT_DIM / 8;  // of eight dims, two pieces each
 constexpr int kM4MergeAhead = 4;
 constexpr int kM4MergeFew = 16;  // chunks of a row, on average, that 4 waves take
@@ -559,21 +539,21 @@ __global__ __launch_bounds__(W* kWave) void mla_fp4_merge_kernel(const Mla4Args 
   const int lane = threadIdx.x & (kWave - 1), wv = wave_id();
   const int nhb = m4_blocks(A.H), heads = m4_heads(A.H), per = kM4Quads * 2 * heads / kWave;
   const int hb = (int)(blockIdx.x / per), b = (int)blockIdx.y;
-  const M4Plan p = m4_plan_row(A, b, lane);
-  if (p.count == 1) return;  // (the same in the whole workgroup)
+  const int2 plan = A.units ? make_int2(b * A.per_row, A.per_row) : A.plan[b];
+  const int first = plan.x, count = plan.y;
+  if (count == 1) return;  // (the same in the whole workgroup)
   const int eights = heads / 8, at8 = (int)(blockIdx.x % per);
   const int x = at8 % eights * 8 + (lane & 7), q = at8 / eights * 8 + (lane >> 3), head = hb * kM4Heads + x;
-  const bool in = head < A.H;
   const v4f* part = reinterpret_cast<const v4f*>(A.part_o);
   float mx = -INFINITY, L = 0.f;
   v4f acc = {0.f, 0.f, 0.f, 0.f};
-  for (int c0 = wv; c0 < p.count; c0 += W * kM4MergeAhead) {
+  for (int c0 = wv; c0 < count; c0 += W * kM4MergeAhead) {
     float m[kM4MergeAhead], l[kM4MergeAhead], next = mx;
     v4f a[kM4MergeAhead];
 #pragma unroll
     for (int k = 0; k < kM4MergeAhead; ++k) {  // (past the last: chunk c0 again, for nothing)
-      const bool have = c0 + k * W < p.count;
-      const long at = (long)(p.first + (have ? c0 + k * W : c0)) * nhb + hb;
+      const bool have = c0 + k * W < count;
+      const long at = (long)(first + (have ? c0 + k * W : c0)) * nhb + hb;
       const float2 ml = reinterpret_cast<const float2*>(A.part_ml)[at * heads + x];
       const v4f v = part[(at * (kM4Quads * 2) + q) * heads + x];
       m[k] = have ? ml.x : -INFINITY;
@@ -598,7 +578,7 @@ __global__ __launch_bounds__(W* kWave) void mla_fp4_merge_kernel(const Mla4Args 
   sl[wv][lane] = L;
   so[wv][lane] = acc;
   __syncthreads();
-  if (wv || !in) return;
+  if (wv || head >= A.H) return;
   for (int w = 1; w < W; ++w) mx = fmaxf(mx, sm[w][lane]);
   L = 0.f;
   acc = v4f{0.f, 0.f, 0.f, 0.f};
@@ -619,6 +599,10 @@ __global__ __launch_bounds__(W* kWave) void mla_fp4_merge_kernel(const Mla4Args 
 // (kM4Ragged rows and fewer).  Measured around 0's choice: 32 rows of 2048
 // selected keys, 16 heads: 26.0 us at 2 a row, 19.4 at 4, 18.5 at 8 (0's), 23.5
 // at 16; 8 rows of 16K keys, 128 heads: 76.8 at 4, 52.0 at 8 (0's), 55.8 at 16.
+// Dense rows share by length wherever there are more chunks than rows: 100 rows
+// of 64 heads, one of 16K keys and 99 of 500, take 23.8 us (a chunk each: 245);
+// 100 of 2000 keys 45.7 (39.2).  At the chip's fill, 64 rows of 128 heads, a chunk
+// a row is the default: 43.7 us for 1024 to 2048 keys, 68 with two a row.
 static int m4_chunks(int B, int H, int nsplit) {
   const long want = nsplit > 0 ? (long)B * nsplit : (long)(device_cu_count() / m4_blocks(H));
   return (int)std::max((long)B, B <= kM4Ragged ? std::min(want, (long)kM4MergeMax) : want);
@@ -628,8 +612,9 @@ static int m4_chunks(int B, int H, int nsplit) {
 // workspace, so calls over both formats may take turns with one.
 size_t mla_fp4_workspace_bytes(int B, int H, int nsplit) {
   const int chunks = m4_chunks(B, H, nsplit);
-  if (chunks / B <= 1) return 16;  // unsplit rows: none is read
-  return attn_workspace_bytes(B, H, 0) + (size_t)chunks * m4_blocks(H) * m4_heads(H) * (DSA_LATENT_DIM + 2) * sizeof(float);
+  if (chunks <= B) return 16;  // unsplit rows: none is read
+  return attn_workspace_bytes(B, H, 0) + (size_t)chunks * m4_blocks(H) * m4_heads(H) * (DSA_LATENT_DIM + 2) * sizeof(float) +
+         (size_t)B * sizeof(int2);
 }
 
 hipError_t launch_mla_fp4(Mla4Args A, int nsplit, void* workspace, hipStream_t s) {
@@ -645,9 +630,10 @@ hipError_t launch_mla_fp4(Mla4Args A, int nsplit, void* workspace, hipStream_t s
   A.chunks = m4_chunks(A.B, A.H, nsplit);
   A.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + attn_workspace_bytes(A.B, A.H, 0));
   A.part_ml = A.part_o + (size_t)A.chunks * blocks * m4_heads(A.H) * DSA_LATENT_DIM;
+  A.plan = reinterpret_cast<int2*>(A.part_ml + (size_t)A.chunks * blocks * m4_heads(A.H) * 2);
   const int per_row = A.chunks / A.B;
   int grid_chunks = A.chunks;
-  if (per_row <= 1 || !A.dense_pt || A.B > kM4Ragged) {  // the same split for every row
+  if (A.chunks <= A.B || !A.dense_pt || A.B > kM4Ragged) {  // the same split for every row
     A.units = (row_units + per_row - 1) / per_row;
     A.per_row = (row_units + A.units - 1) / A.units;
     grid_chunks = A.B * A.per_row;
