@@ -21,11 +21,12 @@
 // moving.  So a tile passes through LDS once in 4 bits: a transpose of the bf16
 // values there cost 16 clocks a KB written.
 //
-// Measured: 8 rows of 16K keys, 128 heads: 51 us in a graph, merge included.  A
-// tile takes 4.5K clocks, 2.7K of them the matrix unit's (1.9 GHz with all CUs
-// at it); the start of a chunk 4 us (entries, then rows and queries), its end
-// and the launch 4.  The same work in workgroups of 4 waves that each score and
-// then sum, two a CU: 58 us (2.9 us a tile on an idle CU, 1.9 here).  64 heads a
+// Measured: 8 rows of 16K keys, 128 heads: 50 us in a graph, merge included.  A
+// tile takes 4.4K clocks, 2.7K of them the matrix unit's, with all CUs at it
+// (which then run at 1.9 GHz: 0.98 PFLOP/s of scores and sums, four fifths of
+// what a large bf16 product reaches, besides V^T); the start of a chunk 4 us
+// (entries, then rows and queries), its end and the launch 4.  The same work in workgroups of 4 waves that each score and
+// then sum, two a CU: 58 us (2.9 us a tile on an idle CU, 1.8 here).  64 heads a
 // workgroup: a tenth fewer matrix operations, but twice the partial sums of as
 // many workgroups: 70 us.
 //
@@ -164,9 +165,9 @@ __device__ __forceinline__ int m4_plan_chunk(const Mla4Args& A, int id, int lane
 
 template <bool DENSE>
 __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A) {
-  extern __shared__ __align__(16) unsigned char smem[];  // rows | probabilities
+  extern __shared__ __align__(16) unsigned char smem[];  // three tiles' rows
   __shared__ __align__(16) float ref[2][kM4Heads][kM4Groups], wl[kM4Heads][kM4Groups];
-  __shared__ __align__(16) uint32_t there[4][4];  // a bit a key of a tile's
+  __shared__ __align__(16) uint32_t there[4][kM4Groups];  // a bit a key, of a tile and the three around it
   const int t = threadIdx.x, lane = t & (kWave - 1), wave = wave_id();
   const int n = lane & 31, h = lane >> 5;
   // a chunk's head blocks on one XCD (workgroup number modulo 8), whose L2
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A
     const uint32_t j = min((uint32_t)tl * kM4Unit + jl, keys - 1);
     return idx_row[DENSE ? j >> 6 : j];
   };
-  int e0 = 0, e1 = 0, e2 = 0, e3 = 0;
+  int e0 = 0, e1 = 0, e2 = 0, e3 = 0;  // of the next tiles
   if (wave >= 4 && tiles) e0 = entry(0), e1 = entry(1), e2 = entry(2), e3 = entry(3);
   // the queries' way in: lines of 64 bytes of 16 heads
   const uint8_t* qsrc = reinterpret_cast<const uint8_t*>(A.q) + (long)b * A.H * (DSA_QK_DIM * 2) + p16;
@@ -315,13 +316,14 @@ __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A
 
   // Sums: 128 dims of all the tile's keys and heads, a tile behind the scores;
   // and the rows' way in, a tile before them.
+  //
   // A key's slot; -1: not there (row 0 is read then, and its probability is 0).
   const auto slot = [&](int tl, int e) {
     const uint32_t j = (uint32_t)tl * kM4Unit + jl;
     const long sl = DENSE ? (long)e * DSA_PAGE_TOKENS + (j & (DSA_PAGE_TOKENS - 1)) : (long)e;
     return j < keys && e >= 0 && sl < A.kv_rows ? (int)sl : -1;
   };
-  // Tile tl's rows to LDS, 16-byte piece by piece: pieces 4k .. 4k + 3 of 16
+  // A tile's rows to LDS, 32 a wave, 16-byte piece by piece: pieces 4k .. 4k + 3 of 16
   // rows a load (64 bytes a row together), then the last pieces.  Piece q < 24
   // of row r of a group lies at m4_piece(r) + 1024 (q / 4) + 16 ((q % 4) ^ m4_swz(r)),
   // piece 24 at kM4Last + 16 r: 8 rows' reads of one piece fall on 8 bank
@@ -355,9 +357,9 @@ __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A
   };
   // s_waitcnt vmcnt(k): all but the last k loads; 13 are a tile's
   constexpr int kNone = 0x0f70, kOneTile = 0x0f7d;
-  // (a write to LDS would wait for loads to it: all three before the first)
-  const Way w0 = way(0, slot(0, e0), 0), w1 = way(1, slot(1, e1), kM4Tile), w2 = way(2, slot(2, e2), 2 * kM4Tile);
-  int sl = slot(3, e3), e = 0;
+  // (a write to LDS would wait for loads to it: both before the first)
+  const Way w0 = way(0, slot(0, e0), 0), w1 = way(1, slot(1, e1), kM4Tile);
+  int sl = slot(2, e2), e = e3;
   if (tiles) fetch(w0);
   __builtin_amdgcn_s_waitcnt(kOneTile);
   m4_meet();  // the queries are there
@@ -386,20 +388,15 @@ __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A
     __builtin_amdgcn_s_waitcnt(kNone);
   m4_meet();  // tile 0 is there
   if (tiles) {
-    if (tiles > 2) {
-      e = entry(4);
-      fetch(w2);
-      m4_meet();  // (the first maximum)
-      __builtin_amdgcn_s_waitcnt(kOneTile);
-    } else {
-      m4_meet();
-      __builtin_amdgcn_s_waitcnt(kNone);
-    }
+    m4_meet();  // (the first maximum)
+    __builtin_amdgcn_s_waitcnt(kNone);
     m4_meet();  // tile 0's probabilities and tile 1's rows
   }
   uint32_t buf = 0;
-#pragma unroll 1
-  for (int tl = 0; tl < tiles; ++tl) {
+  // tile tl; MORE: tile tl + 2 comes to where tile tl - 1 was, in a loop of its own,
+  // because with branches between them the products move down to their uses
+  const auto sum_tile = [&](int tl, auto more) {
+    constexpr bool MORE = decltype(more)::value;
     const unsigned char* const rows = smem + buf;
     const v4f own = *reinterpret_cast<const v4f*>(&ref[tl & 1][n][0]);
     const float now = fmaxf(fmaxf(own[0], own[1]), fmaxf(own[2], own[3]));
@@ -443,17 +440,15 @@ __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    // tile tl + 2 to where tile tl - 1 was (the first three are on their way)
-    const bool more = tl && tl + 2 < tiles;
     Way next = {};
-    if (more) {
+    if constexpr (MORE) {
       next = way(tl + 2, sl, buf == 0 ? (kM4Buffers - 1) * kM4Tile : buf - kM4Tile);
       sl = slot(tl + 3, e);
       e = entry(tl + 4);
     }
     __builtin_amdgcn_sched_barrier(0);
     // Block i: keys 32 (i / 4) .., dims 128 wv + 32 (i % 4) ..; its values (V^T
-    // by the fp4 product) are two blocks ahead of their use.
+    // by the fp4 product) are two blocks ahead of their use, rounded one ahead.
     const auto values = [&](int i) {
       const int kb = i >> 2, g = i >> 1 & 1;
       v16f v;
@@ -464,27 +459,41 @@ __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A
                : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, p, v, 4, 4, 0, (int)sc[kb], 0, 0x7f7f7f7f);
     };
     v16f v[2] = {values(0), values(1)};
+    uint32_t w[2][8];
+    const auto round4 = [&](int i, int k) {  // half k of block i's values
+#pragma unroll
+      for (int e = 4 * k; e < 4 * k + 4; ++e) w[i & 1][e] = pack_bf16x2(v[i & 1][2 * e], v[i & 1][2 * e + 1]);
+    };
+    round4(0, 0);
+    round4(0, 1);
 #pragma unroll
     for (int i = 0; i < 4 * kM4Groups; ++i) {
-      uint32_t w[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(v[i & 1][2 * e], v[i & 1][2 * e + 1]);
-      __builtin_amdgcn_sched_barrier(0);  // (the next values go where these were)
+      // three products, the next block's roundings between them
+      __builtin_amdgcn_sched_barrier(0);
       if (i + 2 < 4 * kM4Groups) v[i & 1] = values(i + 2);
       v16f& acc = o[i & 3];
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m4_bf8(make_uint4(w[0], w[1], w[2], w[3])), m4_bf8(pr[i / 4 * 2]), acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m4_bf8(make_uint4(w[4], w[5], w[6], w[7])), m4_bf8(pr[i / 4 * 2 + 1]), acc, 0, 0, 0);
-      if (more) {
+      const uint32_t* a = w[i & 1];
 #pragma unroll
-        for (int k = 2 * i; k < 2 * i + 2; ++k)
-          if (k < 13) load(next, k);
+      for (int k = 0; k < 2; ++k) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + 1 < 4 * kM4Groups) round4(i + 1, k);
+        if constexpr (MORE)
+          if (2 * i + k < 13) load(next, 2 * i + k);
+        __builtin_amdgcn_sched_barrier(0);
+        acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m4_bf8(make_uint4(a[4 * k], a[4 * k + 1], a[4 * k + 2], a[4 * k + 3])),
+                                                      m4_bf8(pr[i / 4 * 2 + k]), acc, 0, 0, 0);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_sched_barrier(0);
     __builtin_amdgcn_s_waitcnt(kNone);  // the rows of tile tl + 2
-    if (tl + 1 < tiles) m4_meet();
+    if (MORE || tl + 1 < tiles) m4_meet();
     buf = buf == (kM4Buffers - 1) * kM4Tile ? 0u : buf + kM4Tile;
-  }
+  };
+  int tl = 0;
+#pragma unroll 1
+  for (; tl + 2 < tiles; ++tl) sum_tile(tl, std::true_type{});
+#pragma unroll 1
+  for (; tl < tiles; ++tl) sum_tile(tl, std::false_type{});
   __syncthreads();
 
   const v4f ls = *reinterpret_cast<const v4f*>(&wl[n][0]);

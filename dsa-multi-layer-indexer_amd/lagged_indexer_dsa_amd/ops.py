@@ -47,7 +47,7 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 def _nbytes(t: torch.Tensor) -> int:
-    return t.numel() * t.element_size()
+    return t.nbytes
 
 
 def _need_bytes(name: str, t: torch.Tensor, nbytes: int) -> None:
@@ -58,7 +58,7 @@ def _need_bytes(name: str, t: torch.Tensor, nbytes: int) -> None:
 
 
 def _need_shape(name: str, t: torch.Tensor, shape: tuple, dtype) -> None:
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
         raise RuntimeError(f"{name} must be contiguous {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
 
 
