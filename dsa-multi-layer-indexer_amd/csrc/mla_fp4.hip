@@ -248,11 +248,11 @@ __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A
 #pragma unroll
       for (int i = 0; i < 8; ++i) code[i] = *reinterpret_cast<const uint4*>(rows + code_at[i & 1] + 1024 * (i >> 1));
       const uint32_t ok = there[tl & 3][kg];
-      v16f s[2];
+      v16f s;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[0][e] = s[1][e] = 0.f;
+      for (int e = 0; e < 16; ++e) s[e] = 0.f;
       const auto product = [&](int kk, const uint4& k) {
-        s[kk & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m4_bf8(k), m4_bf8(qf[kk]), s[kk & 1], 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(m4_bf8(k), m4_bf8(qf[kk]), s, 0, 0, 0);
       };
       const uint32_t scw[4] = {scv.x, scv.y, scv.z, scv.w};
 #pragma unroll
@@ -265,17 +265,21 @@ __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) product(32 + u, *reinterpret_cast<const uint4*>(rows + rope_at[u]));
-      // element e is key 8 (e / 4) + 4h + e % 4 of head n
-      float tmax = -INFINITY;
+      // element e is key 8 (e / 4) + 4h + e % 4 of head n; the scale waits for
+      // the exponent's fma, unless it turns the order of the scores round
+      float tmax = -INFINITY, scale = A.sm_log2;
+      if (!(scale > 0.f)) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[0][e] = (s[0][e] + s[1][e]) * A.sm_log2;
+        for (int e = 0; e < 16; ++e) s[e] *= scale;
+        scale = 1.f;
+      }
       if (ok != ~0u) {  // keys that are not there
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[0][e] = (ok >> (4 * h)) & (1u << (8 * (e >> 2) + (e & 3))) ? s[0][e] : -INFINITY;
+        for (int e = 0; e < 16; ++e) s[e] = (ok >> (4 * h)) & (1u << (8 * (e >> 2) + (e & 3))) ? s[e] : -INFINITY;
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, s[0][e]);
-      tmax = m4_halves(tmax, [](float x, float y) { return fmaxf(x, y); });
+      for (int e = 0; e < 16; ++e) tmax = fmaxf(tmax, s[e]);
+      tmax = m4_halves(tmax, [](float x, float y) { return fmaxf(x, y); }) * scale;
       if (tl == 0) {  // the first tile's maximum is agreed on; later ones are seldom above it
         if (h == 0) ref[1][n][kg] = tmax;
         __syncthreads();
@@ -287,7 +291,8 @@ __global__ __launch_bounds__(kM4Threads, 2) void mla_fp4_kernel(const Mla4Args A
       float sum = 0.f;
 #pragma unroll
       for (int e = 0; e < 16; e += 2) {
-        pk[e >> 1] = pack_bf16x2(__builtin_amdgcn_exp2f(s[0][e] - at), __builtin_amdgcn_exp2f(s[0][e + 1] - at));
+        pk[e >> 1] = pack_bf16x2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale, -at)),
+                                 __builtin_amdgcn_exp2f(__builtin_fmaf(s[e + 1], scale, -at)));
         // the sum of the rounded probabilities, the ones that are multiplied
         // with the values: the weights then add up to one
         sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pk[e >> 1]), __builtin_bit_cast(v2bf, 0x3f803f80u), sum,

@@ -151,6 +151,23 @@ def test_every_count_of_tiles(dev, H, nsplit):
     _check(out, q, O.dequant_latent_rows_fp4(rows), idx)
 
 
+@pytest.mark.parametrize("sm", [0.0, -SM, 0.02])
+def test_other_scales(dev, sm):
+    """A scale that is not positive is applied before the maximum is taken.
+    (None is larger than the default, so the bound above holds.)"""
+    from lagged_indexer_dsa_amd import ops
+
+    print(f"[fp4 scale] {sm}", flush=True)
+    rng = np.random.default_rng(8)
+    rows, q = _pool(21, 900), _q(21, 2, 32)
+    idx = np.stack([rng.permutation(900)[:700] for _ in range(2)]).astype(np.int32)
+    idx[0, rng.random(700) < 0.3] = -1
+    idx[1, 300:] = -1
+    for nsplit in (1, 0):
+        out = ops.sparse_mla_decode(_dev(q, dev, True), _dev(rows, dev), _dev(idx, dev), sm_scale=sm, nsplit=nsplit)
+        _check(out, q, O.dequant_latent_rows_fp4(rows), idx, sm)
+
+
 def test_sharp_and_growing_scores(dev):
     """Scores whose maximum rises along the row by far more than the sums'
     slack, and rows where one key outweighs the others."""
