@@ -33,6 +33,15 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+// sum over 16 lanes, the same value in each
+__device__ __forceinline__ float sum16(float v) {
+  const auto sh = [](auto ctrl, float x) { return __uint_as_float(dpp_u32<decltype(ctrl)::value, 0xf>(__float_as_uint(x), 0u)); };
+  v += sh(std::integral_constant<int, 0x121>{}, v);
+  v += sh(std::integral_constant<int, 0x122>{}, v);
+  v += sh(std::integral_constant<int, 0x124>{}, v);
+  return v + sh(std::integral_constant<int, 0x128>{}, v);
+}
+
 // V vectors of 8 elements a lane, as they come from memory.
 template <int DT, int V>
 struct RawRow {
@@ -58,18 +67,62 @@ __device__ __forceinline__ void unpack8(const uint4* v, float* x) {
     }
   }
 }
-// Row `p`'s vectors of thread t of T (zeros past D).
-template <int DT, int V>
+// Row `p`'s vectors of thread t of T (zeros past D).  WIDE: on 16-byte
+// boundaries and whole; otherwise the loads are as wide, but may lie across a
+// boundary (global memory allows that), and the last vector comes one by one.
+template <int DT, int V, bool WIDE>
 __device__ __forceinline__ void load_raw(const void* p, int t, int T, int D, RawRow<DT, V>& r) {
   constexpr int es = DT == kF32 ? 4 : 2, k = DT == kF32 ? 2 : 1;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int i = 8 * (v * T + t);
+    const uint8_t* at = static_cast<const uint8_t*>(p) + (long)i * es;
+    if (WIDE ? i < D : i + 8 <= D) {
+      if constexpr (WIDE) {
 #pragma unroll
-    for (int c = 0; c < k; ++c)
-      r.v[v][c] = i < D ? reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p) + (long)i * es)[c]
-                        : make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < k; ++c) r.v[v][c] = reinterpret_cast<const uint4*>(at)[c];
+      } else {
+        __builtin_memcpy(r.v[v], __builtin_assume_aligned(at, es), 16 * k);
+      }
+      continue;
+    }
+#pragma unroll
+    for (int c = 0; c < k; ++c) r.v[v][c] = make_uint4(0, 0, 0, 0);
+    if constexpr (!WIDE) {
+      uint32_t w[4 * k] = {};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i + e < D) {
+          if constexpr (DT == kF32) w[e] = reinterpret_cast<const uint32_t*>(at)[e];
+          else w[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(at)[e] << (16 * (e & 1));
+        }
+#pragma unroll
+      for (int c = 0; c < k; ++c) r.v[v][c] = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+    }
   }
+}
+// Elements i .. i + 7, all there; and those of a row of D that are to be stored.
+template <int DT, bool WIDE>
+__device__ __forceinline__ void load_row8(const void* p, int i, float* x) {
+  constexpr int es = DT == kF32 ? 4 : 2;
+  if constexpr (WIDE) {
+    load8<DT>(p, i, x);
+  } else {
+    uint4 w[DT == kF32 ? 2 : 1];
+    __builtin_memcpy(w, __builtin_assume_aligned(static_cast<const uint8_t*>(p) + (long)i * es, es), sizeof(w));
+    load8<DT>(w, 0, x);
+  }
+}
+template <int DT, bool WIDE>
+__device__ __forceinline__ void store_row8(void* p, long row, int i, const float* x, int D) {
+  if (WIDE || i + 8 > D) {
+    store8<DT, WIDE>(p, row + i, x, row + D);
+    return;
+  }
+  constexpr int es = DT == kF32 ? 4 : 2;
+  uint4 w[DT == kF32 ? 2 : 1];
+  store8<DT, true>(w, 0, x, 0);
+  __builtin_memcpy(__builtin_assume_aligned(static_cast<uint8_t*>(p) + (row + i) * es, es), w, sizeof(w));
 }
 
 // A workgroup of T threads holds a row, V vectors of 8 elements each (vector v
@@ -79,9 +132,12 @@ __device__ __forceinline__ void load_raw(const void* p, int t, int T, int D, Raw
 // weight in registers and the next row in flight from before the reduction on.
 //
 // Bound by its bytes: 8191 rows of 7168 bf16 with a residual, to e4m3 with a
-// scale per 128 values, move 412 MB in 82 us, 5.0 TB/s (a large copy: 5.2).  A
-// row a workgroup, the weight read again for each: 195 us.  One token: 2.9 us,
-// a launch and two trips to memory.
+// scale per 128 values, move 412 MB in 79 us, 5.2 TB/s (as a large copy).  A row
+// a workgroup, the weight read again for each: 195 us.  Without the residual the
+// quantiser's arithmetic is next (42 us for 176 MB).  Rows of 3001 values, which
+// begin between boundaries: 4096 of bf16 with a residual 28 us, of 3000 16 us;
+// value by value they took 62.  One token: 2.9 us, a launch and two trips to
+// memory.
 constexpr int kNormWaves = 16;  // most waves a row
 
 template <int DT, int V, bool WIDE>
@@ -90,24 +146,20 @@ __global__ __launch_bounds__(kNormWaves* kWave) void rms_norm_kernel(const NormA
   __shared__ float red[2][kNormWaves];
   __shared__ uint32_t redm[2][kNormWaves];
   const int T = (int)blockDim.x, waves = T / kWave, t = (int)threadIdx.x, D = A.D, wv = wave_id();
+  const float inv_d = 1.f / (float)D;
+  if (t >= waves && t < kNormWaves) red[0][t] = red[1][t] = 0.f, redm[0][t] = redm[1][t] = 0;
   long row = blockIdx.x;
   const auto at = [&](const void* p, long r, long rs) { return static_cast<const uint8_t*>(p) + r * rs * es; };
   RawRow<DT, V> x, r;
-  if constexpr (WIDE) {
-    load_raw<DT, V>(at(A.x, row, A.xs), t, T, D, x);
-    if (A.r) load_raw<DT, V>(at(A.r, row, A.rs), t, T, D, r);
-  }
+  load_raw<DT, V, WIDE>(at(A.x, row, A.xs), t, T, D, x);
+  if (A.r) load_raw<DT, V, WIDE>(at(A.r, row, A.rs), t, T, D, r);
   float w[V][8];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int i = 8 * (v * T + t);
-    if constexpr (WIDE) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) w[v][e] = 0.f;
-      if (i < D) {
-        if (A.w_f32) load8<kF32>(A.w, i, w[v]);
-        else load8<DT>(A.w, i, w[v]);
-      }
+    if (i + 8 <= D) {
+      if (A.w_f32) load_row8<kF32, WIDE>(A.w, i, w[v]);
+      else load_row8<DT, WIDE>(A.w, i, w[v]);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -120,42 +172,28 @@ __global__ __launch_bounds__(kNormWaves* kWave) void rms_norm_kernel(const NormA
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int i = 8 * (v * T + t);
-      if constexpr (WIDE) {
-        unpack8<DT>(x.v[v], h[v]);
-        if (A.r) {
-          float f[8];
-          unpack8<DT>(r.v[v], f);
+      unpack8<DT>(x.v[v], h[v]);
+      if (A.r) {
+        float f[8];
+        unpack8<DT>(r.v[v], f);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) h[v][e] += f[e];
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          h[v][e] = 0.f;
-          if (i + e < D) {
-            h[v][e] = load_elem<DT>(A.x, row * A.xs + i + e);
-            if (A.r) h[v][e] += load_elem<DT>(A.r, row * A.rs + i + e);
-          }
-        }
+        for (int e = 0; e < 8; ++e) h[v][e] += f[e];
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(h[v][e], h[v][e], ss);
-      if (A.h && (!WIDE || i < D)) store8<DT, WIDE>(A.h, row * A.hs + i, h[v], row * A.hs + D);
+      if (A.h && i < D) store_row8<DT, WIDE>(A.h, row * A.hs, i, h[v], D);
     }
-    if constexpr (WIDE) {
-      if (const long next = row + gridDim.x; next < A.n) {
-        load_raw<DT, V>(at(A.x, next, A.xs), t, T, D, x);
-        if (A.r) load_raw<DT, V>(at(A.r, next, A.rs), t, T, D, r);
-      }
+    if (const long next = row + gridDim.x; next < A.n) {
+      load_raw<DT, V, WIDE>(at(A.x, next, A.xs), t, T, D, x);
+      if (A.r) load_raw<DT, V, WIDE>(at(A.r, next, A.rs), t, T, D, r);
     }
     ss = wave_sum(ss);
     if (waves > 1) {
       if ((t & (kWave - 1)) == 0) red[par][wv] = ss;
       __syncthreads();
-      ss = 0.f;
-      for (int k = 0; k < waves; ++k) ss += red[par][k];
+      ss = sum16(red[par][t & (kNormWaves - 1)]);
     }
-    const float rs = 1.f / sqrtf(ss / (float)D + A.eps);
+    const float rs = rsqrtf(ss * inv_d + A.eps);
 #pragma unroll
     for (int v = 0; v < V; ++v)
 #pragma unroll
@@ -164,7 +202,7 @@ __global__ __launch_bounds__(kNormWaves* kWave) void rms_norm_kernel(const NormA
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int i = 8 * (v * T + t);
-        if (!WIDE || i < D) store8<DT, WIDE>(A.y, row * D + i, h[v], row * D + D);
+        if (i < D) store_row8<DT, WIDE>(A.y, row * D, i, h[v], D);
       }
       continue;
     }
@@ -176,7 +214,7 @@ __global__ __launch_bounds__(kNormWaves* kWave) void rms_norm_kernel(const NormA
       if (waves > 1) {
         if ((t & (kWave - 1)) == 0) redm[par][wv] = am;
         __syncthreads();
-        for (int k = 0; k < waves; ++k) am = max(am, redm[par][k]);
+        am = row16_max(redm[par][t & (kNormWaves - 1)]);
       }
     }
     const int groups = A.group ? (D + 127) / 128 : 1;
@@ -189,6 +227,8 @@ __global__ __launch_bounds__(kNormWaves* kWave) void rms_norm_kernel(const NormA
       uint8_t* dst = A.codes + row * D + i;
       if constexpr (WIDE) {
         *reinterpret_cast<v2u_t*>(dst) = c;
+      } else if (i + 8 <= D) {
+        __builtin_memcpy(dst, &c, 8);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -215,9 +255,11 @@ static hipError_t launch_norm_dim(const NormArgs& A, hipStream_t s) {
   const auto on16 = [](const void* p, long stride) { return (((uintptr_t)p | (uintptr_t)(stride * es)) & 15) == 0; };
   const bool wide = A.D % 8 == 0 && on16(A.x, A.xs) && (!A.r || on16(A.r, A.rs)) && (!A.h || on16(A.h, A.hs)) &&
                     (!A.y || on16(A.y, 0)) && ((uintptr_t)A.codes & 7) == 0 && on16(A.w, 0);
-  // the fewest vectors a thread that 1024 threads allow: 7168 values in one
-  // (896 threads) 82.8 us, in two 84.8, in four 108.7 (8191 rows, as above)
-  if (A.D <= 8192) return launch_norm<DT, 1>(A, wide, s);
+  // the fewest vectors a thread that 1024 threads allow, but two where the
+  // quantiser's arithmetic bounds the row (8191 x 7168 bf16: 42.5 us, in one
+  // vector 47.7; 4096 x 3000: 12.7 and 13.1; 8191 x 1536: 13.8 and 12.4; not
+  // quantised: 40.1 and 37.6).  In four: 67.7 and 45.5 for 7168.
+  if (A.D <= 8192 && (!A.codes || DT == kF32 || A.D <= 2048)) return launch_norm<DT, 1>(A, wide, s);
   if (A.D <= 16384) return launch_norm<DT, 2>(A, wide, s);
   return launch_norm<DT, 4>(A, wide, s);
 }

@@ -87,7 +87,9 @@ __device__ __forceinline__ float row_scale(const float* x) {
 // the first correction is within an ulp, the second then rounds correctly
 // (Markstein's theorem), at 5 instructions a quotient where the compiler's
 // general division takes about 10 and a quarter-rate reciprocal.  A scale
-// that is not finite takes the division.
+// that is not finite takes the division.  scale is the row's own: a quotient is
+// at most 448 (1 + 2^-23), which converts to 448 without a clamp; only where a
+// NaN was passed over (NANS false) does one turn it into -448.
 template <bool NANS>
 __device__ __forceinline__ v2u_t quant8(const float* x, float scale) {
   float y[8];
@@ -105,10 +107,9 @@ __device__ __forceinline__ v2u_t quant8(const float* x, float scale) {
     for (int e = 0; e < 8; ++e) y[e] = x[e] / scale;
   }
   int c[4];
+  if constexpr (!NANS) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    if constexpr (NANS) y[e] = y[e] > 448.f ? 448.f : (y[e] < -448.f ? -448.f : y[e]);  // NaN stays
-    else y[e] = fminf(fmaxf(y[e], -448.f), 448.f);
+    for (int e = 0; e < 8; ++e) y[e] = fminf(fmaxf(y[e], -448.f), 448.f);
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) c[e] = __builtin_amdgcn_cvt_pk_fp8_f32(y[2 * e], y[2 * e + 1], 0, false);
