@@ -114,6 +114,40 @@ def test_norm_many_rows_and_strides(dev):
     assert torch.equal(stream[:, 40:552], (keep[:, 40:552].float() + x.float()).half())
 
 
+@pytest.mark.parametrize("n,D", [(3, 9), (5000, 301), (70, 3001), (9, 9999)])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_norm_rows_between_boundaries(dev, n, D, dtype):
+    """Rows, weights and outputs that begin anywhere: the same bits as from
+    boundaries, in place too, and nothing beside them written."""
+    from lagged_indexer_dsa_amd import ops
+
+    print(f"[norm] between boundaries {(n, D, dtype)}", flush=True)
+    g = torch.Generator(device=dev).manual_seed(n)
+    E = -(-D // 8) * 8 + 16
+    x, r = _rand(dev, g, n, D, dtype=dtype), _rand(dev, g, n, D, dtype=dtype)
+    w = _rand(dev, g, D + 1, dtype=dtype)[1:]
+    xa, ra, wa = torch.zeros(n, E, dtype=dtype, device=dev), torch.zeros(n, E, dtype=dtype, device=dev), w.clone()
+    xa[:, :D], ra[:, :D] = x, r
+    y, h = ops.rms_norm(xa[:, :D], wa, residual=ra[:, :D])           # rows on boundaries
+    ref, _ = O.rms_norm(x.double().cpu().numpy(), w.double().cpu().numpy(), 1e-6, r.double().cpu().numpy())
+    _near(y, ref, F32 + 2.0 ** -23)  # (the sum x + r is off by 2^-24 of itself)
+    for off in (1, 3):
+        wide = torch.full((n, D + 7), 5.0, dtype=dtype, device=dev)
+        wide[:, off:off + D] = r
+        big = torch.full((n * D + 16,), 5.0, dtype=dtype, device=dev)
+        out = big[off:off + n * D].view(n, D)
+        y2, h2 = ops.rms_norm(x, w, residual=wide[:, off:off + D], out=out, out_residual=wide[:, off:off + D])
+        assert torch.equal(y2, y) and torch.equal(h2, h)
+        assert (wide[:, :off] == 5).all() and (wide[:, off + D:] == 5).all()
+        assert (big[:off] == 5).all() and (big[off + n * D:] == 5).all()
+        for group in (128, 0):
+            c0, s0, _ = ops.rms_norm_quant(xa[:, :D], wa, residual=ra[:, :D], group=group)
+            cb = torch.full((n * D + 16,), 9, dtype=torch.uint8, device=dev)
+            c1, s1, _ = ops.rms_norm_quant(x, w, residual=r, group=group, out_q=cb[off:off + n * D].view(n, D))
+            assert torch.equal(c0, c1) and torch.equal(s0, s1)
+            assert (cb[:off] == 9).all() and (cb[off + n * D:] == 9).all()
+
+
 def test_norm_extremes(dev):
     from lagged_indexer_dsa_amd import ops
 
