@@ -523,11 +523,12 @@ int dsa_read_latent_rows(const void* kv_pool, int64_t kv_rows, int row_bytes, co
  * dsa_mla_fp4_workspace_bytes(B, H, nsplit) bytes, no initialisation; calls
  * that overlap in time must not share it.  A workspace large enough for both
  * may serve (3), (3a) and these in turn: the barriers at its start are left as
- * they are.  nsplit: the chunks of keys a row is
- * cut into, 1 to 128 (0: what fills the device once); dense rows (256 or fewer)
- * share B * nsplit chunks (512 at most) by their lengths, so where a row is cut, and the
- * last bits of its output, depend on the other rows' lengths (the same call
- * always gives the same).  No workgroup waits for another.
+ * they are.  nsplit: the chunks of keys a row is cut into, 1 to 128, or 0 for
+ * as many as fill the device once (one a row, where there are that many rows).
+ * 256 or fewer dense rows share B * nsplit chunks (512 at most) by their
+ * lengths, so where a row is cut, and the last bits of its output, depend on
+ * the other rows' lengths; the same call always gives the same.  No workgroup
+ * waits for another.
  */
 size_t dsa_mla_fp4_workspace_bytes(int B, int H, int nsplit);
 int dsa_sparse_mla_decode_fp4(const void* q_bf16, const void* kv_pool, int64_t kv_rows, const int32_t* idx,
