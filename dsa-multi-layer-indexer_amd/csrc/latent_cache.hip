@@ -16,9 +16,9 @@
 // 0.8 of the 9 us below; a division and a root in place of the reciprocal root 3
 // more.)
 //
-// 8191 tokens, latent to 400 bytes and index key: 9.0 us for 18 MB, bound by the
+// 8191 tokens, latent to 400 bytes and index key: 8.6 us for 18 MB, bound by the
 // arithmetic of the norm and the two quantisers (half of it) and the chain from
-// the position over the page to the store.  One token: 2.5 us.
+// the position over the page to the store.  One token: 2.2 us.
 #include "dsa_kernels.h"
 #include "quant_core.h"
 
@@ -195,7 +195,7 @@ hipError_t launch_append_tokens(const AppendArgs& A, int dtype, int row_bytes, h
 //
 // Bound by its bytes: 65536 rows of 400 bytes to 1152: 102 MB in 20.5 us (5.0
 // TB/s, what a large copy reaches); 1, 4 and 8 rows a wave: 21.2, 21.5, 20.1.
-// 777 rows of 656 bytes: 3.0 us, a launch and two trips to memory; 8 a wave: 3.8.
+// 777 rows of 656 bytes: 2.9 us, a launch and two trips to memory; 8 a wave: 3.8.
 constexpr int kReadRows = 2;
 
 template <int BYTES>
