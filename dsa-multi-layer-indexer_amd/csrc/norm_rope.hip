@@ -150,9 +150,15 @@ __global__ __launch_bounds__(kNormWaves* kWave) void rms_norm_kernel(const NormA
   if (t >= waves && t < kNormWaves) red[0][t] = red[1][t] = 0.f, redm[0][t] = redm[1][t] = 0;
   long row = blockIdx.x;
   const auto at = [&](const void* p, long r, long rs) { return static_cast<const uint8_t*>(p) + r * rs * es; };
+  // four vectors of the next row do not fit beside this one's: 2000 x 18432 bf16
+  // with a residual took 66 us with them (spilled), 52 without, fp32 176 and 118
+  constexpr bool kAhead = V < 4;
   RawRow<DT, V> x, r;
-  load_raw<DT, V, WIDE>(at(A.x, row, A.xs), t, T, D, x);
-  if (A.r) load_raw<DT, V, WIDE>(at(A.r, row, A.rs), t, T, D, r);
+  const auto load = [&](long row) {
+    load_raw<DT, V, WIDE>(at(A.x, row, A.xs), t, T, D, x);
+    if (A.r) load_raw<DT, V, WIDE>(at(A.r, row, A.rs), t, T, D, r);
+  };
+  if (kAhead) load(row);
   float w[V][8];
 #pragma unroll
   for (int v = 0; v < V; ++v) {
@@ -167,6 +173,7 @@ __global__ __launch_bounds__(kNormWaves* kWave) void rms_norm_kernel(const NormA
     }
   }
   for (int par = 0; row < A.n; row += gridDim.x, par ^= 1) {
+    if (!kAhead) load(row);
     float h[V][8];
     float ss = 0.f;
 #pragma unroll
@@ -183,10 +190,7 @@ __global__ __launch_bounds__(kNormWaves* kWave) void rms_norm_kernel(const NormA
       for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(h[v][e], h[v][e], ss);
       if (A.h && i < D) store_row8<DT, WIDE>(A.h, row * A.hs, i, h[v], D);
     }
-    if (const long next = row + gridDim.x; next < A.n) {
-      load_raw<DT, V, WIDE>(at(A.x, next, A.xs), t, T, D, x);
-      if (A.r) load_raw<DT, V, WIDE>(at(A.r, next, A.rs), t, T, D, r);
-    }
+    if (kAhead && row + gridDim.x < A.n) load(row + gridDim.x);
     ss = wave_sum(ss);
     if (waves > 1) {
       if ((t & (kWave - 1)) == 0) red[par][wv] = ss;
@@ -258,7 +262,7 @@ static hipError_t launch_norm_dim(const NormArgs& A, hipStream_t s) {
   // the fewest vectors a thread that 1024 threads allow, but two where the
   // quantiser's arithmetic bounds the row (8191 x 7168 bf16: 42.5 us, in one
   // vector 47.7; 4096 x 3000: 12.7 and 13.1; 8191 x 1536: 13.8 and 12.4; not
-  // quantised: 40.1 and 37.6).  In four: 67.7 and 45.5 for 7168.
+  // quantised: 40.1 and 37.6).  In four, without the next row: 42.2 and 39.1.
   if (A.D <= 8192 && (!A.codes || DT == kF32 || A.D <= 2048)) return launch_norm<DT, 1>(A, wide, s);
   if (A.D <= 16384) return launch_norm<DT, 2>(A, wide, s);
   return launch_norm<DT, 4>(A, wide, s);
