@@ -380,7 +380,7 @@ extern "C" {
 
 const char* dsa_last_error(void) { return g_err; }
 
-const char* dsa_version(void) { return "dsa_mli 0.5.0 gfx950"; }
+const char* dsa_version(void) { return "dsa_mli 0.6.0 gfx950"; }
 
 size_t dsa_layer_args_bytes(void) { return sizeof(dsa_layer_args); }
 
@@ -822,9 +822,20 @@ int dsa_read_latent_rows(const void* kv_pool, int64_t kv_rows, int row_bytes, co
                     "read latent rows");
 }
 
+static bool mla_shape(int B, int H, int nsplit) {
+  return B >= 1 && B <= 65535 && H >= 16 && H % 16 == 0 && H <= 16 * 64 && nsplit >= 0 && nsplit <= 128;
+}
+
 size_t dsa_mla_fp4_workspace_bytes(int B, int H, int nsplit) {
-  if (B < 1 || B > 65535 || H < 16 || H % 16 || H > 16 * 64 || nsplit < 0 || nsplit > 128) return 0;
-  return dsa::mla_fp4_workspace_bytes(B, H, nsplit);
+  return mla_shape(B, H, nsplit) ? dsa::mla_fp4_workspace_bytes(B, H, nsplit) : 0;
+}
+
+size_t dsa_mla_shared_workspace_bytes(int B, int H, int nsplit) {
+  return mla_shape(B, H, nsplit) ? dsa::mla_shared_workspace_bytes(B, H, nsplit) : 0;
+}
+
+int64_t dsa_mla_fp4_workspace_in(size_t shared_bytes, int B, int H, int nsplit) {
+  return mla_shape(B, H, nsplit) ? (int64_t)dsa::mla_fp4_workspace_in(shared_bytes, B, H, nsplit) : -1;
 }
 
 static int mla_fp4(const void* q_bf16, const void* kv_pool, int64_t kv_rows, const int32_t* idx,

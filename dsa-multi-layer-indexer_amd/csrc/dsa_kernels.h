@@ -200,6 +200,8 @@ struct Mla4Args {
   int chunks, units, per_row;
 };
 size_t mla_fp4_workspace_bytes(int B, int H, int nsplit);
+long mla_fp4_workspace_in(size_t bytes, int B, int H, int nsplit);
+size_t mla_shared_workspace_bytes(int B, int H, int nsplit);
 hipError_t launch_mla_fp4(Mla4Args A, int nsplit, void* workspace, hipStream_t s);
 
 }  // namespace dsa

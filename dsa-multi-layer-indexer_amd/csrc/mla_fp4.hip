@@ -622,13 +622,41 @@ static int m4_chunks(int B, int H, int nsplit) {
   return (int)std::max((long)B, B <= kM4Ragged ? std::min(want, (long)kM4MergeMax) : want);
 }
 
-// The partials lie behind the barriers that the 8-bit decode keeps in a
-// workspace, so calls over both formats may take turns with one.
-size_t mla_fp4_workspace_bytes(int B, int H, int nsplit) {
+// Partial sums and plan of a call; 0: unsplit rows, none is read.
+static size_t mla_fp4_partial_bytes(int B, int H, int nsplit) {
   const int chunks = m4_chunks(B, H, nsplit);
-  if (chunks <= B) return 16;  // unsplit rows: none is read
-  return attn_workspace_bytes(B, H, 0) + (size_t)chunks * m4_blocks(H) * m4_heads(H) * (DSA_LATENT_DIM + 2) * sizeof(float) +
-         (size_t)B * sizeof(int2);
+  if (chunks <= B) return 0;
+  return (size_t)chunks * m4_blocks(H) * m4_heads(H) * (DSA_LATENT_DIM + 2) * sizeof(float) + (size_t)B * sizeof(int2);
+}
+
+// The partials lie behind as many barriers as an 8-bit call of the same rows and
+// heads keeps at a workspace's start.  A call of more rows keeps more of them:
+// mla_fp4_workspace_in() below moves this call's workspace behind those.
+size_t mla_fp4_workspace_bytes(int B, int H, int nsplit) {
+  const size_t partials = mla_fp4_partial_bytes(B, H, nsplit);
+  return partials ? attn_workspace_bytes(B, H, 0) + partials : 16;
+}
+
+// The bytes at the start of a workspace of `bytes` that may hold barriers: an
+// 8-bit call that fits has a barrier and one split's partials at least for each
+// of its (row, head group)s.
+static size_t mla_barrier_room(size_t bytes) { return bytes / attn_workspace_bytes(1, 16, 1) * attn_workspace_bytes(1, 16, 0); }
+
+// Where in a workspace that 8-bit calls of any rows and heads share a 4-bit call
+// has its own, so that its partials begin behind every barrier; -1: too small.
+long mla_fp4_workspace_in(size_t bytes, int B, int H, int nsplit) {
+  const size_t partials = mla_fp4_partial_bytes(B, H, nsplit), room = mla_barrier_room(bytes);
+  if (!partials) return bytes >= 16 ? 0 : -1;
+  const size_t own = attn_workspace_bytes(B, H, 0), from = std::max(room, own);
+  return bytes >= from + partials ? (long)(from - own) : -1;
+}
+
+// Bytes for calls over both formats; nsplit 0: of every split count.
+size_t mla_shared_workspace_bytes(int B, int H, int nsplit) {
+  const size_t partials = std::max(mla_fp4_partial_bytes(B, H, nsplit), mla_fp4_partial_bytes(B, H, nsplit ? nsplit : 128));
+  size_t bytes = attn_workspace_bytes(B, H, nsplit ? nsplit : 128);
+  for (size_t need; (need = partials + std::max(mla_barrier_room(bytes), attn_workspace_bytes(B, H, 0))) > bytes;) bytes = need;
+  return (bytes + 15) / 16 * 16;
 }
 
 hipError_t launch_mla_fp4(Mla4Args A, int nsplit, void* workspace, hipStream_t s) {

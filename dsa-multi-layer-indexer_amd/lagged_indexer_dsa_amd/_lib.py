@@ -117,6 +117,8 @@ SIGNATURES = {
     "dsa_append_tokens": (_i32, [ctypes.c_char_p, _vp]),
     "dsa_read_latent_rows": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _vp]),
     "dsa_mla_fp4_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i32]),
+    "dsa_mla_shared_workspace_bytes": (ctypes.c_size_t, [_i32, _i32, _i32]),
+    "dsa_mla_fp4_workspace_in": (_i64, [ctypes.c_size_t, _i32, _i32, _i32]),
     "dsa_sparse_mla_decode_fp4": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp]),
     "dsa_dense_mla_decode_fp4": (_i32, [_vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _f32, _vp]),
 }

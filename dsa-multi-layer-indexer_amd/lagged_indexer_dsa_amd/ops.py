@@ -154,12 +154,15 @@ def select_rows(scores: torch.Tensor, k: int, pad_value: int) -> torch.Tensor | 
 def sparse_mla_workspace(B: int, H: int, nsplit: int, device) -> torch.Tensor:
     """Zero-filled workspace (split partials + the splits' barriers; every
     call leaves the barriers ready), for pools of either row format.  nsplit=0
-    sizes it for any split count."""
-    lib = _lib.load()
-    nbytes = lib.dsa_sparse_mla_workspace_bytes(B, H, nsplit)
+    sizes it for any split count.
+
+    Calls over 400-byte rows of any B and H that it is enough for may use it, in
+    turn with calls over 656-byte rows.  Those must all be of one B * H: their
+    partials begin behind as many barriers as the call itself has.
+    """
+    nbytes = _lib.load().dsa_mla_shared_workspace_bytes(B, H, nsplit)
     if nbytes == 0:
         raise RuntimeError(f"bad sparse MLA workspace shape B={B} H={H} nsplit={nsplit}")
-    nbytes = max(nbytes, *(lib.dsa_mla_fp4_workspace_bytes(B, H, n) for n in (nsplit, nsplit or 128)))
     return torch.zeros(nbytes // 4, dtype=torch.float32, device=device)
 
 
@@ -196,7 +199,8 @@ def _here(dev: int, *tensors: torch.Tensor | None) -> None:
 
 
 def _fp4_call(q, kv_pool, sm_scale, nsplit: int, workspace, out, *others):
-    """What a decode call over 400-byte rows checks besides its keys."""
+    """What a decode call over 400-byte rows checks besides its keys; ws: the
+    address in the workspace that the call gets."""
     qs = q.shape
     if len(qs) != 3 or qs[2] != QK_DIM or q.dtype != torch.bfloat16:
         raise RuntimeError("q must be [B, H, 576] bfloat16")
@@ -204,18 +208,24 @@ def _fp4_call(q, kv_pool, sm_scale, nsplit: int, workspace, out, *others):
         raise RuntimeError("kv_pool must be [rows, 400] uint8")
     B, H, _ = qs
     _here(q.get_device(), kv_pool, workspace, out, *others)
-    nbytes = _lib.load().dsa_mla_fp4_workspace_bytes(B, H, nsplit)
+    lib = _lib.load()
     if workspace is None:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    else:
-        _need_bytes("4-bit MLA workspace", workspace, nbytes)
+        workspace = torch.empty(lib.dsa_mla_fp4_workspace_bytes(B, H, nsplit), dtype=torch.uint8, device=q.device)
+        ws = workspace.data_ptr()
+    else:  # behind the barriers that calls over 656-byte rows may have in it
+        at = lib.dsa_mla_fp4_workspace_in(_nbytes(workspace), B, H, nsplit)
+        if at < 0:
+            raise RuntimeError(f"the 4-bit MLA workspace of {_nbytes(workspace)} bytes is not enough for B={B} H={H} "
+                               f"nsplit={nsplit} (ops.sparse_mla_workspace: "
+                               f"{lib.dsa_mla_shared_workspace_bytes(B, H, nsplit)} bytes)")
         if not workspace.is_contiguous():
             raise RuntimeError("the 4-bit MLA workspace must be contiguous")
+        ws = workspace.data_ptr() + at
     if out is None:
         out = torch.empty(B, H, LATENT_DIM, dtype=torch.bfloat16, device=q.device)
     else:
         _need_shape("out", out, (B, H, LATENT_DIM), torch.bfloat16)
-    return B, H, QK_DIM ** -0.5 if sm_scale is None else float(sm_scale), workspace, out
+    return B, H, QK_DIM ** -0.5 if sm_scale is None else float(sm_scale), workspace, ws, out
 
 
 def sparse_mla_decode(q: torch.Tensor, kv_pool: torch.Tensor, idx: torch.Tensor,
@@ -231,11 +241,11 @@ def sparse_mla_decode(q: torch.Tensor, kv_pool: torch.Tensor, idx: torch.Tensor,
     """
     _dev(q, kv_pool, idx)
     if kv_pool.dim() == 2 and kv_pool.shape[1] == FP4_ROW_BYTES:
-        B, H, sm_scale, workspace, out = _fp4_call(q, kv_pool, sm_scale, nsplit, workspace, out, idx)
+        B, H, sm_scale, workspace, ws, out = _fp4_call(q, kv_pool, sm_scale, nsplit, workspace, out, idx)
         if idx.dim() != 2 or idx.shape[0] != B or idx.dtype != torch.int32:
             raise RuntimeError("idx must be [B, topk] int32")
-        _lib.call("dsa_sparse_mla_decode_fp4", q.data_ptr(), kv_pool.data_ptr(), kv_pool.shape[0], idx.data_ptr(),
-                  workspace.data_ptr(), out.data_ptr(), B, H, idx.shape[1], nsplit, sm_scale, _stream())
+        _lib.call("dsa_sparse_mla_decode_fp4", q.data_ptr(), kv_pool.data_ptr(), kv_pool.shape[0], idx.data_ptr(), ws,
+                  out.data_ptr(), B, H, idx.shape[1], nsplit, sm_scale, _stream())
         return out
     if q.dim() != 3 or q.shape[2] != QK_DIM or q.dtype != torch.bfloat16:
         raise RuntimeError("q must be [B, H, 576] bfloat16")
@@ -275,13 +285,13 @@ def dense_mla_decode(q: torch.Tensor, kv_pool: torch.Tensor, page_table: torch.T
     """
     _dev(q, kv_pool, page_table, seq_lens)
     if kv_pool.dim() == 2 and kv_pool.shape[1] == FP4_ROW_BYTES:
-        B, H, sm_scale, workspace, out = _fp4_call(q, kv_pool, sm_scale, nsplit, workspace, out, page_table, seq_lens)
+        B, H, sm_scale, workspace, ws, out = _fp4_call(q, kv_pool, sm_scale, nsplit, workspace, out, page_table, seq_lens)
         if page_table.dim() != 2 or page_table.shape[0] != B or page_table.dtype != torch.int32:
             raise RuntimeError("page_table must be [B, pt_stride] int32")
         _need_shape("seq_lens", seq_lens, (B,), torch.int32)
         _lib.call("dsa_dense_mla_decode_fp4", q.data_ptr(), kv_pool.data_ptr(), kv_pool.shape[0],
-                  page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(), workspace.data_ptr(),
-                  out.data_ptr(), B, H, nsplit, sm_scale, _stream())
+                  page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(), ws, out.data_ptr(), B, H, nsplit,
+                  sm_scale, _stream())
         return out
     if q.dim() != 3 or q.shape[2] != QK_DIM or q.dtype != torch.bfloat16:
         raise RuntimeError("q must be [B, H, 576] bfloat16")

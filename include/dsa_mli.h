@@ -194,7 +194,9 @@ int dsa_select_rows(const float* scores, const int32_t* seq_lens, int64_t* out_i
  *             partials plus one barrier per (row, head group) through which
  *             the splits merge together; zero-fill it once before the first
  *             call, every call leaves the barriers ready for the next.
- *             Calls that overlap in time must not share it.
+ *             Calls that overlap in time must not share it, nor calls of
+ *             another B * H: the partials begin behind the call's own barriers,
+ *             where a call of more rows or heads has barriers still.
  *   out       [B, H, 512] bf16
  * H must be a multiple of 16; 1 <= nsplit <= 128 (nsplit=0: automatic, and
  * a workspace sized with nsplit=0 fits any nsplit).
@@ -521,16 +523,24 @@ int dsa_read_latent_rows(const void* kv_pool, int64_t kv_rows, int row_bytes, co
 /*
  * (12) (3) and (3a) over a pool of 400-byte rows.  workspace:
  * dsa_mla_fp4_workspace_bytes(B, H, nsplit) bytes, no initialisation; calls
- * that overlap in time must not share it.  A workspace large enough for both
- * may serve (3), (3a) and these in turn: the barriers at its start are left as
- * they are.  nsplit: the chunks of keys a row is cut into, 1 to 128, or 0 for
- * as many as fill the device once (one a row, where there are that many rows).
+ * that overlap in time must not share it.  The partial sums begin
+ * dsa_sparse_mla_barrier_bytes(B, H, 0) bytes in, what is before them is left as
+ * it is.  Calls of any B and H over 400-byte rows may take turns with one
+ * workspace.  (3), (3a) and (4), of one B * H, may take turns with them if the
+ * workspace, of w bytes in all (dsa_mla_shared_workspace_bytes(B, H, nsplit) for
+ * both formats, zero-filled), is given to a 4-bit call from
+ * dsa_mla_fp4_workspace_in(w, B, H, nsplit) bytes on: its partial sums then lie
+ * behind every barrier of any call that w is enough for.  (-1: w is not enough.)
+ * nsplit: the chunks of keys a row is cut into, 1 to 128, or 0 for as many as
+ * fill the device once (one a row, where there are that many rows).
  * 256 or fewer dense rows share B * nsplit chunks (512 at most) by their
  * lengths, so where a row is cut, and the last bits of its output, depend on
  * the other rows' lengths; the same call always gives the same.  No workgroup
  * waits for another.
  */
 size_t dsa_mla_fp4_workspace_bytes(int B, int H, int nsplit);
+size_t dsa_mla_shared_workspace_bytes(int B, int H, int nsplit);
+int64_t dsa_mla_fp4_workspace_in(size_t shared_bytes, int B, int H, int nsplit);
 int dsa_sparse_mla_decode_fp4(const void* q_bf16, const void* kv_pool, int64_t kv_rows, const int32_t* idx,
                               void* workspace, void* out_bf16, int B, int H, int topk, int nsplit, float sm_scale,
                               void* stream);

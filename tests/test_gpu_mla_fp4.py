@@ -256,6 +256,50 @@ def test_one_workspace_for_both_formats(dev):
     assert _lib.sync_timeouts() == 0
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_calls_of_other_batches_on_one_workspace(dev, captured):
+    """A workspace for the largest batch: 4-bit calls of fewer rows (whose partial
+    sums would begin where the larger batch has barriers) between 8-bit calls of
+    all of them, each like the call with a workspace of its own."""
+    from lagged_indexer_dsa_amd import _lib, formats as F, ops
+
+    print(f"[fp4] other batches on one workspace, captured {captured}", flush=True)
+    g = torch.Generator(device=dev).manual_seed(12)
+    lat, rope = torch.randn(4096, 512, device=dev, generator=g), torch.randn(4096, 64, device=dev, generator=g)
+    p8, p4 = F.pack_latent_rows(lat, rope), F.pack_latent_rows_fp4(lat, rope)
+    q = torch.randn(8, 32, 576, device=dev, generator=g).to(torch.bfloat16)
+    idx = torch.stack([torch.randperm(4096, generator=g, device=dev)[:2048] for _ in range(8)]).int()
+    pt = torch.arange(64, device=dev, dtype=torch.int32).reshape(8, 8)
+    lens = torch.tensor([512, 3, 500, 0, 129, 64, 400, 1], dtype=torch.int32, device=dev)
+    ws = ops.sparse_mla_workspace(8, 32, 0, dev)
+    outs = [torch.zeros(b, h, 512, dtype=torch.bfloat16, device=dev) for b, h in ((8, 32), (1, 16), (8, 32), (3, 32), (8, 16))]
+    q1, q5 = q[:1, :16].contiguous(), q[:, :16].contiguous()
+    calls = [lambda w, o: ops.sparse_mla_decode(q, p8, idx, nsplit=4, workspace=w, out=o),
+             lambda w, o: ops.sparse_mla_decode(q1, p4, idx[:1], workspace=w, out=o),
+             lambda w, o: ops.dense_mla_decode(q, p8, pt, lens, nsplit=3, workspace=w, out=o),
+             lambda w, o: ops.dense_mla_decode(q[:3], p4, pt[:3], lens[:3], nsplit=6, workspace=w, out=o),
+             lambda w, o: ops.sparse_mla_decode(q5, p4, idx, nsplit=16, workspace=w, out=o)]
+    _lib.sync_timeouts(reset=True)
+    want = [f(ops.sparse_mla_workspace(8, 32, 0, dev), None).clone() for f in calls]
+    run = [lambda f=f, o=o: f(ws, o) for f, o in zip(calls, outs)]
+    if captured:
+        for k, f in enumerate(run):
+            f()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                f()
+            run[k] = graph.replay
+    for turn in range(3):
+        for o in outs:
+            o.zero_()
+        for k in (1, 0, 3, 2, 4, 0, 1, 2):
+            run[k]()
+        torch.cuda.synchronize()
+        for k, (o, w) in enumerate(zip(outs, want)):
+            assert torch.equal(o, w), f"turn {turn}, call {k}"
+    assert _lib.sync_timeouts() == 0
+
+
 def test_graphs_on_one_workspace_and_calls_at_once(dev):
     """Two captured calls of other sizes and formats share a workspace and are
     replayed in turn; calls on two streams with a workspace each run together."""

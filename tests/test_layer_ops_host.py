@@ -265,3 +265,50 @@ def test_workspace_for_any_split_count(lib):
         for n in range(0, 129):
             assert nbytes >= lib.dsa_mla_fp4_workspace_bytes(B, H, n), (B, H, n)
             assert nbytes >= lib.dsa_sparse_mla_workspace_bytes(B, H, n), (B, H, n)
+
+
+def _barriers(B, H):
+    return B * (H // 16) * 25 * 64 * 4
+
+
+@pytest.mark.parametrize("B,H,nsplit", [(8, 16, 0), (32, 16, 8), (8, 128, 0), (1, 16, 0), (2, 16, 8), (3, 48, 1),
+                                        (100, 64, 2), (300, 16, 3), (64, 128, 0)])
+def test_4bit_partials_are_clear_of_every_barrier(lib, B, H, nsplit):
+    """One workspace, 8-bit calls of any rows and heads that it is enough for (a
+    barrier a row and 16 heads, at its start), 4-bit calls likewise: where the
+    4-bit ones write lies behind all of those barriers and inside the workspace."""
+    total = lib.dsa_mla_shared_workspace_bytes(B, H, nsplit)
+    shapes = [(b, h, n) for b in (1, 2, 3, 5, 8, 31, 32, 33, 100, 256, 257, 300) for h in (16, 32, 48, 64, 128, 1024)
+              for n in (0, 1, 2, 3, 8, 64, 65, 128)] + [(B, H, n) for n in range(129)]
+    # (what an 8-bit call needs is least for one split)
+    last = max(_barriers(b, h) for b, h, _ in shapes if lib.dsa_sparse_mla_workspace_bytes(b, h, 1) <= total)
+    assert last >= _barriers(B, H)
+    took = refused = 0
+    for b, h, n in shapes:
+        at, need = lib.dsa_mla_fp4_workspace_in(total, b, h, n), lib.dsa_mla_fp4_workspace_bytes(b, h, n)
+        if at < 0:
+            refused += 1
+        elif need > 16:                                      # (16: nothing is read or written)
+            took += 1
+            assert last <= at + _barriers(b, h) and at + need <= total and at % 16 == 0, (b, h, n)
+    assert took and refused
+    if nsplit == 0:  # sized for every count of splits, and for fewer rows
+        assert all(lib.dsa_mla_fp4_workspace_in(total, b, H, n) >= 0 for b in range(1, B + 1) for n in range(129))
+    else:
+        assert lib.dsa_mla_fp4_workspace_in(total, B, H, nsplit) >= 0
+    # the partials begin where those of an 8-bit call of these rows and heads would, counted from there
+    assert lib.dsa_sparse_mla_barrier_bytes(B, H, 0) == _barriers(B, H)
+
+
+def test_shared_workspace_contract(lib):
+    assert lib.dsa_mla_shared_workspace_bytes(1, 15, 8) == 0 and lib.dsa_mla_shared_workspace_bytes(0, 16, 8) == 0
+    assert lib.dsa_mla_shared_workspace_bytes(1, 16, 129) == 0
+    f = lib.dsa_mla_fp4_workspace_in
+    assert f(1 << 30, 1, 15, 8) == -1 and f(1 << 30, 1, 16, -1) == -1 and f(0, 1, 16, 8) == -1
+    assert f(16, 7, 16, 1) == 0 and f(15, 7, 16, 1) == -1    # unsplit rows read none
+    from lagged_indexer_dsa_amd import ops
+
+    for B, H, n in ((1, 16, 8), (5, 32, 1), (4, 16, 0)):
+        assert ops.sparse_mla_workspace(B, H, n, "cpu").nbytes == lib.dsa_mla_shared_workspace_bytes(B, H, n)
+    with pytest.raises(RuntimeError):
+        ops.sparse_mla_workspace(1, 24, 8, "cpu")
