@@ -33,7 +33,9 @@ def _dev(*tensors: torch.Tensor) -> None:
             raise RuntimeError("lagged_indexer_dsa_amd ops need contiguous tensors")
 
 
-_current_device = torch._C._cuda_getDevice
+def _current_device() -> int:
+    # (looked up in the call: a torch without a GPU backend has no such function)
+    return torch._C._cuda_getDevice()
 
 
 def _stream() -> int:

@@ -8,6 +8,7 @@ from __future__ import annotations
 import math
 import shutil
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -153,6 +154,32 @@ def test_ops_refuse_cpu_tensors():
                                                torch.zeros(4, 400, dtype=torch.uint8), i[None])):
         with pytest.raises(RuntimeError, match="no CPU path"):
             call()
+
+
+def test_import_on_a_torch_without_a_gpu_backend():
+    """Such a torch has none of the device functions that a call looks up: the
+    package imports, and its ops refuse CPU tensors with their own message."""
+    from conftest import PKG_ROOT
+
+    code = f"""
+import sys, torch
+for name in [n for n in dir(torch._C) if n.startswith("_cuda_")]:
+    delattr(torch._C, name)
+sys.path.insert(0, {str(PKG_ROOT)!r})
+from lagged_indexer_dsa_amd import ops
+i = torch.zeros(2, dtype=torch.int32)
+for call in (lambda: ops.rms_norm(torch.zeros(2, 64), torch.ones(64)),
+             lambda: ops.read_latent_rows(torch.zeros(4, 400, dtype=torch.uint8), i),
+             lambda: ops.sparse_mla_decode(torch.zeros(1, 16, 576, dtype=torch.bfloat16),
+                                           torch.zeros(4, 656, dtype=torch.uint8), i[None])):
+    try:
+        call()
+        sys.exit("no refusal")
+    except RuntimeError as e:
+        assert "no CPU path" in str(e), e
+"""
+    res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr[-2000:]
 
 
 def test_decode_layer_refuses_4bit_pool():
