@@ -48,7 +48,9 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// Where a token goes.  slot < 0: nowhere (no request, page, row or table row).
+// Where a token goes, in both caches.  slot < 0: nowhere (no request, page or
+// table row, or a place that one of the caches that are given does not have: a
+// key whose latent row is not there could be selected).
 struct Place {
   int pos;
   long page, slot;
@@ -59,7 +61,8 @@ __device__ __forceinline__ Place place_of(const AppendArgs& A, int t) {
   if (r < 0 || r >= A.B || p.pos < 0 || p.pos / DSA_PAGE_TOKENS >= A.pt_stride || (A.table && p.pos >= A.table_rows))
     return p;
   p.page = A.page_table[(long)r * A.pt_stride + p.pos / DSA_PAGE_TOKENS];
-  p.slot = p.page < 0 ? -1 : p.page * DSA_PAGE_TOKENS + p.pos % DSA_PAGE_TOKENS;
+  p.slot = p.page * DSA_PAGE_TOKENS + p.pos % DSA_PAGE_TOKENS;
+  if (p.page < 0 || (A.latent && p.slot >= A.kv_rows) || (A.keys && p.page >= A.num_pages)) p.slot = -1;
   return p;
 }
 
@@ -81,7 +84,7 @@ __device__ __forceinline__ void append_latent_row(const AppendArgs& A, int t) {
     else load8<DT, WIDE>(A.norm_w, 8 * lane, w);
   }
   const Place p = place_of(A, t);
-  if (p.slot < 0 || p.slot >= A.kv_rows) return;
+  if (p.slot < 0) return;
   float c = 1.f, s = 0.f;
   if (A.table) {
     c = A.table[(long)p.pos * DSA_ROPE_DIM + pair];
@@ -129,7 +132,7 @@ __device__ __forceinline__ void append_key(const AppendArgs& A, int t) {
   const bool turned = A.table && i < DSA_ROPE_DIM / 8;
   if (turned && !A.index_interleaved) load8<DT, WIDE>(A.keys, src + 8 * (i ^ 4), o);
   const Place p = place_of(A, t);
-  if (p.page < 0 || p.page >= A.num_pages) return;
+  if (p.slot < 0) return;
   if (turned) {
     constexpr int kHalf = DSA_ROPE_DIM / 2;
     const float* cs = A.table + (long)p.pos * DSA_ROPE_DIM;

@@ -712,8 +712,9 @@ def append_tokens(page_table: torch.Tensor, rows: torch.Tensor, pos: torch.Tenso
     scale per 32).  keys [n, 128]: the first 64 turned, into index_k [pages,
     8448].  Either pair may be left out.  latent and keys are fp32, bf16 or
     fp16, rows any one stride apart; norm_weight of the same type or fp32.  A
-    token without a request, page, slot or table row is skipped; two tokens of
-    one slot must hold the same values.
+    token without a request, page, slot or table row is skipped, in both caches
+    where one of them has no place for it; two tokens of one slot must hold the
+    same values.
     Reference: sglang overlay P:252-363, P:789; dsa_layer.py:92-143.
     """
     dev = rows.get_device()

@@ -493,8 +493,8 @@ int dsa_rotary(const dsa_rotary_args* args, void* stream);
  *     index_k as in (6).
  *   latent, keys and a norm_weight that is not fp32 are of one type; row
  *   strides in elements.  A token whose request, position, page, slot or table
- *   row is out of range is skipped.  Two tokens of a call with one slot must
- *   hold the same values.
+ *   row is out of range is skipped, in both caches if it is out of one's.  Two
+ *   tokens of a call with one slot must hold the same values.
  * Replaces: forward_hide_operands' key side (P:252-363, P:789) with the norm
  * and rope before it (DL:92-143).
  */

@@ -203,6 +203,40 @@ def test_tokens_without_a_place_are_skipped(dev, bits):
 
 
 @pytest.mark.parametrize("bits", [8, 4])
+@pytest.mark.parametrize("kv_rows,pages", [(128, 4), (256, 2), (150, 3)])
+def test_a_token_is_in_both_caches_or_in_none(dev, bits, kv_rows, pages):
+    """Caches of other capacities: what one has no place for, the other does not
+    hold either; a call for one of them goes by that one's capacity."""
+    from lagged_indexer_dsa_amd import ops
+
+    print(f"[append] caches of other capacities {(bits, kv_rows, pages)}", flush=True)
+    row = 656 if bits == 8 else 400
+    pt = torch.tensor([[3, 1, 2, 0]], dtype=torch.int32, device=dev)
+    pos = torch.arange(5, 256, 10, dtype=torch.int32, device=dev)
+    rows = torch.zeros_like(pos)
+    g = torch.Generator(device=dev).manual_seed(5)
+    lat, keys = torch.randn(len(pos), 576, device=dev, generator=g), torch.randn(len(pos), 128, device=dev, generator=g)
+    slots = pt[0].long()[pos.long() // 64] * 64 + pos.long() % 64
+    in_kv, in_idx = slots < kv_rows, slots // 64 < pages
+    assert bool((in_kv & in_idx).any()) and bool((~(in_kv & in_idx)).any())
+
+    def held(**kw):
+        pool = torch.full((kv_rows, row), 0x11, dtype=torch.uint8, device=dev)
+        idx = torch.full((pages, 8448), 0x22, dtype=torch.uint8, device=dev)
+        both = dict(kv_pool=pool, latent=lat, index_k=idx, keys=keys)
+        ops.append_tokens(pt, rows, pos, **{k: v for k, v in both.items() if k in kw["of"]})
+        a = (pool != 0x11).any(1).nonzero().flatten()
+        codes, scales = idx[:, :8192].reshape(pages * 64, 128), idx[:, 8192:].reshape(pages * 64, 4)
+        b, s = (codes != 0x22).any(1).nonzero().flatten(), (scales != 0x22).any(1).nonzero().flatten()
+        assert torch.equal(b, s)
+        return a.tolist(), b.tolist()
+    want = lambda m: sorted(slots[m].tolist())  # noqa: E731
+    assert held(of=("kv_pool", "latent", "index_k", "keys")) == (want(in_kv & in_idx), want(in_kv & in_idx))
+    assert held(of=("kv_pool", "latent")) == (want(in_kv), [])
+    assert held(of=("index_k", "keys")) == ([], want(in_idx))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
 def test_slots_past_2_31_bytes(dev, bits):
     from lagged_indexer_dsa_amd import ops
 
