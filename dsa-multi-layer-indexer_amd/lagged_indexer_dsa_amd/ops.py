@@ -710,7 +710,9 @@ def append_tokens(page_table: torch.Tensor, rows: torch.Tensor, pos: torch.Tenso
     is given (:func:`rotary`'s pairs and table), into kv_pool: [rows, 656]
     uint8 (e4m3, a scale per 128) or [rows, 400] (4-bit e2m1, a power-of-two
     scale per 32).  keys [n, 128]: the first 64 turned, into index_k [pages,
-    8448].  Either pair may be left out.  latent and keys are fp32, bf16 or
+    8448].  A NaN makes its 128 values' (4 bits: 32 values') scale NaN, where
+    :func:`append_index_keys` and :func:`append_latent_rows` pass it over.  Either
+    pair may be left out.  latent and keys are fp32, bf16 or
     fp16, rows any one stride apart; norm_weight of the same type or fp32.  A
     token without a request, page, slot or table row is skipped, in both caches
     where one of them has no place for it; two tokens of one slot must hold the

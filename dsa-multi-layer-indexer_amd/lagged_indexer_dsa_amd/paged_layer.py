@@ -18,8 +18,10 @@ timed hot path.  Shapes the kernels accept: kv_lora_rank 512, rope 64
 attention heads a multiple of 16.
 
 With ``kv_bits=4`` the latent pool holds 400-byte rows (39 % less cache); the
-keys and rows of new tokens are then stored by ``ops.append_tokens`` and the
-attention is a launch of its own beside the layer's scan and top-k.
+latent rows of new tokens are then stored by ``ops.append_tokens``, the index
+keys as with 8 bits (the selections do not depend on kv_bits, for keys with a
+NaN either), and the attention is a launch of its own ahead of the layer's scan
+and top-k.
 
 Index convention: selections cross this API as token positions, int64
 ``[B, 1, topk]`` like ``select_topk`` returns them, with the sentinel
@@ -88,11 +90,11 @@ class PagedDSALayer:
         posb = pos.repeat(B)
         keys = index_k.reshape(B * S, INDEX_DIM).to(torch.bfloat16).contiguous()
         latent = kv.reshape(B * S, QK_DIM).to(torch.bfloat16).contiguous()
+        # (append_tokens has another rule for a key with a NaN: its scale is NaN)
+        ops.append_index_keys(self.index_k, self.page_table, rows, posb, keys)
         if self.kv_bits == 4:
-            ops.append_tokens(self.page_table, rows, posb, kv_pool=self.kv_pool, latent=latent, index_k=self.index_k,
-                              keys=keys)
+            ops.append_tokens(self.page_table, rows, posb, kv_pool=self.kv_pool, latent=latent)
         else:
-            ops.append_index_keys(self.index_k, self.page_table, rows, posb, keys)
             slots = (rows.long() * self.cap + posb.long()).to(torch.int32)
             ops.append_latent_rows(self.kv_pool, slots, latent)
         self.length += S

@@ -490,7 +490,9 @@ int dsa_rotary(const dsa_rotary_args* args, void* stream);
  *     byte 255.  The last 64 turned by (9)'s rule when cos_sin [table_rows, 64]
  *     is given, rounded to bf16.
  *   keys [n, 128] (NULL: none): the first 64 values turned, quantised into
- *     index_k as in (6).
+ *     index_k by (6)'s rule, but a NaN makes the key's scale and codes NaN
+ *     ((6)'s append passes it over: its code is -448, the scale that of the
+ *     other values).
  *   latent, keys and a norm_weight that is not fp32 are of one type; row
  *   strides in elements.  A token whose request, position, page, slot or table
  *   row is out of range is skipped, in both caches if it is out of one's.  Two

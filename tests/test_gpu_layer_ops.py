@@ -199,3 +199,26 @@ def test_paged_layer_with_a_4bit_pool(dev, batch):
         assert _lib.sync_timeouts() == 0
         with pytest.raises(ValueError):
             PagedDSALayer(layer, batch=1, max_ctx=64, device=dev, kv_bits=5)
+
+
+def test_paged_layers_keep_the_same_index_keys(dev):
+    """Keys with a NaN or an infinity too: the index cache, and so the selection,
+    is the same with latent rows of 8 and of 4 bits."""
+    from lagged_indexer_dsa_amd.paged_layer import PagedDSALayer
+
+    print("[layer ops] index keys with NaN", flush=True)
+    layer = _Layer(torch.Generator().manual_seed(7)).to(dev)
+    g = torch.Generator(device=dev).manual_seed(3)
+    keys, kv = torch.randn(2, 70, 128, device=dev, generator=g), torch.randn(2, 70, 576, device=dev, generator=g)
+    keys[0, 3, 17], keys[1, 69, 100], keys[1, 5, 0] = float("nan"), float("nan"), float("inf")
+    keys[0, 64] = float("nan")
+    p4, p8 = (PagedDSALayer(layer, batch=2, max_ctx=128, device=dev, kv_bits=b) for b in (4, 8))
+    for p in (p4, p8):
+        p._append(keys[:, :69], kv[:, :69])
+        p._append(keys[:, 69:], kv[:, 69:])
+    assert torch.equal(p4.index_k, p8.index_k) and bool(p4.index_k.any())
+    back = O.dequant_latent_rows_fp4(p4.kv_pool.cpu().numpy())
+    ref = O.pack_latent_rows_fp4(kv[:, :, :512].to(torch.bfloat16).float().cpu().numpy().reshape(140, 512),
+                                 kv[:, :, 512:].float().cpu().numpy().reshape(140, 64))
+    rows = np.r_[0:70, 128:198]
+    assert np.array_equal(back[rows], O.dequant_latent_rows_fp4(ref))
