@@ -53,8 +53,8 @@ constexpr int kM4Heads = 32;         // heads a workgroup
 constexpr int kM4Group = 32;         // keys a wave scores
 constexpr int kM4Groups = 4;         // of a tile
 constexpr int kM4Unit = kM4Groups * kM4Group;  // keys a tile: chunks are multiples
-constexpr int kM4MergeMax = 512;     // chunks of a row
-constexpr int kM4Ragged = 256;       // rows that share chunks by their lengths
+constexpr int kM4MergeMax = 512;     // chunks of up to kM4Ragged rows together
+constexpr int kM4Ragged = 256;       // most rows that share chunks by their lengths
 constexpr float kM4Rise = 16.f;      // log2 growth of the maximum that rescales the sums
 constexpr int kM4Buffers = 3;        // tiles of rows: summed, scored, on their way
 constexpr int kM4GroupLds = kM4Group * DSA_FP4_ROW_BYTES;
@@ -609,8 +609,9 @@ __global__ __launch_bounds__(W* kWave) void mla_fp4_merge_kernel(const Mla4Args 
 }
 
 // Chunks the rows share: nsplit a row, or (0) what fills the chip once, one
-// workgroup a CU; at most kM4MergeMax where one row may take them all
-// (kM4Ragged rows and fewer).  Measured around 0's choice: 32 rows of 2048
+// workgroup a CU; at most kM4MergeMax for kM4Ragged rows and fewer, dense or
+// selected (one dense row may take them all; the partials then stay within 17 MB
+// for 16 heads, and twice the chip's CUs are there already).  Measured around 0's choice: 32 rows of 2048
 // selected keys, 16 heads: 26.0 us at 2 a row, 19.4 at 4, 18.5 at 8 (0's), 23.5
 // at 16; 8 rows of 16K keys, 128 heads: 76.8 at 4, 52.0 at 8 (0's), 55.8 at 16.
 // Dense rows share by length wherever there are more chunks than rows: 100 rows

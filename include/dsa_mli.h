@@ -534,11 +534,13 @@ int dsa_read_latent_rows(const void* kv_pool, int64_t kv_rows, int row_bytes, co
  * dsa_mla_fp4_workspace_in(w, B, H, nsplit) bytes on: its partial sums then lie
  * behind every barrier of any call that w is enough for.  (-1: w is not enough.)
  * nsplit: the chunks of keys a row is cut into, 1 to 128, or 0 for as many as
- * fill the device once (one a row, where there are that many rows).
- * 256 or fewer dense rows share B * nsplit chunks (512 at most) by their
+ * fill the device once (one a row, where there are that many rows).  Up to 256
+ * rows are cut into 512 chunks at most together (or one a row), so fewer than
+ * nsplit each where B * nsplit is more.  Dense rows, up to 256, share them by their
  * lengths, so where a row is cut, and the last bits of its output, depend on
- * the other rows' lengths; the same call always gives the same.  No workgroup
- * waits for another.
+ * the other rows' lengths; the same call always gives the same.  More dense rows
+ * are each cut alike, by what the page table has room for.  No workgroup waits for
+ * another.
  */
 size_t dsa_mla_fp4_workspace_bytes(int B, int H, int nsplit);
 size_t dsa_mla_shared_workspace_bytes(int B, int H, int nsplit);

@@ -151,6 +151,27 @@ def test_every_count_of_tiles(dev, H, nsplit):
     _check(out, q, O.dequant_latent_rows_fp4(rows), idx)
 
 
+@pytest.mark.parametrize("B,nsplit,least", [(8, 128, 64), (3, 128, 128), (200, 4, 2)])
+def test_long_selections_in_as_many_chunks_as_there_may_be(dev, B, nsplit, least):
+    """512 chunks for all rows together: a larger split count gives the bits of the
+    one that reaches them."""
+    from lagged_indexer_dsa_amd import _lib, ops
+
+    topk = 16384 if B < 100 else 700
+    print(f"[fp4 chunks] {(B, topk, nsplit)}", flush=True)
+    rng = np.random.default_rng(B)
+    rows, q = _pool(33, topk + 1000), _q(33, B, 16)
+    idx = np.stack([rng.permutation(topk + 1000)[:topk] for _ in range(B)]).astype(np.int32)
+    idx[rng.random(idx.shape) < 0.01] = -1
+    args = _dev(q, dev, True), _dev(rows, dev), _dev(idx, dev)
+    out = ops.sparse_mla_decode(*args, nsplit=nsplit)
+    _check(out, q, O.dequant_latent_rows_fp4(rows), idx)
+    assert torch.equal(out, ops.sparse_mla_decode(*args, nsplit=least))
+    size = _lib.load().dsa_mla_fp4_workspace_bytes
+    # (partials of a chunk and 16 heads; 25 lines of 64 words a barrier; a row's plan)
+    assert size(B, 16, nsplit) == min(512, B * nsplit) * 16 * 514 * 4 + B * (25 * 64 * 4 + 8)
+
+
 @pytest.mark.parametrize("sm", [0.0, -SM, 0.02])
 def test_other_scales(dev, sm):
     """A scale that is not positive is applied before the maximum is taken.
