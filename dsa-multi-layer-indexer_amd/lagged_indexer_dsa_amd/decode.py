@@ -54,7 +54,7 @@ class DecodeLayer:
         self.scores = torch.empty(B, self.slab_stride, dtype=torch.float32, device=dev)
         self.topk_scratch = topk_scratch(B, self.slab_stride, dev)
         self.next_idx = torch.full((B, self.topk), -1, dtype=torch.int32, device=dev)
-        self.workspace = sparse_mla_workspace(B, self.q_bf16.shape[1], self.nsplit, dev)
+        self.workspace = sparse_mla_workspace(B, self.q_bf16.shape[1], self.nsplit, dev, kv_bits=8)
         self.out = torch.zeros(B, self.q_bf16.shape[1], 512, dtype=torch.bfloat16, device=dev)
 
     @property

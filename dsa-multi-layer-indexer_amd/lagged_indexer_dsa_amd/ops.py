@@ -153,16 +153,21 @@ def select_rows(scores: torch.Tensor, k: int, pad_value: int) -> torch.Tensor | 
     return out
 
 
-def sparse_mla_workspace(B: int, H: int, nsplit: int, device) -> torch.Tensor:
+def sparse_mla_workspace(B: int, H: int, nsplit: int, device, kv_bits: int | None = None) -> torch.Tensor:
     """Zero-filled workspace (split partials + the splits' barriers; every
     call leaves the barriers ready), for pools of either row format.  nsplit=0
-    sizes it for any split count.
+    sizes it for any split count; kv_bits=8 for pools of 656-byte rows only (for
+    a few rows less than half the bytes).
 
     Calls over 400-byte rows of any B and H that it is enough for may use it, in
     turn with calls over 656-byte rows.  Those must all be of one B * H: their
     partials begin behind as many barriers as the call itself has.
     """
-    nbytes = _lib.load().dsa_mla_shared_workspace_bytes(B, H, nsplit)
+    lib = _lib.load()
+    if kv_bits not in (None, 4, 8):
+        raise ValueError(f"latent rows are kept in 8 or 4 bits, got {kv_bits}")
+    size = lib.dsa_sparse_mla_workspace_bytes if kv_bits == 8 else lib.dsa_mla_shared_workspace_bytes
+    nbytes = size(B, H, nsplit)
     if nbytes == 0:
         raise RuntimeError(f"bad sparse MLA workspace shape B={B} H={H} nsplit={nsplit}")
     return torch.zeros(nbytes // 4, dtype=torch.float32, device=device)

@@ -72,7 +72,7 @@ class PagedDSALayer:
         self.next_idx = torch.full((B, self.topk), -1, dtype=torch.int32, device=dev)
         self.attend = torch.full((B, self.topk), -1, dtype=torch.int32, device=dev)
         self.nsplit = int(nsplit)
-        self.workspace = ops.sparse_mla_workspace(B, self.H, self.nsplit, dev)
+        self.workspace = ops.sparse_mla_workspace(B, self.H, self.nsplit, dev, kv_bits=self.kv_bits)
         self.out = torch.zeros(B, self.H, LATENT_DIM, dtype=torch.bfloat16, device=dev)
         self.q_fp8 = torch.empty(B, self.Hidx, INDEX_DIM, dtype=torch.uint8, device=dev)
         self.w = torch.empty(B, self.Hidx, dtype=torch.float32, device=dev)

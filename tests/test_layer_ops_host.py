@@ -339,3 +339,22 @@ def test_shared_workspace_contract(lib):
         assert ops.sparse_mla_workspace(B, H, n, "cpu").nbytes == lib.dsa_mla_shared_workspace_bytes(B, H, n)
     with pytest.raises(RuntimeError):
         ops.sparse_mla_workspace(1, 24, 8, "cpu")
+
+
+def test_workspace_of_8bit_layers(lib):
+    """A layer over 656-byte rows holds what its calls need and no 4-bit partials."""
+    from lagged_indexer_dsa_amd import ops
+    from lagged_indexer_dsa_amd.decode import DecodeLayer
+
+    for B, H, n in ((1, 16, 0), (3, 32, 8), (100, 16, 0)):
+        want = lib.dsa_sparse_mla_workspace_bytes(B, H, n)
+        assert ops.sparse_mla_workspace(B, H, n, "cpu", kv_bits=8).nbytes == want
+        for bits in (None, 4):
+            assert ops.sparse_mla_workspace(B, H, n, "cpu", kv_bits=bits).nbytes == lib.dsa_mla_shared_workspace_bytes(B, H, n)
+        layer = DecodeLayer(q_fp8=None, w=None, index_k=None, q_bf16=torch.zeros(B, H, 576, dtype=torch.bfloat16),
+                            kv_pool=torch.zeros(64, 656, dtype=torch.uint8),
+                            page_table=torch.zeros(B, 1, dtype=torch.int32), seq_lens=torch.zeros(B, dtype=torch.int32),
+                            slab_stride=64, nsplit=n)
+        assert layer.workspace.nbytes == want
+    with pytest.raises(ValueError):
+        ops.sparse_mla_workspace(1, 16, 0, "cpu", kv_bits=6)
