@@ -151,6 +151,38 @@ def test_every_count_of_tiles(dev, H, nsplit):
     _check(out, q, O.dequant_latent_rows_fp4(rows), idx)
 
 
+@pytest.mark.parametrize("nsplit", [1, 0, 3])
+@pytest.mark.parametrize("H", [16, 48])
+def test_one_key_at_every_border(dev, H, nsplit):
+    """Rows whose queries look like one key, which then holds nearly all of the
+    weight (a score of about 24 where others are near 1): the output is that key's
+    value, so the loss of any one at a border of a tile (128 keys), of a wave's
+    part (32), of a page (64) or of a row's end shows in every dim."""
+    from lagged_indexer_dsa_amd import ops
+
+    print(f"[fp4 borders] {(H, nsplit)}", flush=True)
+    n = 2500
+    at = np.unique(np.clip([128 * k + d for k in range(20) for d in (-1, 0)] + [31, 32, 33, 63, 64, 65, 95, 96, 2495, 2499], 0, n - 1))
+    B, pts = len(at), -(-n // 64)
+    rng = np.random.default_rng(H + nsplit)
+    rows = O.pack_latent_rows_fp4(rng.standard_normal((pts * 64, 512)).astype(np.float32),
+                                  rng.standard_normal((pts * 64, 64)).astype(np.float32))
+    kv = O.dequant_latent_rows_fp4(rows)
+    pt = rng.permutation(pts).astype(np.int32)
+    j = np.arange(n)
+    slots = pt[j // 64].astype(np.int64) * 64 + j % 64
+    q = O.bf16_rn(kv[slots[at]][:, None] * np.linspace(0.9, 1.1, H, dtype=np.float32)[None, :, None])
+    idx = np.repeat(slots[None], B, 0)
+    weight = np.exp(np.einsum("bhd,bd->bh", q.astype(np.float64), kv[slots[at]].astype(np.float64)) * SM)
+    assert weight.min() > 100 * n * np.exp(2.0)                    # the key outweighs the rest
+    qd, pool, ptd = _dev(q, dev, True), _dev(rows, dev), _dev(np.repeat(pt[None], B, 0), dev)
+    _check(ops.sparse_mla_decode(qd, pool, _dev(idx.astype(np.int32), dev), nsplit=nsplit), q, kv, idx)
+    # dense: the whole row; rows that end with the key; rows that end just before it
+    for lens in (np.full(B, n), at + 1, at):
+        cut = np.where(j[None] < lens[:, None], idx, -1)
+        _check(ops.dense_mla_decode(qd, pool, ptd, _dev(lens.astype(np.int32), dev), nsplit=nsplit), q, kv, cut)
+
+
 @pytest.mark.parametrize("B,nsplit,least", [(8, 128, 64), (3, 128, 128), (200, 4, 2)])
 def test_long_selections_in_as_many_chunks_as_there_may_be(dev, B, nsplit, least):
     """512 chunks for all rows together: a larger split count gives the bits of the
