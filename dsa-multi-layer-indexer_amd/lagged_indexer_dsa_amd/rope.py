@@ -70,6 +70,8 @@ def rope_frequencies(dim: int, theta: float = 10000.0, scaling: RopeScaling | No
         return dim * math.log(scaling.original_max_pos / (2 * math.pi * turns)) / (2 * math.log(theta))
     lo = max(math.floor(pair_of(scaling.beta_fast)), 0)
     hi = min(math.ceil(pair_of(scaling.beta_slow)), dim - 1)
+    if hi <= 0:  # not even the first pair turns beta_slow times
+        return f / scaling.factor
     ramp = ((i - lo) / max(hi - lo, 1e-3)).clamp(0.0, 1.0)
     return f * (1.0 - ramp) + f / scaling.factor * ramp
 

@@ -60,6 +60,23 @@ def test_scaled_frequencies():
     assert float(t[0, 0]) == 1.0
 
 
+def test_yarn_where_no_pair_turns_often():
+    """A trained context in which even the fastest pair turns less than beta_slow
+    times: every pair is slowed by the factor, the first too; one in which the
+    slowest turns more than beta_fast times: none is."""
+    from lagged_indexer_dsa_amd.rope import RopeScaling, rope_frequencies
+
+    f = rope_frequencies(64, 10000.0)
+    for kw in (dict(original_max_pos=6), dict(original_max_pos=1), dict(original_max_pos=100, beta_slow=20.0),
+               dict(original_max_pos=4, beta_fast=1.0)):
+        assert 0.5 * kw["original_max_pos"] / math.pi < kw.get("beta_slow", 1.0)       # pair 0's turns
+        assert torch.allclose(rope_frequencies(64, 10000.0, RopeScaling("yarn", 8.0, **kw)), f / 8, rtol=1e-15), kw
+    assert torch.equal(rope_frequencies(64, 10000.0, RopeScaling("yarn", 8.0, original_max_pos=1 << 24)), f)
+    # at the first pair's own count of turns the ramp begins with it
+    y = rope_frequencies(64, 10000.0, RopeScaling("yarn", 8.0, original_max_pos=200, beta_slow=1.0, beta_fast=40.0))
+    assert y[0] == f[0] and torch.allclose(y[-1], f[-1] / 8, rtol=1e-15)
+
+
 def test_rope_refusals():
     from lagged_indexer_dsa_amd.rope import RopeScaling, build_rope_table
 
