@@ -160,6 +160,14 @@ struct RopeArgs {
   long max_pos;
   int heads, tokens;  // filled by the launcher: of each, those of a workgroup
 };
+// A launch holds fewer than 2^32 threads (the runtime cuts larger ones down, and
+// says nothing): n items as launches of `most` at a time.  launch(first, count).
+template <class F>
+hipError_t in_launches(long n, long most, F launch) {
+  for (long at = 0; at < n; at += most)
+    if (const hipError_t e = launch(at, n - at < most ? n - at : most)) return e;
+  return hipSuccess;
+}
 hipError_t launch_rms_norm(const NormArgs& A, int dtype, hipStream_t s);
 hipError_t launch_rotary(const RopeArgs& A, int dtype, hipStream_t s);
 

@@ -175,11 +175,17 @@ static hipError_t launch_append_dt(const AppendArgs& A, int row_bytes, hipStream
   const auto on16 = [](const void* p, long stride) { return (((uintptr_t)p | (uintptr_t)(stride * es)) & 15) == 0; };
   const bool wide = (!A.latent || on16(A.latent, A.latent_stride)) && (!A.keys || on16(A.keys, A.keys_stride)) &&
                     on16(A.norm_w, 0);
-  const long units = (A.latent ? A.n : 0) + (A.keys ? (A.n + 3L) / 4 : 0);
-  const dim3 grid((unsigned)((units + kAppendUnits - 1) / kAppendUnits));
   const auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(kAppendThreads), 0, s, A);
-    return hipGetLastError();
+    // (a token has up to a wave and a quarter)
+    return in_launches(A.n, 1L << 25, [&](long at, long n) {
+      AppendArgs P = A;
+      P.rows += at, P.pos += at, P.n = (int)n;
+      if (A.latent) P.latent = static_cast<const uint8_t*>(A.latent) + at * A.latent_stride * es;
+      if (A.keys) P.keys = static_cast<const uint8_t*>(A.keys) + at * A.keys_stride * es;
+      const long units = (A.latent ? n : 0) + (A.keys ? (n + 3) / 4 : 0);
+      hipLaunchKernelGGL(kernel, dim3((unsigned)((units + kAppendUnits - 1) / kAppendUnits)), dim3(kAppendThreads), 0, s, P);
+      return hipGetLastError();
+    });
   };
   if (row_bytes == DSA_LATENT_ROW_BYTES)
     return wide ? go(append_tokens_kernel<DT, true, DSA_LATENT_ROW_BYTES>)
@@ -250,14 +256,14 @@ hipError_t launch_read_latent(const void* pool, long kv_rows, int row_bytes, con
                               hipStream_t s) {
   if (n <= 0) return hipSuccess;
   constexpr int per = kAppendUnits * kReadRows;
-  const dim3 grid((unsigned)(((long)n + per - 1) / per));
-  const uint8_t* p = static_cast<const uint8_t*>(pool);
-  uint16_t* o = static_cast<uint16_t*>(out);
-  if (row_bytes == DSA_LATENT_ROW_BYTES)
-    hipLaunchKernelGGL(read_latent_kernel<DSA_LATENT_ROW_BYTES>, grid, dim3(kAppendThreads), 0, s, p, kv_rows, slots, n, o);
-  else
-    hipLaunchKernelGGL(read_latent_kernel<DSA_FP4_ROW_BYTES>, grid, dim3(kAppendThreads), 0, s, p, kv_rows, slots, n, o);
-  return hipGetLastError();
+  const auto kernel = row_bytes == DSA_LATENT_ROW_BYTES ? read_latent_kernel<DSA_LATENT_ROW_BYTES>
+                                                        : read_latent_kernel<DSA_FP4_ROW_BYTES>;
+  return in_launches(n, 1L << 26, [&](long at, long rows) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((rows + per - 1) / per)), dim3(kAppendThreads), 0, s,
+                       static_cast<const uint8_t*>(pool), kv_rows, slots + at, (int)rows,
+                       static_cast<uint16_t*>(out) + at * DSA_QK_DIM);
+    return hipGetLastError();
+  });
 }
 
 }  // namespace dsa

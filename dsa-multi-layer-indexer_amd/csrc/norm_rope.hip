@@ -385,18 +385,23 @@ static hipError_t launch_rotary_dt(RopeArgs A, hipStream_t s) {
   // a workgroup: as many heads of a token as fit, then as many tokens
   A.heads = items >= kRopeThreads ? 1 : std::min(A.H, kRopeThreads / items);
   A.tokens = std::max(1, kRopeThreads / (A.heads * items));
-  const long x = ((long)A.n + A.tokens - 1) / A.tokens;
+  const auto blocks = [&](long n) { return (n + A.tokens - 1) / A.tokens; };
   // few tokens: their heads over several workgroups (a token of 128 heads of
   // 192 values: 3.4 us; in one workgroup 6.3)
   const int turns = (A.H + A.heads - 1) / A.heads;
-  const int y = (int)std::max(1L, std::min({(long)turns, 65535L, 2L * device_cu_count() / x}));
-  const dim3 grid((unsigned)x, (unsigned)y);
-  const auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(kRopeThreads), 0, s, A);
+  const int y = (int)std::max(1L, std::min({(long)turns, 65535L, 2L * device_cu_count() / blocks(A.n)}));
+  const auto kernel = A.interleaved ? (wide ? rotary_kernel<DT, true, true> : rotary_kernel<DT, false, true>)
+                                    : (wide ? rotary_kernel<DT, true, false> : rotary_kernel<DT, false, false>);
+  constexpr long kMostBlocks = (1L << 31) / kRopeThreads;
+  return in_launches(A.n, kMostBlocks * A.tokens, [&](long at, long n) {
+    RopeArgs P = A;
+    P.x = static_cast<const uint8_t*>(A.x) + at * A.xn * es;
+    P.out = static_cast<uint8_t*>(A.out) + at * A.on * es;
+    P.pos = static_cast<const uint8_t*>(A.pos) + at * (A.pos64 ? 8 : 4);
+    P.n = (int)n;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks(n), (unsigned)y), dim3(kRopeThreads), 0, s, P);
     return hipGetLastError();
-  };
-  if (A.interleaved) return wide ? go(rotary_kernel<DT, true, true>) : go(rotary_kernel<DT, false, true>);
-  return wide ? go(rotary_kernel<DT, true, false>) : go(rotary_kernel<DT, false, false>);
+  });
 }
 
 hipError_t launch_rotary(const RopeArgs& A, int dtype, hipStream_t s) {

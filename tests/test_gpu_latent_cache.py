@@ -257,6 +257,53 @@ def test_slots_past_2_31_bytes(dev, bits):
     assert np.array_equal(ops.read_latent_rows(pool, slots).float().cpu().numpy(), vals)
 
 
+def test_append_of_more_tokens_than_a_launch_holds(dev):
+    """A wave a token: 2^26 are more than a launch has.  Nearly all are padding;
+    those with a place are at the borders of the launches it takes."""
+    from lagged_indexer_dsa_amd import ops
+
+    print("[append] 2^26 + 9 tokens", flush=True)
+    n = (1 << 26) + 9
+    at = torch.tensor([0, 1, (1 << 25) - 1, 1 << 25, (1 << 25) + 3, (1 << 26) - 1, 1 << 26, n - 2, n - 1], device=dev)
+    rows = torch.full((n,), -1, dtype=torch.int32, device=dev)
+    pos = torch.zeros(n, dtype=torch.int32, device=dev)
+    rows[at] = 0
+    pos[at] = 7 * torch.arange(len(at), device=dev, dtype=torch.int32)
+    g = torch.Generator(device=dev).manual_seed(4)
+    lat, keys = torch.randn(1, 576, device=dev, generator=g), torch.randn(1, 128, device=dev, generator=g)
+    pt = torch.tensor([[1]], dtype=torch.int32, device=dev)
+    pool, idx = torch.zeros(128, 400, dtype=torch.uint8, device=dev), torch.zeros(2, 8448, dtype=torch.uint8, device=dev)
+    ops.append_tokens(pt, rows, pos, kv_pool=pool, latent=lat.expand(n, 576), index_k=idx, keys=keys.expand(n, 128))
+    slots = [64 + 7 * k for k in range(len(at))]
+    assert pool.any(1).nonzero().flatten().tolist() == slots
+    assert idx[:, :8192].reshape(128, 128).any(1).nonzero().flatten().tolist() == slots
+    x = lat.cpu().numpy()
+    assert np.array_equal(pool[slots].cpu().numpy(), np.repeat(_pack(4, x[:, :512], x[:, 512:]), len(at), 0))
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_read_in_more_than_one_launch(dev, bits):
+    """2^26 rows a launch; 77 GB of values."""
+    from lagged_indexer_dsa_amd import ops
+
+    n = (1 << 26) + 9
+    if torch.cuda.mem_get_info(dev)[0] < 90 << 30:
+        torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info(dev)[0] < 90 << 30:
+        pytest.skip("needs 90 GB of device memory")
+    print(f"[read] 2^26 + 9 rows {bits}", flush=True)
+    rng = np.random.default_rng(bits)
+    rows = _pack(bits, rng.standard_normal((3, 512)), rng.standard_normal((3, 64)))
+    f = O.dequant_latent_rows if bits == 8 else O.dequant_latent_rows_fp4
+    vals = torch.cat([torch.from_numpy(f(rows)), torch.zeros(1, 576)]).to(dev).to(torch.bfloat16)
+    slots = (torch.arange(n, device=dev) % 4).int()       # (3: outside the pool, zeros)
+    out = ops.read_latent_rows(torch.from_numpy(rows).to(dev), slots)
+    for a in range(0, n, 1 << 22):
+        assert torch.equal(out[a:a + (1 << 22)], vals[slots[a:a + (1 << 22)].long()])
+    del out
+    torch.cuda.empty_cache()
+
+
 def test_append_and_read_refusals(dev):
     from lagged_indexer_dsa_amd import ops
 

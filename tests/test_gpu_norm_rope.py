@@ -283,6 +283,21 @@ def test_rotary_slices_and_padding(dev):
     assert ops.rotary(q[:0], pos[:0], table).shape == (0, 16, 192)
 
 
+def test_rotary_of_more_tokens_than_a_launch_holds(dev):
+    """2^24 workgroups of 256 threads are more than a launch has."""
+    from lagged_indexer_dsa_amd import ops
+
+    print("[rotary] 2^24 + 5 tokens", flush=True)
+    n, H = (1 << 24) + 5, 129                             # 129 pairs: a workgroup a token
+    x = torch.ones(n, H, 2, dtype=torch.bfloat16, device=dev)
+    table = torch.tensor([[0.5, 0.25], [2.0, 0.0], [0.0, 1.0]], device=dev)
+    turned = torch.tensor([[0.25, 0.75], [2.0, 2.0], [-1.0, 1.0], [1.0, 1.0]], device=dev).to(torch.bfloat16)
+    pos = (torch.arange(n, device=dev) % 4).int()         # (3: not in the table)
+    assert ops.rotary(x, pos, table, out=x) is x
+    for a in range(0, n, 1 << 21):
+        assert torch.equal(x[a:a + (1 << 21)], turned[pos[a:a + (1 << 21)].long()][:, None].expand(-1, H, 2))
+
+
 def test_rotary_refusals(dev):
     from lagged_indexer_dsa_amd import ops
 
