@@ -612,12 +612,14 @@ __global__ __launch_bounds__(W* kWave) void mla_fp4_merge_kernel(const Mla4Args 
 // workgroup a CU; at most kM4MergeMax for kM4Ragged rows and fewer, dense or
 // selected (one dense row may take them all; the partials then stay within 17 MB
 // for 16 heads, and twice the chip's CUs are there already).  Measured around 0's choice: 32 rows of 2048
-// selected keys, 16 heads: 26.0 us at 2 a row, 19.4 at 4, 18.5 at 8 (0's), 23.5
-// at 16; 8 rows of 16K keys, 128 heads: 76.8 at 4, 52.0 at 8 (0's), 55.8 at 16.
+// selected keys, 16 heads: 23.9 us at 2 a row, 18.7 at 4, 17.6 at 8 (0's), 23.4
+// at 16; 8 rows of 16K keys, 128 heads: 66.5 at 4, 47.2 at 8 (0's), 52.7 at 16.
 // Dense rows share by length wherever there are more chunks than rows: 100 rows
-// of 64 heads, one of 16K keys and 99 of 500, take 23.8 us (a chunk each: 245);
-// 100 of 2000 keys 45.7 (39.2).  At the chip's fill, 64 rows of 128 heads, a chunk
-// a row is the default: 43.7 us for 1024 to 2048 keys, 68 with two a row.
+// of 64 heads, one of 16K keys and 99 of 500, take 23.7 us (a chunk each: 219);
+// 100 of 2000 keys 43.8 (37.0).  At the chip's fill a chunk a row is the default:
+// 64 rows of 128 heads and 1024 to 2048 keys 37.8 us, 61.7 with two a row.  So a
+// long row among short ones is not cut there: 128 rows of 64 heads, one of 16K
+// keys and 127 of 500, take 219 us, with two a row asked for 36.
 static int m4_chunks(int B, int H, int nsplit) {
   const long want = nsplit > 0 ? (long)B * nsplit : (long)(device_cu_count() / m4_blocks(H));
   return (int)std::max((long)B, B <= kM4Ragged ? std::min(want, (long)kM4MergeMax) : want);

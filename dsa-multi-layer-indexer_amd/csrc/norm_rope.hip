@@ -134,10 +134,12 @@ __device__ __forceinline__ void store_row8(void* p, long row, int i, const float
 // Bound by its bytes: 8191 rows of 7168 bf16 with a residual, to e4m3 with a
 // scale per 128 values, move 412 MB in 79 us, 5.2 TB/s (as a large copy).  A row
 // a workgroup, the weight read again for each: 195 us.  Without the residual the
-// quantiser's arithmetic is next (42 us for 176 MB).  Rows of 3001 values, which
-// begin between boundaries: 4096 of bf16 with a residual 28 us, of 3000 16 us;
-// value by value they took 62.  One token: 2.9 us, a launch and two trips to
-// memory.
+// quantiser's arithmetic is next (42 us for 176 MB).  With a scale
+// per row: 79 and 44.  Rows of 3001 values, which begin between boundaries: 4096
+// of bf16 with a residual 25 us, of 3000 16 us: the same bytes from memory (both
+// ways within 1 %), but 2.5 times the accesses to the L1 by loads and stores that
+// lie across a boundary; value by value they took 62.  One token: 2.7 us, a launch
+// and two trips to memory.
 constexpr int kNormWaves = 16;  // most waves a row
 
 template <int DT, int V, bool WIDE>
@@ -285,7 +287,8 @@ hipError_t launch_rms_norm(const NormArgs& A, int dtype, hipStream_t s) {
 // are in flight.
 //
 // Bound by its bytes: 64 values of each of 128 heads of 4097 tokens, 384 bytes
-// apart on the way in, take 32 us for 134 MB (4.2 TB/s).  One item a thread,
+// apart on the way in, take 32 us for 134 MB (4.2 TB/s); in place 27, with the
+// other 128 values copied 79 (403 MB, 5.1 TB/s); halves as pairs 30 and 86.  One item a thread,
 // the table read again for every head: 44 us; batches of 1, 2 and 8 heads:
 // 33.0, 32.4 and 32.6.  32 tokens of 16 heads: 3.1 us, a launch and its latency.
 constexpr int kRopeThreads = 256, kRopeBatch = 4;

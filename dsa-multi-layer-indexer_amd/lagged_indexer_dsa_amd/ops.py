@@ -613,7 +613,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual:
     x [..., D] fp32, bf16 or fp16 (rows any one stride apart, D up to 32768),
     residual of the same shape and type, weight [D] of x's type or fp32.
     out_residual may be residual itself; otherwise outputs must not overlap
-    inputs.  h is rounded to x's type only as it is stored.
+    inputs (a tensor reaches from its first element to its last, so an output
+    between an input's rows is refused too).  h is rounded to x's type only as it is stored.
     Reference: dsa_layer.py:32-52 RMSNorm.
     """
     res = _norm(x, weight, eps, residual, (out,), 0, out_residual)
@@ -646,7 +647,8 @@ def rotary(x: torch.Tensor, pos: torch.Tensor, cos_sin: torch.Tensor, interleave
     fp32 (``rope.build_rope_table``).  Pairs are i and i + R/2 or, interleaved,
     2i and 2i + 1; inverse turns back (and is the gradient's direction).  out:
     x itself (only the turned values are touched), a tensor that does not
-    overlap it, or None for a new one; the other values are copied then.  A
+    overlap it (from first element to last: not the gaps between x's heads), or
+    None for a new one; the other values are copied then.  A
     token whose position is not in the table (padding, say -1) is not turned.
     Reference: rope.py:25-84 apply_rotary.
     """

@@ -534,7 +534,8 @@ int dsa_read_latent_rows(const void* kv_pool, int64_t kv_rows, int row_bytes, co
  * dsa_mla_fp4_workspace_in(w, B, H, nsplit) bytes on: its partial sums then lie
  * behind every barrier of any call that w is enough for.  (-1: w is not enough.)
  * nsplit: the chunks of keys a row is cut into, 1 to 128, or 0 for as many as
- * fill the device once (one a row, where there are that many rows).  Up to 256
+ * fill the device once (one a row, where there are that many rows: 2 or more are
+ * then faster for dense rows of very different lengths).  Up to 256
  * rows are cut into 512 chunks at most together (or one a row), so fewer than
  * nsplit each where B * nsplit is more.  Dense rows, up to 256, share them by their
  * lengths, so where a row is cut, and the last bits of its output, depend on
