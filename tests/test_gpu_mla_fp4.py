@@ -221,6 +221,46 @@ def test_other_scales(dev, sm):
         _check(out, q, O.dequant_latent_rows_fp4(rows), idx, sm)
 
 
+@pytest.mark.parametrize("nsplit", [1, 2, 0])
+def test_tiles_without_a_key(dev, nsplit):
+    """Tiles, waves' parts of one and whole chunks whose keys are masked, first, in
+    the middle and last, with NaN and infinities in the rows they would name and in
+    row 0 (which is read in their place): the keys that are there, alone."""
+    from lagged_indexer_dsa_amd import ops
+
+    print(f"[fp4 masked tiles] {nsplit}", flush=True)
+    n = 1300
+    rows, q = _pool(41, 1344), _q(41, 9, 32)
+    rows[0, 256:272], rows[0, 272:400:2] = 255, 0xff
+    rows[1, 272:274] = np.array([0xff80], np.uint16).view(np.uint8)            # rope: minus infinity
+    idx = np.repeat(np.arange(20, 20 + n)[None], 9, 0)
+    idx[0, :300] = -1                                  # the first two tiles and a part of the third
+    idx[1, :n - 1] = -1                                # the last key alone
+    idx[2, 1:] = -1                                    # the first alone
+    idx[3, 128:1280] = 1 << 30                         # all but the first tile and what follows the tenth
+    idx[4, :] = -5                                     # none
+    idx[5, :] = np.where(np.arange(n) // 32 % 2, idx[5], -1)                   # every second wave's part
+    idx[6, :] = np.where(np.arange(n) // 128 % 2, idx[6], 1344)                # every second tile
+    idx[7, 96:] = -1
+    idx[8, :640] = -1                                  # with two chunks, nearly the first
+    out = ops.sparse_mla_decode(_dev(q, dev, True), _dev(rows, dev), _dev(idx.astype(np.int32), dev), nsplit=nsplit)
+    clean = rows.copy()
+    clean[:2] = 0
+    kv = O.dequant_latent_rows_fp4(clean)
+    _check(out, q, kv, idx)
+    # pages that are not there, in a table of 21
+    pt = np.repeat(np.arange(21, dtype=np.int32)[None], 9, 0)
+    pt[:, 0] = -1                                      # (the page of rows 0 and 1)
+    pt[0, :6], pt[1, :20], pt[2, 2:], pt[3, 2:19] = -1, 21, -1, 1 << 25
+    pt[4], pt[5, ::2], pt[6, 4:12], pt[7, 1:20] = -7, -1, -1, -1
+    lens = np.array([1344, 1344, 1300, 1344, 1344, 1343, 1281, 1344, 70], dtype=np.int32)
+    j = np.arange(1344)
+    page = pt[:, j // 64].astype(np.int64)
+    cut = np.where((page >= 0) & (page < 21) & (j[None] < lens[:, None]), page * 64 + j % 64, -1)
+    out = ops.dense_mla_decode(_dev(q, dev, True), _dev(rows, dev), _dev(pt, dev), _dev(lens, dev), nsplit=nsplit)
+    _check(out, q, kv, cut)
+
+
 def test_sharp_and_growing_scores(dev):
     """Scores whose maximum rises along the row by far more than the sums'
     slack, and rows where one key outweighs the others."""
