@@ -380,7 +380,7 @@ extern "C" {
 
 const char* dsa_last_error(void) { return g_err; }
 
-const char* dsa_version(void) { return "dsa_mli 0.6.0 gfx950"; }
+const char* dsa_version(void) { return "dsa_mli 0.7.0 gfx950"; }
 
 size_t dsa_layer_args_bytes(void) { return sizeof(dsa_layer_args); }
 
@@ -868,6 +868,66 @@ int dsa_dense_mla_decode_fp4(const void* q_bf16, const void* kv_pool, int64_t kv
               "dsa_dense_mla_decode_fp4: pt_stride too large");
   return mla_fp4(q_bf16, kv_pool, kv_rows, nullptr, page_table, pt_stride, seq_lens, workspace, out_bf16, B, H,
                  pt_stride * DSA_PAGE_TOKENS, nsplit, sm_scale, stream);
+}
+
+int dsa_quantize_rows(const dsa_quant_args* a, void* stream) {
+  DSA_REQUIRE(a && a->n >= 0, DSA_ERR_INVALID_ARG, "dsa_quantize_rows: args with n >= 0 are required");
+  if (a->n == 0) return DSA_OK;
+  DSA_REQUIRE(a->x && a->codes && a->scales, DSA_ERR_INVALID_ARG, "dsa_quantize_rows: null pointer");
+  DSA_REQUIRE(a->dtype >= 0 && a->dtype <= 2, DSA_ERR_INVALID_ARG,
+              "dsa_quantize_rows: dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+  DSA_REQUIRE(a->D >= 1 && a->D <= DSA_NORM_MAX_DIM, DSA_ERR_UNSUPPORTED, "dsa_quantize_rows: D must be in [1, %d] (got %d)",
+              DSA_NORM_MAX_DIM, a->D);
+  DSA_REQUIRE(a->group == 0 || a->group == 128, DSA_ERR_UNSUPPORTED, "dsa_quantize_rows: group must be 128 or 0 (got %d)",
+              a->group);
+  DSA_REQUIRE(a->x_stride >= 0 && (!a->gate || a->gate_stride >= 0), DSA_ERR_INVALID_ARG, "dsa_quantize_rows: bad row stride");
+  dsa::QuantRowsArgs A{};
+  A.x = a->x, A.gate = a->gate, A.codes = static_cast<uint8_t*>(a->codes), A.scales = a->scales;
+  A.xs = (long)a->x_stride, A.gs = (long)a->gate_stride, A.n = a->n, A.D = a->D, A.group = a->group;
+  return hip_status(dsa::launch_quantize_rows(A, a->dtype, (hipStream_t)stream), "quantize rows");
+}
+
+int dsa_fp8_matmul(const dsa_matmul_args* a, void* stream) {
+  DSA_REQUIRE(a && a->rows >= 0 && a->N >= 0, DSA_ERR_INVALID_ARG, "dsa_fp8_matmul: args with rows and N >= 0 are required");
+  if (a->rows == 0 || a->N == 0) return DSA_OK;
+  DSA_REQUIRE(a->a && a->a_scale && a->w && a->w_scale && a->out, DSA_ERR_INVALID_ARG, "dsa_fp8_matmul: null pointer");
+  DSA_REQUIRE(a->experts >= 1 && (a->experts == 1 || a->offsets), DSA_ERR_INVALID_ARG,
+              "dsa_fp8_matmul: %d experts need offsets", a->experts);
+  DSA_REQUIRE(a->K >= 16 && a->K % 16 == 0 && a->K <= DSA_MATMUL_MAX_K, DSA_ERR_UNSUPPORTED,
+              "dsa_fp8_matmul: K must be a multiple of 16 up to %d (got %d)", DSA_MATMUL_MAX_K, a->K);
+  const int groups = (a->K + 127) / 128;
+  DSA_REQUIRE(a->a_groups == 1 || a->a_groups == groups, DSA_ERR_INVALID_ARG,
+              "dsa_fp8_matmul: a row has 1 or %d scales (got %d)", groups, a->a_groups);
+  DSA_REQUIRE(a->out_dtype >= 0 && a->out_dtype <= 2, DSA_ERR_INVALID_ARG,
+              "dsa_fp8_matmul: out_dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
+  DSA_REQUIRE(aligned16(a->a) && aligned16(a->w), DSA_ERR_INVALID_ARG, "dsa_fp8_matmul: a and w must be 16-byte aligned");
+  // (its launches hold a workgroup of at most 512 threads per 16 x 128 outputs)
+  DSA_REQUIRE(((int64_t)a->rows / 128 + a->experts) * ((a->N + 15) / 16) < (int64_t)1 << 23, DSA_ERR_UNSUPPORTED,
+              "dsa_fp8_matmul: %d rows of %d outputs are too many for a launch", a->rows, a->N);
+  dsa::MatmulArgs A{};
+  A.a = static_cast<const uint8_t*>(a->a), A.a_scale = a->a_scale;
+  A.w = static_cast<const uint8_t*>(a->w), A.w_scale = a->w_scale;
+  A.offsets = a->offsets, A.out = a->out;
+  A.rows = a->rows, A.N = a->N, A.K = a->K, A.experts = a->experts, A.a_groups = a->a_groups, A.out_dtype = a->out_dtype;
+  return hip_status(dsa::launch_fp8_matmul(A, (hipStream_t)stream), "fp8 matmul");
+}
+
+int dsa_chunk_scan(const void* q_fp8, const float* w, const void* index_k, int64_t num_pages, const int32_t* page_table,
+                   const int32_t* q_start, const int32_t* seq_lens, float* scores, int n, int B, int Hidx, int pt_stride,
+                   int slab_stride, void* stream) {
+  DSA_REQUIRE(n >= 0 && B >= 0, DSA_ERR_INVALID_ARG, "dsa_chunk_scan: n and B must be >= 0");
+  if (n == 0 || B == 0) return DSA_OK;
+  DSA_REQUIRE(q_start, DSA_ERR_INVALID_ARG, "dsa_chunk_scan: null pointer argument");
+  if (const int rc = check_scan(q_fp8, w, index_k, num_pages, page_table, seq_lens, scores, 1, Hidx, pt_stride, slab_stride))
+    return rc;
+  DSA_REQUIRE(aligned16(w), DSA_ERR_INVALID_ARG, "dsa_chunk_scan: w must be 16-byte aligned");
+  DSA_REQUIRE(slab_stride <= 1 << 28 && pt_stride <= 1 << 22, DSA_ERR_UNSUPPORTED,
+              "dsa_chunk_scan: slab_stride must be <= 2^28 and pt_stride <= 2^22");
+  dsa::ChunkScanArgs C{};
+  C.q8 = static_cast<const uint8_t*>(q_fp8), C.w = w, C.pages = static_cast<const uint8_t*>(index_k);
+  C.num_pages = (long)num_pages, C.page_table = page_table, C.q_start = q_start, C.seq_lens = seq_lens, C.scores = scores;
+  C.n = n, C.B = B, C.Hidx = Hidx, C.pt_stride = pt_stride, C.slab_stride = slab_stride;
+  return hip_status(dsa::launch_chunk_scan(C, (hipStream_t)stream), "chunk scan");
 }
 
 }  // extern "C"

@@ -95,6 +95,35 @@ __device__ __forceinline__ void dequant16(const uint4& v, float sc, uint4& lo, u
   hi.w = pack_bf16x2(f[14] * sc, f[15] * sc);
 }
 
+// 32 e4m3 bytes of a lane -> the four bf16 operands of 8 values each (exact).
+struct Bf32 {
+  v8bf v[4];
+};
+__device__ __forceinline__ Bf32 e4m3x32_to_bf16(const v8i& x) {
+  Bf32 o;
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * s + i], 1.f, false));
+      w[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x[2 * s + i], 1.f, true));
+    }
+    __builtin_memcpy(&o.v[s], w, 16);
+  }
+  return o;
+}
+// A block of 128 of a 16 x 16 product from such operands.  (The matrix unit's
+// 8-bit products keep 13 bits below the largest of each 8 of them, measured:
+// 1.5e-5 of a result's size for normal inputs; its bf16 products all 24,
+// 9e-9, at half the rate.)
+__device__ __forceinline__ v4f mfma_bf16_128(const Bf32& a, const Bf32& b) {
+  v4f d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < 4; ++s) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[s], b.v[s], d, 0, 0, 0);
+  return d;
+}
+
 __device__ __forceinline__ int wave_id() {
   return __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
 }

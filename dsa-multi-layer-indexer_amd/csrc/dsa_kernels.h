@@ -126,6 +126,46 @@ size_t prefill_logits_workspace_bytes(int B, int S, int H, int T);
 hipError_t launch_prefill_logits(const void* q, int qt, const void* k, int kt, const void* w, int wt, void* workspace,
                                  float* out, int B, int S, int H, int T, hipStream_t s);
 
+// Indexer scores of the new tokens of several requests over the paged index
+// keys (prefill_logits.hip).
+struct ChunkScanArgs {
+  const uint8_t* q8;     // [n, Hidx, 128] e4m3
+  const float* w;        // [n, Hidx]
+  const uint8_t* pages;  // [num_pages, 8448]
+  const int* page_table; // [B, pt_stride]
+  const int* q_start;    // [B + 1]
+  const int* seq_lens;   // [B]
+  float* scores;         // [n, slab_stride]
+  long num_pages;
+  int n, B, Hidx, pt_stride, slab_stride;
+};
+hipError_t launch_chunk_scan(const ChunkScanArgs& C, hipStream_t s);
+
+// Rows to e4m3 (quant_rows.hip).  Strides in elements.
+struct QuantRowsArgs {
+  const void* x;      // [n, D], row stride xs
+  const void* gate;   // the same, row stride gs, or nullptr
+  uint8_t* codes;     // [n, D] contiguous
+  float* scales;      // [n, ceil(D / 128)], or [n] with group 0
+  long xs, gs;
+  int n, D, group;
+  int segs;           // filled by the launcher
+};
+hipError_t launch_quantize_rows(const QuantRowsArgs& A, int dtype, hipStream_t s);
+
+// Products of e4m3 rows and weights (fp8_matmul.hip).
+struct MatmulArgs {
+  const uint8_t* a;      // [rows, K] e4m3
+  const float* a_scale;  // [rows, a_groups]
+  const uint8_t* w;      // [experts, N, K] e4m3
+  const float* w_scale;  // [experts, ceil(N / 128), ceil(K / 128)]
+  const int* offsets;    // [experts + 1], or nullptr: one expert has all rows
+  void* out;             // [rows, N]
+  int rows, N, K, experts, a_groups, out_dtype;
+  int kblocks, nblocks, otiles, rtiles, wide_out;  // filled by the launcher
+};
+hipError_t launch_fp8_matmul(MatmulArgs A, hipStream_t s);
+
 // Decode-step operand preparation (quant.hip).
 hipError_t launch_quant_query(const void* q_bf16, const float* w, void* codes, float* w_out, long rows,
                               hipStream_t s);

@@ -61,12 +61,45 @@ struct LogitsArgs {
   const uint8_t* k8;   // [B, Tp, 128], Tp = T rounded up to 64
   const float* ks;     // [B, Tp]
   float* out;          // [B*S, T]
-  int B, S, T, ktiles, rows_per_wg, groups;
+  int B, S, T, ktiles, rows_per_wg, groups;  // CHUNK: groups before this launch's
+  ChunkScanArgs chunk; // CHUNK
 };
 
 typedef __attribute__((address_space(3))) void* lg_lds_ptr;
 
-template <int NHG>
+// The chunk's rows and the keys they see: request b's rows [first, end), row
+// first + i at position pos + i.  The group-th group of `size` rows, counted
+// over the requests in turn; first == end where there is none.
+struct ChunkGroup {
+  int b, first, end, pos;
+};
+__device__ __forceinline__ ChunkGroup find_group(const int* q_start, const int* seq_lens, int B, int n, int group,
+                                                 int size) {
+  const int lane = threadIdx.x & (kWave - 1);
+  for (int b0 = 0; b0 < B; b0 += kWave) {
+    const int b = min(b0 + lane, B - 1);
+    const int lo = min(max(q_start[b], 0), n), hi = b0 + lane < B ? min(max(q_start[b + 1], lo), n) : lo;
+    const int len = max(seq_lens[b], 0);
+    const int mine = (hi - lo + size - 1) / size;
+    const int incl = (int)wave_scan_incl<0>((uint32_t)mine);
+    const uint64_t at = __ballot(group < incl);
+    if (at) {
+      const int l = __builtin_ctzll(at);
+      const int x = __builtin_amdgcn_readlane(lo, l), y = __builtin_amdgcn_readlane(hi, l);
+      const int first = x + (group - __builtin_amdgcn_readlane(incl - mine, l)) * size;
+      return {b0 + l, first, min(y, first + size), __builtin_amdgcn_readlane(len, l) - (y - first)};
+    }
+    group -= __builtin_amdgcn_readlane(incl, kWave - 1);
+  }
+  return {0, 0, 0, 0};
+}
+
+// CHUNK: the rows are the new tokens of several requests and the keys those of
+// the paged cache, a wave's 64 one page; a row's scores end at its own
+// position, -inf behind.  Its products are the matrix unit's bf16 ones, of the
+// same values: their sums keep fp32's 24 bits, where the 8-bit ones' are off
+// by 1.5e-5 of a score's size.
+template <int NHG, bool CHUNK>
 __global__ __launch_bounds__(kLgThreads, 4) void prefill_logits_kernel(const LogitsArgs A) {
   constexpr int kHeads = 16 * NHG;
   constexpr uint32_t kQBytes = kHeads * DSA_INDEX_DIM;           // one row's queries
@@ -75,18 +108,46 @@ __global__ __launch_bounds__(kLgThreads, 4) void prefill_logits_kernel(const Log
   const int t = threadIdx.x, lane = t & (kWave - 1), wv = wave_id();
   const int kr = lane & 15, kc = lane >> 4;
   const int kt = blockIdx.x % A.ktiles;
-  const int grp = (blockIdx.x / A.ktiles) % A.groups, b = blockIdx.x / (A.ktiles * A.groups);
-  const int s0 = grp * A.rows_per_wg, s1 = min(A.S, s0 + A.rows_per_wg);
+  const int grp = CHUNK ? A.groups + blockIdx.x / A.ktiles : (blockIdx.x / A.ktiles) % A.groups;
+  int b = CHUNK ? 0 : blockIdx.x / (A.ktiles * A.groups);
+  int s0 = grp * A.rows_per_wg, s1 = min(A.S, s0 + A.rows_per_wg);
+  int pos = 0;  // CHUNK: of row s0
   const int tp = (A.T + 63) / 64 * 64;
   const int g0 = kt * kLgKeys + wv * 64;  // this wave's keys (none when past Tp)
+  if constexpr (CHUNK) {
+    const ChunkGroup g = find_group(A.chunk.q_start, A.chunk.seq_lens, A.chunk.B, A.S, grp, A.rows_per_wg);
+    if (g.first >= g.end) return;
+    s0 = __builtin_amdgcn_readfirstlane(g.first);
+    s1 = __builtin_amdgcn_readfirstlane(g.end);
+    pos = __builtin_amdgcn_readfirstlane(g.pos);
+    const int last = min(pos + (s1 - s0), A.chunk.pt_stride * 64);  // keys that any of the rows sees
+    if (kt * kLgKeys >= last) {
+      for (int s = s0; s < s1; ++s)
+        if (g0 + lane < A.T) A.out[(long)s * A.T + g0 + lane] = -INFINITY;
+      return;
+    }
+    b = __builtin_amdgcn_readfirstlane(g.b);
+  }
 
   // ---- the wave's keys: 4 chunks of 16, lane (kr, kc) holds key kr's bytes
   // [32 kc, +32); and key `lane`'s scale ----
   v8i kb[4];
   float ksc = 0.f;
+  bool paged = false;  // CHUNK: the wave's page is one of the cache's
   {
-    const bool in = g0 < tp;
-    const __amdgpu_buffer_rsrc_t r = dev_rsrc(A.k8 + ((long)b * tp + (in ? g0 : 0)) * DSA_INDEX_DIM, in ? 64 * DSA_INDEX_DIM : 0);
+    const uint8_t* keys;
+    bool in = g0 < tp;
+    if constexpr (CHUNK) {
+      const int pt = min(g0 / 64, A.chunk.pt_stride - 1);
+      const int page = __builtin_amdgcn_readfirstlane(A.chunk.page_table[(long)b * A.chunk.pt_stride + pt]);
+      paged = in = g0 / 64 == pt && page >= 0 && (long)page < A.chunk.num_pages;
+      keys = A.k8 + (in ? (long)page * DSA_INDEX_PAGE_BYTES : 0);
+      if (in) ksc = reinterpret_cast<const float*>(keys + 64 * DSA_INDEX_DIM)[lane];
+    } else {
+      keys = A.k8 + ((long)b * tp + (in ? g0 : 0)) * DSA_INDEX_DIM;
+      if (in) ksc = A.ks[(long)b * tp + g0 + lane];
+    }
+    const __amdgpu_buffer_rsrc_t r = dev_rsrc(keys, in ? 64 * DSA_INDEX_DIM : 0);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int off = (16 * j + kr) * DSA_INDEX_DIM + 32 * kc;
@@ -94,11 +155,14 @@ __global__ __launch_bounds__(kLgThreads, 4) void prefill_logits_kernel(const Log
       const uint4 y = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off + 16, 0, 0));
       kb[j] = v8i{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
     }
-    if (in) ksc = A.ks[(long)b * tp + g0 + lane];
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) asm volatile("" : "+v"(kb[j]));  // waited for here
   asm volatile("" : "+v"(ksc));
+  Bf32 kbf[CHUNK ? 4 : 1];
+  if constexpr (CHUNK)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) kbf[j] = e4m3x32_to_bf16(kb[j]);
 
   // ---- staging: 16-byte chunk c of a stage's queries is chunk c & 7 of head
   // row c >> 3; in LDS its low bits are xored with the head row / 2, so that
@@ -106,8 +170,9 @@ __global__ __launch_bounds__(kLgThreads, 4) void prefill_logits_kernel(const Log
   // loads (m0: the wave's base, 16 bytes a lane); rows past the last repeat
   // it. ----
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lg_lds_ptr)buf;
-  const uint8_t* qb = A.q8 + (long)b * A.S * kQBytes;
-  const float* wb = A.w + (long)b * A.S * kHeads;
+  const long req = CHUNK ? 0 : (long)b * A.S;  // the request's first row
+  const uint8_t* qb = A.q8 + req * kQBytes;
+  const float* wb = A.w + req * kHeads;
   const auto issue = [&](int s, uint32_t at) {
 #pragma unroll
     for (int it = 0; it < NHG; ++it) {
@@ -147,10 +212,13 @@ __global__ __launch_bounds__(kLgThreads, 4) void prefill_logits_kernel(const Log
       const uint4 y = *reinterpret_cast<const uint4*>(q + hg * (16 * DSA_INDEX_DIM) + qoff1);
       const v4f wr = *reinterpret_cast<const v4f*>(w + hg * 64 + kc * 16);
       const v8i qa = v8i{(int)x.x, (int)x.y, (int)x.z, (int)x.w, (int)y.x, (int)y.y, (int)y.z, (int)y.w};
+      Bf32 qbf;
+      if constexpr (CHUNK) qbf = e4m3x32_to_bf16(qa);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const v4f z = {0.f, 0.f, 0.f, 0.f};
-        const v4f d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(qa, kb[j], z, 0, 0, 0, 0, 0, 0);
+        v4f d = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (CHUNK) d = mfma_bf16_128(qbf, kbf[j]);
+        else d = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(qa, kb[j], d, 0, 0, 0, 0, 0, 0);
         // ReLU on the float's bits (see the decode scan)
 #pragma unroll
         for (int r = 0; r < 4; ++r) a[j] += wr[r] * __int_as_float(max(__float_as_int(d[r]), 0));
@@ -160,10 +228,12 @@ __global__ __launch_bounds__(kLgThreads, 4) void prefill_logits_kernel(const Log
     const float ys = add32(a[1], a[3]);
     const auto r16 = __builtin_amdgcn_permlane16_swap(__float_as_uint(xs), __float_as_uint(ys), false, false);
     const float acc = __uint_as_float(r16[0]) + __uint_as_float(r16[1]);
+    float v = acc * ksc;
+    if constexpr (CHUNK) v = paged && g0 + lane <= pos + (s - s0) ? v : -INFINITY;
     // always issued (the wait below counts it); keys past T are outside the
     // resource and dropped
-    const __amdgpu_buffer_rsrc_t o = dev_rsrc(A.out + ((long)b * A.S + s) * A.T, (uint32_t)A.T * 4u);
-    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc * ksc), o, 4 * (g0 + lane), 0, 0);
+    const __amdgpu_buffer_rsrc_t o = dev_rsrc(A.out + (req + s) * A.T, (uint32_t)A.T * 4u);
+    __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), o, 4 * (g0 + lane), 0, 0);
   };
 
   uint32_t at = 0;
@@ -206,6 +276,18 @@ static hipError_t launch_quant_rows(const void* x, int dt, int B, int T, int str
   return hipGetLastError();
 }
 
+template <bool CHUNK>
+static hipError_t launch_logits(const LogitsArgs& A, int H, dim3 grid, hipStream_t s) {
+  const dim3 block(kLgThreads);
+  switch (H / 16) {
+    case 1: hipLaunchKernelGGL((prefill_logits_kernel<1, CHUNK>), grid, block, 0, s, A); break;
+    case 2: hipLaunchKernelGGL((prefill_logits_kernel<2, CHUNK>), grid, block, 0, s, A); break;
+    case 3: hipLaunchKernelGGL((prefill_logits_kernel<3, CHUNK>), grid, block, 0, s, A); break;
+    default: hipLaunchKernelGGL((prefill_logits_kernel<4, CHUNK>), grid, block, 0, s, A); break;
+  }
+  return hipGetLastError();
+}
+
 hipError_t launch_prefill_logits(const void* q, int qt, const void* k, int kt, const void* w, int wt, void* workspace,
                                  float* out, int B, int S, int H, int T, hipStream_t s) {
   const int tp = logits_tp(T);
@@ -236,14 +318,30 @@ hipError_t launch_prefill_logits(const void* q, int qt, const void* k, int kt, c
   const long per = std::max(1L, 2L * device_cu_count() / std::max(1L, (long)A.ktiles * B));
   A.rows_per_wg = (int)((((long)S + per - 1) / per + kLgStage - 1) / kLgStage * kLgStage);
   A.groups = (S + A.rows_per_wg - 1) / A.rows_per_wg;
-  const dim3 grid((unsigned)((long)A.ktiles * A.groups * B)), block(kLgThreads);
-  switch (H / 16) {
-    case 1: hipLaunchKernelGGL(prefill_logits_kernel<1>, grid, block, 0, s, A); break;
-    case 2: hipLaunchKernelGGL(prefill_logits_kernel<2>, grid, block, 0, s, A); break;
-    case 3: hipLaunchKernelGGL(prefill_logits_kernel<3>, grid, block, 0, s, A); break;
-    default: hipLaunchKernelGGL(prefill_logits_kernel<4>, grid, block, 0, s, A); break;
-  }
-  return hipGetLastError();
+  const dim3 grid((unsigned)((long)A.ktiles * A.groups * B));
+  return launch_logits<false>(A, H, grid, s);
+}
+
+// The chunk's rows in groups: as many workgroups as the chip holds at once, a
+// group of one request's.
+hipError_t launch_chunk_scan(const ChunkScanArgs& C, hipStream_t s) {
+  LogitsArgs A{};
+  A.q8 = C.q8;
+  A.w = C.w;
+  A.k8 = C.pages;
+  A.out = C.scores;
+  A.chunk = C;
+  A.S = C.n;
+  A.T = C.slab_stride;
+  A.ktiles = (A.T + kLgKeys - 1) / kLgKeys;
+  const long per = std::max(1L, 2L * device_cu_count() / A.ktiles);
+  A.rows_per_wg = (int)std::min(((C.n + per - 1) / per + kLgStage - 1) / kLgStage * kLgStage, 1L << 16);
+  // every request's last group may be short
+  const long groups = (long)C.n / A.rows_per_wg + std::min(C.B, C.n);
+  return in_launches(groups, ((1L << 32) - 1) / kLgThreads / A.ktiles, [&](long first, long count) {
+    A.groups = (int)first;
+    return launch_logits<true>(A, C.Hidx, dim3((unsigned)(count * A.ktiles)), s);
+  });
 }
 
 }  // namespace dsa

@@ -33,6 +33,7 @@ QK_DIM = 576
 LATENT_ROW_BYTES = 656
 FP4_ROW_BYTES = 400
 NORM_MAX_DIM = 32768
+MATMUL_MAX_K = 131072
 TOPK_MAX_CTX = 262144
 SELECTION_MAX_CTX = 524288
 
@@ -67,11 +68,13 @@ class LayerArgs(ctypes.Structure):
     ]
 
 
-# dsa_norm_args, dsa_rotary_args, dsa_append_args, packed in one go (a field of
+# dsa_norm_args and the other argument structures of ops, packed in one go (a field of
 # a ctypes structure costs about as much as the whole packing)
 NORM_ARGS = struct.Struct("@7P3qd5i0q")
 ROTARY_ARGS = struct.Struct("@4P5q9i0q")
 APPEND_ARGS = struct.Struct("@9P5qd8i0q")
+QUANT_ARGS = struct.Struct("@4P2q4i0q")
+MATMUL_ARGS = struct.Struct("@6P6i0q")
 
 _LIB: ctypes.CDLL | None = None
 
@@ -121,6 +124,9 @@ SIGNATURES = {
     "dsa_mla_fp4_workspace_in": (_i64, [ctypes.c_size_t, _i32, _i32, _i32]),
     "dsa_sparse_mla_decode_fp4": (_i32, [_vp, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp]),
     "dsa_dense_mla_decode_fp4": (_i32, [_vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _f32, _vp]),
+    "dsa_quantize_rows": (_i32, [ctypes.c_char_p, _vp]),
+    "dsa_fp8_matmul": (_i32, [ctypes.c_char_p, _vp]),
+    "dsa_chunk_scan": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
 }
 
 

@@ -46,6 +46,20 @@ def quantize_index_query(q: torch.Tensor, w: torch.Tensor) -> tuple[torch.Tensor
     return codes.contiguous(), (w.float() * sq).contiguous()
 
 
+def quantize_weight(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Weights [..., N, K] -> (codes uint8 [..., N, K], scales f32 [...,
+    ceil(N/128), ceil(K/128)]), a scale per 128 x 128 block by the rowwise rule
+    (the blocks at the edges may be smaller): what ``ops.fp8_matmul`` takes
+    (reference inference/modeling/kernels.py:120-221)."""
+    *lead, N, K = w.shape
+    nb, kb = -(-N // 128), -(-K // 128)
+    x = torch.nn.functional.pad(w.float(), (0, kb * 128 - K, 0, nb * 128 - N))
+    x = x.reshape(*lead, nb, 128, kb, 128).transpose(-3, -2).reshape(*lead, nb, kb, 128 * 128)
+    q, scale = quantize_rowwise(x)
+    q = q.reshape(*lead, nb, kb, 128, 128).transpose(-3, -2).reshape(*lead, nb * 128, kb * 128)
+    return q[..., :N, :K].contiguous(), scale
+
+
 def random_page_table(seq_lens: list[int], pt_stride: int, num_pages: int,
                       generator: torch.Generator | None = None) -> torch.Tensor:
     """Distinct physical pages for every row's logical pages, drawn as one

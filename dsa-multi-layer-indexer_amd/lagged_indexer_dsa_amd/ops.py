@@ -18,6 +18,7 @@ from ._lib import (
     INDEX_PAGE_BYTES,
     LATENT_DIM,
     LATENT_ROW_BYTES,
+    MATMUL_MAX_K,
     NORM_MAX_DIM,
     PAGE_TOKENS,
     QK_DIM,
@@ -808,4 +809,184 @@ def read_latent_rows(kv_pool: torch.Tensor, slots: torch.Tensor, out: torch.Tens
         _need_shape("out", out, (n, QK_DIM), torch.bfloat16)
     _lib.call("dsa_read_latent_rows", kv_pool.data_ptr(), kv_rows, row_bytes, slots.data_ptr(), n, out.data_ptr(),
               torch._C._cuda_getCurrentRawStream(dev))
+    return out
+
+
+# ---- 8-bit products: row quantiser, products with block scales ----
+
+def quantize_rows(x: torch.Tensor, gate: torch.Tensor | None = None, group: int = 128,
+                  out_q: torch.Tensor | None = None, out_scale: torch.Tensor | None = None):
+    """x, or x * silu(gate), in e4m3: (codes uint8 [..., D], scales fp32
+    [..., groups]), by :func:`rms_norm_quant`'s rule.
+
+    x [..., D] fp32, bf16 or fp16 (rows any one stride apart, D up to 32768),
+    gate of the same shape and type (the two halves of one projection).  group
+    128: a scale per 128 values (the last group may be short); group 0: one per
+    row.  scale = max(amax, 1e-6) / 448; a NaN makes its group's scale and codes
+    NaN.  Outputs must not overlap inputs.
+    Reference: act_quant (inference/modeling/kernels.py:35-117).
+    """
+    if group not in (0, 128):
+        raise RuntimeError(f"group must be 128 or 0, got {group}")
+    shape, dt = x.shape, x.dtype
+    dtype = _PACK_DTYPES.get(dt)
+    if dtype is None:
+        raise RuntimeError(f"x must be float32, bfloat16 or float16, got {dt}")
+    dev = x.get_device()
+    D = shape[-1] if shape else 0
+    if not 1 <= D <= NORM_MAX_DIM:
+        raise RuntimeError(f"x must be [..., D] with D from 1 to {NORM_MAX_DIM}, got {tuple(shape)}")
+    _here(dev, gate, out_q, out_scale)
+    n = x.numel() // D
+    xs, gs, gp = _row_stride("x", x, n, D), 0, 0
+    if gate is not None:
+        if gate.dtype != dt or gate.shape != shape:
+            raise RuntimeError(f"gate must be {dt} {tuple(shape)}, got {gate.dtype} {tuple(gate.shape)}")
+        gs, gp = _row_stride("gate", gate, n, D), gate.data_ptr()
+    sshape = (*shape[:-1], -(-D // 128) if group else 1)
+    if out_q is None:
+        out_q = torch.empty(shape, dtype=torch.uint8, device=x.device)
+    else:
+        _need_shape("out_q", out_q, shape, torch.uint8)
+        if n:
+            _need_apart("out_q", out_q, x, gate)
+    if out_scale is None:
+        out_scale = torch.empty(sshape, dtype=torch.float32, device=x.device)
+    else:
+        _need_shape("out_scale", out_scale, sshape, torch.float32)
+        if n:
+            _need_apart("out_scale", out_scale, x, gate, out_q)
+    if n:
+        a = _lib.QUANT_ARGS.pack(x.data_ptr(), gp, out_q.data_ptr(), out_scale.data_ptr(), xs, gs, n, D, dtype, group)
+        _lib.call("dsa_quantize_rows", a, torch._C._cuda_getCurrentRawStream(dev))
+    return out_q, out_scale
+
+
+def _matmul(a, a_scale, w, w_scale, offsets, dtype, out):
+    """Checks and launch of a product; w [experts, N, K] or [N, K]."""
+    for name, t in (("a", a), ("w", w)):
+        if t.dtype != torch.uint8 and t.dtype != torch.float8_e4m3fn:
+            raise RuntimeError(f"{name} must hold e4m3 codes (uint8 or float8_e4m3fn), got {t.dtype}")
+        if not t.is_contiguous():
+            raise RuntimeError(f"{name} must be contiguous")
+    dev = a.get_device()
+    _here(dev, a_scale, w, w_scale, offsets, out)
+    ash, wsh = a.shape, w.shape
+    if len(wsh) != (2 if offsets is None else 3) or not ash or ash[-1] != wsh[-1]:
+        raise RuntimeError(f"a must be [..., K] and w {'[N, K]' if offsets is None else '[experts, N, K]'}, got "
+                           f"{tuple(ash)} and {tuple(wsh)}")
+    K, N = wsh[-1], wsh[-2]
+    if not 16 <= K <= MATMUL_MAX_K or K % 16:
+        raise RuntimeError(f"K must be a multiple of 16 up to {MATMUL_MAX_K}, got {K}")
+    n = a.numel() // K
+    groups = -(-K // 128)
+    ss = a_scale.shape
+    if a_scale.dtype != torch.float32 or not a_scale.is_contiguous() or ss[:-1] != ash[:-1] or len(ss) != len(ash) or \
+            ss[-1] not in (1, groups):
+        raise RuntimeError(f"a_scale must be contiguous float32 {(*ash[:-1], groups)}, or 1 a row, got {a_scale.dtype} "
+                           f"{tuple(ss)}")
+    _need_shape("w_scale", w_scale, (*wsh[:-2], -(-N // 128), groups), torch.float32)
+    experts = 1
+    if offsets is not None:
+        experts = wsh[0]
+        _need_shape("offsets", offsets, (experts + 1,), torch.int32)
+    if out is None:
+        if dtype not in _PACK_DTYPES:
+            raise RuntimeError(f"the output must be float32, bfloat16 or float16, got {dtype}")
+        out = torch.empty(*ash[:-1], N, dtype=dtype, device=a.device)
+    else:
+        dtype = out.dtype
+        if dtype not in _PACK_DTYPES:
+            raise RuntimeError(f"out must be float32, bfloat16 or float16, got {dtype}")
+        _need_shape("out", out, (*ash[:-1], N), dtype)
+        if n and N:
+            _need_apart("out", out, a, a_scale, w if w.numel() else None, w_scale if w.numel() else None, offsets)
+    if n and N and experts:
+        p = _lib.MATMUL_ARGS.pack(a.data_ptr(), a_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(),
+                                  0 if offsets is None else offsets.data_ptr(), out.data_ptr(), n, N, K, experts, ss[-1],
+                                  _PACK_DTYPES[dtype])
+        _lib.call("dsa_fp8_matmul", p, torch._C._cuda_getCurrentRawStream(dev))
+    return out
+
+
+def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+               dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rows a [..., K] times weights w [N, K]^T, both e4m3 codes, summed in fp32
+    -> [..., N] of ``dtype`` (fp32, bf16 or fp16), or of out's type.
+
+    a_scale [..., ceil(K/128)] fp32, or [..., 1] for one scale a row: what
+    :func:`rms_norm_quant` and :func:`quantize_rows` give; w_scale [ceil(N/128),
+    ceil(K/128)] fp32, a scale per 128 x 128 block (``formats.quantize_weight``).
+    K a multiple of 16; everything contiguous.  Which kernel runs, and the order
+    of its sum, depends on the number of rows: a row alone and among others may
+    differ in the last bits.
+    Reference: fp8_gemm (inference/modeling/kernels.py:120-221).
+    """
+    return _matmul(a, a_scale, w, w_scale, None, dtype, out)
+
+
+def fp8_matmul_grouped(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor,
+                       offsets: torch.Tensor, dtype: torch.dtype = torch.bfloat16,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`fp8_matmul` with the weights of experts: rows offsets[e] ..
+    offsets[e + 1] - 1 of a [n, K] times w[e] of w [experts, N, K].
+
+    offsets [experts + 1] int32 on the device, not falling, from 0 or later to
+    at most n; w_scale [experts, ceil(N/128), ceil(K/128)].  An expert may have
+    no row; rows outside all of them are left as they are (new outputs: undefined).
+    """
+    if a.dim() != 2:
+        raise RuntimeError(f"a must be [n, K], got {tuple(a.shape)}")
+    if offsets is None:
+        raise RuntimeError("offsets are needed")
+    return _matmul(a, a_scale, w, w_scale, offsets, dtype, out)
+
+
+# ---- a chunk of new tokens over the paged caches ----
+
+def _chunk(page_table, q_start, seq_lens) -> int:
+    """What the chunk ops check of their requests; returns how many there are."""
+    pts = page_table.shape
+    if len(pts) != 2 or 0 in pts or page_table.dtype != torch.int32 or not page_table.is_contiguous():
+        raise RuntimeError("page_table must be contiguous [B, pt_stride] int32")
+    B = pts[0]
+    _need_shape("q_start", q_start, (B + 1,), torch.int32)
+    _need_shape("seq_lens", seq_lens, (B,), torch.int32)
+    return B
+
+
+def chunk_scan(q_fp8: torch.Tensor, w: torch.Tensor, index_k: torch.Tensor, page_table: torch.Tensor,
+               q_start: torch.Tensor, seq_lens: torch.Tensor, slab_stride: int,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`indexer_scan` for more than one row a request: rows q_start[b] ..
+    q_start[b + 1] - 1 are the last tokens of request b, whose index keys (theirs
+    too) are the first seq_lens[b] of the paged cache; a row's scores end at its
+    own position.
+
+    q_fp8 [n,Hidx,128] e4m3 codes; w [n,Hidx] f32 (q-scale folded in); index_k
+    [P,8448] uint8; page_table [B,pt] int32; q_start [B+1] int32, not falling;
+    seq_lens [B] int32  ->  scores [n, slab_stride] f32 (-inf behind the row's
+    position, and all of them for a row before position 0).  Rows of no request
+    are left as they are (new scores: undefined).
+    Reference: attention_core.py:27-63 indexer_logits, apply_causal_mask.
+    """
+    q_fp8 = q_fp8.view(torch.uint8) if q_fp8.dtype == torch.float8_e4m3fn else q_fp8
+    _here(q_fp8.get_device(), w, index_k, page_table, q_start, seq_lens, out)
+    qs = q_fp8.shape
+    if len(qs) != 3 or qs[2] != INDEX_DIM or q_fp8.dtype != torch.uint8 or not q_fp8.is_contiguous():
+        raise RuntimeError("q_fp8 must be contiguous [n, Hidx, 128] e4m3 bytes")
+    n, Hidx, _ = qs
+    _need_shape("w", w, (n, Hidx), torch.float32)
+    ks = index_k.shape
+    if len(ks) != 2 or ks[1] != INDEX_PAGE_BYTES or index_k.dtype != torch.uint8 or not index_k.is_contiguous():
+        raise RuntimeError("index_k must be contiguous [pages, 8448] uint8")
+    B = _chunk(page_table, q_start, seq_lens)
+    if out is None:
+        out = torch.empty(n, slab_stride, dtype=torch.float32, device=q_fp8.device)
+    else:
+        _need_shape("out", out, (n, slab_stride), torch.float32)
+    if n:
+        _lib.call("dsa_chunk_scan", q_fp8.data_ptr(), w.data_ptr(), index_k.data_ptr(), ks[0], page_table.data_ptr(),
+                  q_start.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), n, B, Hidx, page_table.shape[1], slab_stride,
+                  _stream())
     return out

@@ -58,6 +58,7 @@ extern "C" {
 #define DSA_LATENT_ROW_BYTES 656  /* 512 + 4*4 + 64*2 */
 #define DSA_FP4_ROW_BYTES 400     /* 512/2 + 16 + 64*2 */
 #define DSA_NORM_MAX_DIM 32768    /* longest row of dsa_rms_norm */
+#define DSA_MATMUL_MAX_K 131072   /* longest row of dsa_fp8_matmul */
 #define DSA_TOPK_MAX_CTX 262144   /* longest row the top-k select accepts */
 #define DSA_SELECTION_MAX_CTX 524288 /* longest context of dsa_selection_set */
 
@@ -552,6 +553,68 @@ int dsa_sparse_mla_decode_fp4(const void* q_bf16, const void* kv_pool, int64_t k
 int dsa_dense_mla_decode_fp4(const void* q_bf16, const void* kv_pool, int64_t kv_rows, const int32_t* page_table,
                              int pt_stride, const int32_t* seq_lens, void* workspace, void* out_bf16, int B, int H,
                              int nsplit, float sm_scale, void* stream);
+
+/*
+ * (13) Rows to e4m3: y = x, or x * g / (1 + e^-g) with a gate g, in fp32;
+ * scale = max(amax |y|, 1e-6) / 448 per 128 values (group 128: scales [n,
+ * ceil(D/128)], the last group may be short) or per row (group 0: [n, 1]),
+ * codes [n, D] e4m3_rne(y / scale), contiguous; a NaN makes its group's scale
+ * and codes NaN.  x and gate [n, D] of one type, row strides in elements.
+ * 1 <= D <= DSA_NORM_MAX_DIM.  Outputs must not overlap inputs.
+ * Replaces: act_quant (inference/modeling/kernels.py:35-117).
+ */
+typedef struct dsa_quant_args {
+  const void *x, *gate; /* gate may be NULL */
+  void* codes;
+  float* scales;
+  int64_t x_stride, gate_stride;
+  int n, D, dtype, group;
+} dsa_quant_args;
+int dsa_quantize_rows(const dsa_quant_args* args, void* stream);
+
+/*
+ * (14) Product of e4m3 rows with e4m3 weights, by blocks b of 128 values of K
+ * (the last may be short):
+ *   out[t, o] = sum_b sa[t, b] sw[o / 128, b] sum_{k in b} a[t, k] w[o, k]
+ * in fp32, rounded once to out_dtype.
+ *   a [rows, K], a_scale [rows, a_groups]: a_groups = ceil(K/128), or 1 for one
+ *   scale a row; w [experts, N, K], w_scale [experts, ceil(N/128),
+ *   ceil(K/128)]; out [rows, N].  K a multiple of 16 up to DSA_MATMUL_MAX_K;
+ *   a and w 16-byte aligned; everything contiguous.
+ *   offsets NULL (experts 1): all rows with the one weight.  offsets [experts +
+ *   1] int32, on the device, not falling: rows offsets[e] .. offsets[e+1] - 1
+ *   with expert e's weights; rows outside are neither read nor written.
+ * Which kernel runs depends on rows / experts, and with it the order of the sum
+ * over b: equal calls give equal bits.
+ * Replaces: fp8_gemm (inference/modeling/kernels.py:120-221), with the weights
+ * of the experts of a mixture besides.
+ */
+typedef struct dsa_matmul_args {
+  const void* a;
+  const float* a_scale;
+  const void* w;
+  const float* w_scale;
+  const int32_t* offsets;
+  void* out;
+  int rows, N, K, experts, a_groups, out_dtype;
+} dsa_matmul_args;
+int dsa_fp8_matmul(const dsa_matmul_args* args, void* stream);
+
+/*
+ * (15) The indexer's scores of a chunk: new tokens of several requests over
+ * their cached keys.  Rows q_start[b] .. q_start[b+1] - 1 of q are the last
+ * tokens of request b, whose cache holds seq_lens[b] tokens with them: row i is
+ * at position p = seq_lens[b] - (q_start[b+1] - i) and
+ *   scores[i, g] as (1) for g <= p, -inf for p < g < slab_stride.
+ *   q_fp8 [n, Hidx, 128], w [n, Hidx] (16-byte aligned), page_table [B,
+ *   pt_stride], q_start [B + 1] (not falling), scores [n, slab_stride].
+ * A row at a negative position sees no key; a key in a page outside the cache
+ * scores -inf; rows of no request are left as they are.
+ * Replaces: (1) for more than one row a request (attention_core.py:27-63).
+ */
+int dsa_chunk_scan(const void* q_fp8, const float* w, const void* index_k, int64_t num_pages, const int32_t* page_table,
+                   const int32_t* q_start, const int32_t* seq_lens, float* scores, int n, int B, int Hidx, int pt_stride,
+                   int slab_stride, void* stream);
 
 #ifdef __cplusplus
 }
