@@ -930,6 +930,36 @@ int dsa_chunk_scan(const void* q_fp8, const float* w, const void* index_k, int64
   return hip_status(dsa::launch_chunk_scan(C, (hipStream_t)stream), "chunk scan");
 }
 
+static bool chunk_shape(int n, int H) {
+  return n >= 1 && H >= 16 && H % 16 == 0 && H <= 16 * 64 && (int64_t)n * H < (int64_t)1 << 31;
+}
+
+size_t dsa_chunk_attention_workspace_bytes(int n, int H) { return chunk_shape(n, H) ? dsa::chunk_workspace_bytes(n, H) : 0; }
+
+int dsa_chunk_attention(const void* q_bf16, const void* kv_pool, int64_t kv_rows, int row_bytes, const int32_t* page_table,
+                        const int32_t* q_start, const int32_t* seq_lens, void* workspace, void* out_bf16, int n, int B, int H,
+                        int pt_stride, float sm_scale, void* stream) {
+  DSA_REQUIRE(n >= 0 && B >= 0, DSA_ERR_INVALID_ARG, "dsa_chunk_attention: n and B must be >= 0");
+  if (n == 0 || B == 0) return DSA_OK;
+  DSA_REQUIRE(q_bf16 && kv_pool && page_table && q_start && seq_lens && workspace && out_bf16, DSA_ERR_INVALID_ARG,
+              "dsa_chunk_attention: null pointer argument");
+  DSA_REQUIRE(H >= 16 && H % 16 == 0 && H <= 16 * 64, DSA_ERR_UNSUPPORTED,
+              "dsa_chunk_attention: H must be a positive multiple of 16 (got %d)", H);
+  DSA_REQUIRE(chunk_shape(n, H), DSA_ERR_UNSUPPORTED, "dsa_chunk_attention: n * H must be < 2^31");
+  DSA_REQUIRE(kv_rows >= 1, DSA_ERR_INVALID_ARG, "dsa_chunk_attention: kv_rows must be >= 1");
+  DSA_REQUIRE(row_bytes == DSA_LATENT_ROW_BYTES || row_bytes == DSA_FP4_ROW_BYTES, DSA_ERR_UNSUPPORTED,
+              "dsa_chunk_attention: row_bytes must be %d or %d (got %d)", DSA_LATENT_ROW_BYTES, DSA_FP4_ROW_BYTES, row_bytes);
+  DSA_REQUIRE(pt_stride >= 1 && pt_stride <= 1 << 22, DSA_ERR_UNSUPPORTED, "dsa_chunk_attention: pt_stride must be in [1, 2^22]");
+  DSA_REQUIRE(aligned16(q_bf16) && aligned16(kv_pool) && aligned16(workspace) && ((uintptr_t)out_bf16 & 7) == 0,
+              DSA_ERR_INVALID_ARG, "dsa_chunk_attention: q, kv_pool and workspace must be 16-byte aligned, out 8-byte");
+  dsa::ChunkAttnArgs A{};
+  A.q = static_cast<const uint16_t*>(q_bf16), A.pool = static_cast<const uint8_t*>(kv_pool), A.kv_rows = (long)kv_rows;
+  A.page_table = page_table, A.q_start = q_start, A.seq_lens = seq_lens, A.out = static_cast<uint16_t*>(out_bf16);
+  A.sm_log2 = sm_scale * 1.4426950408889634f;
+  A.n = n, A.B = B, A.H = H, A.pt_stride = pt_stride;
+  return hip_status(dsa::launch_chunk_attention(A, row_bytes, workspace, (hipStream_t)stream), "chunk attention");
+}
+
 }  // extern "C"
 // Internal: choose the cooperative (1, default) or single-workgroup (0)
 // select inside the decode launch; read (and optionally reset) the count of

@@ -1,0 +1,603 @@
+// Attention of new tokens over the paged latent cache (gfx950): the last tokens
+// of several requests at once, each over its request's keys up to its own.
+//
+//   out[r, :] = sum_j softmax_j(sm * q[r, :] . k_j) * k_j[:512]
+//
+// over the keys j <= pos(i), where row r = (token i, head h).  All heads share
+// the keys, so a request's rows, tokens times heads, are one tall matrix against
+// them: the tile of prefill.hip, 128 rows against 32 keys, whose softmax and
+// operand layout this kernel has too.  What differs is where the keys come from
+// and how the work is cut.
+//
+// Keys: a tile is half a page, one contiguous piece of the pool.  It goes from
+// memory straight to LDS as it is (656 or 400 bytes a row), two places, and the
+// workgroup dequantises it once, into a bf16 tile for its 128 rows: tile t + 1
+// while tile t is multiplied and t + 2 is on its way.  (Rows unpacked to bf16 in
+// memory first, as prefill.hip has them, cost 2.75 times a row's bytes besides,
+// which is more than the attention of up to a few hundred rows.)
+//
+// Work: the (row tile, key tile) pairs of all requests lie on one line, and each
+// workgroup, one a CU, takes an equal share of it, whatever the requests'
+// lengths: the tiles in the middle of its share whole, at most one tile that
+// began before it and one that ends behind it in part.  Parts leave their sums
+// and reference points in the workspace, where a second launch joins them in the
+// order of the keys.
+#include <algorithm>
+
+#include "dsa_kernels.h"
+#include "prefill_core.h"
+#include "quant_core.h"
+
+namespace dsa {
+
+#define DSA_INLINE __attribute__((always_inline))  // (a lambda left out of line keeps its captures in memory)
+
+constexpr int kCaTileCost = 64;   // keys' worth of a row tile's start and end
+constexpr int kCaShare = 256;     // the least share of a workgroup, in keys of a row tile
+
+// A workgroup's place on the line of work: request, row tile, key tile of it.
+struct ChunkPos {
+  int b, tile, kt;
+};
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// A request's part of the batch: its rows, tiles and the position of its first
+// token (negative: tokens before the first key).
+struct ChunkReq {
+  int first, T, tiles, P;
+};
+__device__ __forceinline__ ChunkReq chunk_req(const ChunkAttnArgs& A, int b) {
+  ChunkReq r;
+  r.first = min(max(A.q_start[b], 0), A.n);
+  r.T = min(max(A.q_start[b + 1], r.first), A.n) - r.first;
+  r.tiles = (int)(((long)r.T * A.H + kPfRows - 1) / kPfRows);
+  r.P = max(A.seq_lens[b], 0) - r.T;
+  return r;
+}
+// Cost of a request's first `t` row tiles, H times keys: 128 rows further down
+// are 128 / H tokens, and as many keys, further, from none (tokens before the
+// first key) up to what the page table holds.  Within a tile it is at most 64 +
+// 8 keys and 1 above the keys that the tile sees, so two places kCaShare apart
+// are in different key tiles: no share lies inside a tile without a part of it.
+__device__ __forceinline__ long chunk_cost(const ChunkAttnArgs& A, const ChunkReq& r, long t) {
+  const long HP = (long)A.H * r.P, most = (long)A.H * A.pt_stride * DSA_PAGE_TOKENS;
+  const long none = HP < 0 ? min(t, -HP / kPfRows) : 0;  // tiles without a key
+  const long from = max(0L, min(HP, most));
+  const long grow = min(t - none, max(0L, (most - from) / kPfRows));
+  return t * A.H * kCaTileCost + grow * from + kPfRows / 2 * grow * (grow + 1) + (t - none - grow) * most;
+}
+// Keys that any row of a tile sees.
+__device__ __forceinline__ int chunk_keys(const ChunkAttnArgs& A, const ChunkReq& r, int tile) {
+  const long R = (long)r.T * A.H;
+  const int s_hi = (int)((min((tile + 1L) * kPfRows, R) - 1) / A.H);
+  return max(0, min(r.P + s_hi + 1, A.pt_stride * DSA_PAGE_TOKENS));
+}
+
+__device__ __forceinline__ long wave_prefix(long v) {
+  const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const long u = __shfl_up(v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+__device__ __forceinline__ long lane_value(long v, int l) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)v, l), hi = (uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), l);
+  return (long)((uint64_t)hi << 32 | lo);
+}
+
+// The place at x of the line; every wave finds it for itself.
+__device__ __forceinline__ ChunkPos chunk_find(const ChunkAttnArgs& A, long x) {
+  const int lane = threadIdx.x & (kWave - 1);
+  for (int b0 = 0; b0 < A.B; b0 += kWave) {
+    long mine = 0;
+    if (b0 + lane < A.B) {
+      const ChunkReq r = chunk_req(A, b0 + lane);
+      mine = chunk_cost(A, r, r.tiles);
+    }
+    const long incl = wave_prefix(mine);
+    const uint64_t at = __ballot(x < incl);
+    if (!at) {
+      x -= lane_value(incl, kWave - 1);
+      continue;
+    }
+    const int l = __builtin_ctzll(at), b = b0 + l;
+    x -= lane_value(incl - mine, l);
+    const ChunkReq r = chunk_req(A, b);
+    // the last tile whose start is not behind x, 64 candidates at a time
+    long lo = 0, step = 1;
+    while (step * kWave < r.tiles) step *= kWave;
+    for (;; step /= kWave) {
+      const long t = lo + lane * step;
+      const uint64_t ok = __ballot(t < r.tiles && chunk_cost(A, r, t) <= x);
+      lo += (__builtin_popcountll(ok) - 1) * step;
+      if (step == 1) break;
+    }
+    const int tile = uniform((int)lo);
+    const long c0 = chunk_cost(A, r, tile), c1 = chunk_cost(A, r, tile + 1);
+    const int kts = (chunk_keys(A, r, tile) + kPfKeys - 1) / kPfKeys;
+    return {uniform(b), tile, uniform((int)((x - c0) * kts / (c1 - c0)))};
+  }
+  return {A.B, 0, 0};
+}
+
+// Workgroups that take a share: as many as there are, or fewer shares that are
+// worth their join.
+__device__ __forceinline__ long chunk_total(const ChunkAttnArgs& A) {
+  const int lane = threadIdx.x & (kWave - 1);
+  long sum = 0;
+  for (int b0 = 0; b0 < A.B; b0 += kWave) {
+    long mine = 0;
+    if (b0 + lane < A.B) {
+      const ChunkReq r = chunk_req(A, b0 + lane);
+      mine = chunk_cost(A, r, r.tiles);
+    }
+    sum += lane_value(wave_prefix(mine), kWave - 1);
+  }
+  return sum;
+}
+
+// A row's 8 values at 8 lane of a tile's row in LDS -> bf16.
+template <int ROW>
+__device__ __forceinline__ uint4 latent8(const uint8_t* row, int lane) {
+  uint4 o;
+  if constexpr (ROW == DSA_LATENT_ROW_BYTES) {
+    const v2u_t c = *reinterpret_cast<const v2u_t*>(row + 8 * lane);
+    const float s = *reinterpret_cast<const float*>(row + DSA_LATENT_DIM + 4 * (lane >> 4));
+    float f[8];
+    e4m3x4_to_f32(c[0], f);
+    e4m3x4_to_f32(c[1], f + 4);
+    o.x = pack_bf16x2(f[0] * s, f[1] * s);
+    o.y = pack_bf16x2(f[2] * s, f[3] * s);
+    o.z = pack_bf16x2(f[4] * s, f[5] * s);
+    o.w = pack_bf16x2(f[6] * s, f[7] * s);
+  } else {
+    const uint32_t c = *reinterpret_cast<const uint32_t*>(row + 4 * lane);
+    o = dequant8_fp4(c, __uint_as_float((uint32_t)row[DSA_LATENT_DIM / 2 + (lane >> 2)] << 23));
+  }
+  return o;
+}
+__device__ __forceinline__ bool any_nonfinite(const uint4& v) {
+  const auto bad = [](uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; };
+  return bad(v.x) || bad(v.y) || bad(v.z) || bad(v.w);
+}
+
+template <int ROW>
+__global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const ChunkAttnArgs A) {
+  constexpr int kRaw = kPfKeys * ROW;       // bytes of a tile in the pool
+  constexpr int kRawChunks = kRaw / 16;     // 1312 or 800
+  constexpr int kRawLoads = (kRawChunks + kPfThreads - 1) / kPfThreads;
+  static_assert(kRaw % 16 == 0, "whole chunks");
+  __shared__ __align__(16) uint16_t kb[2 * kPfKeys * DSA_QK_DIM];
+  __shared__ __align__(16) uint8_t raw[2 * kRaw];
+  __shared__ int redo;
+  const int t = threadIdx.x, lane = t & (kWave - 1), wv = wave_id();
+  const int n = lane & 31, h = lane >> 5;
+
+  // this workgroup's share; neighbours on the line run on one XCD, whose L2
+  // then holds the keys they have in common
+  const int G = (int)gridDim.x;
+  const int g = (int)(blockIdx.x % 8u) * (G / 8) + (int)(blockIdx.x / 8u);  // (G is a multiple of 8)
+  const long total = chunk_total(A);
+  const int shares = (int)min((long)G, max(1L, total / ((long)A.H * kCaShare)));
+  if (t == 0) A.part[g] = int4{-1, 0, 0, 0};
+  if (g >= shares || total == 0) return;
+  ChunkPos at = chunk_find(A, total * g / shares);
+  const ChunkPos end = g + 1 == shares ? ChunkPos{A.B, 0, 0} : chunk_find(A, total * (g + 1) / shares);
+
+  // K operand: row n (+32), chunk 2kk + h
+  uint32_t koff[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) koff[i] = (uint32_t)(n * (DSA_QK_DIM * 2) + ((2 * i + h) ^ pf_swz(n)) * 16);
+  // V operand (transposed read): lane a of a 16-lane group addresses key 4h +
+  // (a >> 2) (+8), dims 16 * (group & 1) + 4 (a & 3)
+  const int a16 = lane & 15, g1 = (lane >> 4) & 1;
+  uint32_t voff[2][2];
+#pragma unroll
+  for (int par = 0; par < 2; ++par)
+#pragma unroll
+    for (int e8 = 0; e8 < 2; ++e8) {
+      const int r = 4 * h + (a16 >> 2) + 8 * e8;
+      const int j = 4 * par + 2 * g1 + ((a16 >> 1) & 1);
+      voff[par][e8] = (uint32_t)(r * (DSA_QK_DIM * 2) + (j ^ pf_swz(r)) * 16 + 8 * (a16 & 1));
+    }
+  const uint32_t raw0 = (uint32_t)(uintptr_t)(lvoid_ptr)raw;
+  const long pool_bytes = A.kv_rows * ROW;
+
+  while (at.b < end.b || (at.b == end.b && (at.tile < end.tile || (at.tile == end.tile && at.kt < end.kt)))) {
+    ChunkReq rq = chunk_req(A, at.b);
+    rq = {uniform(rq.first), uniform(rq.T), uniform(rq.tiles), uniform(rq.P)};
+    if (at.tile >= rq.tiles) {  // the next request
+      at = {at.b + 1, 0, 0};
+      continue;
+    }
+    const int R = rq.T * A.H, r0 = at.tile * kPfRows;
+    const int kend = uniform(chunk_keys(A, rq, at.tile)), ktiles = (kend + kPfKeys - 1) / kPfKeys;
+    const int kfull = uniform(rq.P + r0 / A.H + 1);  // keys every row sees
+    const int t0 = at.kt;
+    const int t1 = at.b == end.b && at.tile == end.tile ? end.kt : ktiles;
+    const bool whole = t0 == 0 && t1 == ktiles;
+    const int* pages = A.page_table + (long)at.b * A.pt_stride;
+
+    const int row = min(r0 + kPfRowsPerWave * wv + n, R - 1);
+    const int limit = min(rq.P + row / A.H + 1, kend);
+    const uint16_t* qrow = A.q + ((long)rq.first * A.H + row) * DSA_QK_DIM + 8 * h;
+
+    // rows of tile tl that hold keys (0: its page is none of the cache's), and
+    // where its bytes are
+    const auto rows_of = [&](int page, int tl) DSA_INLINE {
+      const long slot = (long)page * DSA_PAGE_TOKENS + (tl & 1) * kPfKeys;
+      if (page < 0 || slot >= A.kv_rows) return 0;
+      return (int)min((long)min(kPfKeys, kend - tl * kPfKeys), A.kv_rows - slot);
+    };
+    const auto page_of = [&](int tl) DSA_INLINE { return pages[max(min(tl, t1 - 1), 0) >> 1]; };
+    // Direct-to-LDS loads, written out because the compiler, which cannot tell
+    // the buffers apart, would wait for them before the next LDS read: the
+    // wait is the barrier's, one tile later.  m0 holds the wave's LDS base, to
+    // which the hardware adds 16 bytes a lane.
+    const auto issue = [&](int page, int tl, uint32_t buf) DSA_INLINE {
+      if (!rows_of(page, tl)) return;  // uniform
+      const long base = ((long)page * DSA_PAGE_TOKENS + (tl & 1) * kPfKeys) * ROW;
+      const uint32_t last = (uint32_t)min((long)kRaw, pool_bytes - base) - 16u;  // rows behind the pool's end: read its last
+      const uint8_t* src = A.pool + base;
+#pragma unroll
+      for (int it = 0; it < kRawLoads; ++it) {
+        const int c = it * kPfThreads + t;
+        if (c < kRawChunks) {
+          const uint32_t off = min(16u * (uint32_t)c, last);
+          const uint32_t dst = __builtin_amdgcn_readfirstlane(raw0 + buf + (uint32_t)(it * kPfThreads + wv * kWave) * 16u);
+          asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                       :
+                       : "s"(dst), "v"(off), "s"(src)
+                       : "memory", "m0");
+        }
+      }
+    };
+    // Wave w dequantises rows w, w + 4, ..., 8 values a lane.  In a tile that
+    // some rows do not see to its end (EDGE), 0 * NaN would reach those rows'
+    // outputs: a key with a non-finite latent value (its score is NaN or an
+    // infinity whatever the query) keeps a NaN in its rope, which only the
+    // scores read, and zeros where the values are read; rows without a key are
+    // zeros.
+    const auto convert = [&](uint32_t from, uint16_t* to, int rows, auto edge) DSA_INLINE {
+      const uint8_t* src = raw + from;
+      uint32_t bad = 0;
+#pragma unroll
+      for (int i = 0; i < kPfKeys / kPfWaves; ++i) {
+        const int r = wv + kPfWaves * i;
+        uint4 v = latent8<ROW>(src + r * ROW, lane);
+        if constexpr (decltype(edge)::value) {
+          const bool nan = __ballot(any_nonfinite(v)) != 0;
+          if (nan || r >= rows) v = make_uint4(0, 0, 0, 0);
+          bad |= nan ? 1u << i : 0u;
+        }
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(to) + r * (DSA_QK_DIM * 2) +
+                                  ((lane & ~7) | ((lane & 7) ^ pf_swz(r))) * 16) = v;
+      }
+      // the rope of the wave's 8 rows, 8 lanes a row
+      const int i = lane >> 3, r = wv + kPfWaves * i;
+      uint4 v = *reinterpret_cast<const uint4*>(src + r * ROW + ROW - 128 + 16 * (lane & 7));
+      if constexpr (decltype(edge)::value) {
+        if (r >= rows) v = make_uint4(0, 0, 0, 0);
+        else if (bad & (1u << i)) v.x = 0x7fc07fc0u;
+      }
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(to) + r * (DSA_QK_DIM * 2) + 64 * 16 + ((lane & 7) ^ pf_swz(r)) * 16) = v;
+    };
+    const auto dequantise = [&](int tl, int page, uint32_t from, uint16_t* to) DSA_INLINE {
+      const int rows = rows_of(page, tl);
+      if (tl * kPfKeys + kPfKeys > kfull || rows < kPfKeys) convert(from, to, rows, std::true_type{});
+      else convert(from, to, rows, std::false_type{});
+    };
+
+    v16f o[16];
+    float m = -INFINITY, l = 0.f;
+    bool over = false;
+    uint4 qf[36];
+
+    const auto compute = [&](auto max_only, int tl, int rows, const uint16_t* buf) DSA_INLINE {
+      const uint8_t* kp = reinterpret_cast<const uint8_t*>(buf);
+      v16f s[2];
+      uint4 kf[kPfDepth];
+      const auto k_frag = [&](int kk) DSA_INLINE { return *reinterpret_cast<const uint4*>(kp + koff[kk & 3] + (kk >> 2) * 128); };
+#pragma unroll
+      for (int i = 0; i < kPfDepth; ++i) kf[i] = k_frag(i);
+#pragma unroll
+      for (int kk = 0; kk < 36; ++kk) {
+        const v4i ka = as_v4i(kf[kk % kPfDepth]), qb = as_v4i(qf[kk]);
+        if (kk < 2)
+          asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s[kk]) : "v"(ka), "v"(qb));
+        else
+          asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s[kk & 1]) : "v"(ka), "v"(qb));
+        if (kk + kPfDepth < 36) kf[kk % kPfDepth] = k_frag(kk + kPfDepth);
+      }
+      // the matrix unit's results may be read 19 wait states after the last issue
+      asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]));
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[0][e] += s[1][e];
+      // scores in the log2 domain; keys at or past the row's limit: -inf.
+      // Element i is the tile's key 8 (i / 4) + 4h + (i % 4).
+      const int k0 = tl * kPfKeys;
+      const bool edge = k0 + kPfKeys > kfull || rows < kPfKeys;  // uniform
+      const int seen = min(limit - k0, rows) - 4 * h;
+      float tmax = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float v = s[0][i] * A.sm_log2;
+        if (edge) v = 8 * (i >> 2) + (i & 3) < seen ? v : -INFINITY;
+        s[0][i] = v;
+        tmax = fmaxf(tmax, v);
+      }
+      tmax = half_swap_max(tmax);
+      if constexpr (decltype(max_only)::value) {
+        m = fmaxf(m, tmax);
+        return;
+      }
+      // The reference point of a row's softmax is its first tile's maximum and
+      // stays: any point gives the same result while no probability overflows.
+      // A row that rises more than 2^32 above it is redone from its true
+      // maximum (below).
+      m = m == -INFINITY ? tmax : m;
+      over |= tmax > m + kPfRise;
+      const float mr = m == -INFINITY ? 0.f : m;
+      uint32_t pk[8];
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        s[0][i] = __builtin_amdgcn_exp2f(s[0][i] - mr);
+        s[0][i + 1] = __builtin_amdgcn_exp2f(s[0][i + 1] - mr);
+        pk[i >> 1] = pack_bf16x2(s[0][i], s[0][i + 1]);
+        // the sum of the rounded probabilities, the ones PV multiplies: the
+        // weights then add up to one
+        l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pk[i >> 1]), __builtin_bit_cast(v2bf, 0x3f803f80u), l,
+                                            false);
+      }
+      const auto v_frag = [&](int i) DSA_INLINE {
+        const int ks = i >> 4, dt = i & 15;
+        const uint32_t imm = (dt >> 1) * 128 + ks * (16 * DSA_QK_DIM * 2);
+        const v4s_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(kp + voff[dt & 1][0] + imm));
+        const v4s_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_ptr)(kp + voff[dt & 1][1] + imm));
+        uint4 vf;
+        __builtin_memcpy(&vf.x, &lo, 8);
+        __builtin_memcpy(&vf.z, &hi, 8);
+        return vf;
+      };
+      // Where a row has much of its weight in this tile, what the rounding left
+      // of the probabilities follows as a second product (prefill.hip has the
+      // errors and times of the choices).
+      const auto second = [&](uint32_t* w) DSA_INLINE {
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          w[i >> 1] = pack_bf16x2(s[0][i] - __uint_as_float(pk[i >> 1] << 16),
+                                  s[0][i + 1] - __uint_as_float(pk[i >> 1] & 0xffff0000u));
+          l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w[i >> 1]), __builtin_bit_cast(v2bf, 0x3f803f80u), l,
+                                              false);
+        }
+      };
+      const auto product = [&](const uint4& v, const uint32_t* p, int i) DSA_INLINE {
+        const uint32_t* pr = p + 4 * (i >> 4);
+        o[i & 15] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(v), as_bf8(make_uint4(pr[0], pr[1], pr[2], pr[3])),
+                                                            o[i & 15], 0, 0, 0);
+      };
+      uint4 vf[kPfDepth];
+      const bool two = kend < kPfBothKeys ||
+                       __ballot(__builtin_amdgcn_exp2f(tmax - mr) > kPfSecond * half_swap_sum(l)) != 0;  // uniform
+      // one copy of the products in the code: unrolled, or as two branches, the
+      // accumulators cross the vector file at the join and spill
+#pragma nounroll
+      for (int term = 0;; ++term) {
+#pragma unroll
+        for (int i = 0; i < kPfDepth; ++i) vf[i] = v_frag(i);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          product(vf[i % kPfDepth], pk, i);
+          if (i + kPfDepth < 32) vf[i % kPfDepth] = v_frag(i + kPfDepth);
+        }
+        if (term || !two) break;
+        second(pk);
+      }
+    };
+
+    const auto pass = [&](auto max_only) DSA_INLINE {
+      int p0 = uniform(page_of(t0)), p1 = uniform(page_of(t0 + 1));
+      int p2 = page_of(t0 + 2);
+      asm volatile("" : "+v"(p2));  // waited for here
+      issue(p0, t0, 0u);
+      if (t0 + 1 < t1) issue(p1, t0 + 1, kRaw);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      dequantise(t0, p0, 0u, kb);
+      uint32_t cur = 0;  // of the tile's two places
+      for (int tl = t0; tl < t1; ++tl) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // tile tl is in bf16, tile tl + 1 has landed; what held tl - 1 and tl's bytes is free
+        const int pn = uniform(p2);
+        if (tl + 2 < t1) {
+          p2 = page_of(tl + 3);
+          asm volatile("" : "+v"(p2));  // waited for here, before the loads
+          issue(pn, tl + 2, cur * kRaw);
+        }
+        if (tl + 1 < t1) dequantise(tl + 1, p1, (cur ^ 1u) * kRaw, kb + (cur ^ 1u) * (kPfTileBytes / 2));
+        // (always: a branch around the products takes the accumulators through
+        // the vector file)
+        compute(max_only, tl, rows_of(p0, tl), kb + cur * (kPfTileBytes / 2));
+        p0 = p1;
+        p1 = pn;
+        cur ^= 1u;
+      }
+      __syncthreads();
+    };
+#pragma unroll
+    for (int kk = 0; kk < 36; ++kk) qf[kk] = *reinterpret_cast<const uint4*>(qrow + 16 * kk);
+    // waited for here: later the wait would count the key loads in flight too
+#pragma unroll
+    for (int kk = 0; kk < 36; ++kk) asm volatile("" : : "v"(as_v4i(qf[kk])));
+    if (t == 0) redo = 0;
+    for (int round = 0;; ++round) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+      l = 0.f;
+      over = false;
+      pass(std::false_type{});
+      if (round) break;
+      if (__ballot(over) && lane == 0) redo = 1;
+      __syncthreads();
+      if (!uniform(redo)) break;
+      m = -INFINITY;
+      pass(std::true_type{});
+    }
+    __syncthreads();  // (everyone has read redo)
+
+    l = half_swap_sum(l);
+    if (r0 + kPfRowsPerWave * wv + n < R) {
+      // lane (n, h) holds dims 32 dt + 8 (i / 4) + 4h + (i % 4) of its row
+      if (whole) {
+        const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);  // a row without a key gives 0, NaN stays
+        uint16_t* orow = A.out + ((long)rq.first * A.H + row) * DSA_LATENT_DIM + 4 * h;
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            v2u_t w;
+            w[0] = pack_bf16x2(o[dt][i] * inv, o[dt][i + 1] * inv);
+            w[1] = pack_bf16x2(o[dt][i + 2] * inv, o[dt][i + 3] * inv);
+            *reinterpret_cast<v2u_t*>(orow + 32 * dt + 2 * i) = w;
+          }
+      } else {
+        // the part of a tile that began before this share, or of the one that ends behind it
+        const long pr = (long)(2 * g + (t0 == 0)) * A.part_rows + (row - r0);
+        float* po = A.part_o + pr * DSA_LATENT_DIM + 4 * h;
+#pragma unroll
+        for (int dt = 0; dt < 16; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; i += 4) {
+            v4f w = {o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
+            *reinterpret_cast<v4f*>(po + 32 * dt + 2 * i) = w;
+          }
+        if (h == 0) {
+          A.part_ml[2 * pr] = m;
+          A.part_ml[2 * pr + 1] = l;
+        }
+      }
+    }
+    if (t == 0 && !whole) {
+      int4 d = A.part[g];
+      if (t0 == 0) d.x = at.b, d.y = at.tile;       // began here, goes on in the next share
+      else d.z = t1 == ktiles ? 2 : 1;              // began before: ends here, or not
+      A.part[g] = d;
+    }
+    if (at.b == end.b && at.tile == end.tile) break;
+    at = {at.b, at.tile + 1, 0};
+  }
+}
+
+// Joins a row's parts: out = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m), m =
+// max m_s.  Workgroup (i, r): row r of the i-th row tile that more than one
+// share has part of; wave w takes the parts w, w + 4, ... (8 dims a lane), then
+// the four sums meet in LDS, always in the same order.
+__global__ __launch_bounds__(kPfThreads) void chunk_merge_kernel(const ChunkAttnArgs A, int G) {
+  __shared__ float sl[kPfWaves];
+  __shared__ v4f so[kPfWaves][2 * kWave];
+  const int lane = threadIdx.x & (kWave - 1), wv = wave_id();
+  const int r = (int)(blockIdx.x % (unsigned)A.part_rows);
+  int left = (int)(blockIdx.x / (unsigned)A.part_rows), first = -1;
+  for (int g0 = 0; g0 < G && first < 0; g0 += kWave) {
+    uint64_t has = __ballot(g0 + lane < G && A.part[min(g0 + lane, G - 1)].x >= 0);
+    const int here = __builtin_popcountll(has);
+    if (left >= here) {
+      left -= here;
+      continue;
+    }
+    for (; left > 0; --left) has &= has - 1;
+    first = g0 + __builtin_ctzll(has);
+  }
+  if (first < 0) return;
+  const int4 d = A.part[first];
+  const ChunkReq rq = chunk_req(A, d.x);
+  const long row = (long)d.y * kPfRows + r;
+  if (row >= (long)rq.T * A.H) return;
+  int parts = 1;  // the first share's, then those up to the one where the tile ends
+  for (int g0 = first + 1; g0 < G; g0 += kWave) {
+    const uint64_t ends = __ballot(g0 + lane < G && A.part[min(g0 + lane, G - 1)].z == 2);
+    if (ends) {
+      parts += __builtin_ctzll(ends) + 1;
+      break;
+    }
+    parts += kWave;
+  }
+  const auto slot = [&](int s) { return (long)(s ? 2 * (first + s) : 2 * first + 1) * A.part_rows + r; };
+  float m = -INFINITY;
+  for (int s = lane; s < parts; s += kWave) m = fmaxf(m, A.part_ml[2 * slot(s)]);
+  m = wave_max(m);
+  const float mr = m == -INFINITY ? 0.f : m;
+  float L = 0.f;
+  v4f x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
+  constexpr int kU = 4;
+  for (int s0 = wv; s0 < parts; s0 += kU * kPfWaves) {
+    v4f a[kU], c[kU];
+    float ms[kU], ls[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int s = s0 + u * kPfWaves;
+      const long pr = slot(s < parts ? s : wv);  // past the last: read again, weight 0
+      const v4f* po = reinterpret_cast<const v4f*>(A.part_o + pr * DSA_LATENT_DIM) + 2 * lane;
+      a[u] = po[0];
+      c[u] = po[1];
+      ms[u] = A.part_ml[2 * pr];
+      ls[u] = A.part_ml[2 * pr + 1];
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      if (s0 + u * kPfWaves >= parts) break;  // uniform
+      const float w = exp2f(ms[u] - mr);
+      L += ls[u] * w;
+      x0 += a[u] * w;
+      x1 += c[u] * w;
+    }
+  }
+  so[wv][2 * lane] = x0;
+  so[wv][2 * lane + 1] = x1;
+  if (lane == 0) sl[wv] = L;
+  __syncthreads();
+  const float tot = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+  const float inv = tot > 0.f ? 1.f / tot : (tot == tot ? 0.f : tot);
+  if (threadIdx.x < 2 * kWave) {
+    const int i = threadIdx.x;
+    const v4f o = (so[0][i] + so[1][i]) + (so[2][i] + so[3][i]);
+    v2u_t w;
+    w[0] = pack_bf16x2(o[0] * inv, o[1] * inv);
+    w[1] = pack_bf16x2(o[2] * inv, o[3] * inv);
+    *reinterpret_cast<v2u_t*>(A.out + ((long)rq.first * A.H + row) * DSA_LATENT_DIM + 4 * i) = w;
+  }
+}
+
+static int chunk_shares() { return std::max(8, device_cu_count() / 8 * 8); }
+static int chunk_part_rows(int n, int H) { return (int)std::min<long>(kPfRows, (long)n * H); }
+
+// [a workgroup's two parts | (reference point, sum) of their rows | what they are parts of]
+size_t chunk_workspace_bytes(int n, int H) {
+  const size_t G = (size_t)chunk_shares();
+  return 2 * G * chunk_part_rows(n, H) * (DSA_LATENT_DIM + 2) * sizeof(float) + G * sizeof(int4);
+}
+
+hipError_t launch_chunk_attention(ChunkAttnArgs A, int row_bytes, void* workspace, hipStream_t s) {
+  const int G = chunk_shares();
+  A.part_rows = chunk_part_rows(A.n, A.H);
+  A.part_o = static_cast<float*>(workspace);
+  A.part_ml = A.part_o + (size_t)2 * G * A.part_rows * DSA_LATENT_DIM;
+  A.part = reinterpret_cast<int4*>(A.part_ml + (size_t)2 * G * A.part_rows * 2);
+  const dim3 block(kPfThreads);
+  if (row_bytes == DSA_LATENT_ROW_BYTES)
+    hipLaunchKernelGGL(chunk_attention_kernel<DSA_LATENT_ROW_BYTES>, dim3(G), block, 0, s, A);
+  else
+    hipLaunchKernelGGL(chunk_attention_kernel<DSA_FP4_ROW_BYTES>, dim3(G), block, 0, s, A);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  // row tiles there may be, and those that two shares can have part of
+  const long tiles = (long)A.n * A.H / kPfRows + std::min(A.B, A.n);
+  const long split = std::min<long>(tiles, G - 1);
+  hipLaunchKernelGGL(chunk_merge_kernel, dim3((unsigned)(split * A.part_rows)), block, 0, s, A, G);
+  return hipGetLastError();
+}
+
+}  // namespace dsa

@@ -141,6 +141,28 @@ struct ChunkScanArgs {
 };
 hipError_t launch_chunk_scan(const ChunkScanArgs& C, hipStream_t s);
 
+// Attention of the new tokens of several requests over the paged latent cache
+// (chunk_attention.hip).
+struct ChunkAttnArgs {
+  const uint16_t* q;     // [n, H, 576] bf16
+  const uint8_t* pool;   // [kv_rows, 656 or 400]
+  long kv_rows;
+  const int* page_table; // [B, pt_stride]
+  const int* q_start;    // [B + 1]
+  const int* seq_lens;   // [B]
+  uint16_t* out;         // [n, H, 512] bf16
+  float sm_log2;         // sm_scale * log2(e)
+  int n, B, H, pt_stride;
+  // filled by the launcher
+  float* part_o;         // [2 * shares][part_rows][512]
+  float* part_ml;        // [2 * shares][part_rows][2]
+  int4* part;            // [shares]: request (-1: none) and row tile that begin here and go on;
+                         // 1, 2: the first piece began before and goes on, ends here
+  int part_rows;
+};
+size_t chunk_workspace_bytes(int n, int H);
+hipError_t launch_chunk_attention(ChunkAttnArgs A, int row_bytes, void* workspace, hipStream_t s);
+
 // Rows to e4m3 (quant_rows.hip).  Strides in elements.
 struct QuantRowsArgs {
   const void* x;      // [n, D], row stride xs

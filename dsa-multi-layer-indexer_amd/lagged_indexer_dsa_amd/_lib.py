@@ -126,6 +126,8 @@ SIGNATURES = {
     "dsa_dense_mla_decode_fp4": (_i32, [_vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _f32, _vp]),
     "dsa_quantize_rows": (_i32, [ctypes.c_char_p, _vp]),
     "dsa_fp8_matmul": (_i32, [ctypes.c_char_p, _vp]),
+    "dsa_chunk_attention_workspace_bytes": (ctypes.c_size_t, [_i32, _i32]),
+    "dsa_chunk_attention": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _f32, _vp]),
     "dsa_chunk_scan": (_i32, [_vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp]),
 }
 

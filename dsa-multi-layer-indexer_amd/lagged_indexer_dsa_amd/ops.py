@@ -990,3 +990,56 @@ def chunk_scan(q_fp8: torch.Tensor, w: torch.Tensor, index_k: torch.Tensor, page
                   q_start.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), n, B, Hidx, page_table.shape[1], slab_stride,
                   _stream())
     return out
+
+
+def chunk_workspace(n: int, H: int, device) -> torch.Tensor:
+    """Workspace of :func:`chunk_attention` calls of up to n rows of up to H
+    heads (no initialisation needed; at most 135 MB)."""
+    nbytes = _lib.load().dsa_chunk_attention_workspace_bytes(n, H)
+    if nbytes == 0:
+        raise RuntimeError(f"bad chunk attention shape n={n} H={H}")
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def chunk_attention(q: torch.Tensor, kv_pool: torch.Tensor, page_table: torch.Tensor, q_start: torch.Tensor,
+                    seq_lens: torch.Tensor, sm_scale: float | None = None, workspace: torch.Tensor | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """:func:`dense_mla_decode` for more than one row a request: rows q_start[b]
+    .. q_start[b + 1] - 1 are the last tokens of request b, whose latent rows
+    (theirs too) are the first seq_lens[b] of the paged cache; each attends the
+    tokens up to its own.
+
+    q [n,H,576] bf16; kv_pool [rows,656] or [rows,400] uint8; page_table [B,pt]
+    int32; q_start [B+1] int32, not falling; seq_lens [B] int32  ->  out
+    [n,H,512] bf16 (0 for a row before position 0).  Rows of no request are left
+    as they are (a new out: undefined).  workspace: :func:`chunk_workspace` of
+    at least this n and H; calls that overlap in time must not share one.  For a
+    sparse layer's chunk each row is a row of :func:`sparse_mla_decode`.
+    Reference: attention_core.py:142-160 dense_mla_core.
+    """
+    qs, ps = q.shape, kv_pool.shape
+    dev = q.get_device()
+    _here(dev, kv_pool, page_table, q_start, seq_lens, workspace, out)
+    if len(qs) != 3 or qs[2] != QK_DIM or q.dtype != torch.bfloat16 or not q.is_contiguous():
+        raise RuntimeError("q must be contiguous [n, H, 576] bfloat16")
+    n, H, _ = qs
+    if len(ps) != 2 or (ps[1] != LATENT_ROW_BYTES and ps[1] != FP4_ROW_BYTES) or not ps[0] or \
+            kv_pool.dtype != torch.uint8 or not kv_pool.is_contiguous():
+        raise RuntimeError("kv_pool must be contiguous [rows, 656] or [rows, 400] uint8")
+    B = _chunk(page_table, q_start, seq_lens)
+    if out is None:
+        out = torch.empty(n, H, LATENT_DIM, dtype=torch.bfloat16, device=q.device)
+    else:
+        _need_shape("out", out, (n, H, LATENT_DIM), torch.bfloat16)
+    if n:
+        if workspace is None:
+            workspace = chunk_workspace(n, H, q.device)
+        else:
+            if not workspace.is_contiguous():
+                raise RuntimeError("the chunk attention workspace must be contiguous")
+            _need_bytes("chunk attention workspace", workspace, _lib.load().dsa_chunk_attention_workspace_bytes(n, H))
+        _lib.call("dsa_chunk_attention", q.data_ptr(), kv_pool.data_ptr(), ps[0], ps[1], page_table.data_ptr(),
+                  q_start.data_ptr(), seq_lens.data_ptr(), workspace.data_ptr(), out.data_ptr(), n, B, H,
+                  page_table.shape[1], QK_DIM ** -0.5 if sm_scale is None else float(sm_scale),
+                  torch._C._cuda_getCurrentRawStream(dev))
+    return out

@@ -616,6 +616,28 @@ int dsa_chunk_scan(const void* q_fp8, const float* w, const void* index_k, int64
                    const int32_t* q_start, const int32_t* seq_lens, float* scores, int n, int B, int Hidx, int pt_stride,
                    int slab_stride, void* stream);
 
+/*
+ * (16) Dense attention of a chunk: (15)'s rows, each over the latent rows of its
+ * request's tokens up to its own.
+ *   out[i, h, :] = sum_{g <= p} softmax_g(sm_scale * q[i, h, :] . kv_g) * kv_g[:512]
+ * with kv_g as (3) (656-byte rows) or (12) (400-byte rows) reads them.
+ *   q [n, H, 576] bf16, out [n, H, 512] bf16, kv_pool [kv_rows, row_bytes],
+ *   page_table [B, pt_stride], q_start [B + 1] (not falling), seq_lens [B];
+ *   H a multiple of 16, n * H < 2^31.
+ *   workspace dsa_chunk_attention_workspace_bytes(n, H) bytes, no
+ *   initialisation (at most 135 MB; not falling in n and H); calls that overlap
+ *   in time must not share it.
+ * A key in a page, or at a slot, outside the pool is masked; a row that sees no
+ * key gives 0; rows of no request are left as they are.  Where a row's keys are
+ * divided, and so the last bits of its output, depends on the other rows and
+ * the device's CU count: equal calls give equal bits.
+ * Replaces: dense_mla_core (attention_core.py:142-160) over a paged cache.
+ */
+size_t dsa_chunk_attention_workspace_bytes(int n, int H);
+int dsa_chunk_attention(const void* q_bf16, const void* kv_pool, int64_t kv_rows, int row_bytes, const int32_t* page_table,
+                        const int32_t* q_start, const int32_t* seq_lens, void* workspace, void* out_bf16, int n, int B, int H,
+                        int pt_stride, float sm_scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
