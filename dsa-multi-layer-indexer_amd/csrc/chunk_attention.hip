@@ -34,6 +34,13 @@ namespace dsa {
 
 constexpr int kCaTileCost = 64;   // keys' worth of a row tile's start and end
 constexpr int kCaShare = 256;     // the least share of a workgroup, in keys of a row tile
+// A row's reference point lies this far above its first tile's maximum (in
+// log2), and a score may rise this far above the reference: any point gives the
+// same sums (bf16 and fp32 have 8 bits of exponent, and a probability's error is
+// relative) while no probability overflows, and one that underflows is below
+// 2^-90 of the row's largest.  A row of scores that rise by more, 96 in log2,
+// is redone from its true maximum.
+constexpr float kCaAbove = 32.f, kCaRise = 64.f;
 
 // A workgroup's place on the line of work: request, row tile, key tile of it.
 struct ChunkPos {
@@ -162,6 +169,8 @@ __device__ __forceinline__ bool any_nonfinite(const uint4& v) {
   return bad(v.x) || bad(v.y) || bad(v.z) || bad(v.w);
 }
 
+typedef const __attribute__((address_space(4))) int* const_int_ptr;
+
 template <int ROW>
 __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const ChunkAttnArgs A) {
   constexpr int kRaw = kPfKeys * ROW;       // bytes of a tile in the pool
@@ -217,7 +226,9 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
     const int t0 = at.kt;
     const int t1 = at.b == end.b && at.tile == end.tile ? end.kt : ktiles;
     const bool whole = t0 == 0 && t1 == ktiles;
-    const int* pages = A.page_table + (long)at.b * A.pt_stride;
+    // (in the constant address space: scalar loads, which do not wait in line
+    // with the keys'; nothing writes the table meanwhile)
+    const auto* pages = (const_int_ptr)(A.page_table + (long)at.b * A.pt_stride);
 
     const int row = min(r0 + kPfRowsPerWave * wv + n, R - 1);
     const int limit = min(rq.P + row / A.H + 1, kend);
@@ -262,26 +273,27 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
     const auto convert = [&](uint32_t from, uint16_t* to, int rows, auto edge) DSA_INLINE {
       const uint8_t* src = raw + from;
       uint32_t bad = 0;
+      int ln = lane;
+      asm volatile("" : "+v"(ln));  // (addresses formed here: kept over the loop they would be spilled)
 #pragma unroll
       for (int i = 0; i < kPfKeys / kPfWaves; ++i) {
         const int r = wv + kPfWaves * i;
-        uint4 v = latent8<ROW>(src + r * ROW, lane);
+        uint4 v = latent8<ROW>(src + r * ROW, ln);
         if constexpr (decltype(edge)::value) {
           const bool nan = __ballot(any_nonfinite(v)) != 0;
           if (nan || r >= rows) v = make_uint4(0, 0, 0, 0);
           bad |= nan ? 1u << i : 0u;
         }
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(to) + r * (DSA_QK_DIM * 2) +
-                                  ((lane & ~7) | ((lane & 7) ^ pf_swz(r))) * 16) = v;
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(to) + r * (DSA_QK_DIM * 2) + 16 * (ln ^ pf_swz(r))) = v;
       }
       // the rope of the wave's 8 rows, 8 lanes a row
-      const int i = lane >> 3, r = wv + kPfWaves * i;
-      uint4 v = *reinterpret_cast<const uint4*>(src + r * ROW + ROW - 128 + 16 * (lane & 7));
+      const int i = ln >> 3, r = wv + kPfWaves * i;
+      uint4 v = *reinterpret_cast<const uint4*>(src + r * ROW + ROW - 128 + 16 * (ln & 7));
       if constexpr (decltype(edge)::value) {
         if (r >= rows) v = make_uint4(0, 0, 0, 0);
         else if (bad & (1u << i)) v.x = 0x7fc07fc0u;
       }
-      *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(to) + r * (DSA_QK_DIM * 2) + 64 * 16 + ((lane & 7) ^ pf_swz(r)) * 16) = v;
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(to) + r * (DSA_QK_DIM * 2) + 64 * 16 + ((ln & 7) ^ pf_swz(r)) * 16) = v;
     };
     const auto dequantise = [&](int tl, int page, uint32_t from, uint16_t* to) DSA_INLINE {
       const int rows = rows_of(page, tl);
@@ -332,12 +344,8 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
         m = fmaxf(m, tmax);
         return;
       }
-      // The reference point of a row's softmax is its first tile's maximum and
-      // stays: any point gives the same result while no probability overflows.
-      // A row that rises more than 2^32 above it is redone from its true
-      // maximum (below).
-      m = m == -INFINITY ? tmax : m;
-      over |= tmax > m + kPfRise;
+      m = m == -INFINITY ? tmax + kCaAbove : m;
+      over |= tmax > m + kCaRise;
       const float mr = m == -INFINITY ? 0.f : m;
       uint32_t pk[8];
 #pragma unroll
@@ -397,9 +405,7 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
     };
 
     const auto pass = [&](auto max_only) DSA_INLINE {
-      int p0 = uniform(page_of(t0)), p1 = uniform(page_of(t0 + 1));
-      int p2 = page_of(t0 + 2);
-      asm volatile("" : "+v"(p2));  // waited for here
+      int p0 = page_of(t0), p1 = page_of(t0 + 1), p2 = page_of(t0 + 2);
       issue(p0, t0, 0u);
       if (t0 + 1 < t1) issue(p1, t0 + 1, kRaw);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -409,18 +415,15 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
       for (int tl = t0; tl < t1; ++tl) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();  // tile tl is in bf16, tile tl + 1 has landed; what held tl - 1 and tl's bytes is free
-        const int pn = uniform(p2);
-        if (tl + 2 < t1) {
-          p2 = page_of(tl + 3);
-          asm volatile("" : "+v"(p2));  // waited for here, before the loads
-          issue(pn, tl + 2, cur * kRaw);
-        }
+        const int p3 = page_of(tl + 3);
         if (tl + 1 < t1) dequantise(tl + 1, p1, (cur ^ 1u) * kRaw, kb + (cur ^ 1u) * (kPfTileBytes / 2));
+        if (tl + 2 < t1) issue(p2, tl + 2, cur * kRaw);
         // (always: a branch around the products takes the accumulators through
         // the vector file)
         compute(max_only, tl, rows_of(p0, tl), kb + cur * (kPfTileBytes / 2));
         p0 = p1;
-        p1 = pn;
+        p1 = p2;
+        p2 = p3;
         cur ^= 1u;
       }
       __syncthreads();
