@@ -40,6 +40,8 @@ constexpr int kCaShare = 256;     // the least share of a workgroup, in keys of 
 // relative) while no probability overflows, and one that underflows is below
 // 2^-90 of the row's largest.  A row of scores that rise by more, 96 in log2,
 // is redone from its true maximum.
+constexpr int kCaHeld = 34;       // of the 36 fragments of a row's query, those in registers
+constexpr int kCaDepth = 5, kCaDepthK = 6;
 constexpr float kCaAbove = 32.f, kCaRise = 64.f;
 
 // A workgroup's place on the line of work: request, row tile, key tile of it.
@@ -144,26 +146,44 @@ __device__ __forceinline__ long chunk_total(const ChunkAttnArgs& A) {
   return sum;
 }
 
-// A row's 8 values at 8 lane of a tile's row in LDS -> bf16.
+// 8 values of a row in LDS, the codes at 8 lane and their scale, to bf16 in
+// three steps that take their place between products.
 template <int ROW>
-__device__ __forceinline__ uint4 latent8(const uint8_t* row, int lane) {
-  uint4 o;
-  if constexpr (ROW == DSA_LATENT_ROW_BYTES) {
-    const v2u_t c = *reinterpret_cast<const v2u_t*>(row + 8 * lane);
-    const float s = *reinterpret_cast<const float*>(row + DSA_LATENT_DIM + 4 * (lane >> 4));
-    float f[8];
-    e4m3x4_to_f32(c[0], f);
-    e4m3x4_to_f32(c[1], f + 4);
-    o.x = pack_bf16x2(f[0] * s, f[1] * s);
-    o.y = pack_bf16x2(f[2] * s, f[3] * s);
-    o.z = pack_bf16x2(f[4] * s, f[5] * s);
-    o.w = pack_bf16x2(f[6] * s, f[7] * s);
-  } else {
-    const uint32_t c = *reinterpret_cast<const uint32_t*>(row + 4 * lane);
-    o = dequant8_fp4(c, __uint_as_float((uint32_t)row[DSA_LATENT_DIM / 2 + (lane >> 2)] << 23));
+struct Latent8 {
+  static constexpr bool kE4m3 = ROW == DSA_LATENT_ROW_BYTES;
+  v2u_t c;
+  float s, f[8];
+  __device__ __forceinline__ void load_codes(const uint8_t* row, int lane) {
+    if constexpr (kE4m3) c = *reinterpret_cast<const v2u_t*>(row + 8 * lane);
+    else c[0] = *reinterpret_cast<const uint32_t*>(row + 4 * lane);
   }
-  return o;
-}
+  __device__ __forceinline__ void load_scale(const uint8_t* row, int lane) {
+    if constexpr (kE4m3) s = *reinterpret_cast<const float*>(row + DSA_LATENT_DIM + 4 * (lane >> 4));
+    else s = __uint_as_float((uint32_t)row[DSA_LATENT_DIM / 2 + (lane >> 2)] << 23);
+  }
+  __device__ __forceinline__ void unpack() {
+    if constexpr (kE4m3) {
+      e4m3x4_to_f32(c[0], f);
+      e4m3x4_to_f32(c[1], f + 4);
+    } else {
+      f[0] = __uint_as_float(c[0]);
+    }
+  }
+  __device__ __forceinline__ void scale() {
+    if constexpr (kE4m3) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= s;
+    } else {
+      const uint4 v = dequant8_fp4(__float_as_uint(f[0]), s);
+      f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+    }
+  }
+  __device__ __forceinline__ uint4 bf16() const {
+    if constexpr (kE4m3)
+      return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+};
 __device__ __forceinline__ bool any_nonfinite(const uint4& v) {
   const auto bad = [](uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; };
   return bad(v.x) || bad(v.y) || bad(v.z) || bad(v.w);
@@ -177,8 +197,10 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
   constexpr int kRawChunks = kRaw / 16;     // 1312 or 800
   constexpr int kRawLoads = (kRawChunks + kPfThreads - 1) / kPfThreads;
   static_assert(kRaw % 16 == 0, "whole chunks");
-  __shared__ __align__(16) uint16_t kb[2 * kPfKeys * DSA_QK_DIM];
+  constexpr uint32_t kRawFlip = kRaw;  // (the two places: 0 and kRaw)
+  __shared__ __align__(16) uint8_t kb[3 * kPfTileBytes];
   __shared__ __align__(16) uint8_t raw[2 * kRaw];
+  __shared__ uint4 ql[kPfWaves][36 - kCaHeld][kWave];  // fragments of the query that find no registers
   __shared__ int redo;
   const int t = threadIdx.x, lane = t & (kWave - 1), wv = wave_id();
   const int n = lane & 31, h = lane >> 5;
@@ -264,100 +286,135 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
         }
       }
     };
-    // Wave w dequantises rows w, w + 4, ..., 8 values a lane.  In a tile that
-    // some rows do not see to its end (EDGE), 0 * NaN would reach those rows'
-    // outputs: a key with a non-finite latent value (its score is NaN or an
-    // infinity whatever the query) keeps a NaN in its rope, which only the
-    // scores read, and zeros where the values are read; rows without a key are
-    // zeros.
-    const auto convert = [&](uint32_t from, uint16_t* to, int rows, auto edge) DSA_INLINE {
-      const uint8_t* src = raw + from;
-      uint32_t bad = 0;
-      int ln = lane;
+    // Wave w dequantises rows w, w + 4, ... of the next tile, 8 values a lane,
+    // between its products of this one: `from` its bytes, `to` its bf16 place.
+    constexpr int kSteps = kPfKeys / kPfWaves;
+    Latent8<ROW> lat;
+    uint4 rope;
+    int ln = lane;
+    const auto conv_begin = [&](const uint8_t* from) DSA_INLINE {
+      ln = lane;
       asm volatile("" : "+v"(ln));  // (addresses formed here: kept over the loop they would be spilled)
-#pragma unroll
-      for (int i = 0; i < kPfKeys / kPfWaves; ++i) {
-        const int r = wv + kPfWaves * i;
-        uint4 v = latent8<ROW>(src + r * ROW, ln);
-        if constexpr (decltype(edge)::value) {
-          const bool nan = __ballot(any_nonfinite(v)) != 0;
-          if (nan || r >= rows) v = make_uint4(0, 0, 0, 0);
-          bad |= nan ? 1u << i : 0u;
-        }
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(to) + r * (DSA_QK_DIM * 2) + 16 * (ln ^ pf_swz(r))) = v;
-      }
-      // the rope of the wave's 8 rows, 8 lanes a row
-      const int i = ln >> 3, r = wv + kPfWaves * i;
-      uint4 v = *reinterpret_cast<const uint4*>(src + r * ROW + ROW - 128 + 16 * (ln & 7));
-      if constexpr (decltype(edge)::value) {
-        if (r >= rows) v = make_uint4(0, 0, 0, 0);
-        else if (bad & (1u << i)) v.x = 0x7fc07fc0u;
-      }
-      *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(to) + r * (DSA_QK_DIM * 2) + 64 * 16 + ((ln & 7) ^ pf_swz(r)) * 16) = v;
+      lat.load_codes(from + wv * ROW, ln);
+      lat.load_scale(from + wv * ROW, ln);
     };
-    const auto dequantise = [&](int tl, int page, uint32_t from, uint16_t* to) DSA_INLINE {
+    const auto conv_slice = [&](int i, const uint8_t* from, uint8_t* to) DSA_INLINE {
+      const int st = i / 4, r = wv + kPfWaves * st;  // slices 4 st .. 4 st + 3: row st
+      const uint8_t* const nextrow = from + (r + kPfWaves) * ROW;
+      if (i % 4 == 0) {
+        lat.unpack();
+        if (st + 1 < kSteps) lat.load_codes(nextrow, ln);
+      } else if (i % 4 == 1) {
+        lat.scale();
+        if (st + 1 < kSteps) lat.load_scale(nextrow, ln);
+      } else if (i % 4 == 2) {
+        *reinterpret_cast<uint4*>(to + r * (DSA_QK_DIM * 2) + 16 * (ln ^ pf_swz(r))) = lat.bf16();
+      } else if (st == kSteps - 2) {  // the rope of the wave's 8 rows, 8 lanes a row
+        rope = *reinterpret_cast<const uint4*>(from + (wv + kPfWaves * (ln >> 3)) * ROW + ROW - 128 + 16 * (ln & 7));
+      } else if (st == kSteps - 1) {
+        const int rr = wv + kPfWaves * (ln >> 3);
+        *reinterpret_cast<uint4*>(to + rr * (DSA_QK_DIM * 2) + 64 * 16 + ((ln & 7) ^ pf_swz(rr)) * 16) = rope;
+      }
+    };
+    // In a tile that some rows do not see to its end, 0 * NaN would reach those
+    // rows' outputs: a key with a non-finite latent value (its score is NaN or
+    // an infinity whatever the query) keeps a NaN in its rope, which only the
+    // scores read, and zeros where the values are read; rows without a key are
+    // zeros.  (A wave's own rows: no barrier.)
+    const auto conv_end = [&](int tl, int page, uint8_t* to) DSA_INLINE {
       const int rows = rows_of(page, tl);
-      if (tl * kPfKeys + kPfKeys > kfull || rows < kPfKeys) convert(from, to, rows, std::true_type{});
-      else convert(from, to, rows, std::false_type{});
+      if (tl * kPfKeys + kPfKeys <= kfull && rows == kPfKeys) return;  // uniform
+#pragma nounroll
+      for (int i = 0; i < kSteps; ++i) {
+        const int r = wv + kPfWaves * i;
+        uint8_t* dst = to + r * (DSA_QK_DIM * 2);
+        const bool nan = __ballot(any_nonfinite(reinterpret_cast<const uint4*>(dst)[lane])) != 0;
+        if (nan || r >= rows) reinterpret_cast<uint4*>(dst)[lane] = make_uint4(0, 0, 0, 0);
+        if ((nan || r >= rows) && lane < 8) {
+          const uint32_t x = r < rows ? 0x7fc07fc0u : 0u;
+          reinterpret_cast<uint4*>(dst)[kWave + lane] = make_uint4(x, x, x, x);
+        }
+      }
     };
 
     v16f o[16];
     float m = -INFINITY, l = 0.f;
     bool over = false;
-    uint4 qf[36];
+    uint4 qf[kCaHeld];
+    v16f s;       // scores of a tile, then its probabilities
+    v16f sn;      // the next tile's scores
 
-    const auto compute = [&](auto max_only, int tl, int rows, const uint16_t* buf) DSA_INLINE {
-      const uint8_t* kp = reinterpret_cast<const uint8_t*>(buf);
-      v16f s[2];
-      uint4 kf[kPfDepth];
-      const auto k_frag = [&](int kk) DSA_INLINE { return *reinterpret_cast<const uint4*>(kp + koff[kk & 3] + (kk >> 2) * 128); };
+    const auto k_frag = [&](const uint8_t* kp, int kk) DSA_INLINE {
+      return *reinterpret_cast<const uint4*>(kp + koff[kk & 3] + (kk >> 2) * 128);
+    };
+    // K Q^T of a tile, a slice of other work after each product (the compiler
+    // would gather either)
+    const auto scores = [&](const uint8_t* kp, auto slice) DSA_INLINE {
+      uint4 kf[kCaDepthK];
 #pragma unroll
-      for (int i = 0; i < kPfDepth; ++i) kf[i] = k_frag(i);
+      for (int i = 0; i < kCaDepthK; ++i) kf[i] = k_frag(kp, i);
 #pragma unroll
       for (int kk = 0; kk < 36; ++kk) {
-        const v4i ka = as_v4i(kf[kk % kPfDepth]), qb = as_v4i(qf[kk]);
-        if (kk < 2)
-          asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(s[kk]) : "v"(ka), "v"(qb));
+        const v4i ka = as_v4i(kf[kk % kCaDepthK]), qb = as_v4i(kk < kCaHeld ? qf[kk] : ql[wv][kk - kCaHeld][lane]);
+        if (kk == 0)
+          asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(sn) : "v"(ka), "v"(qb));
         else
-          asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(s[kk & 1]) : "v"(ka), "v"(qb));
-        if (kk + kPfDepth < 36) kf[kk % kPfDepth] = k_frag(kk + kPfDepth);
+          asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+v"(sn) : "v"(ka), "v"(qb));
+        if (kk + kCaDepthK < 36) kf[kk % kCaDepthK] = k_frag(kp, kk + kCaDepthK);
+        slice(kk);
+        __builtin_amdgcn_sched_barrier(0);
       }
       // the matrix unit's results may be read 19 wait states after the last issue
-      asm volatile("s_nop 15\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]));
+      asm volatile("s_nop 15\n\ts_nop 7" : "+v"(sn));
+    };
+    // The next tile's scores become this one's: in the log2 domain, keys at or
+    // past the row's limit -inf.  Element i is the tile's key 8 (i / 4) + 4h + (i % 4).
+    const auto take_scores = [&](int tl, int rows) DSA_INLINE {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[0][e] += s[1][e];
-      // scores in the log2 domain; keys at or past the row's limit: -inf.
-      // Element i is the tile's key 8 (i / 4) + 4h + (i % 4).
+      for (int e = 0; e < 16; ++e) s[e] = sn[e] * A.sm_log2;
       const int k0 = tl * kPfKeys;
-      const bool edge = k0 + kPfKeys > kfull || rows < kPfKeys;  // uniform
-      const int seen = min(limit - k0, rows) - 4 * h;
-      float tmax = -INFINITY;
+      if (k0 + kPfKeys > kfull || rows < kPfKeys) {  // uniform
+        const int seen = min(limit - k0, rows) - 4 * h;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float v = s[0][i] * A.sm_log2;
-        if (edge) v = 8 * (i >> 2) + (i & 3) < seen ? v : -INFINITY;
-        s[0][i] = v;
-        tmax = fmaxf(tmax, v);
+        for (int i = 0; i < 16; ++i) s[i] = 8 * (i >> 2) + (i & 3) < seen ? s[i] : -INFINITY;
       }
-      tmax = half_swap_max(tmax);
-      if constexpr (decltype(max_only)::value) {
-        m = fmaxf(m, tmax);
-        return;
-      }
-      m = m == -INFINITY ? tmax + kCaAbove : m;
-      over |= tmax > m + kCaRise;
-      const float mr = m == -INFINITY ? 0.f : m;
-      uint32_t pk[8];
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        s[0][i] = __builtin_amdgcn_exp2f(s[0][i] - mr);
-        s[0][i + 1] = __builtin_amdgcn_exp2f(s[0][i + 1] - mr);
-        pk[i >> 1] = pack_bf16x2(s[0][i], s[0][i + 1]);
+    };
+
+    // A tile's softmax, in slices: 0-7 its maximum, 8 the reference point, 9-24
+    // the probabilities, 25-32 their bf16 pairs and sum.
+    float tmax = -INFINITY, mr = 0.f;
+    uint32_t pk[8];
+    const auto softmax_slice = [&](int i) DSA_INLINE {
+      if (i < 8) {
+        tmax = i ? fmaxf(tmax, fmaxf(s[2 * i], s[2 * i + 1])) : fmaxf(s[0], s[1]);
+      } else if (i == 8) {
+        tmax = half_swap_max(tmax);
+        m = m == -INFINITY ? tmax + kCaAbove : m;
+        over |= tmax > m + kCaRise;
+        mr = m == -INFINITY ? 0.f : m;
+      } else if (i < 25) {
+        s[i - 9] = __builtin_amdgcn_exp2f(s[i - 9] - mr);
+      } else if (i < 33) {
+        const int e = i - 25;
+        pk[e] = pack_bf16x2(s[2 * e], s[2 * e + 1]);
         // the sum of the rounded probabilities, the ones PV multiplies: the
         // weights then add up to one
+        l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pk[e]), __builtin_bit_cast(v2bf, 0x3f803f80u), l, false);
+      }
+    };
+    // Where a row has much of its weight in this tile, what the rounding left of
+    // the probabilities follows as a second product (prefill.hip has the errors
+    // and times of the choices).
+    const auto second = [&]() DSA_INLINE {
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        pk[i >> 1] = pack_bf16x2(s[i] - __uint_as_float(pk[i >> 1] << 16), s[i + 1] - __uint_as_float(pk[i >> 1] & 0xffff0000u));
         l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pk[i >> 1]), __builtin_bit_cast(v2bf, 0x3f803f80u), l,
                                             false);
       }
+    };
+    // O^T += V^T P^T of a tile, the tile after next's dequantisation between
+    const auto values = [&](const uint8_t* kp, const uint8_t* from, uint8_t* to) DSA_INLINE {
       const auto v_frag = [&](int i) DSA_INLINE {
         const int ks = i >> 4, dt = i & 15;
         const uint32_t imm = (dt >> 1) * 128 + ks * (16 * DSA_QK_DIM * 2);
@@ -368,71 +425,95 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
         __builtin_memcpy(&vf.z, &hi, 8);
         return vf;
       };
-      // Where a row has much of its weight in this tile, what the rounding left
-      // of the probabilities follows as a second product (prefill.hip has the
-      // errors and times of the choices).
-      const auto second = [&](uint32_t* w) DSA_INLINE {
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-          w[i >> 1] = pack_bf16x2(s[0][i] - __uint_as_float(pk[i >> 1] << 16),
-                                  s[0][i + 1] - __uint_as_float(pk[i >> 1] & 0xffff0000u));
-          l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, w[i >> 1]), __builtin_bit_cast(v2bf, 0x3f803f80u), l,
-                                              false);
-        }
-      };
-      const auto product = [&](const uint4& v, const uint32_t* p, int i) DSA_INLINE {
-        const uint32_t* pr = p + 4 * (i >> 4);
-        o[i & 15] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(v), as_bf8(make_uint4(pr[0], pr[1], pr[2], pr[3])),
-                                                            o[i & 15], 0, 0, 0);
-      };
-      uint4 vf[kPfDepth];
+      uint4 vf[kCaDepth];
       const bool two = kend < kPfBothKeys ||
                        __ballot(__builtin_amdgcn_exp2f(tmax - mr) > kPfSecond * half_swap_sum(l)) != 0;  // uniform
       // one copy of the products in the code: unrolled, or as two branches, the
-      // accumulators cross the vector file at the join and spill
+      // accumulators cross the vector file at the join and spill (the second
+      // term's run dequantises once more, to the same values)
 #pragma nounroll
       for (int term = 0;; ++term) {
+        conv_begin(from);
 #pragma unroll
-        for (int i = 0; i < kPfDepth; ++i) vf[i] = v_frag(i);
+        for (int i = 0; i < kCaDepth; ++i) vf[i] = v_frag(i);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 32; ++i) {
-          product(vf[i % kPfDepth], pk, i);
-          if (i + kPfDepth < 32) vf[i % kPfDepth] = v_frag(i + kPfDepth);
+          const uint32_t* pr = pk + 4 * (i >> 4);
+          o[i & 15] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+              as_bf8(vf[i % kCaDepth]), as_bf8(make_uint4(pr[0], pr[1], pr[2], pr[3])), o[i & 15], 0, 0, 0);
+          if (i + kCaDepth < 32) vf[i % kCaDepth] = v_frag(i + kCaDepth);
+          conv_slice(i, from, to);
+          __builtin_amdgcn_sched_barrier(0);
         }
         if (term || !two) break;
-        second(pk);
+        second();
       }
     };
 
+    // A tile passes through: bytes (two places), bf16 (three), scores, values.
+    // While tile tl is summed, tl + 1 is scored, tl + 2 dequantised, and tl + 3 on
+    // its way.
     const auto pass = [&](auto max_only) DSA_INLINE {
       int p0 = page_of(t0), p1 = page_of(t0 + 1), p2 = page_of(t0 + 2);
       issue(p0, t0, 0u);
       if (t0 + 1 < t1) issue(p1, t0 + 1, kRaw);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      dequantise(t0, p0, 0u, kb);
-      uint32_t cur = 0;  // of the tile's two places
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        conv_begin(raw + j * kRaw);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) conv_slice(i, raw + j * kRaw, kb + j * kPfTileBytes);
+        conv_end(t0 + j, j ? p1 : p0, kb + j * kPfTileBytes);
+      }
+      __syncthreads();  // two tiles in bf16, their bytes' places free
+      if (t0 + 2 < t1) issue(p2, t0 + 2, 0u);
+      scores(kb, [](int) {});
+      take_scores(t0, rows_of(p0, t0));
+      const uint8_t* here = kb;
+      uint8_t *next = kb + kPfTileBytes, *after = kb + 2 * kPfTileBytes;
+      uint32_t at_raw = 0;  // tile tl + 2's bytes
       for (int tl = t0; tl < t1; ++tl) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();  // tile tl is in bf16, tile tl + 1 has landed; what held tl - 1 and tl's bytes is free
+        __syncthreads();  // tile tl + 1 is in bf16, tl + 2 has landed; what held tl - 1 and tl + 1's bytes is free
         const int p3 = page_of(tl + 3);
-        if (tl + 1 < t1) dequantise(tl + 1, p1, (cur ^ 1u) * kRaw, kb + (cur ^ 1u) * (kPfTileBytes / 2));
-        if (tl + 2 < t1) issue(p2, tl + 2, cur * kRaw);
-        // (always: a branch around the products takes the accumulators through
-        // the vector file)
-        compute(max_only, tl, rows_of(p0, tl), kb + cur * (kPfTileBytes / 2));
-        p0 = p1;
+        if (tl + 3 < t1) issue(p3, tl + 3, at_raw ^ kRawFlip);
+        // (always, also where there is no next tile: a branch around the
+        // products takes the accumulators through the vector file)
+        if constexpr (decltype(max_only)::value) {
+          scores(next, [](int) {});
+#pragma unroll
+          for (int i = 0; i < 16; ++i) tmax = i ? fmaxf(tmax, s[i]) : s[0];
+          m = fmaxf(m, half_swap_max(tmax));
+          conv_begin(raw + at_raw);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) conv_slice(i, raw + at_raw, after);
+        } else {
+          scores(next, softmax_slice);
+          values(here, raw + at_raw, after);
+        }
+        take_scores(tl + 1, rows_of(p1, tl + 1));
+        if (tl + 2 < t1) conv_end(tl + 2, p2, after);
         p1 = p2;
         p2 = p3;
-        cur ^= 1u;
+        at_raw ^= kRawFlip;
+        uint8_t* const old = const_cast<uint8_t*>(here);
+        here = next;
+        next = after;
+        after = old;
       }
       __syncthreads();
     };
 #pragma unroll
-    for (int kk = 0; kk < 36; ++kk) qf[kk] = *reinterpret_cast<const uint4*>(qrow + 16 * kk);
+    for (int kk = 0; kk < 36; ++kk) {
+      const uint4 v = *reinterpret_cast<const uint4*>(qrow + 16 * kk);
+      if (kk < kCaHeld) qf[kk] = v;
+      else ql[wv][kk - kCaHeld][lane] = v;  // (read by this lane alone)
+    }
     // waited for here: later the wait would count the key loads in flight too
 #pragma unroll
-    for (int kk = 0; kk < 36; ++kk) asm volatile("" : : "v"(as_v4i(qf[kk])));
+    for (int kk = 0; kk < kCaHeld; ++kk) asm volatile("" : : "v"(as_v4i(qf[kk])));
     if (t == 0) redo = 0;
     for (int round = 0;; ++round) {
 #pragma unroll
