@@ -40,8 +40,7 @@ constexpr int kCaShare = 256;     // the least share of a workgroup, in keys of 
 // relative) while no probability overflows, and one that underflows is below
 // 2^-90 of the row's largest.  A row of scores that rise by more, 96 in log2,
 // is redone from its true maximum.
-constexpr int kCaHeld = 34;       // of the 36 fragments of a row's query, those in registers
-constexpr int kCaDepth = 5, kCaDepthK = 6;
+constexpr int kCaDepthK = 8, kCaDepthV = 6;  // operand fragments read ahead of their MFMA
 constexpr float kCaAbove = 32.f, kCaRise = 64.f;
 
 // A workgroup's place on the line of work: request, row tile, key tile of it.
@@ -200,7 +199,6 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
   constexpr uint32_t kRawFlip = kRaw;  // (the two places: 0 and kRaw)
   __shared__ __align__(16) uint8_t kb[3 * kPfTileBytes];
   __shared__ __align__(16) uint8_t raw[2 * kRaw];
-  __shared__ uint4 ql[kPfWaves][36 - kCaHeld][kWave];  // fragments of the query that find no registers
   __shared__ int redo;
   const int t = threadIdx.x, lane = t & (kWave - 1), wv = wave_id();
   const int n = lane & 31, h = lane >> 5;
@@ -340,7 +338,7 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
     v16f o[16];
     float m = -INFINITY, l = 0.f;
     bool over = false;
-    uint4 qf[kCaHeld];
+    uint4 qf[36];
     v16f s;       // scores of a tile, then its probabilities
     v16f sn;      // the next tile's scores
 
@@ -355,7 +353,7 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
       for (int i = 0; i < kCaDepthK; ++i) kf[i] = k_frag(kp, i);
 #pragma unroll
       for (int kk = 0; kk < 36; ++kk) {
-        const v4i ka = as_v4i(kf[kk % kCaDepthK]), qb = as_v4i(kk < kCaHeld ? qf[kk] : ql[wv][kk - kCaHeld][lane]);
+        const v4i ka = as_v4i(kf[kk % kCaDepthK]), qb = as_v4i(qf[kk]);
         if (kk == 0)
           asm("v_mfma_f32_32x32x16_bf16 %0, %1, %2, 0" : "=&v"(sn) : "v"(ka), "v"(qb));
         else
@@ -402,17 +400,6 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
         l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pk[e]), __builtin_bit_cast(v2bf, 0x3f803f80u), l, false);
       }
     };
-    // Where a row has much of its weight in this tile, what the rounding left of
-    // the probabilities follows as a second product (prefill.hip has the errors
-    // and times of the choices).
-    const auto second = [&]() DSA_INLINE {
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        pk[i >> 1] = pack_bf16x2(s[i] - __uint_as_float(pk[i >> 1] << 16), s[i + 1] - __uint_as_float(pk[i >> 1] & 0xffff0000u));
-        l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, pk[i >> 1]), __builtin_bit_cast(v2bf, 0x3f803f80u), l,
-                                            false);
-      }
-    };
     // O^T += V^T P^T of a tile, the tile after next's dequantisation between
     const auto values = [&](const uint8_t* kp, const uint8_t* from, uint8_t* to) DSA_INLINE {
       const auto v_frag = [&](int i) DSA_INLINE {
@@ -425,29 +412,19 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
         __builtin_memcpy(&vf.z, &hi, 8);
         return vf;
       };
-      uint4 vf[kCaDepth];
-      const bool two = kend < kPfBothKeys ||
-                       __ballot(__builtin_amdgcn_exp2f(tmax - mr) > kPfSecond * half_swap_sum(l)) != 0;  // uniform
-      // one copy of the products in the code: unrolled, or as two branches, the
-      // accumulators cross the vector file at the join and spill (the second
-      // term's run dequantises once more, to the same values)
-#pragma nounroll
-      for (int term = 0;; ++term) {
-        conv_begin(from);
+      uint4 vf[kCaDepthV];
+      conv_begin(from);
 #pragma unroll
-        for (int i = 0; i < kCaDepth; ++i) vf[i] = v_frag(i);
+      for (int i = 0; i < kCaDepthV; ++i) vf[i] = v_frag(i);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const uint32_t* pr = pk + 4 * (i >> 4);
+        o[i & 15] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            as_bf8(vf[i % kCaDepthV]), as_bf8(make_uint4(pr[0], pr[1], pr[2], pr[3])), o[i & 15], 0, 0, 0);
+        if (i + kCaDepthV < 32) vf[i % kCaDepthV] = v_frag(i + kCaDepthV);
+        conv_slice(i, from, to);
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const uint32_t* pr = pk + 4 * (i >> 4);
-          o[i & 15] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              as_bf8(vf[i % kCaDepth]), as_bf8(make_uint4(pr[0], pr[1], pr[2], pr[3])), o[i & 15], 0, 0, 0);
-          if (i + kCaDepth < 32) vf[i % kCaDepth] = v_frag(i + kCaDepth);
-          conv_slice(i, from, to);
-          __builtin_amdgcn_sched_barrier(0);
-        }
-        if (term || !two) break;
-        second();
       }
     };
 
@@ -506,14 +483,10 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
       __syncthreads();
     };
 #pragma unroll
-    for (int kk = 0; kk < 36; ++kk) {
-      const uint4 v = *reinterpret_cast<const uint4*>(qrow + 16 * kk);
-      if (kk < kCaHeld) qf[kk] = v;
-      else ql[wv][kk - kCaHeld][lane] = v;  // (read by this lane alone)
-    }
+    for (int kk = 0; kk < 36; ++kk) qf[kk] = *reinterpret_cast<const uint4*>(qrow + 16 * kk);
     // waited for here: later the wait would count the key loads in flight too
 #pragma unroll
-    for (int kk = 0; kk < kCaHeld; ++kk) asm volatile("" : : "v"(as_v4i(qf[kk])));
+    for (int kk = 0; kk < 36; ++kk) asm volatile("" : : "v"(as_v4i(qf[kk])));
     if (t == 0) redo = 0;
     for (int round = 0;; ++round) {
 #pragma unroll
