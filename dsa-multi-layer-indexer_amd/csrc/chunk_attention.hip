@@ -40,6 +40,7 @@ constexpr int kCaShare = 256;     // the least share of a workgroup, in keys of 
 // relative) while no probability overflows, and one that underflows is below
 // 2^-90 of the row's largest.  A row of scores that rise by more, 96 in log2,
 // is redone from its true maximum.
+constexpr int kCaTouch = 6;       // tiles ahead that are brought into the L2
 constexpr int kCaDepthK = 8, kCaDepthV = 6;  // operand fragments read ahead of their MFMA
 constexpr float kCaAbove = 32.f, kCaRise = 64.f;
 
@@ -57,7 +58,7 @@ __device__ __forceinline__ ChunkReq chunk_req(const ChunkAttnArgs& A, int b) {
   ChunkReq r;
   r.first = min(max(A.q_start[b], 0), A.n);
   r.T = min(max(A.q_start[b + 1], r.first), A.n) - r.first;
-  r.tiles = (int)(((long)r.T * A.H + kPfRows - 1) / kPfRows);
+  r.tiles = (int)(((uint32_t)r.T * (uint32_t)A.H + kPfRows - 1u) / kPfRows);  // (T * H below 2^31)
   r.P = max(A.seq_lens[b], 0) - r.T;
   return r;
 }
@@ -75,8 +76,8 @@ __device__ __forceinline__ long chunk_cost(const ChunkAttnArgs& A, const ChunkRe
 }
 // Keys that any row of a tile sees.
 __device__ __forceinline__ int chunk_keys(const ChunkAttnArgs& A, const ChunkReq& r, int tile) {
-  const long R = (long)r.T * A.H;
-  const int s_hi = (int)((min((tile + 1L) * kPfRows, R) - 1) / A.H);
+  const uint32_t R = (uint32_t)r.T * (uint32_t)A.H;  // (below 2^31)
+  const int s_hi = (int)((min((tile + 1u) * (uint32_t)kPfRows, R) - 1u) / (uint32_t)A.H);
   return max(0, min(r.P + s_hi + 1, A.pt_stride * DSA_PAGE_TOKENS));
 }
 
@@ -124,7 +125,10 @@ __device__ __forceinline__ ChunkPos chunk_find(const ChunkAttnArgs& A, long x) {
     const int tile = uniform((int)lo);
     const long c0 = chunk_cost(A, r, tile), c1 = chunk_cost(A, r, tile + 1);
     const int kts = (chunk_keys(A, r, tile) + kPfKeys - 1) / kPfKeys;
-    return {uniform(b), tile, uniform((int)((x - c0) * kts / (c1 - c0)))};
+    // (in fp64: its divisions are short; any rounding of both ends of a share is
+    // the same for the share that ends there and the one that begins)
+    const int kt = (int)((double)(x - c0) * kts / (double)(c1 - c0));
+    return {uniform(b), tile, uniform(max(0, min(kt, kts - 1)))};
   }
   return {A.B, 0, 0};
 }
@@ -199,6 +203,7 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
   constexpr uint32_t kRawFlip = kRaw;  // (the two places: 0 and kRaw)
   __shared__ __align__(16) uint8_t kb[3 * kPfTileBytes];
   __shared__ __align__(16) uint8_t raw[2 * kRaw];
+  __shared__ uint32_t touched[kPfThreads];  // what brings a tile into the L2 leaves here
   __shared__ int redo;
   const int t = threadIdx.x, lane = t & (kWave - 1), wv = wave_id();
   const int n = lane & 31, h = lane >> 5;
@@ -208,11 +213,12 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
   const int G = (int)gridDim.x;
   const int g = (int)(blockIdx.x % 8u) * (G / 8) + (int)(blockIdx.x / 8u);  // (G is a multiple of 8)
   const long total = chunk_total(A);
-  const int shares = (int)min((long)G, max(1L, total / ((long)A.H * kCaShare)));
+  const int shares = (int)min((double)G, max(1.0, (double)total / ((double)A.H * kCaShare)));
   if (t == 0) A.part[g] = int4{-1, 0, 0, 0};
   if (g >= shares || total == 0) return;
-  ChunkPos at = chunk_find(A, total * g / shares);
-  const ChunkPos end = g + 1 == shares ? ChunkPos{A.B, 0, 0} : chunk_find(A, total * (g + 1) / shares);
+  const double share = (double)total / shares;
+  ChunkPos at = chunk_find(A, (long)(share * g));
+  const ChunkPos end = g + 1 == shares ? ChunkPos{A.B, 0, 0} : chunk_find(A, (long)(share * (g + 1)));
 
   // K operand: row n (+32), chunk 2kk + h
   uint32_t koff[4];
@@ -230,7 +236,7 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
       const int j = 4 * par + 2 * g1 + ((a16 >> 1) & 1);
       voff[par][e8] = (uint32_t)(r * (DSA_QK_DIM * 2) + (j ^ pf_swz(r)) * 16 + 8 * (a16 & 1));
     }
-  const uint32_t raw0 = (uint32_t)(uintptr_t)(lvoid_ptr)raw;
+  const uint32_t raw0 = (uint32_t)(uintptr_t)(lvoid_ptr)raw, touch0 = (uint32_t)(uintptr_t)(lvoid_ptr)touched;
   const long pool_bytes = A.kv_rows * ROW;
 
   while (at.b < end.b || (at.b == end.b && (at.tile < end.tile || (at.tile == end.tile && at.kt < end.kt)))) {
@@ -283,6 +289,19 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
                        : "memory", "m0");
         }
       }
+    };
+    // Brings a tile's lines into the L2, one a thread: one load a wave, always,
+    // the newest that the loop's wait may leave in flight.  (A tile a CU in
+    // flight is 5 MB; memory's 3 us and 5 TB/s take three.)
+    const auto touch = [&](int page, int tl) DSA_INLINE {
+      const long base = rows_of(page, tl) ? ((long)page * DSA_PAGE_TOKENS + (tl & 1) * kPfKeys) * ROW : 0;
+      const uint32_t last = (uint32_t)min((long)kRaw, pool_bytes - base) - 16u;
+      const uint32_t off = min(128u * (uint32_t)t, last);
+      const uint32_t dst = __builtin_amdgcn_readfirstlane(touch0 + (uint32_t)wv * (kWave * 4u));
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+                   :
+                   : "s"(dst), "v"(off), "s"(A.pool + base)
+                   : "memory", "m0");
     };
     // Wave w dequantises rows w, w + 4, ... of the next tile, 8 values a lane,
     // between its products of this one: `from` its bytes, `to` its bf16 place.
@@ -451,10 +470,11 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
       const uint8_t* here = kb;
       uint8_t *next = kb + kPfTileBytes, *after = kb + 2 * kPfTileBytes;
       uint32_t at_raw = 0;  // tile tl + 2's bytes
+      touch(p2, t0 + 2);
       for (int tl = t0; tl < t1; ++tl) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(1)" ::: "memory");  // (all but the newest, touch()'s)
         __syncthreads();  // tile tl + 1 is in bf16, tl + 2 has landed; what held tl - 1 and tl + 1's bytes is free
-        const int p3 = page_of(tl + 3);
+        const int p3 = page_of(tl + 3), far = min(tl + kCaTouch, t1 - 1), pf = page_of(far);
         if (tl + 3 < t1) issue(p3, tl + 3, at_raw ^ kRawFlip);
         // (always, also where there is no next tile: a branch around the
         // products takes the accumulators through the vector file)
@@ -470,6 +490,7 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
           scores(next, softmax_slice);
           values(here, raw + at_raw, after);
         }
+        touch(pf, far);
         take_scores(tl + 1, rows_of(p1, tl + 1));
         if (tl + 2 < t1) conv_end(tl + 2, p2, after);
         p1 = p2;
@@ -549,15 +570,18 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
 }
 
 // Joins a row's parts: out = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m), m =
-// max m_s.  Workgroup (i, r): row r of the i-th row tile that more than one
-// share has part of; wave w takes the parts w, w + 4, ... (8 dims a lane), then
-// the four sums meet in LDS, always in the same order.
-__global__ __launch_bounds__(kPfThreads) void chunk_merge_kernel(const ChunkAttnArgs A, int G) {
+// max m_s.  A workgroup: `per` rows of the i-th row tile that more than one
+// share has part of.  With few parts a wave takes a row; with many the four
+// waves take the parts of one row in turn (w, w + 4, ...; 8 dims a lane) and
+// meet in LDS, always in the same order.
+constexpr int kCaFewParts = 8;
+__global__ __launch_bounds__(kPfThreads) void chunk_merge_kernel(const ChunkAttnArgs A, int G, int per) {
   __shared__ float sl[kPfWaves];
   __shared__ v4f so[kPfWaves][2 * kWave];
   const int lane = threadIdx.x & (kWave - 1), wv = wave_id();
-  const int r = (int)(blockIdx.x % (unsigned)A.part_rows);
-  int left = (int)(blockIdx.x / (unsigned)A.part_rows), first = -1;
+  const int blocks = (A.part_rows + per - 1) / per;
+  const int r_lo = (int)(blockIdx.x % (unsigned)blocks) * per;
+  int left = (int)(blockIdx.x / (unsigned)blocks), first = -1;
   for (int g0 = 0; g0 < G && first < 0; g0 += kWave) {
     uint64_t has = __ballot(g0 + lane < G && A.part[min(g0 + lane, G - 1)].x >= 0);
     const int here = __builtin_popcountll(has);
@@ -571,8 +595,7 @@ __global__ __launch_bounds__(kPfThreads) void chunk_merge_kernel(const ChunkAttn
   if (first < 0) return;
   const int4 d = A.part[first];
   const ChunkReq rq = chunk_req(A, d.x);
-  const long row = (long)d.y * kPfRows + r;
-  if (row >= (long)rq.T * A.H) return;
+  const long row0 = (long)d.y * kPfRows, R = (long)rq.T * A.H;
   int parts = 1;  // the first share's, then those up to the one where the tile ends
   for (int g0 = first + 1; g0 < G; g0 += kWave) {
     const uint64_t ends = __ballot(g0 + lane < G && A.part[min(g0 + lane, G - 1)].z == 2);
@@ -582,49 +605,63 @@ __global__ __launch_bounds__(kPfThreads) void chunk_merge_kernel(const ChunkAttn
     }
     parts += kWave;
   }
-  const auto slot = [&](int s) { return (long)(s ? 2 * (first + s) : 2 * first + 1) * A.part_rows + r; };
-  float m = -INFINITY;
-  for (int s = lane; s < parts; s += kWave) m = fmaxf(m, A.part_ml[2 * slot(s)]);
-  m = wave_max(m);
-  const float mr = m == -INFINITY ? 0.f : m;
-  float L = 0.f;
-  v4f x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
-  constexpr int kU = 4;
-  for (int s0 = wv; s0 < parts; s0 += kU * kPfWaves) {
-    v4f a[kU], c[kU];
-    float ms[kU], ls[kU];
+  const bool few = parts <= kCaFewParts;
+  const int step = few ? 1 : kPfWaves, mine = few ? 0 : wv;
+  for (int r = r_lo + (few ? wv : 0); r < min(r_lo + per, A.part_rows) && row0 + r < R; r += few ? kPfWaves : 1) {
+    const auto slot = [&](int s) { return (long)(s ? 2 * (first + s) : 2 * first + 1) * A.part_rows + r; };
+    float m = -INFINITY;
+    for (int s = lane; s < parts; s += kWave) m = fmaxf(m, A.part_ml[2 * slot(s)]);
+    m = wave_max(m);
+    const float mr = m == -INFINITY ? 0.f : m;
+    float L = 0.f;
+    v4f x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
+    constexpr int kU = 4;
+    for (int s0 = mine; s0 < parts; s0 += kU * step) {
+      v4f a[kU], c[kU];
+      float ms[kU], ls[kU];
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      const int s = s0 + u * kPfWaves;
-      const long pr = slot(s < parts ? s : wv);  // past the last: read again, weight 0
-      const v4f* po = reinterpret_cast<const v4f*>(A.part_o + pr * DSA_LATENT_DIM) + 2 * lane;
-      a[u] = po[0];
-      c[u] = po[1];
-      ms[u] = A.part_ml[2 * pr];
-      ls[u] = A.part_ml[2 * pr + 1];
-    }
+      for (int u = 0; u < kU; ++u) {
+        const int s = s0 + u * step;
+        const long pr = slot(s < parts ? s : mine);  // past the last: read again, weight 0
+        const v4f* po = reinterpret_cast<const v4f*>(A.part_o + pr * DSA_LATENT_DIM) + 2 * lane;
+        a[u] = po[0];
+        c[u] = po[1];
+        ms[u] = A.part_ml[2 * pr];
+        ls[u] = A.part_ml[2 * pr + 1];
+      }
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      if (s0 + u * kPfWaves >= parts) break;  // uniform
-      const float w = exp2f(ms[u] - mr);
-      L += ls[u] * w;
-      x0 += a[u] * w;
-      x1 += c[u] * w;
+      for (int u = 0; u < kU; ++u) {
+        if (s0 + u * step >= parts) break;  // uniform
+        const float w = exp2f(ms[u] - mr);
+        L += ls[u] * w;
+        x0 += a[u] * w;
+        x1 += c[u] * w;
+      }
     }
-  }
-  so[wv][2 * lane] = x0;
-  so[wv][2 * lane + 1] = x1;
-  if (lane == 0) sl[wv] = L;
-  __syncthreads();
-  const float tot = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-  const float inv = tot > 0.f ? 1.f / tot : (tot == tot ? 0.f : tot);
-  if (threadIdx.x < 2 * kWave) {
-    const int i = threadIdx.x;
-    const v4f o = (so[0][i] + so[1][i]) + (so[2][i] + so[3][i]);
-    v2u_t w;
-    w[0] = pack_bf16x2(o[0] * inv, o[1] * inv);
-    w[1] = pack_bf16x2(o[2] * inv, o[3] * inv);
-    *reinterpret_cast<v2u_t*>(A.out + ((long)rq.first * A.H + row) * DSA_LATENT_DIM + 4 * i) = w;
+    uint16_t* const out = A.out + ((long)rq.first * A.H + row0 + r) * DSA_LATENT_DIM;
+    if (few) {
+      const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
+      x0 *= inv;
+      x1 *= inv;
+      reinterpret_cast<uint4*>(out)[lane] =
+          make_uint4(pack_bf16x2(x0[0], x0[1]), pack_bf16x2(x0[2], x0[3]), pack_bf16x2(x1[0], x1[1]), pack_bf16x2(x1[2], x1[3]));
+      continue;
+    }
+    so[wv][2 * lane] = x0;
+    so[wv][2 * lane + 1] = x1;
+    if (lane == 0) sl[wv] = L;
+    __syncthreads();
+    const float tot = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    const float inv = tot > 0.f ? 1.f / tot : (tot == tot ? 0.f : tot);
+    if (threadIdx.x < 2 * kWave) {
+      const int i = threadIdx.x;
+      const v4f o = (so[0][i] + so[1][i]) + (so[2][i] + so[3][i]);
+      v2u_t w;
+      w[0] = pack_bf16x2(o[0] * inv, o[1] * inv);
+      w[1] = pack_bf16x2(o[2] * inv, o[3] * inv);
+      *reinterpret_cast<v2u_t*>(out + 4 * i) = w;
+    }
+    __syncthreads();
   }
 }
 
@@ -653,7 +690,10 @@ hipError_t launch_chunk_attention(ChunkAttnArgs A, int row_bytes, void* workspac
   // row tiles there may be, and those that two shares can have part of
   const long tiles = (long)A.n * A.H / kPfRows + std::min(A.B, A.n);
   const long split = std::min<long>(tiles, G - 1);
-  hipLaunchKernelGGL(chunk_merge_kernel, dim3((unsigned)(split * A.part_rows)), block, 0, s, A, G);
+  // rows a workgroup: about 8 workgroups a CU
+  const int per = (int)std::min(16L, std::max(1L, split * A.part_rows / (8L * G)));
+  const long blocks = split * ((A.part_rows + per - 1) / per);
+  hipLaunchKernelGGL(chunk_merge_kernel, dim3((unsigned)blocks), block, 0, s, A, G, per);
   return hipGetLastError();
 }
 
