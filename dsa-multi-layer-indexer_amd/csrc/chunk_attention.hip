@@ -33,14 +33,13 @@ namespace dsa {
 #define DSA_INLINE __attribute__((always_inline))  // (a lambda left out of line keeps its captures in memory)
 
 constexpr int kCaTileCost = 64;   // keys' worth of a row tile's start and end
-constexpr int kCaShare = 256;     // the least share of a workgroup, in keys of a row tile
+constexpr int kCaShare = 128;     // the least share of a workgroup, in keys of a row tile
 // A row's reference point lies this far above its first tile's maximum (in
 // log2), and a score may rise this far above the reference: any point gives the
 // same sums (bf16 and fp32 have 8 bits of exponent, and a probability's error is
 // relative) while no probability overflows, and one that underflows is below
 // 2^-90 of the row's largest.  A row of scores that rise by more, 96 in log2,
 // is redone from its true maximum.
-constexpr int kCaTouch = 6;       // tiles ahead that are brought into the L2
 constexpr int kCaDepthK = 8, kCaDepthV = 6;  // operand fragments read ahead of their MFMA
 constexpr float kCaAbove = 32.f, kCaRise = 64.f;
 
@@ -203,7 +202,6 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
   constexpr uint32_t kRawFlip = kRaw;  // (the two places: 0 and kRaw)
   __shared__ __align__(16) uint8_t kb[3 * kPfTileBytes];
   __shared__ __align__(16) uint8_t raw[2 * kRaw];
-  __shared__ uint32_t touched[kPfThreads];  // what brings a tile into the L2 leaves here
   __shared__ int redo;
   const int t = threadIdx.x, lane = t & (kWave - 1), wv = wave_id();
   const int n = lane & 31, h = lane >> 5;
@@ -236,7 +234,7 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
       const int j = 4 * par + 2 * g1 + ((a16 >> 1) & 1);
       voff[par][e8] = (uint32_t)(r * (DSA_QK_DIM * 2) + (j ^ pf_swz(r)) * 16 + 8 * (a16 & 1));
     }
-  const uint32_t raw0 = (uint32_t)(uintptr_t)(lvoid_ptr)raw, touch0 = (uint32_t)(uintptr_t)(lvoid_ptr)touched;
+  const uint32_t raw0 = (uint32_t)(uintptr_t)(lvoid_ptr)raw;
   const long pool_bytes = A.kv_rows * ROW;
 
   while (at.b < end.b || (at.b == end.b && (at.tile < end.tile || (at.tile == end.tile && at.kt < end.kt)))) {
@@ -289,19 +287,6 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
                        : "memory", "m0");
         }
       }
-    };
-    // Brings a tile's lines into the L2, one a thread: one load a wave, always,
-    // the newest that the loop's wait may leave in flight.  (A tile a CU in
-    // flight is 5 MB; memory's 3 us and 5 TB/s take three.)
-    const auto touch = [&](int page, int tl) DSA_INLINE {
-      const long base = rows_of(page, tl) ? ((long)page * DSA_PAGE_TOKENS + (tl & 1) * kPfKeys) * ROW : 0;
-      const uint32_t last = (uint32_t)min((long)kRaw, pool_bytes - base) - 16u;
-      const uint32_t off = min(128u * (uint32_t)t, last);
-      const uint32_t dst = __builtin_amdgcn_readfirstlane(touch0 + (uint32_t)wv * (kWave * 4u));
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
-                   :
-                   : "s"(dst), "v"(off), "s"(A.pool + base)
-                   : "memory", "m0");
     };
     // Wave w dequantises rows w, w + 4, ... of the next tile, 8 values a lane,
     // between its products of this one: `from` its bytes, `to` its bf16 place.
@@ -470,11 +455,10 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
       const uint8_t* here = kb;
       uint8_t *next = kb + kPfTileBytes, *after = kb + 2 * kPfTileBytes;
       uint32_t at_raw = 0;  // tile tl + 2's bytes
-      touch(p2, t0 + 2);
       for (int tl = t0; tl < t1; ++tl) {
-        asm volatile("s_waitcnt vmcnt(1)" ::: "memory");  // (all but the newest, touch()'s)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();  // tile tl + 1 is in bf16, tl + 2 has landed; what held tl - 1 and tl + 1's bytes is free
-        const int p3 = page_of(tl + 3), far = min(tl + kCaTouch, t1 - 1), pf = page_of(far);
+        const int p3 = page_of(tl + 3);
         if (tl + 3 < t1) issue(p3, tl + 3, at_raw ^ kRawFlip);
         // (always, also where there is no next tile: a branch around the
         // products takes the accumulators through the vector file)
@@ -490,7 +474,6 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
           scores(next, softmax_slice);
           values(here, raw + at_raw, after);
         }
-        touch(pf, far);
         take_scores(tl + 1, rows_of(p1, tl + 1));
         if (tl + 2 < t1) conv_end(tl + 2, p2, after);
         p1 = p2;

@@ -93,17 +93,16 @@ __device__ __forceinline__ int2 expert_rows(const MatmulArgs& A, int e) {
 
 // ---- few rows ----
 
-constexpr int kRwWaves = 8;
-constexpr int kRwThreads = kRwWaves * kWave;
-
 // One workgroup: 16 MT outputs of one expert, 16 TT of its rows at a time.
-// Wave w takes the blocks w, w + 8, ... of k: it reads its operands from memory
-// straight in the product's layout (lane (r, c) holds bytes [32 c, + 32) of row
-// r: whole 128-byte lines), the next block's while this one multiplies; the
-// waves' sums meet in LDS, in the order of the waves.
-template <int MT, int TT, bool EXACT>
-__global__ __launch_bounds__(kRwThreads, TT * MT > 4 || EXACT ? 2 : 4) void rows_kernel(const MatmulArgs A) {
-  __shared__ v4f part[kRwWaves][MT * TT][kWave];
+// Wave w of W takes the blocks w, w + W, ... of k: it reads its operands from
+// memory straight in the product's layout (lane (r, c) holds bytes [32 c, + 32)
+// of row r: whole 128-byte lines), the weights kRwAhead blocks ahead, the rows,
+// which the L2 holds, two; the waves' sums meet in LDS, in the order of the
+// waves.
+constexpr int kRwAhead = 4;
+template <int MT, int TT, int W, bool EXACT>
+__global__ __launch_bounds__(W* kWave, W >= 16 ? 4 : (MT * TT >= 8 ? 2 : 3)) void rows_kernel(const MatmulArgs A) {
+  __shared__ v4f part[W][MT * TT][kWave];
   const int lane = threadIdx.x & (kWave - 1), wv = wave_id();
   const int r = lane & 15, c = lane >> 4;
   const int ot = (int)(blockIdx.x % (unsigned)A.otiles), e = (int)(blockIdx.x / (unsigned)A.otiles);
@@ -114,10 +113,16 @@ __global__ __launch_bounds__(kRwThreads, TT * MT > 4 || EXACT ? 2 : 4) void rows
   const uint8_t* wrow[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) wrow[m] = wbase + (long)min(o0 + 16 * m + r, A.N - 1) * A.K + 32 * c;
-
-  struct Block {
-    v8i w[MT], a[TT];
-    float s[TT];
+  // the wave's i-th block; behind its last, the last again (read, not used)
+  const int count = A.kblocks > wv ? (A.kblocks - 1 - wv) / W + 1 : 0;
+  const auto block_of = [&](int i) { return wv + W * max(min(i, count - 1), 0); };
+  // 32 bytes of a row, zeros behind its end (of the last, short block)
+  const auto load32 = [&](const uint8_t* row, int b) {
+    const int left = A.K - b * 128 - 32 * c;
+    const uint4* p = reinterpret_cast<const uint4*>(row + (long)b * 128);
+    const uint4 z = make_uint4(0, 0, 0, 0);
+    if (left >= 32) return two16(p[0], p[1]);
+    return two16(left > 0 ? p[0] : z, z);
   };
   for (int t0 = range.x; t0 < range.y; t0 += 16 * TT) {
     const uint8_t* arow[TT];
@@ -128,20 +133,20 @@ __global__ __launch_bounds__(kRwThreads, TT * MT > 4 || EXACT ? 2 : 4) void rows
       arow[t] = A.a + row * A.K + 32 * c;
       srow[t] = A.a_scale + row * A.a_groups;
     }
-    const auto load = [&](int b, Block& x) {
-      const int left = A.K - b * 128 - 32 * c;  // bytes of the row from this lane's on
-      const uint4 z = make_uint4(0, 0, 0, 0);
+    v8i wq[kRwAhead][MT], aq[2][TT];
+    float sq[2][TT];
+    const auto load_w = [&](int i, int u) {
+      const int b = block_of(i);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const uint4* p = reinterpret_cast<const uint4*>(wrow[m] + (long)b * 128);
-        x.w[m] = two16(left > 0 ? p[0] : z, left > 16 ? p[1] : z);
-      }
-      const float ws = sw[b];
+      for (int m = 0; m < MT; ++m) wq[u][m] = load32(wrow[m], b);
+    };
+    const auto load_a = [&](int i, int u) {
+      const int b = block_of(i);
+      const float ws = sw[min(b, A.kblocks - 1)];
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
-        const uint4* p = reinterpret_cast<const uint4*>(arow[t] + (long)b * 128);
-        x.a[t] = two16(left > 0 ? p[0] : z, left > 16 ? p[1] : z);
-        x.s[t] = srow[t][A.a_groups == 1 ? 0 : b] * ws;
+        aq[u][t] = load32(arow[t], b);
+        sq[u][t] = srow[t][A.a_groups == 1 ? 0 : min(b, A.kblocks - 1)] * ws;
       }
     };
     v4f acc[MT][TT];
@@ -149,35 +154,48 @@ __global__ __launch_bounds__(kRwThreads, TT * MT > 4 || EXACT ? 2 : 4) void rows
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int t = 0; t < TT; ++t) acc[m][t] = v4f{0.f, 0.f, 0.f, 0.f};
-    Block cur, nxt;
-    if (wv < A.kblocks) load(wv, cur);
-    for (int b = wv; b < A.kblocks; b += kRwWaves) {
-      if (b + kRwWaves < A.kblocks) load(b + kRwWaves, nxt);
-      Operand<EXACT> wf[MT], af;
+    if (count > 0) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m) wf[m].set(cur.w[m]);
+      for (int u = 0; u < kRwAhead; ++u) load_w(u, u);
+      load_a(0, 0);
+      load_a(1, 1);
+      for (int i0 = 0; i0 < count; i0 += kRwAhead) {
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        af.set(cur.a[t]);
+        for (int u = 0; u < kRwAhead; ++u) {
+          Operand<EXACT> wf[MT], af[TT];
+          float s[TT];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const v4f d = block_product(wf[m], af);
+          for (int m = 0; m < MT; ++m) wf[m].set(wq[u][m]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[m][t][i] = __builtin_fmaf(cur.s[t], d[i], acc[m][t][i]);
+          for (int t = 0; t < TT; ++t) {
+            af[t].set(aq[u & 1][t]);
+            s[t] = i0 + u < count ? sq[u & 1][t] : 0.f;
+          }
+          if (i0 + u < count) {  // uniform
+#pragma unroll
+            for (int t = 0; t < TT; ++t)
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                const v4f d = block_product(wf[m], af[t]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc[m][t][q] = __builtin_fmaf(s[t], d[q], acc[m][t][q]);
+              }
+          }
+          load_w(i0 + u + kRwAhead, u);
+          load_a(i0 + u + 2, u & 1);
         }
       }
-      cur = nxt;
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int t = 0; t < TT; ++t) part[wv][m * TT + t][lane] = acc[m][t];
     __syncthreads();
-    // tile i of 64 lanes' sums to wave i (mod 8)
-    for (int i = wv; i < MT * TT; i += kRwWaves) {
+    // tile i of 64 lanes' sums to wave i (mod W)
+    for (int i = wv; i < MT * TT; i += W) {
       v4f s = part[0][i][lane];
 #pragma unroll
-      for (int w = 1; w < kRwWaves; ++w) s += part[w][i][lane];
+      for (int w = 1; w < W; ++w) s += part[w][i][lane];
       const int row = t0 + 16 * (i % TT) + r, o = o0 + 16 * (i / TT) + 4 * c;
       const float v[4] = {s[0], s[1], s[2], s[3]};
       if (row < range.y && o < A.N) store_out4(A, row, o, v);
@@ -217,8 +235,13 @@ __device__ __forceinline__ int2 find_rows(const MatmulArgs& A, int tile, int& ex
 // One workgroup: BO outputs x BT rows, WO x WT waves of (16 MO) x (16 TT).
 // A block of 128 k at a time goes from memory straight to LDS, two places, the
 // next block's on its way while this one multiplies.  A row's 8 16-byte chunks
-// lie with their low bits xored with row / 2, so that the 16 rows of an operand
-// read fall in distinct banks.
+// lie with their number xored with the row's, so that 8 rows of an operand read
+// (what one clock takes) fall in distinct banks.  The rows' scales come 8 blocks
+// at a time (loaded a block at a time into registers they cost a quarter of the
+// time: as many lines as the operands, and a wait).
+constexpr int kMmScales = 8;  // blocks' scales brought at a time
+typedef const __attribute__((address_space(4))) float* const_float_ptr;
+
 template <int WO, int WT, int MO, int TT, bool EXACT>
 __global__ __launch_bounds__(WO* WT* kWave, 2) void tile_kernel(const MatmulArgs A) {
   constexpr int BO = WO * MO * 16, BT = WT * TT * 16, kThreads = WO * WT * kWave;
@@ -227,6 +250,7 @@ __global__ __launch_bounds__(WO* WT* kWave, 2) void tile_kernel(const MatmulArgs
   static_assert(kLoads * kThreads == (BO + BT) * 8, "whole loads");
   static_assert((BO * 8) % kThreads == 0, "a load is of weights or of rows");
   __shared__ __align__(16) uint8_t lds[2 * kStage];
+  __shared__ float ss[2][BT][kMmScales];
   const int t = threadIdx.x, lane = t & (kWave - 1), wv = wave_id();
   const int r = lane & 15, c = lane >> 4;
   const int wo = wv % WO, wt = wv / WO;
@@ -248,26 +272,20 @@ __global__ __launch_bounds__(WO* WT* kWave, 2) void tile_kernel(const MatmulArgs
 
   const uint8_t* wbase = A.w + (long)e * A.N * A.K;
   const uint8_t* abase = A.a + (long)rows.x * A.K;
-  uint32_t off[kLoads];  // of this thread's chunks from wbase + o0 * K or abase
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int p = i * kThreads + t, row = p >> 3, j = (p & 7) ^ ((row >> 1) & 7);
-    const int src = row < BO ? min(row, A.N - 1 - o0) : min(row - BO, rows.y - 1 - rows.x);
-    off[i] = (uint32_t)src * (uint32_t)A.K + 16u * j;
-  }
   const uint32_t lds0 = (uint32_t)(uintptr_t)(mm_lds_ptr)lds;
   const auto issue = [&](int b, uint32_t buf) {
     // in the last, short block a chunk behind the row's end reads the row's
-    // last instead; the product masks it
+    // last instead; zeros take its place before the product
     const int jmax = min(8, (A.K - b * 128) / 16) - 1;
+    const int row0 = t >> 3, j = min((t & 7) ^ (row0 & 7), jmax);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const uint8_t* base = (i * kThreads < BO * 8 ? wbase + (long)o0 * A.K : abase) + (long)b * 128;
-      uint32_t o = off[i];
-      if (jmax < 7) {  // uniform
-        const int p = i * kThreads + t, j = (p & 7) ^ ((p >> 4) & 7);
-        o -= 16u * (uint32_t)max(0, j - jmax);
-      }
+      constexpr int kRows = kThreads / 8;  // rows a load; (a multiple of 8: the swizzle is the thread's)
+      static_assert(kRows % 8 == 0, "the swizzle");
+      const bool weights = i * kRows < BO;
+      const int last = weights ? A.N - 1 - o0 : rows.y - 1 - rows.x, first = weights ? i * kRows : i * kRows - BO;
+      const uint8_t* base = (weights ? wbase + (long)o0 * A.K : abase) + (long)b * 128;
+      const uint32_t o = (uint32_t)min(first + row0, last) * (uint32_t)A.K + 16u * j;
       const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + buf + (uint32_t)(i * kThreads + wv * kWave) * 16u);
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                    :
@@ -275,15 +293,28 @@ __global__ __launch_bounds__(WO* WT* kWave, 2) void tile_kernel(const MatmulArgs
                    : "memory", "m0");
     }
   };
-  // scales: this lane's token of each row tile, and the wave's outputs' block
-  const float* srow[TT];
-#pragma unroll
-  for (int i = 0; i < TT; ++i)
-    srow[i] = A.a_scale + (long)min(rows.x + (wt * TT + i) * 16 + r, rows.y - 1) * A.a_groups;
-  const float* sw = A.w_scale + ((long)e * A.nblocks + min(o0 + wo * MO * 16, A.N - 1) / 128) * A.kblocks;
+  // the scales of the wave's outputs' block, by scalar loads
+  const auto* sw = (const_float_ptr)(A.w_scale + ((long)e * A.nblocks + min(o0 + wo * MO * 16, A.N - 1) / 128) * A.kblocks);
   static_assert(MO * 16 <= 128 && 128 % (MO * 16) == 0, "a wave's outputs share a block");
+  // those of the rows, kMmScales blocks from b on
+  const float* sbase = A.a_scale + (long)rows.x * A.a_groups;
+  const uint32_t ss0 = (uint32_t)(uintptr_t)(mm_lds_ptr)ss;
+  const auto issue_scales = [&](int b, int place) {
+    constexpr int kEach = BT * kMmScales / kThreads;
+    static_assert(kEach * kThreads == BT * kMmScales, "whole loads");
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int p = i * kThreads + t;
+      const uint32_t row = (uint32_t)min(p / kMmScales, rows.y - 1 - rows.x), k = (uint32_t)min(b + p % kMmScales, A.a_groups - 1);
+      const uint32_t dst = __builtin_amdgcn_readfirstlane(ss0 + (uint32_t)(place * (BT * kMmScales) + i * kThreads + wv * kWave) * 4u);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
+                   :
+                   : "s"(dst), "v"(4u * (row * (uint32_t)A.a_groups + k)), "s"(sbase)
+                   : "memory", "m0");
+    }
+  };
 
-  const uint32_t swz0 = (uint32_t)(((2 * c) ^ ((r >> 1) & 7)) * 16), swz1 = (uint32_t)(((2 * c + 1) ^ ((r >> 1) & 7)) * 16);
+  const uint32_t swz0 = (uint32_t)(((2 * c) ^ (r & 7)) * 16), swz1 = (uint32_t)(((2 * c + 1) ^ (r & 7)) * 16);
   const uint32_t wofs = (uint32_t)(wo * MO * 16 + r) * 128u, aofs = (uint32_t)(BO + wt * TT * 16 + r) * 128u;
   v4f acc[MO][TT];
 #pragma unroll
@@ -292,58 +323,62 @@ __global__ __launch_bounds__(WO* WT* kWave, 2) void tile_kernel(const MatmulArgs
     for (int i = 0; i < TT; ++i) acc[m][i] = v4f{0.f, 0.f, 0.f, 0.f};
   const bool idle = rows.x + wt * TT * 16 >= rows.y || o0 + wo * MO * 16 >= A.N;  // none of the wave's tiles is needed
 
-  const auto compute = [&](const uint8_t* buf, const float* s, auto tail, int left) {
+  const auto compute = [&](const uint8_t* buf, const float* s) {
     const auto frag = [&](uint32_t at) {
-      uint4 x = *reinterpret_cast<const uint4*>(buf + at + swz0), y = *reinterpret_cast<const uint4*>(buf + at + swz1);
-      if constexpr (decltype(tail)::value) {
-        const uint4 z = make_uint4(0, 0, 0, 0);
-        x = left > 0 ? x : z;
-        y = left > 16 ? y : z;
-      }
       Operand<EXACT> f;
-      f.set(two16(x, y));
+      f.set(two16(*reinterpret_cast<const uint4*>(buf + at + swz0), *reinterpret_cast<const uint4*>(buf + at + swz1)));
       return f;
     };
-    Operand<EXACT> a[TT];
+    // A tile's results enter the sums one row of tiles later, beside its products.
+    Operand<EXACT> a[TT], w = frag(wofs);
 #pragma unroll
     for (int i = 0; i < TT; ++i) a[i] = frag(aofs + (uint32_t)i * (16 * 128));
+    v4f d[TT];
 #pragma unroll
-    for (int m = 0; m < MO; ++m) {
-      const Operand<EXACT> w = frag(wofs + (uint32_t)m * (16 * 128));
+    for (int m = 0; m <= MO; ++m) {
+      Operand<EXACT> wn = w;
+      if (m + 1 < MO) wn = frag(wofs + (uint32_t)(m + 1) * (16 * 128));
 #pragma unroll
       for (int i = 0; i < TT; ++i) {
-        const v4f d = block_product(w, a[i]);
+        v4f x = d[i];
+        if (m < MO) x = block_product(w, a[i]);
+        if (m > 0)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) acc[m][i][q] = __builtin_fmaf(s[i], d[q], acc[m][i][q]);
+          for (int q = 0; q < 4; ++q) acc[m - 1][i][q] = __builtin_fmaf(s[i], d[i][q], acc[m - 1][i][q]);
+        d[i] = x;
       }
+      w = wn;
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
-  float s[TT], ns[TT];
-  const auto scales = [&](int b, float* x) {
-    const float ws = sw[b];
-#pragma unroll
-    for (int i = 0; i < TT; ++i) x[i] = srow[i][A.a_groups == 1 ? 0 : b] * ws;
-  };
-  scales(0, ns);
+  issue_scales(0, 0);
   issue(0, 0u);
+  float nw = sw[0];
   uint32_t cur = 0;
   for (int b = 0; b < A.kblocks; ++b) {
-#pragma unroll
-    for (int i = 0; i < TT; ++i) {
-      s[i] = ns[i];
-      asm volatile("" : "+v"(s[i]));  // waited for here, before the next block's loads
-    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // block b has landed (every wave's loads), the other place is free
+    const float w = nw;
     if (b + 1 < A.kblocks) {
-      scales(b + 1, ns);
+      nw = sw[b + 1];
+      if ((b + 1) % kMmScales == 0) issue_scales(b + 1, (b + 1) / kMmScales & 1);
       issue(b + 1, kStage - cur);
     }
+    const int left = A.K - b * 128;
+    if (left < 128) {  // uniform, the last block: zeros behind the rows' ends
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int p = i * kThreads + t, j = (p & 7) ^ ((p >> 3) & 7);
+        if (16 * j >= left) *reinterpret_cast<uint4*>(lds + cur + 16 * p) = make_uint4(0, 0, 0, 0);
+      }
+      __syncthreads();
+    }
     if (!idle) {
-      const int left = A.K - b * 128;
-      if (left >= 128) compute(lds + cur, s, std::false_type{}, 0);
-      else compute(lds + cur, s, std::true_type{}, left - 32 * c);
+      float s[TT];
+#pragma unroll
+      for (int i = 0; i < TT; ++i) s[i] = ss[b / kMmScales & 1][(wt * TT + i) * 16 + r][b % kMmScales] * w;
+      compute(lds + cur, s);
     }
     cur = kStage - cur;
   }
@@ -360,10 +395,10 @@ __global__ __launch_bounds__(WO* WT* kWave, 2) void tile_kernel(const MatmulArgs
   }
 }
 
-template <int MT, int TT, bool EXACT>
+template <int MT, int TT, int W, bool EXACT>
 static hipError_t launch_rows(MatmulArgs A, hipStream_t s) {
   A.otiles = (A.N + 16 * MT - 1) / (16 * MT);
-  hipLaunchKernelGGL((rows_kernel<MT, TT, EXACT>), dim3((unsigned)((long)A.otiles * A.experts)), dim3(kRwThreads), 0, s, A);
+  hipLaunchKernelGGL((rows_kernel<MT, TT, W, EXACT>), dim3((unsigned)((long)A.otiles * A.experts)), dim3(W * kWave), 0, s, A);
   return hipGetLastError();
 }
 
@@ -382,9 +417,13 @@ static hipError_t launch_tiles(MatmulArgs A, hipStream_t s) {
 template <bool EXACT>
 static hipError_t launch_matmul(const MatmulArgs& A, hipStream_t s) {
   const long per = ((long)A.rows + A.experts - 1) / A.experts;
-  if (per <= 16) return launch_rows<1, 1, EXACT>(A, s);
-  if (per <= 32) return launch_rows<2, 2, EXACT>(A, s);
-  if (per <= 64) return launch_rows<2, 4, EXACT>(A, s);
+  if (per <= 64) {
+    // few outputs: a workgroup's waves are all the loads its CU has under way
+    const bool narrow = (long)A.experts * ((A.N + 15) / 16) <= 2L * device_cu_count();
+    if (per <= 16 && A.experts == 1) return narrow ? launch_rows<1, 1, 16, EXACT>(A, s) : launch_rows<2, 1, 4, EXACT>(A, s);
+    if (per <= 32) return narrow ? launch_rows<1, 2, 16, EXACT>(A, s) : launch_rows<2, 2, 4, EXACT>(A, s);
+    return narrow ? launch_rows<1, 4, 8, EXACT>(A, s) : launch_rows<2, 4, 4, EXACT>(A, s);
+  }
   return launch_tiles<2, 2, 4, 4, EXACT>(A, s);
 }
 
