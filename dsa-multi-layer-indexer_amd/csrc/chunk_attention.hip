@@ -30,8 +30,6 @@
 
 namespace dsa {
 
-#define DSA_INLINE __attribute__((always_inline))  // (a lambda left out of line keeps its captures in memory)
-
 constexpr int kCaTileCost = 64;   // keys' worth of a row tile's start and end
 constexpr int kCaShare = 128;     // the least share of a workgroup, in keys of a row tile
 // A row's reference point lies this far above its first tile's maximum (in

@@ -35,6 +35,9 @@ typedef uint32_t v2u_t __attribute__((ext_vector_type(2)));
 
 constexpr int kWave = 64;
 
+// (a lambda that is left out of line keeps its captures in memory)
+#define DSA_INLINE __attribute__((always_inline))
+
 // Order-preserving map fp32 -> u32 used by every ranking in this library:
 // larger key == ranks higher.  -0.0 is folded onto +0.0 and every NaN onto
 // the top key, so the order is total and matches the comparison the

@@ -31,6 +31,7 @@
 namespace dsa {
 
 typedef __attribute__((address_space(3))) void* mm_lds_ptr;
+typedef const __attribute__((address_space(4))) float* const_float_ptr;  // (scalar loads)
 
 // The product of a block of 128, by the matrix unit's 8-bit products or, for
 // outputs that show their error (EXACT: fp32), by its bf16 ones.
@@ -96,57 +97,51 @@ __device__ __forceinline__ int2 expert_rows(const MatmulArgs& A, int e) {
 // One workgroup: 16 MT outputs of one expert, 16 TT of its rows at a time.
 // Wave w of W takes the blocks w, w + W, ... of k: it reads its operands from
 // memory straight in the product's layout (lane (r, c) holds bytes [32 c, + 32)
-// of row r: whole 128-byte lines), the weights kRwAhead blocks ahead, the rows,
+// of row r: whole 128-byte lines), the weights kAhead blocks ahead, the rows,
 // which the L2 holds, two; the waves' sums meet in LDS, in the order of the
 // waves.
-constexpr int kRwAhead = 4;
 template <int MT, int TT, int W, bool EXACT>
-__global__ __launch_bounds__(W* kWave, W >= 16 ? 4 : (MT * TT >= 8 ? 2 : 3)) void rows_kernel(const MatmulArgs A) {
+__global__ __launch_bounds__(W* kWave, W >= 16 ? 4 : 3) void rows_kernel(const MatmulArgs A) {
+  constexpr int kAhead = EXACT ? 2 : 4;  // (as many as find registers)
   __shared__ v4f part[W][MT * TT][kWave];
   const int lane = threadIdx.x & (kWave - 1), wv = wave_id();
   const int r = lane & 15, c = lane >> 4;
   const int ot = (int)(blockIdx.x % (unsigned)A.otiles), e = (int)(blockIdx.x / (unsigned)A.otiles);
   const int2 range = expert_rows(A, e);
   const int o0 = ot * 16 * MT;
-  const uint8_t* wbase = A.w + (long)e * A.N * A.K;
-  const float* sw = A.w_scale + ((long)e * A.nblocks + o0 / 128) * A.kblocks;  // (16 MT outputs share a block)
-  const uint8_t* wrow[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) wrow[m] = wbase + (long)min(o0 + 16 * m + r, A.N - 1) * A.K + 32 * c;
+  // Operands through buffer resources: what lies behind a row's end or the last
+  // row is out of range and reads as zero, without a branch among the loads.
+  constexpr uint32_t kNowhere = 0x80000000u;
+  const __amdgpu_buffer_rsrc_t wr = dev_rsrc(A.w + ((long)e * A.N + o0) * A.K, (uint32_t)min(16 * MT, A.N - o0) * (uint32_t)A.K);
+  const auto* sw = (const_float_ptr)(A.w_scale + ((long)e * A.nblocks + o0 / 128) * A.kblocks);  // (16 MT outputs share a block)
   // the wave's i-th block; behind its last, the last again (read, not used)
   const int count = A.kblocks > wv ? (A.kblocks - 1 - wv) / W + 1 : 0;
   const auto block_of = [&](int i) { return wv + W * max(min(i, count - 1), 0); };
-  // 32 bytes of a row, zeros behind its end (of the last, short block)
-  const auto load32 = [&](const uint8_t* row, int b) {
+  const auto load32 = [&](const __amdgpu_buffer_rsrc_t& res, uint32_t row, int b) DSA_INLINE {
     const int left = A.K - b * 128 - 32 * c;
-    const uint4* p = reinterpret_cast<const uint4*>(row + (long)b * 128);
-    const uint4 z = make_uint4(0, 0, 0, 0);
-    if (left >= 32) return two16(p[0], p[1]);
-    return two16(left > 0 ? p[0] : z, z);
+    const uint32_t at = row * (uint32_t)A.K + (uint32_t)(b * 128 + 32 * c);
+    return two16(__builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(res, left > 0 ? at : kNowhere, 0, 0)),
+                 __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(res, left > 16 ? at + 16 : kNowhere, 0, 0)));
   };
   for (int t0 = range.x; t0 < range.y; t0 += 16 * TT) {
-    const uint8_t* arow[TT];
-    const float* srow[TT];
-#pragma unroll
-    for (int t = 0; t < TT; ++t) {
-      const long row = min(t0 + 16 * t + r, range.y - 1);
-      arow[t] = A.a + row * A.K + 32 * c;
-      srow[t] = A.a_scale + row * A.a_groups;
-    }
-    v8i wq[kRwAhead][MT], aq[2][TT];
-    float sq[2][TT];
-    const auto load_w = [&](int i, int u) {
+    const int here = min(16 * TT, range.y - t0);
+    const __amdgpu_buffer_rsrc_t ar = dev_rsrc(A.a + (long)t0 * A.K, (uint32_t)here * (uint32_t)A.K);
+    const __amdgpu_buffer_rsrc_t sr = dev_rsrc(A.a_scale + (long)t0 * A.a_groups, (uint32_t)here * (uint32_t)A.a_groups * 4u);
+    v8i wq[kAhead][MT], aq[2][TT];
+    float sq[2][TT], swq[2];
+    const auto load_w = [&](int i, int u) DSA_INLINE {
       const int b = block_of(i);
 #pragma unroll
-      for (int m = 0; m < MT; ++m) wq[u][m] = load32(wrow[m], b);
+      for (int m = 0; m < MT; ++m) wq[u][m] = load32(wr, (uint32_t)(16 * m + r), b);
     };
-    const auto load_a = [&](int i, int u) {
-      const int b = block_of(i);
-      const float ws = sw[min(b, A.kblocks - 1)];
+    const auto load_a = [&](int i, int u) DSA_INLINE {
+      const int b = min(block_of(i), A.kblocks - 1);
+      swq[u] = sw[b];
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
-        aq[u][t] = load32(arow[t], b);
-        sq[u][t] = srow[t][A.a_groups == 1 ? 0 : min(b, A.kblocks - 1)] * ws;
+        aq[u][t] = load32(ar, (uint32_t)(16 * t + r), b);
+        const uint32_t at = 4u * ((uint32_t)(16 * t + r) * (uint32_t)A.a_groups + (uint32_t)(A.a_groups == 1 ? 0 : b));
+        sq[u][t] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(sr, at, 0, 0));
       }
     };
     v4f acc[MT][TT];
@@ -156,12 +151,12 @@ __global__ __launch_bounds__(W* kWave, W >= 16 ? 4 : (MT * TT >= 8 ? 2 : 3)) voi
       for (int t = 0; t < TT; ++t) acc[m][t] = v4f{0.f, 0.f, 0.f, 0.f};
     if (count > 0) {
 #pragma unroll
-      for (int u = 0; u < kRwAhead; ++u) load_w(u, u);
+      for (int u = 0; u < kAhead; ++u) load_w(u, u);
       load_a(0, 0);
       load_a(1, 1);
-      for (int i0 = 0; i0 < count; i0 += kRwAhead) {
+      const auto blocks = [&](int i0, auto more) DSA_INLINE {
 #pragma unroll
-        for (int u = 0; u < kRwAhead; ++u) {
+        for (int u = 0; u < kAhead; ++u) {
           Operand<EXACT> wf[MT], af[TT];
           float s[TT];
 #pragma unroll
@@ -169,7 +164,7 @@ __global__ __launch_bounds__(W* kWave, W >= 16 ? 4 : (MT * TT >= 8 ? 2 : 3)) voi
 #pragma unroll
           for (int t = 0; t < TT; ++t) {
             af[t].set(aq[u & 1][t]);
-            s[t] = i0 + u < count ? sq[u & 1][t] : 0.f;
+            s[t] = sq[u & 1][t] * swq[u & 1];
           }
           if (i0 + u < count) {  // uniform
 #pragma unroll
@@ -181,10 +176,13 @@ __global__ __launch_bounds__(W* kWave, W >= 16 ? 4 : (MT * TT >= 8 ? 2 : 3)) voi
                 for (int q = 0; q < 4; ++q) acc[m][t][q] = __builtin_fmaf(s[t], d[q], acc[m][t][q]);
               }
           }
-          load_w(i0 + u + kRwAhead, u);
-          load_a(i0 + u + 2, u & 1);
+          if (decltype(more)::value) load_w(i0 + u + kAhead, u);
+          if (decltype(more)::value || u + 2 < kAhead) load_a(i0 + u + 2, u & 1);
         }
-      }
+      };
+      int i0 = 0;
+      for (; i0 + kAhead < count; i0 += kAhead) blocks(i0, std::true_type{});
+      blocks(i0, std::false_type{});  // the last ones, with nothing behind them to load
     }
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -240,18 +238,17 @@ __device__ __forceinline__ int2 find_rows(const MatmulArgs& A, int tile, int& ex
 // at a time (loaded a block at a time into registers they cost a quarter of the
 // time: as many lines as the operands, and a wait).
 constexpr int kMmScales = 8;  // blocks' scales brought at a time
-typedef const __attribute__((address_space(4))) float* const_float_ptr;
-
-template <int WO, int WT, int MO, int TT, bool EXACT>
-__global__ __launch_bounds__(WO* WT* kWave, 2) void tile_kernel(const MatmulArgs A) {
+template <int WO, int WT, int MO, int TT, int KG, bool EXACT>
+__global__ __launch_bounds__(KG* WO* WT* kWave, 2) void tile_kernel(const MatmulArgs A) {
   constexpr int BO = WO * MO * 16, BT = WT * TT * 16, kThreads = WO * WT * kWave;
   constexpr uint32_t kStage = (BO + BT) * 128;
   constexpr int kLoads = (BO + BT) * 8 / kThreads;
   static_assert(kLoads * kThreads == (BO + BT) * 8, "whole loads");
   static_assert((BO * 8) % kThreads == 0, "a load is of weights or of rows");
-  __shared__ __align__(16) uint8_t lds[2 * kStage];
-  __shared__ float ss[2][BT][kMmScales];
-  const int t = threadIdx.x, lane = t & (kWave - 1), wv = wave_id();
+  __shared__ __align__(16) uint8_t lds[KG * 2 * kStage];
+  __shared__ float ss[KG][2][BT][kMmScales];
+  // (thread and wave of a group)
+  const int kg = wave_id() / (WO * WT), t = (int)threadIdx.x - kg * kThreads, lane = t & (kWave - 1), wv = wave_id() - kg * (WO * WT);
   const int r = lane & 15, c = lane >> 4;
   const int wo = wv % WO, wt = wv / WO;
 
@@ -272,7 +269,8 @@ __global__ __launch_bounds__(WO* WT* kWave, 2) void tile_kernel(const MatmulArgs
 
   const uint8_t* wbase = A.w + (long)e * A.N * A.K;
   const uint8_t* abase = A.a + (long)rows.x * A.K;
-  const uint32_t lds0 = (uint32_t)(uintptr_t)(mm_lds_ptr)lds;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(mm_lds_ptr)lds + (uint32_t)kg * (2 * kStage);
+  uint8_t* const mine = lds + kg * (2 * kStage);
   const auto issue = [&](int b, uint32_t buf) {
     // in the last, short block a chunk behind the row's end reads the row's
     // last instead; zeros take its place before the product
@@ -296,16 +294,16 @@ __global__ __launch_bounds__(WO* WT* kWave, 2) void tile_kernel(const MatmulArgs
   // the scales of the wave's outputs' block, by scalar loads
   const auto* sw = (const_float_ptr)(A.w_scale + ((long)e * A.nblocks + min(o0 + wo * MO * 16, A.N - 1) / 128) * A.kblocks);
   static_assert(MO * 16 <= 128 && 128 % (MO * 16) == 0, "a wave's outputs share a block");
-  // those of the rows, kMmScales blocks from b on
+  // those of the rows, for the group's kMmScales blocks from the i-th on
   const float* sbase = A.a_scale + (long)rows.x * A.a_groups;
-  const uint32_t ss0 = (uint32_t)(uintptr_t)(mm_lds_ptr)ss;
-  const auto issue_scales = [&](int b, int place) {
+  const uint32_t ss0 = (uint32_t)(uintptr_t)(mm_lds_ptr)ss[kg];
+  const auto issue_scales = [&](int i0, int place) {
     constexpr int kEach = BT * kMmScales / kThreads;
     static_assert(kEach * kThreads == BT * kMmScales, "whole loads");
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int p = i * kThreads + t;
-      const uint32_t row = (uint32_t)min(p / kMmScales, rows.y - 1 - rows.x), k = (uint32_t)min(b + p % kMmScales, A.a_groups - 1);
+      const uint32_t row = (uint32_t)min(p / kMmScales, rows.y - 1 - rows.x), k = (uint32_t)min((i0 + p % kMmScales) * KG + kg, A.a_groups - 1);
       const uint32_t dst = __builtin_amdgcn_readfirstlane(ss0 + (uint32_t)(place * (BT * kMmScales) + i * kThreads + wv * kWave) * 4u);
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2"
                    :
@@ -353,34 +351,52 @@ __global__ __launch_bounds__(WO* WT* kWave, 2) void tile_kernel(const MatmulArgs
   };
 
   issue_scales(0, 0);
-  issue(0, 0u);
-  float nw = sw[0];
+  if (kg < A.kblocks) issue(kg, 0u);
+  float nw = sw[min(kg, A.kblocks - 1)];
   uint32_t cur = 0;
-  for (int b = 0; b < A.kblocks; ++b) {
+  const int steps = (A.kblocks + KG - 1) / KG;
+  for (int i = 0; i < steps; ++i) {
+    const int b = i * KG + kg, nb = b + KG;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();  // block b has landed (every wave's loads), the other place is free
     const float w = nw;
-    if (b + 1 < A.kblocks) {
-      nw = sw[b + 1];
-      if ((b + 1) % kMmScales == 0) issue_scales(b + 1, (b + 1) / kMmScales & 1);
-      issue(b + 1, kStage - cur);
+    if (nb < A.kblocks) {
+      nw = sw[nb];
+      if ((i + 1) % kMmScales == 0) issue_scales(i + 1, (i + 1) / kMmScales & 1);
+      issue(nb, kStage - cur);
     }
-    const int left = A.K - b * 128;
-    if (left < 128) {  // uniform, the last block: zeros behind the rows' ends
+    if (i + 1 == steps && A.K % 128) {  // uniform, the last block is short: zeros behind the rows' ends
+      const int left = A.K - b * 128;
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int p = i * kThreads + t, j = (p & 7) ^ ((p >> 3) & 7);
-        if (16 * j >= left) *reinterpret_cast<uint4*>(lds + cur + 16 * p) = make_uint4(0, 0, 0, 0);
+      for (int j0 = 0; j0 < kLoads; ++j0) {
+        const int p = j0 * kThreads + t, j = (p & 7) ^ ((p >> 3) & 7);
+        if (16 * j >= left) *reinterpret_cast<uint4*>(mine + cur + 16 * p) = make_uint4(0, 0, 0, 0);
       }
       __syncthreads();
     }
-    if (!idle) {
+    if (!idle && b < A.kblocks) {
       float s[TT];
 #pragma unroll
-      for (int i = 0; i < TT; ++i) s[i] = ss[b / kMmScales & 1][(wt * TT + i) * 16 + r][b % kMmScales] * w;
-      compute(lds + cur, s);
+      for (int q = 0; q < TT; ++q) s[q] = ss[kg][i / kMmScales & 1][(wt * TT + q) * 16 + r][i % kMmScales] * w;
+      compute(mine + cur, s);
     }
     cur = kStage - cur;
+  }
+  if constexpr (KG > 1) {  // the other groups' sums, in their order
+    static_assert(KG == 2 && WO * WT * MO * TT * kWave * sizeof(v4f) <= sizeof(lds), "the second group's sums fit");
+    v4f* const sums = reinterpret_cast<v4f*>(lds) + wv * (MO * TT * kWave) + lane;
+    __syncthreads();
+    if (kg)
+#pragma unroll
+      for (int m = 0; m < MO; ++m)
+#pragma unroll
+        for (int i = 0; i < TT; ++i) sums[(m * TT + i) * kWave] = acc[m][i];
+    __syncthreads();
+    if (kg) return;
+#pragma unroll
+    for (int m = 0; m < MO; ++m)
+#pragma unroll
+      for (int i = 0; i < TT; ++i) acc[m][i] += sums[(m * TT + i) * kWave];
   }
   if (idle) return;
 #pragma unroll
@@ -402,29 +418,27 @@ static hipError_t launch_rows(MatmulArgs A, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <int WO, int WT, int MO, int TT, bool EXACT>
-static hipError_t launch_tiles(MatmulArgs A, hipStream_t s) {
-  constexpr int BO = WO * MO * 16, BT = WT * TT * 16;
-  A.otiles = (A.N + BO - 1) / BO;
-  // every expert's last tile may be short
-  A.rtiles = A.offsets ? A.rows / BT + std::min(A.experts, A.rows) : (A.rows + BT - 1) / BT;
+template <int KG, bool EXACT>
+static hipError_t launch_tiles(const MatmulArgs& A, hipStream_t s) {
   const long total = (long)A.rtiles * A.otiles;
-  hipLaunchKernelGGL((tile_kernel<WO, WT, MO, TT, EXACT>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(WO * WT * kWave), 0, s,
-                     A);
+  hipLaunchKernelGGL((tile_kernel<2, 2, 4, 4, KG, EXACT>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(KG * 4 * kWave), 0, s, A);
   return hipGetLastError();
 }
 
 template <bool EXACT>
-static hipError_t launch_matmul(const MatmulArgs& A, hipStream_t s) {
+static hipError_t launch_matmul(MatmulArgs A, hipStream_t s) {
   const long per = ((long)A.rows + A.experts - 1) / A.experts;
-  if (per <= 64) {
-    // few outputs: a workgroup's waves are all the loads its CU has under way
-    const bool narrow = (long)A.experts * ((A.N + 15) / 16) <= 2L * device_cu_count();
+  if (per <= 32) {
+    // few outputs of long rows: a workgroup's waves are all the loads its CU has under way
+    const bool narrow = (long)A.experts * ((A.N + 15) / 16) <= 2L * device_cu_count() && A.kblocks >= 32;
     if (per <= 16 && A.experts == 1) return narrow ? launch_rows<1, 1, 16, EXACT>(A, s) : launch_rows<2, 1, 4, EXACT>(A, s);
-    if (per <= 32) return narrow ? launch_rows<1, 2, 16, EXACT>(A, s) : launch_rows<2, 2, 4, EXACT>(A, s);
-    return narrow ? launch_rows<1, 4, 8, EXACT>(A, s) : launch_rows<2, 4, 4, EXACT>(A, s);
+    return narrow ? launch_rows<1, 2, 16, EXACT>(A, s) : launch_rows<2, 2, 4, EXACT>(A, s);
   }
-  return launch_tiles<2, 2, 4, 4, EXACT>(A, s);
+  A.otiles = (A.N + 127) / 128;
+  // every expert's last tile may be short
+  A.rtiles = A.offsets ? A.rows / 128 + std::min(A.experts, A.rows) : (A.rows + 127) / 128;
+  // no more tiles than CUs: two groups of waves share a tile's blocks
+  return (long)A.rtiles * A.otiles <= device_cu_count() ? launch_tiles<2, EXACT>(A, s) : launch_tiles<1, EXACT>(A, s);
 }
 
 hipError_t launch_fp8_matmul(MatmulArgs A, hipStream_t s) {

@@ -165,8 +165,8 @@ __global__ __launch_bounds__(kLgThreads, 4) void prefill_logits_kernel(const Log
     for (int j = 0; j < 4; ++j) kbf[j] = e4m3x32_to_bf16(kb[j]);
 
   // ---- staging: 16-byte chunk c of a stage's queries is chunk c & 7 of head
-  // row c >> 3; in LDS its low bits are xored with the head row / 2, so that
-  // the 16 heads of an operand read fall in distinct banks.  Direct-to-LDS
+  // row c >> 3; in LDS its number is xored with the head row's, so that 8
+  // heads of an operand read (what one clock takes) fall in distinct banks.  Direct-to-LDS
   // loads (m0: the wave's base, 16 bytes a lane); rows past the last repeat
   // it. ----
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lg_lds_ptr)buf;
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kLgThreads, 4) void prefill_logits_kernel(const Log
 #pragma unroll
     for (int it = 0; it < NHG; ++it) {
       const int c = it * kLgThreads + t;
-      const int hrow = c >> 3, j = (c & 7) ^ ((hrow >> 1) & 7);
+      const int hrow = c >> 3, j = (c & 7) ^ (hrow & 7);
       const int r = min(s + hrow / kHeads, s1 - 1) - s0;
       const uint32_t off = (uint32_t)r * kQBytes + (uint32_t)(hrow % kHeads) * DSA_INDEX_DIM + 16u * j;
       const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + at + (uint32_t)(it * kLgThreads + wv * kWave) * 16u);
@@ -198,8 +198,8 @@ __global__ __launch_bounds__(kLgThreads, 4) void prefill_logits_kernel(const Log
   };
   // the operand's swizzled chunks 2 kc and 2 kc + 1 of head row kr (the
   // xored bits depend on kr alone)
-  const uint32_t qoff0 = (uint32_t)kr * DSA_INDEX_DIM + (uint32_t)((2 * kc) ^ ((kr >> 1) & 7)) * 16u;
-  const uint32_t qoff1 = (uint32_t)kr * DSA_INDEX_DIM + (uint32_t)((2 * kc + 1) ^ ((kr >> 1) & 7)) * 16u;
+  const uint32_t qoff0 = (uint32_t)kr * DSA_INDEX_DIM + (uint32_t)((2 * kc) ^ (kr & 7)) * 16u;
+  const uint32_t qoff1 = (uint32_t)kr * DSA_INDEX_DIM + (uint32_t)((2 * kc + 1) ^ (kr & 7)) * 16u;
   const auto add32 = [](float x, float y) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
