@@ -23,6 +23,12 @@ keys as with 8 bits (the selections do not depend on kv_bits, for keys with a
 NaN either), and the attention is a launch of its own ahead of the layer's scan
 and top-k.
 
+A chunk of new tokens (a part of a prompt after a cached prefix, or drafted
+tokens) goes through ``chunk_attention_and_indices``: appended together, then
+the dense attention of ``ops.chunk_attention`` or the rows' selections by
+``ops.sparse_mla_decode``, and the indexer's scores by ``ops.chunk_scan`` with
+one select over all rows.
+
 Index convention: selections cross this API as token positions, int64
 ``[B, 1, topk]`` like ``select_topk`` returns them, with the sentinel
 ``S_kv`` (the row length) for unused entries.  They come back in ascending
@@ -78,6 +84,7 @@ class PagedDSALayer:
         self.w = torch.empty(B, self.Hidx, dtype=torch.float32, device=dev)
         self._rows = torch.arange(B, dtype=torch.int32, device=dev)
         self._base = (torch.arange(B, dtype=torch.int64, device=dev) * self.cap)[:, None]
+        self._starts = torch.arange(B + 1, dtype=torch.int32, device=dev)
 
     # ---- cache maintenance ----
     def _append(self, index_k: torch.Tensor, kv: torch.Tensor) -> None:
@@ -178,4 +185,50 @@ class PagedDSALayer:
         o_latent = self.out.float().reshape(self.B, 1, self.H, LATENT_DIM).to(x_norm.dtype)
         hidden = lay._project_output(o_latent)
         nxt = self._to_positions(self.next_idx) if produce_indexer else None
+        return hidden, nxt
+
+    # ---- a chunk of rows ----
+    def chunk_attention_and_indices(self, x_norm: torch.Tensor, rope, attn_indices: torch.Tensor | None,
+                                    produce_indexer: bool = True):
+        """The S rows at positions ``length`` .. ``length + S - 1`` ([B, S,
+        hidden], rope caches for those positions): their keys and latent rows are
+        appended first, then each row attends ``attn_indices`` [B, S, topk] (those
+        up to its own position) or, when None, every token up to its own, and, if
+        asked, this layer's indexer selects among the same tokens.  Returns
+        (attention hidden output [B, S, hidden], next indices [B, S, topk] or
+        None) (dsa_layer.py:145-192 over a cached prefix)."""
+        if x_norm.dim() != 3 or x_norm.shape[0] != self.B or x_norm.shape[1] < 1:
+            raise ValueError(f"x_norm must be [{self.B}, S, hidden], got {tuple(x_norm.shape)}")
+        S = x_norm.shape[1]
+        n = self.B * S
+        if attn_indices is not None and attn_indices.shape != (self.B, S, self.topk):
+            raise ValueError(f"indices must be [{self.B}, {S}, {self.topk}], got {tuple(attn_indices.shape)}")
+        lay = self.layer
+        c_q = lay.q_latent(x_norm)
+        q, kv = lay._mla_qkv(x_norm, c_q, rope)
+        index_q, index_k, weights = lay._indexer_qkw(x_norm, c_q, rope)
+        pos = torch.arange(self.length, self.length + S, device=x_norm.device)
+        self._append(index_k, kv)
+        q_bf16 = q.reshape(n, self.H, QK_DIM).to(torch.bfloat16).contiguous()
+        starts = self._starts * S
+        if attn_indices is None:
+            out = ops.chunk_attention(q_bf16, self.kv_pool, self.page_table, starts, self.seq_lens)
+        else:
+            idx = attn_indices.long()
+            seen = (idx >= 0) & (idx <= pos[None, :, None])
+            slots = torch.where(seen, idx + self._base[:, None], torch.full_like(idx, -1))
+            out = ops.sparse_mla_decode(q_bf16, self.kv_pool, slots.reshape(n, self.topk).to(torch.int32))
+        hidden = lay._project_output(out.float().reshape(self.B, S, self.H, LATENT_DIM).to(x_norm.dtype))
+        if not produce_indexer:
+            return hidden, None
+        q_fp8, w = ops.quantize_index_query(index_q.reshape(n, self.Hidx, INDEX_DIM).to(torch.bfloat16).contiguous(),
+                                            weights.reshape(n, self.Hidx).float().contiguous())
+        slab = max(-(-self.length // PAGE_TOKENS) * PAGE_TOKENS, self.topk)
+        scores = ops.chunk_scan(q_fp8, w, self.index_k, self.page_table, starts, self.seq_lens, slab)
+        # the scores behind a row's position are -inf, which the select pads
+        nxt = ops.select_rows(scores, self.topk, self.length)
+        if nxt is None:
+            lens = torch.full((n,), slab, dtype=torch.int32, device=scores.device)
+            nxt = ops.topk(scores, lens, self.topk, pad_value=self.length).long()
+        nxt = nxt.reshape(self.B, S, self.topk).sort(dim=-1)[0]  # ascending, the sentinel behind
         return hidden, nxt
