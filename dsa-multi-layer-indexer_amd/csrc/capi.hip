@@ -901,7 +901,8 @@ int dsa_fp8_matmul(const dsa_matmul_args* a, void* stream) {
   DSA_REQUIRE(a->out_dtype >= 0 && a->out_dtype <= 2, DSA_ERR_INVALID_ARG,
               "dsa_fp8_matmul: out_dtype must be 0 (fp32), 1 (bf16) or 2 (fp16)");
   DSA_REQUIRE(aligned16(a->a) && aligned16(a->w), DSA_ERR_INVALID_ARG, "dsa_fp8_matmul: a and w must be 16-byte aligned");
-  // (its launches hold a workgroup of at most 512 threads per 16 x 128 outputs)
+  // (a launch is below 2^32 threads: 256 for 32 outputs of an expert's rows, 1024 for 16 only in grids of few
+  // workgroups, 256 or 512 for a tile of 128 x 128)
   DSA_REQUIRE(((int64_t)a->rows / 128 + a->experts) * ((a->N + 15) / 16) < (int64_t)1 << 23, DSA_ERR_UNSUPPORTED,
               "dsa_fp8_matmul: %d rows of %d outputs are too many for a launch", a->rows, a->N);
   dsa::MatmulArgs A{};

@@ -22,6 +22,18 @@
 // began before it and one that ends behind it in part.  Parts leave their sums
 // and reference points in the workspace, where a second launch joins them in the
 // order of the keys.
+//
+// Bound by the matrix unit at the clock that its power leaves (1.55 to 1.9 GHz
+// under this load): 1999 tokens of 16 heads after 16001 keys in 1.24 ms (953
+// TFLOP/s; a library product of 8192 x 8192 x 8192 reaches 1435), 9 ragged chunks
+// of 64 heads over 4-bit rows in 1.05 ms (877).  With few rows a key tile's
+// latency shows: 16 requests of 4 tokens and 16 heads, 64 of a tile's 128 rows, in
+// 104 us (1 TB/s), 3.4 us a key tile against 2.2 for keys in the L2.  Tried and
+// not kept: tiles brought into the L2 ahead (none, or 5% slower); waves without
+// rows that dequantise for the others (139 us for 113, and the large case 1.5 times as
+// slow: a second path takes registers from the first); a second bf16 term of the
+// probabilities (error 0.00144 of the output's norm instead of 0.0015, the plain
+// form's own 0.0014, for 15 to 25% of the time).
 #include <algorithm>
 
 #include "dsa_kernels.h"
@@ -36,10 +48,12 @@ constexpr int kCaShare = 128;     // the least share of a workgroup, in keys of 
 // log2), and a score may rise this far above the reference: any point gives the
 // same sums (bf16 and fp32 have 8 bits of exponent, and a probability's error is
 // relative) while no probability overflows, and one that underflows is below
-// 2^-90 of the row's largest.  A row of scores that rise by more, 96 in log2,
-// is redone from its true maximum.
+// 2^-46 of the row's largest (2^-80 / 2^-126).  A share with a row whose scores
+// rise by more, 144 in log2, is summed again from the rows' true maxima
+// (a span of 96 redid whole shares for one key of 11 times the others' size, 187 in
+// log2: 2.8 ms where 1.3 do).
 constexpr int kCaDepthK = 8, kCaDepthV = 6;  // operand fragments read ahead of their MFMA
-constexpr float kCaAbove = 32.f, kCaRise = 64.f;
+constexpr float kCaAbove = 80.f, kCaRise = 64.f;
 
 // A workgroup's place on the line of work: request, row tile, key tile of it.
 struct ChunkPos {
@@ -339,7 +353,6 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
 
     v16f o[16];
     float m = -INFINITY, l = 0.f;
-    bool over = false;
     uint4 qf[36];
     v16f s;       // scores of a tile, then its probabilities
     v16f sn;      // the next tile's scores
@@ -382,7 +395,7 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
 
     // A tile's softmax, in slices: 0-7 its maximum, 8 the reference point, 9-24
     // the probabilities, 25-32 their bf16 pairs and sum.
-    float tmax = -INFINITY, mr = 0.f;
+    float tmax = -INFINITY, top = -INFINITY, mr = 0.f;  // (top: of all tiles)
     uint32_t pk[8];
     const auto softmax_slice = [&](int i) DSA_INLINE {
       if (i < 8) {
@@ -390,7 +403,7 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
       } else if (i == 8) {
         tmax = half_swap_max(tmax);
         m = m == -INFINITY ? tmax + kCaAbove : m;
-        over |= tmax > m + kCaRise;
+        top = fmaxf(top, tmax);
         mr = m == -INFINITY ? 0.f : m;
       } else if (i < 25) {
         s[i - 9] = __builtin_amdgcn_exp2f(s[i - 9] - mr);
@@ -433,7 +446,7 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
     // A tile passes through: bytes (two places), bf16 (three), scores, values.
     // While tile tl is summed, tl + 1 is scored, tl + 2 dequantised, and tl + 3 on
     // its way.
-    const auto pass = [&](auto max_only) DSA_INLINE {
+    const auto pass = [&]() DSA_INLINE {
       int p0 = page_of(t0), p1 = page_of(t0 + 1), p2 = page_of(t0 + 2);
       issue(p0, t0, 0u);
       if (t0 + 1 < t1) issue(p1, t0 + 1, kRaw);
@@ -460,18 +473,8 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
         if (tl + 3 < t1) issue(p3, tl + 3, at_raw ^ kRawFlip);
         // (always, also where there is no next tile: a branch around the
         // products takes the accumulators through the vector file)
-        if constexpr (decltype(max_only)::value) {
-          scores(next, [](int) {});
-#pragma unroll
-          for (int i = 0; i < 16; ++i) tmax = i ? fmaxf(tmax, s[i]) : s[0];
-          m = fmaxf(m, half_swap_max(tmax));
-          conv_begin(raw + at_raw);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) conv_slice(i, raw + at_raw, after);
-        } else {
-          scores(next, softmax_slice);
-          values(here, raw + at_raw, after);
-        }
+        scores(next, softmax_slice);
+        values(here, raw + at_raw, after);
         take_scores(tl + 1, rows_of(p1, tl + 1));
         if (tl + 2 < t1) conv_end(tl + 2, p2, after);
         p1 = p2;
@@ -496,14 +499,12 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
       l = 0.f;
-      over = false;
-      pass(std::false_type{});
+      pass();
       if (round) break;
-      if (__ballot(over) && lane == 0) redo = 1;
+      if (__ballot(top > m + kCaRise) && lane == 0) redo = 1;
       __syncthreads();
       if (!uniform(redo)) break;
-      m = -INFINITY;
-      pass(std::true_type{});
+      m = top;
     }
     __syncthreads();  // (everyone has read redo)
 
@@ -551,7 +552,8 @@ __global__ __launch_bounds__(kPfThreads, 1) void chunk_attention_kernel(const Ch
 }
 
 // Joins a row's parts: out = sum_s O_s 2^(m_s - m) / sum_s l_s 2^(m_s - m), m =
-// max m_s.  A workgroup: `per` rows of the i-th row tile that more than one
+// max (m_s + log2 l_s): the reference points m_s alone can lie 144 apart from
+// where their parts' weight is.  A workgroup: `per` rows of the i-th row tile that more than one
 // share has part of.  With few parts a wave takes a row; with many the four
 // waves take the parts of one row in turn (w, w + 4, ...; 8 dims a lane) and
 // meet in LDS, always in the same order.
@@ -591,7 +593,7 @@ __global__ __launch_bounds__(kPfThreads) void chunk_merge_kernel(const ChunkAttn
   for (int r = r_lo + (few ? wv : 0); r < min(r_lo + per, A.part_rows) && row0 + r < R; r += few ? kPfWaves : 1) {
     const auto slot = [&](int s) { return (long)(s ? 2 * (first + s) : 2 * first + 1) * A.part_rows + r; };
     float m = -INFINITY;
-    for (int s = lane; s < parts; s += kWave) m = fmaxf(m, A.part_ml[2 * slot(s)]);
+    for (int s = lane; s < parts; s += kWave) m = fmaxf(m, A.part_ml[2 * slot(s)] + log2f(A.part_ml[2 * slot(s) + 1]));
     m = wave_max(m);
     const float mr = m == -INFINITY ? 0.f : m;
     float L = 0.f;

@@ -16,6 +16,10 @@
 // together 81): 1024 rows x 8192 keys x 64 heads in 65 us (2.1
 // PFLOP/s of fp8) where the decode scan's flat form took 146 and torch's
 // quantisation and page layout 200 before it; here that is 14 (two launches).
+// The chunk scan has the same kernel over ragged chunks and paged keys, with its
+// products in bf16 (the 8-bit ones keep 13 bits below the largest of 8 products,
+// which an fp32 score shows): 1023 tokens x 64 heads x 32K keys in 400 us (1.35
+// PFLOP/s of the 2.1 that the matrix unit issues), 4 tokens of 16 requests in 18.
 // Neither 128 keys a wave, nor the products of the next head group issued
 // before this group's sums, nor wave priorities around them moved it by more
 // than 3%.

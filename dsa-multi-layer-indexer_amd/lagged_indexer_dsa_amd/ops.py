@@ -824,7 +824,7 @@ def quantize_rows(x: torch.Tensor, gate: torch.Tensor | None = None, group: int 
     128: a scale per 128 values (the last group may be short); group 0: one per
     row.  scale = max(amax, 1e-6) / 448; a NaN makes its group's scale and codes
     NaN.  Outputs must not overlap inputs.
-    Reference: act_quant (inference/modeling/kernels.py:35-117).
+    Reference: inference/modeling/kernels.py:35-117.
     """
     if group not in (0, 128):
         raise RuntimeError(f"group must be 128 or 0, got {group}")
@@ -920,7 +920,7 @@ def fp8_matmul(a: torch.Tensor, a_scale: torch.Tensor, w: torch.Tensor, w_scale:
     K a multiple of 16; everything contiguous.  Which kernel runs, and the order
     of its sum, depends on the number of rows: a row alone and among others may
     differ in the last bits.
-    Reference: fp8_gemm (inference/modeling/kernels.py:120-221).
+    Reference: inference/modeling/kernels.py:120-221.
     """
     return _matmul(a, a_scale, w, w_scale, None, dtype, out)
 

@@ -561,7 +561,7 @@ int dsa_dense_mla_decode_fp4(const void* q_bf16, const void* kv_pool, int64_t kv
  * codes [n, D] e4m3_rne(y / scale), contiguous; a NaN makes its group's scale
  * and codes NaN.  x and gate [n, D] of one type, row strides in elements.
  * 1 <= D <= DSA_NORM_MAX_DIM.  Outputs must not overlap inputs.
- * Replaces: act_quant (inference/modeling/kernels.py:35-117).
+ * Replaces: inference/modeling/kernels.py:35-117.
  */
 typedef struct dsa_quant_args {
   const void *x, *gate; /* gate may be NULL */
@@ -586,7 +586,7 @@ int dsa_quantize_rows(const dsa_quant_args* args, void* stream);
  *   with expert e's weights; rows outside are neither read nor written.
  * Which kernel runs depends on rows / experts, and with it the order of the sum
  * over b: equal calls give equal bits.
- * Replaces: fp8_gemm (inference/modeling/kernels.py:120-221), with the weights
+ * Replaces: inference/modeling/kernels.py:120-221, with the weights
  * of the experts of a mixture besides.
  */
 typedef struct dsa_matmul_args {

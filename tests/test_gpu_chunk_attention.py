@@ -1,12 +1,14 @@
 """GPU: ops.chunk_attention against float64.
 
-Bound of a row's output, relative to the largest value a row can take, M = max
-|kv| over the keys it sees: the probabilities are rounded to bf16 once (2^-9 of
-each, and the weights' sum is of the rounded ones: at most 2^-9 M + 2^-9 M
-together, less where a second term follows); the scores' products (576 of a whole
-step 2^-23, of the magnitudes' sum) move an exponent by d and a weight by e^d - 1,
-here below 2^-9 for |q| and |kv| of the cases; the output is rounded once (2^-9):
-all within 4 * 2^-9 M.
+Bound of a row's output o, relative to the largest value a row can take, M = max
+|kv| over the keys it sees.  The probabilities are rounded to bf16 once (2^-8 of
+each) and their sum is of the rounded ones, so they move o by at most 2^-8 sum_j
+w_j |v_j - o|, and values within +-M deviate from their mean o by at most M - o^2
+/ M on average; the output's rounding adds 2^-8 |o|: together at most 2^-8 (M +
+|o| - o^2 / M) <= 1.25 * 2^-8 M = 2.5 * 2^-9 M.  The scores' products (576 of a
+whole step 2^-23, of the magnitudes' sum) move an exponent by d and o by at most
+2 d M, here below 1.5 * 2^-9 M for |q| and |kv| of the cases: all within 4 * 2^-9
+M.
 """
 
 from __future__ import annotations
@@ -174,6 +176,30 @@ def test_one_key_outweighs_the_rest(dev):
         c["q"] = torch.zeros_like(c["q"])
         c["q"][..., 0], c["q"][..., 1] = 60.0, 200.0
         _check(_run(ops, c), c, [n], ops)
+
+
+@pytest.mark.parametrize("n", (600, 4000))
+@pytest.mark.parametrize("low,peak,rest", ((0, 140, 135), (-120, 20, 12), (0, 140, 140), (100, 100, -60)))
+def test_parts_with_far_reference_points(dev, n, low, peak, rest):
+    """One share's scores rise by 140 in log2 behind its first keys, while the
+    others begin near that height: every part counts by where its weight is."""
+    from lagged_indexer_dsa_amd import formats as F
+    from lagged_indexer_dsa_amd import ops
+
+    c = _case(dev, 13, [1], [n], 16, 8)
+    kv = torch.randn(len(c["pool"]), 576, device=dev)
+    kv[:, 512:] = 0
+    g = torch.arange(n, device=dev)
+    slots = c["pt"][0].long()[g // 64] * 64 + g % 64
+    level = torch.full((n,), float(rest), device=dev)
+    level[:100] = low
+    level[100] = peak
+    kv[slots, 512] = level
+    c["pool"] = F.pack_latent_rows(kv[:, :512], kv[:, 512:])
+    c["q"][..., 512:] = 0
+    c["q"][..., :512] *= 0.05
+    c["q"][..., 512] = 16.625  # 16.625 / 24 log2(e) = 0.9994
+    _check(_run(ops, c), c, [n], ops)
 
 
 def test_graph_streams_and_shared_workspace(dev):
