@@ -985,6 +985,8 @@ def chunk_scan(q_fp8: torch.Tensor, w: torch.Tensor, index_k: torch.Tensor, page
         out = torch.empty(n, slab_stride, dtype=torch.float32, device=q_fp8.device)
     else:
         _need_shape("out", out, (n, slab_stride), torch.float32)
+        if n:
+            _need_apart("out", out, q_fp8, w, index_k, page_table, q_start, seq_lens)
     if n:
         _lib.call("dsa_chunk_scan", q_fp8.data_ptr(), w.data_ptr(), index_k.data_ptr(), ks[0], page_table.data_ptr(),
                   q_start.data_ptr(), seq_lens.data_ptr(), out.data_ptr(), n, B, Hidx, page_table.shape[1], slab_stride,
@@ -1031,6 +1033,8 @@ def chunk_attention(q: torch.Tensor, kv_pool: torch.Tensor, page_table: torch.Te
         out = torch.empty(n, H, LATENT_DIM, dtype=torch.bfloat16, device=q.device)
     else:
         _need_shape("out", out, (n, H, LATENT_DIM), torch.bfloat16)
+        if n:
+            _need_apart("out", out, q, kv_pool, page_table, q_start, seq_lens, workspace)
     if n:
         if workspace is None:
             workspace = chunk_workspace(n, H, q.device)

@@ -262,3 +262,22 @@ def test_chunk_attention_refusals(dev):
             pytest.fail(f"call {i} was not refused")
     empty = call(q[:0], pool, pt, torch.zeros_like(s), n)
     assert empty.shape == (0, 16, 512)
+
+
+def test_refuses_outputs_over_inputs(dev):
+    """out may share no byte with what the call reads, its workspace among them."""
+    from lagged_indexer_dsa_amd import ops
+
+    c = _case(dev, 14, [2], [70], 16, 8)
+    nbytes = 2 * 16 * 512 * 2
+    ws = ops.chunk_workspace(2, 16, dev)
+    for buf in (c["q"].view(torch.uint8).flatten(), c["pool"].flatten(), ws):
+        out = buf[:nbytes].view(torch.bfloat16).view(2, 16, 512)
+        with pytest.raises(RuntimeError, match="overlaps"):
+            _run(ops, c, workspace=ws, out=out)
+    index_k = torch.zeros(2, 8448, dtype=torch.uint8, device=dev)
+    q8, w = torch.zeros(2, 64, 128, dtype=torch.uint8, device=dev), torch.ones(2, 64, device=dev)
+    for buf in (q8.flatten(), index_k.flatten()):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            ops.chunk_scan(q8, w, index_k, c["pt"], c["starts"], c["lens"], 128,
+                           out=buf[:2 * 128 * 4].view(torch.float32).view(2, 128))
