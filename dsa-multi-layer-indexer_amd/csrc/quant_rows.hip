@@ -20,7 +20,10 @@ constexpr int kQrThreads = 256;
 
 // x * g * sigmoid(g).  e^-g by 2^n 2^f with f from two terms of log2 e, so
 // that the argument's rounding does not grow with |g|; the quotient corrected
-// once by its exact remainder.
+// once by its exact remainder.  Of 75 million codes 141 to 145 are on the wrong
+// side of a border, 130 to 150 where y is a 64-bit silu rounded to fp32; two
+// floats up to the product, with the exponential by its series, make that 117 to
+// 132 and take 104 us for 87.
 __device__ __forceinline__ float silu_times(float g, float x) {
   constexpr float kHi = 1.44269502f, kLo = 1.92596299e-8f;  // log2 e in two floats
   const float n = fminf(fmaxf(rintf(-g * kHi), -200.f), 200.f);
