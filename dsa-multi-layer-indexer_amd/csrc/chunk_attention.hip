@@ -11,8 +11,8 @@
 //
 // Keys: a tile is half a page, one contiguous piece of the pool.  It goes from
 // memory straight to LDS as it is (656 or 400 bytes a row), two places, and the
-// workgroup dequantises it once, into a bf16 tile for its 128 rows: tile t + 1
-// while tile t is multiplied and t + 2 is on its way.  (Rows unpacked to bf16 in
+// workgroup dequantises it once, into a bf16 tile for its 128 rows: tile t + 2
+// while t is summed and t + 1 scored, with t + 3 on its way.  (Rows unpacked to bf16 in
 // memory first, as prefill.hip has them, cost 2.75 times a row's bytes besides,
 // which is more than the attention of up to a few hundred rows.)
 //
