@@ -23,9 +23,9 @@ constexpr int kQrThreads = 256;
 // once by its exact remainder.  Of 75 million codes 141 to 145 are on the wrong
 // side of a border, 130 to 150 where y is a 64-bit silu rounded to fp32; two
 // floats up to the product, with the exponential by its series, make that 117 to
-// 132 and take 104 us for 87.
+// 132 and take a fifth longer.
+constexpr float kHi = 1.44269502f, kLo = 1.92596299e-8f;  // log2 e in two floats
 __device__ __forceinline__ float silu_times(float g, float x) {
-  constexpr float kHi = 1.44269502f, kLo = 1.92596299e-8f;  // log2 e in two floats
   const float n = fminf(fmaxf(rintf(-g * kHi), -200.f), 200.f);
   const float f = __builtin_fmaf(-g, kLo, __builtin_fmaf(-g, kHi, -n));
   const float d = 1.f + __builtin_ldexpf(__builtin_amdgcn_exp2f(f), (int)n);
@@ -36,24 +36,54 @@ __device__ __forceinline__ float silu_times(float g, float x) {
   return q * x;
 }
 
-// Elements i .. i + 7 of a row of D (zeros past its end), gated if GATE.
+// The same for gates from -150 to -86, where the quotient is not a normal number
+// (the reciprocal is flushed to 0 from d = 2^126 on) though an x of 1e30 and more
+// makes the product an ordinary one: x g e^g, its power of two last.  Below, no x
+// brings it to the least scale.
+constexpr float kSmallSilu = -86.f;
+__device__ __forceinline__ bool silu_is_small(float g) { return g < kSmallSilu && g > -150.f; }
+__device__ __forceinline__ float small_silu_times(float g, float x) {
+  const float n = rintf(g * kHi);
+  const float f = __builtin_fmaf(g, kLo, __builtin_fmaf(g, kHi, -n));
+  return __builtin_ldexpf(g * __builtin_amdgcn_exp2f(f) * (x * 0x1p-16f), (int)n + 16);
+}
+
+// Elements i .. i + 7 of a row of D (zeros past its end), gated if GATE; `least`:
+// of the gates seen.
 template <int DT, bool GATE, bool WIDE>
-__device__ __forceinline__ void load_y8(const QuantRowsArgs& A, long row, int i, float* y) {
+__device__ __forceinline__ void load_y8(const QuantRowsArgs& A, long row, int i, float* y, float& least) {
+  float g[8];
   if (!WIDE && i + 8 > A.D) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const bool in = i + e < A.D;
       y[e] = in ? load_elem<DT>(A.x, row * A.xs + i + e) : 0.f;
-      if constexpr (GATE) y[e] = in ? silu_times(load_elem<DT>(A.gate, row * A.gs + i + e), y[e]) : 0.f;
+      if constexpr (GATE) g[e] = in ? load_elem<DT>(A.gate, row * A.gs + i + e) : 0.f;
     }
-    return;
+  } else {
+    load8<DT, WIDE>(A.x, row * A.xs + i, y);
+    if constexpr (GATE) load8<DT, WIDE>(A.gate, row * A.gs + i, g);
   }
-  load8<DT, WIDE>(A.x, row * A.xs + i, y);
   if constexpr (GATE) {
-    float g[8];
-    load8<DT, WIDE>(A.gate, row * A.gs + i, g);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = silu_times(g[e], y[e]);
+    for (int e = 0; e < 8; ++e) {
+      least = fminf(least, g[e]);
+      y[e] = silu_times(g[e], y[e]);
+    }
+  }
+}
+
+// Puts in those of elements i .. i + 7 whose gate is small, read once more: a
+// branch behind all loads that hardly any call takes (selected element by element
+// it cost 5%, branched to between the loads of a whole row 17%).
+template <int DT>
+__device__ __forceinline__ void put_small(const QuantRowsArgs& A, long row, int i, float* y) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (i + e >= A.D) break;
+    const float g = load_elem<DT>(A.gate, row * A.gs + i + e);
+    if (silu_is_small(g)) y[e] = small_silu_times(g, load_elem<DT>(A.x, row * A.xs + i + e));
+    __builtin_amdgcn_sched_barrier(0);  // (gathered, the loads take registers from the other path)
   }
 }
 
@@ -81,7 +111,9 @@ __global__ __launch_bounds__(kQrThreads) void quant_groups_kernel(const QuantRow
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = 0.f;
   } else {
-    load_y8<DT, GATE, WIDE>(A, row, i, y);
+    float least = 0.f;
+    load_y8<DT, GATE, WIDE>(A, row, i, y, least);
+    if (GATE && __builtin_expect(least < kSmallSilu, 0)) put_small<DT>(A, row, i, y);
   }
   const float scale = row_scale<true>(y);
   const v2u_t c = quant8<true>(y, scale);
@@ -90,19 +122,30 @@ __global__ __launch_bounds__(kQrThreads) void quant_groups_kernel(const QuantRow
 }
 
 // One scale a row: a workgroup of T threads a row, up to V vectors of 8 a
-// thread, kept in registers between the maximum and the codes.
+// thread, kept in registers between the maximum and the codes.  (64 registers at
+// most: two workgroups of 1024 a CU, 73 us for gated rows, 86 with one.)
 template <int DT, bool GATE, bool WIDE, int T, int V>
-__global__ __launch_bounds__(T) void quant_whole_rows_kernel(const QuantRowsArgs A) {
+__global__ __launch_bounds__(T, WIDE ? 8 : 1) void quant_whole_rows_kernel(const QuantRowsArgs A) {
   __shared__ uint32_t top[T / kWave];
   const long row = blockIdx.x;
-  float y[V][8];
+  float y[V][8], least = 0.f;
   uint32_t am = 0;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     const int i = 8 * (v * T + (int)threadIdx.x);
     if (i < A.D) {
-      load_y8<DT, GATE, WIDE>(A, row, i, y[v]);
+      load_y8<DT, GATE, WIDE>(A, row, i, y[v], least);
       am = max(am, amax_bits<true>(y[v]));
+    }
+  }
+  if (GATE && __builtin_expect(least < kSmallSilu, 0)) {  // (what they were before is 0 or about the same)
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int i = 8 * (v * T + (int)threadIdx.x);
+      if (i < A.D) {
+        put_small<DT>(A, row, i, y[v]);
+        am = max(am, amax_bits<true>(y[v]));
+      }
     }
   }
   am = wave_reduce<2>(am);
