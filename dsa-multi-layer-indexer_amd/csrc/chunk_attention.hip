@@ -626,8 +626,9 @@ __global__ __launch_bounds__(kPfThreads) void chunk_merge_kernel(const ChunkAttn
       const float inv = L > 0.f ? 1.f / L : (L == L ? 0.f : L);
       x0 *= inv;
       x1 *= inv;
-      reinterpret_cast<uint4*>(out)[lane] =
-          make_uint4(pack_bf16x2(x0[0], x0[1]), pack_bf16x2(x0[2], x0[3]), pack_bf16x2(x1[0], x1[1]), pack_bf16x2(x1[2], x1[3]));
+      v2u_t* const o = reinterpret_cast<v2u_t*>(out) + 2 * lane;  // (out need begin on 8 bytes only)
+      o[0] = v2u_t{pack_bf16x2(x0[0], x0[1]), pack_bf16x2(x0[2], x0[3])};
+      o[1] = v2u_t{pack_bf16x2(x1[0], x1[1]), pack_bf16x2(x1[2], x1[3])};
       continue;
     }
     so[wv][2 * lane] = x0;

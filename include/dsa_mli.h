@@ -623,7 +623,8 @@ int dsa_chunk_scan(const void* q_fp8, const float* w, const void* index_k, int64
  * with kv_g as (3) (656-byte rows) or (12) (400-byte rows) reads them.
  *   q [n, H, 576] bf16, out [n, H, 512] bf16, kv_pool [kv_rows, row_bytes],
  *   page_table [B, pt_stride], q_start [B + 1] (not falling), seq_lens [B];
- *   H a multiple of 16, n * H < 2^31.
+ *   H a multiple of 16 up to 1024, n * H < 2^31; q, kv_pool and workspace begin
+ *   on 16 bytes, out on 8.
  *   workspace dsa_chunk_attention_workspace_bytes(n, H) bytes, no
  *   initialisation (at most 135 MB; not falling in n and H); calls that overlap
  *   in time must not share it.

@@ -40,3 +40,22 @@ def test_gates_below_every_product(dev):
     codes, scales = ops.quantize_rows(torch.full_like(g, 3e38), gate=g)
     assert not bool((codes & 0x7f).any())
     assert bool((scales == torch.tensor(1e-6, device=dev) / 448).all())
+
+
+@pytest.mark.parametrize("new,lens,heads", [([3], [700], 16), ([2], [9000], 128), ([1], [9000], 16), ([40, 1, 300], [400, 5000, 300], 16)],
+                         ids=lambda v: str(v))
+def test_attention_into_an_output_between_boundaries(dev, new, lens, heads):
+    """out on 8 bytes but not on 16: row tiles of few parts, of many, and whole ones."""
+    from lagged_indexer_dsa_amd import ops
+    from test_gpu_chunk_attention import _case, _check, _run
+
+    c = _case(dev, 21, new, lens, heads, 8)
+    want = _run(ops, c)
+    _check(want, c, lens, ops)
+    buf = torch.full((want.numel() + 12,), 3.0, dtype=torch.bfloat16, device=dev)
+    out = buf[4:4 + want.numel()].view(want.shape)
+    assert buf.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 8
+    _run(ops, c, out=out)
+    assert torch.equal(out, want) and bool((buf[:4] == 3).all()) and bool((buf[-8:] == 3).all())
+    with pytest.raises(RuntimeError, match="8-byte"):
+        _run(ops, c, out=buf[1:1 + want.numel()].view(want.shape))
