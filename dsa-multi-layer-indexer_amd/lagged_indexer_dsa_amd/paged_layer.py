@@ -46,6 +46,12 @@ from . import _lib, ops
 from ._lib import INDEX_DIM, LATENT_DIM, PAGE_TOKENS, QK_DIM, LayerArgs
 from .formats import new_latent_pool
 
+# What a chunk's sparse attention and selection take at a time: the rows of the
+# decode and select launches, and scores in memory (2^28: 1 GiB).  A longer chunk
+# goes through in several.
+MAX_ROWS = 65535
+MAX_SCORES = 1 << 28
+
 
 class PagedDSALayer:
     """Paged caches of one layer for ``batch`` rows of up to ``max_ctx``
@@ -210,25 +216,40 @@ class PagedDSALayer:
         pos = torch.arange(self.length, self.length + S, device=x_norm.device)
         self._append(index_k, kv)
         q_bf16 = q.reshape(n, self.H, QK_DIM).to(torch.bfloat16).contiguous()
-        starts = self._starts * S
         if attn_indices is None:
-            out = ops.chunk_attention(q_bf16, self.kv_pool, self.page_table, starts, self.seq_lens)
+            out = ops.chunk_attention(q_bf16, self.kv_pool, self.page_table, self._starts * S, self.seq_lens)
         else:
             idx = attn_indices.long()
             seen = (idx >= 0) & (idx <= pos[None, :, None])
             slots = torch.where(seen, idx + self._base[:, None], torch.full_like(idx, -1))
-            out = ops.sparse_mla_decode(q_bf16, self.kv_pool, slots.reshape(n, self.topk).to(torch.int32))
+            slots = slots.reshape(n, self.topk).to(torch.int32)
+            out = torch.empty(n, self.H, LATENT_DIM, dtype=torch.bfloat16, device=q_bf16.device)
+            for i in range(0, n, MAX_ROWS):
+                ops.sparse_mla_decode(q_bf16[i:i + MAX_ROWS], self.kv_pool, slots[i:i + MAX_ROWS], out=out[i:i + MAX_ROWS])
         hidden = lay._project_output(out.float().reshape(self.B, S, self.H, LATENT_DIM).to(x_norm.dtype))
         if not produce_indexer:
             return hidden, None
         q_fp8, w = ops.quantize_index_query(index_q.reshape(n, self.Hidx, INDEX_DIM).to(torch.bfloat16).contiguous(),
                                             weights.reshape(n, self.Hidx).float().contiguous())
+        q_fp8, w = q_fp8.reshape(self.B, S, self.Hidx, INDEX_DIM), w.reshape(self.B, S, self.Hidx)
         slab = max(-(-self.length // PAGE_TOKENS) * PAGE_TOKENS, self.topk)
-        scores = ops.chunk_scan(q_fp8, w, self.index_k, self.page_table, starts, self.seq_lens, slab)
+        step = max(1, min(MAX_ROWS, MAX_SCORES // slab) // self.B)  # tokens of each request at a time
+        if step >= S:
+            return hidden, self._select_chunk(q_fp8, w, self.seq_lens, slab)
+        return hidden, torch.cat([self._select_chunk(q_fp8[:, i:i + step].contiguous(), w[:, i:i + step].contiguous(),
+                                                     self.seq_lens - max(0, S - i - step), slab)
+                                  for i in range(0, S, step)], dim=1)
+
+    def _select_chunk(self, q_fp8: torch.Tensor, w: torch.Tensor, seq_lens: torch.Tensor, slab: int) -> torch.Tensor:
+        """Selections [B, s, topk] of the queries [B, s, Hidx, 128], each
+        request's the last of its first seq_lens[b] tokens."""
+        s = q_fp8.shape[1]
+        n = self.B * s
+        scores = ops.chunk_scan(q_fp8.reshape(n, self.Hidx, INDEX_DIM), w.reshape(n, self.Hidx), self.index_k,
+                                self.page_table, self._starts * s, seq_lens, slab)
         # the scores behind a row's position are -inf, which the select pads
         nxt = ops.select_rows(scores, self.topk, self.length)
         if nxt is None:
             lens = torch.full((n,), slab, dtype=torch.int32, device=scores.device)
             nxt = ops.topk(scores, lens, self.topk, pad_value=self.length).long()
-        nxt = nxt.reshape(self.B, S, self.topk).sort(dim=-1)[0]  # ascending, the sentinel behind
-        return hidden, nxt
+        return nxt.reshape(self.B, s, self.topk).sort(dim=-1)[0]  # ascending, the sentinel behind

@@ -59,3 +59,68 @@ def test_attention_into_an_output_between_boundaries(dev, new, lens, heads):
     assert torch.equal(out, want) and bool((buf[:4] == 3).all()) and bool((buf[-8:] == 3).all())
     with pytest.raises(RuntimeError, match="8-byte"):
         _run(ops, c, out=buf[1:1 + want.numel()].view(want.shape))
+
+
+def _paged(dev, topk, batch, max_ctx, bits=8):
+    from lagged_indexer_dsa_amd.paged_layer import PagedDSALayer
+    from test_gpu_paged_layer import _Cfg, _Layer
+
+    layer = _Layer(torch.Generator().manual_seed(6))
+    layer.config = type("Small", (_Cfg,), dict(index_topk=topk))()
+    return PagedDSALayer(layer.to(dev), batch=batch, max_ctx=max_ctx, device=dev, kv_bits=bits)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_a_chunk_in_several_launches(dev, bits, monkeypatch):
+    """Attention over selections and selection a few rows at a time: the selections
+    of all rows at once, and the attention but for where its sums are cut (fp32 sums
+    joined in another order, and the output's rounding to bf16: 2^-8 of the largest
+    value, before a projection of 512 of them)."""
+    from _cases import rel_err
+    from lagged_indexer_dsa_amd import paged_layer
+
+    g = torch.Generator().manual_seed(2)
+    B, n0, S = 2, 300, 23
+    prefix, x = torch.randn(B, n0, 256, generator=g).to(dev), torch.randn(B, S, 256, generator=g).to(dev)
+
+    def step(sel):
+        pl = _paged(dev, 64, B, n0 + S, bits)
+        pl.append(prefix, None)
+        return pl.chunk_attention_and_indices(x, None, sel)
+
+    with torch.no_grad():
+        _, sel = step(None)
+        want = step(sel)
+        for rows, scores in ((65535, 2 * 5 * 384), (9, 1 << 28), (1, 1)):
+            monkeypatch.setattr(paged_layer, "MAX_ROWS", rows)
+            monkeypatch.setattr(paged_layer, "MAX_SCORES", scores)
+            got = step(sel)
+            assert torch.equal(got[1], want[1]), (rows, scores)
+            assert rel_err(got[0].cpu().numpy(), want[0].cpu().numpy()) < 2.0 ** -7, (rows, scores)
+
+
+def test_a_chunk_of_more_rows_than_a_launch_takes(dev):
+    """66000 tokens at once, dense and over selections: their selections are the
+    exact ones of their own scores."""
+    import numpy as np
+
+    from lagged_indexer_dsa_amd import ops
+    from oracle import dsa_oracle as O
+
+    S, k = 66000, 64
+    x = torch.randn(1, S, 256, generator=torch.Generator().manual_seed(4)).to(dev)
+    sel = None
+    with torch.no_grad():
+        for i in range(2):
+            print(f"[long chunk] pass {i}", flush=True)
+            pl = _paged(dev, k, 1, S)
+            h, sel = pl.chunk_attention_and_indices(x, None, sel)
+            assert h.shape == x.shape and sel.shape == (1, S, k) and pl.length == S
+        iq, _, w = pl.layer._indexer_qkw(x, pl.layer.q_latent(x), None)
+        for r in (0, 5, 4063, 4064, 65534, 65535, 65999):
+            q8, wf = ops.quantize_index_query(iq[:, r].to(torch.bfloat16).contiguous(), w[:, r].float().contiguous())
+            sc = ops.chunk_scan(q8, wf, pl.index_k, pl.page_table, torch.tensor([0, 1], dtype=torch.int32, device=dev),
+                                torch.tensor([r + 1], dtype=torch.int32, device=dev), pl.cap)
+            want = O.topk_select(sc.cpu().numpy(), np.array([r + 1]), k)[0]
+            want = np.where(want < 0, S, want)
+            assert np.array_equal(np.sort(want), sel[0, r].cpu().numpy()), r
