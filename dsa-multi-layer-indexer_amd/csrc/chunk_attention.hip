@@ -48,12 +48,15 @@ constexpr int kCaShare = 128;     // the least share of a workgroup, in keys of 
 // log2), and a score may rise this far above the reference: any point gives the
 // same sums (bf16 and fp32 have 8 bits of exponent, and a probability's error is
 // relative) while no probability overflows, and one that underflows is below
-// 2^-46 of the row's largest (2^-80 / 2^-126).  A share with a row whose scores
+// 2^-46 of the row's largest (2^-80 / 2^-126).  Its products with the values lie as
+// much lower: a value below 2^-46 makes subnormal sums, which the matrix unit
+// keeps (errors as ever at 2^-56, 0.01 at 2^-64, nothing left at 2^-74; rows that
+// this library packs have no value but 0 below 2^-38).  A share with a row whose scores
 // rise by more, 144 in log2, is summed again from the rows' true maxima
 // (a span of 96 redid whole shares for one key of 11 times the others' size, 187 in
 // log2: 2.8 ms where 1.3 do).
-constexpr int kCaDepthK = 8, kCaDepthV = 6;  // operand fragments read ahead of their MFMA
 constexpr float kCaAbove = 80.f, kCaRise = 64.f;
+constexpr int kCaDepthK = 8, kCaDepthV = 6;  // operand fragments read ahead of their MFMA
 
 // A workgroup's place on the line of work: request, row tile, key tile of it.
 struct ChunkPos {

@@ -1014,9 +1014,11 @@ def chunk_attention(q: torch.Tensor, kv_pool: torch.Tensor, page_table: torch.Te
     q [n,H,576] bf16; kv_pool [rows,656] or [rows,400] uint8; page_table [B,pt]
     int32; q_start [B+1] int32, not falling; seq_lens [B] int32  ->  out
     [n,H,512] bf16 (0 for a row before position 0).  Rows of no request are left
-    as they are (a new out: undefined).  workspace: :func:`chunk_workspace` of
-    at least this n and H; calls that overlap in time must not share one.  For a
-    sparse layer's chunk each row is a row of :func:`sparse_mla_decode`.
+    as they are (a new out: undefined).  Probabilities are rounded to bf16;
+    latent values below 2^-56, which no packer here writes, lose bits.  workspace:
+    :func:`chunk_workspace` of at least this n and H; calls that overlap in time
+    must not share one.  For a sparse layer's chunk each row is a row of
+    :func:`sparse_mla_decode`.
     Reference: attention_core.py:142-160 dense_mla_core.
     """
     qs, ps = q.shape, kv_pool.shape

@@ -628,6 +628,9 @@ int dsa_chunk_scan(const void* q_fp8, const float* w, const void* index_k, int64
  *   workspace dsa_chunk_attention_workspace_bytes(n, H) bytes, no
  *   initialisation (at most 135 MB; not falling in n and H); calls that overlap
  *   in time must not share it.
+ * The probabilities are rounded to bf16 once (the decode ops keep a second term
+ * of large ones).  Latent values count in full from 2^-56 on (the packers write
+ * none but 0 below 2^-38); smaller ones lose bits, and are 0 below 2^-70.
  * A key in a page, or at a slot, outside the pool is masked; a row that sees no
  * key gives 0; rows of no request are left as they are.  Where a row's keys are
  * divided, and so the last bits of its output, depends on the other rows and

@@ -73,3 +73,59 @@ def test_every_tile_once_where_shares_differ(dev):
         print(f"[marked] {k}", flush=True)
         q, pool, pt, s, n, slots, starts = _case(dev, 50 + k, new, lens, 16, 8)
         _check(ops.chunk_attention(q, pool, pt, s, n), q, pool, slots, starts, new, lens)
+
+
+@pytest.mark.parametrize("new,lens,heads", [([1], [5000], 1024), ([5, 2], [300, 77], 1024), ([1] * 3000, [65] * 3000, 16),
+                                            ([0] * 500 + [3] + [0] * 500 + [2] + [0] * 63, [9] * 500 + [4000] + [9] * 500 + [2] + [0] * 63, 32)],
+                         ids=("h1024", "h1024two", "3000r", "empties"))
+def test_most_heads_and_many_requests(dev, new, lens, heads):
+    from lagged_indexer_dsa_amd import ops
+
+    print(f"[marked] {len(new)} requests, heads={heads}", flush=True)
+    q, pool, pt, s, n, slots, starts = _case(dev, 9, new, lens, heads, 8)
+    _check(ops.chunk_attention(q, pool, pt, s, n), q, pool, slots, starts, new, lens)
+
+
+def test_two_calls_at_once(dev):
+    """On two streams, each with its own workspace, beside each other: the bits of
+    each alone."""
+    from lagged_indexer_dsa_amd import ops
+
+    cases = [_case(dev, 3, [600, 3], [5000, 30000], 32, 8), _case(dev, 4, [4] * 16, [3000 + 700 * i for i in range(16)], 16, 4)]
+    want = [ops.chunk_attention(*c[:5]) for c in cases]
+    outs = [[torch.zeros_like(w) for _ in range(6)] for w in want]
+    ws = [ops.chunk_workspace(c[0].shape[0], c[0].shape[1], dev) for c in cases]
+    streams = [torch.cuda.Stream(dev) for _ in cases]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for i in range(6):
+        for c, o, w, st in zip(cases, outs, ws, streams):
+            with torch.cuda.stream(st):
+                ops.chunk_attention(*c[:5], workspace=w, out=o[i])
+    torch.cuda.synchronize()
+    for w, o in zip(want, outs):
+        assert all(torch.equal(x, w) for x in o)
+
+
+@pytest.mark.parametrize("e", [-30, -56, 40])
+def test_small_and_large_latents(dev, e):
+    """Latent values of 2^-56 (far below any that the library's packers write) and
+    2^40 come out as those of 1 do, but for a step of the output (2^-7) where what a
+    sum of products of 2^-136 loses turns its rounding."""
+    from lagged_indexer_dsa_amd import ops
+
+    q, pool, pt, s, n, slots, starts = _case(dev, 8, [5, 1], [700, 9000], 16, 8)
+    want = ops.chunk_attention(q, pool, pt, s, n)
+    pool = pool.clone()
+    scales = pool[:, 512:528].contiguous().view(torch.float32) * 2.0 ** e
+    pool[:, 512:528] = scales.view(torch.uint8)
+    got = ops.chunk_attention(q, pool, pt, s, n)
+    err = (got.double() * 2.0 ** -e - want.double()).abs()
+    assert float((err / want.double().clamp_min(1e-30)).max()) <= 2.0 ** -7
+    _check((got.float() * 2.0 ** -e).to(torch.bfloat16), q, _unscaled(pool, e), slots, starts, [5, 1], [700, 9000])
+
+
+def _unscaled(pool, e):
+    pool = pool.clone()
+    pool[:, 512:528] = (pool[:, 512:528].contiguous().view(torch.float32) * 2.0 ** -e).view(torch.uint8)
+    return pool
