@@ -23,17 +23,26 @@
 // and reference points in the workspace, where a second launch joins them in the
 // order of the keys.
 //
-// Bound by the matrix unit at the clock that its power leaves (1.55 to 1.9 GHz
-// under this load): 1999 tokens of 16 heads after 16001 keys in 1.24 ms (953
-// TFLOP/s; a library product of 8192 x 8192 x 8192 reaches 1435), 9 ragged chunks
-// of 64 heads over 4-bit rows in 1.05 ms (877).  With few rows a key tile's
-// latency shows: 16 requests of 4 tokens and 16 heads, 64 of a tile's 128 rows, in
-// 104 us (1 TB/s), 3.4 us a key tile against 2.2 for keys in the L2.  Tried and
-// not kept: tiles brought into the L2 ahead (none, or 5% slower); waves without
-// rows that dequantise for the others (139 us for 113, and the large case 1.5 times as
-// slow: a second path takes registers from the first); a second bf16 term of the
-// probabilities (error 0.00144 of the output's norm instead of 0.0015, the plain
-// form's own 0.0014, for 15 to 25% of the time).
+// 1999 tokens of 16 heads after 16001 keys take 1.25 ms (945 TFLOP/s; a library
+// product of 8192 x 8192 x 8192 reaches 1435), 9 ragged chunks of 64 heads over
+// 4-bit rows 1.05 ms (877).  Their matrix units are busy 42% and 37% of the clocks
+// (1.85 and 2.0 GHz under this load), LDS 30% and 26% with no conflicts, and a wave,
+// the only one of its SIMD, waits for a fifth of its time: what is left is where
+// products, softmax, unpacking and a tile's first operand reads do not overlap.
+// With few rows a key tile's latency shows: 16 requests of 4 tokens and 16 heads,
+// 64 of a tile's 128 rows, in 102 us (1 TB/s; over 4-bit rows 97), matrix units busy
+// 20%, 3.4 us a key tile against 2.2 for keys in the L2.  Every row tile and part
+// of one begins cold besides: the first loads' offsets are spilled (180 and 192
+// bytes a lane), and 16 of 18 (10 of 12 over 4-bit rows) wait for the load before
+// them when theirs is read back; the steady loop has none of it.
+//
+// The probabilities are one bf16 term: error 0.0016 of the output's norm where fp32
+// ones in torch have 0.0015, nearly all of either the output's rounding.  A second
+// term gives 0.0015 for 15 to 25% of the time (the decode kernels, which wait for
+// memory, take it for large probabilities).  Also tried and not kept: tiles brought
+// into the L2 ahead (none, or 5% slower); waves without rows that dequantise for the
+// others (139 us for 113, and the large case 1.5 times as slow: a second path takes
+// registers from the first).
 #include <algorithm>
 
 #include "dsa_kernels.h"

@@ -23,15 +23,24 @@
 // read once and are the cost: rows_kernel, whose waves divide k and stream the
 // weights from memory into registers, four blocks ahead.  More rows:
 // tile_kernel, tiles of 128 outputs x 128 tokens through LDS.  (33 to 64 rows of
-// 7168 x 7168: 100-145 us by rows_kernel, whose registers run out, 38 by tiles.)
+// 7168 x 7168: 100-145 us by rows_kernel, whose registers run out, 43-45 by tiles.)
+// Tiles divide outputs and rows, and K between two groups of waves at most, so
+// few outputs leave most of the chip idle: 33 to 512 rows of 7168 x 7168 take
+// 43-49 us (floor 11-19), of 2112 x 7168 37-42 (3.3-5.7), and of 128 x 16384
+// 76-87 where 32 rows take 30.  The choice goes by the average over the experts:
+// with 32 at most, an expert of many rows takes them 32 at a time, its weights
+// read again for each (1031 rows of which one of 32 experts has 1000, 4096 x 7168:
+// 174 us, floor 22; 64 experts with 1000 rows in one and 15 in the others 733 us,
+// with 31 each 590, with 70 each 500).
 //
 // Measured, from memory: one token, 2112 x 7168, 8 us (1.9 TB/s: a launch and
 // one wait for memory); 32 rows, 24576 x 1536, 15 us (2.7 TB/s); 128 rows over 32
 // experts of 4096 x 7168, 736 MB of the weights of those that have any, 154 us
-// (4.8 TB/s, a large copy's rate); 4097 rows, 18432 x 7168, 630 us (1.73 PFLOP/s; the matrix
-// unit alone issues these products at 3.8, at the clock that its power leaves);
-// 8191 rows over 32 experts 265 us (0.9 PFLOP/s: 487 MB to move in 97 us, and a
-// last tile of every expert that is part empty).
+// (4.8 TB/s, a large copy's rate); 4097 rows, 18432 x 7168, 635 us (1.7 PFLOP/s), fp32
+// outputs 996; 8191 rows over 32 experts 264 us (0.9 PFLOP/s: 487 MB to move in 97
+// us, and a last tile of every expert that is part empty).  In the large one the
+// matrix unit is busy 38% of the clocks and LDS 48%, more than half of those bank
+// conflicts of the operand reads; waves wait for a third of their time.
 #include <algorithm>
 
 #include "dsa_kernels.h"
@@ -242,8 +251,10 @@ __device__ __forceinline__ int2 find_rows(const MatmulArgs& A, int tile, int& ex
 // One workgroup: BO outputs x BT rows, WO x WT waves of (16 MO) x (16 TT).
 // A block of 128 k at a time goes from memory straight to LDS, two places, the
 // next block's on its way while this one multiplies.  A row's 8 16-byte chunks
-// lie with their number xored with the row's, so that 8 rows of an operand read
-// (what one clock takes) fall in distinct banks.  The rows' scales come 8 blocks
+// lie with their number xored with the row's, which halves the conflicts of the
+// operand reads and leaves 4.9 clocks of an LDS instruction's 8.9 (a lane's chunks
+// 2c and 2c + 1 keep the row's parity, so a read meets half of the banks; rows r
+// and r + 8 of ss share one).  The rows' scales come 8 blocks
 // at a time (loaded a block at a time into registers they cost a quarter of the
 // time: as many lines as the operands, and a wait).
 constexpr int kMmScales = 8;  // blocks' scales brought at a time

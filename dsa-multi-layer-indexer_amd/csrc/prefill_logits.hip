@@ -15,11 +15,13 @@
 // and 57 ns per 4 MFMAs and 32 VALU operations with four waves a SIMD,
 // together 81): 1024 rows x 8192 keys x 64 heads in 65 us (2.1
 // PFLOP/s of fp8) where the decode scan's flat form took 146 and torch's
-// quantisation and page layout 200 before it; here that is 14 (two launches).
+// quantisation and page layout 200 before it; here that is 14 (two launches; 75 in
+// all, with the queries' chunks in LDS as they are or xored with half the row).
 // The chunk scan has the same kernel over ragged chunks and paged keys, with its
 // products in bf16 (the 8-bit ones keep 13 bits below the largest of 8 products,
-// which an fp32 score shows): 1023 tokens x 64 heads x 32K keys in 400 us (1.35
-// PFLOP/s of the 2.1 that the matrix unit issues), 4 tokens of 16 requests in 18.
+// which an fp32 score shows): 1023 tokens x 64 heads x 32K keys in 405 us (1.35
+// PFLOP/s of the 2.1 that the matrix unit issues; it is busy 55% of the clocks, LDS
+// 17%, 7 of them conflicts), 4 tokens of 16 requests in 18.
 // Neither 128 keys a wave, nor the products of the next head group issued
 // before this group's sums, nor wave priorities around them moved it by more
 // than 3%.
@@ -169,9 +171,8 @@ __global__ __launch_bounds__(kLgThreads, 4) void prefill_logits_kernel(const Log
     for (int j = 0; j < 4; ++j) kbf[j] = e4m3x32_to_bf16(kb[j]);
 
   // ---- staging: 16-byte chunk c of a stage's queries is chunk c & 7 of head
-  // row c >> 3; in LDS its number is xored with the head row's, so that 8
-  // heads of an operand read (what one clock takes) fall in distinct banks.  Direct-to-LDS
-  // loads (m0: the wave's base, 16 bytes a lane); rows past the last repeat
+  // row c >> 3; in LDS its number is xored with the head row's (the chunk
+  // form's two operand reads still conflict for 4 clocks each).  Direct-to-LDS loads (m0: the wave's base, 16 bytes a lane); rows past the last repeat
   // it. ----
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lg_lds_ptr)buf;
   const long req = CHUNK ? 0 : (long)b * A.S;  // the request's first row

@@ -9,8 +9,9 @@
 //
 // Bound by memory: 16 lanes hold a group of 128 (8 values each, one load), whose
 // maximum is four steps across the lanes, and a workgroup's 16 groups are one
-// contiguous piece.  Gated rows, 380 MB read and written, take 77 us (4.9 TB/s, a
-// large copy's rate); a token 9 us, a launch and its wait for memory.
+// contiguous piece.  Gated rows, 380 MB read and written, take 79 us (4.8 TB/s, a
+// large copy's rate; 74 with one scale a row); a token 9 us, a launch and its wait
+// for memory.
 #include "dsa_kernels.h"
 #include "quant_core.h"
 
